@@ -466,6 +466,28 @@ int skyrl_logits_bwd(const void* logits, int logits_dtype, int64_t ld_logits, co
                      const float* row_pz, const float* dlogprobs, const float* dentropy, int64_t T, int64_t V,
                      float rcp_temperature, void* dlogits, int64_t ld_dlogits, void* stream);
 
+/* ---- given tokens and the best alternatives ---------------------------------------------------------------------------
+ * The statistics above and, from the same pass, each label's rank and the k columns that sort first, with their log-probabilities; no
+ * counterpart in the reference's trainer.  Columns sort by logit, the larger first, equal ones (-0 equals +0) by column, the lower first,
+ * NaN behind everything.
+ *   ranks int64 [T]: 1 + the number of columns that sort before the label; 0 where the label lies outside [0, V) or its logit is NaN.  A
+ *     label among the alternatives stands at place rank - 1.
+ *   top_ids int64 [T, k], top_logprobs fp32 [T, k], contiguous: best first.  0 <= k <= min(V, SKYRL_LOGITS_TOP_MAX).
+ * A row without any logit above -inf has log-probabilities -inf (row_lse too), entropy and row_pz 0 and columns 0 .. k - 1; its gradient is
+ * zero.  Any of logprobs, entropy, row_lse, row_pz and ranks may be NULL, top_ids and top_logprobs with k = 0.
+ * skyrl_logits_top_bwd writes
+ *   dlogits = ( g (onehot[label] - p) - dentropy p (y - row_pz) + sum_j dtop_j (onehot[top_ids_j] - p) ) * rcp_temperature
+ * with g = dlogprobs where the label lies in [0, V) and 0 elsewhere (the log-probability is the constant 0 there).  dlogprobs, dentropy
+ * and dtop (fp32 [T, k]) may each be NULL, not all three; alternatives outside [0, V) have no term.  dlogits as in skyrl_logits_bwd.  Every
+ * result is the same bits on each call. */
+#define SKYRL_LOGITS_TOP_MAX 128
+int skyrl_logits_top_fwd(const void* logits, int logits_dtype, int64_t ld_logits, const int64_t* labels, int64_t T, int64_t V, int64_t k,
+                         float rcp_temperature, float* logprobs, float* entropy, float* row_lse, float* row_pz, int64_t* ranks,
+                         float* top_logprobs, int64_t* top_ids, void* stream);
+int skyrl_logits_top_bwd(const void* logits, int logits_dtype, int64_t ld_logits, const int64_t* labels, const float* row_lse,
+                         const float* row_pz, const float* dlogprobs, const float* dentropy, const int64_t* top_ids, const float* dtop,
+                         int64_t T, int64_t V, int64_t k, float rcp_temperature, void* dlogits, int64_t ld_dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

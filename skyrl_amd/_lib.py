@@ -102,6 +102,11 @@ SIGNATURES = {
     "skyrl_logits_bwd": (
         ctypes.c_int,
         [_c_p, ctypes.c_int, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_i64, _c_p]),
+    "skyrl_logits_top_fwd": (
+        ctypes.c_int, [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float] + [_c_p] * 8),
+    "skyrl_logits_top_bwd": (
+        ctypes.c_int,
+        [_c_p, ctypes.c_int, _c_i64] + [_c_p] * 7 + [_c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_i64, _c_p]),
     "skyrl_logprob_diff_metrics": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p]),
     "skyrl_lmhead_mfma_probe": (ctypes.c_int, [_c_p, ctypes.c_int, ctypes.c_int, _c_p, _c_p]),
     "skyrl_lmhead_atomic_floor_probe": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p]),

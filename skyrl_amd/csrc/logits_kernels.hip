@@ -21,130 +21,16 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <cmath>
-
-#include "../../include/skyrl_lmhead.h"
+#include "logits_rows.hpp"
 
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+using namespace logits;
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kLowest = -3.0e38f;  // start of a running maximum: finite, so that (-inf) - max is -inf and never NaN
-// A logit of -inf (a masked vocabulary entry) has probability exactly 0; in the products z * p it is taken as this finite
-// value so that 0 * inf does not turn the row into NaN (the reference's entropy does return NaN there, torch_utils.py:99-100).
-constexpr float kMostNegativeFactor = -1.0e30f;
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBwdThreads = 1024;
 constexpr int kInFlight = 4;  // 16-byte loads a thread has in flight
-
-// Eight bf16 or four fp32 logits of one 16-byte piece, widened to fp32.
-template <bool F32>
-struct Piece {
-  static constexpr int kElems = F32 ? 4 : 8;
-  float v[kElems];
-  __device__ __forceinline__ void load(const void* p) {
-    const uint4 raw = *(const uint4*)p;
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    if (F32) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    }
-  }
-};
-
-// Where the 16-byte pieces of a row lie: logits [head, head + pieces * E); the other `single` logits are numbered head first.
-struct RowPieces {
-  int head, pieces, single;
-};
-template <bool F32>
-__device__ __forceinline__ RowPieces row_pieces(const char* row, int V, bool vector_ok) {
-  constexpr int E = Piece<F32>::kElems, ES = F32 ? 4 : 2;
-  int head = (int)((16u - (uint32_t)((uintptr_t)row & 15u)) & 15u) / ES;
-  head = head < V ? head : V;
-  const int pieces = vector_ok ? (V - head) / E : 0;
-  return RowPieces{head, pieces, V - pieces * E};
-}
-__device__ __forceinline__ int single_column(const RowPieces& r, int elems, int i) { return i < r.head ? i : i + r.pieces * elems; }
-
-__device__ __forceinline__ float load_one(const void* base, size_t i, bool f32) {
-  return f32 ? ((const float*)base)[i] : __uint_as_float((uint32_t)((const uint16_t*)base)[i] << 16);
-}
-
-__device__ __forceinline__ uint16_t bf16_bits(float x) {
-  typedef __attribute__((ext_vector_type(2))) float f32x2;
-  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-  const f32x2 pair = {x, 0.f};
-  const bf16x2 b = __builtin_convertvector(pair, bf16x2);
-  return (uint16_t)(*(const uint32_t*)&b & 0xffffu);
-}
-
-// Running statistics of a row in base 2, with y2 = z * log2e / temperature:  m = max y2,  s = sum 2^(y2 - m),
-// e = sum (y2 - m) * 2^(y2 - m).  The third sum is kept relative to the maximum, like the other two, so that a large common
-// offset of a row's logits costs no accuracy:  entropy = ln s - ln 2 * e / s,  logprob = ln 2 * (y2[label] - m) - ln s.
-struct Stats {
-  float m, s, e;
-};
-
-template <bool ENT>
-__device__ __forceinline__ void absorb(Stats& st, float z, float scale2) {
-  const float t = fmaf(z, scale2, -st.m);
-  const float p = __builtin_amdgcn_exp2f(t);
-  st.s += p;
-  if (ENT) st.e = fmaf(fmaxf(t, kMostNegativeFactor), p, st.e);
-}
-
-// Sums taken relative to maximum `from`, re-expressed relative to `to` >= from.
-__device__ __forceinline__ void rebase(float& s, float& e, float from, float to) {
-  const float d = fmaxf(from - to, kMostNegativeFactor);  // <= 0; finite, so that d * 0 is 0 for an empty sum
-  const float c = __builtin_amdgcn_exp2f(d);
-  e = c * fmaf(d, s, e);
-  s *= c;
-}
-
-// Raise the running maximum to at least `cand` (a value of y2).
-__device__ __forceinline__ void raise_max(Stats& st, float cand) {
-  if (cand > st.m) {
-    rebase(st.s, st.e, st.m, cand);
-    st.m = cand;
-  }
-}
-
-__device__ __forceinline__ void merge(Stats& a, const Stats& b) {
-  const float m = fmaxf(a.m, b.m);
-  float bs = b.s, be = b.e;
-  rebase(a.s, a.e, a.m, m);
-  rebase(bs, be, b.m, m);
-  a.s += bs;
-  a.e += be;
-  a.m = m;
-}
-
-// The row's statistics in every thread.
-__device__ __forceinline__ Stats block_merge(Stats st, Stats* sm) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    Stats other;
-    other.m = __shfl_xor(st.m, o, 64);
-    other.s = __shfl_xor(st.s, o, 64);
-    other.e = __shfl_xor(st.e, o, 64);
-    merge(st, other);
-  }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (lane == 0) sm[wave] = st;
-  __syncthreads();
-  Stats all = sm[0];
-  for (int w = 1; w < kWaves; ++w) merge(all, sm[w]);
-  return all;
-}
 
 // Statistics of row `row`.
 template <bool F32, bool ENT>
@@ -191,7 +77,7 @@ __global__ __launch_bounds__(kThreads) void logits_fwd_rows(const void* __restri
   __shared__ Stats sm[kWaves];
   const int64_t row = blockIdx.x;
   const float scale2 = rcp_temp * kLog2e;
-  const Stats st = block_merge(row_stats<F32, ENT>(logits, ld, row, V, scale2), sm);
+  const Stats st = block_merge<kWaves>(row_stats<F32, ENT>(logits, ld, row, V, scale2), sm);
   if (threadIdx.x == 0) {
     const float log_s = logf(st.s);
     const float lse = fmaf(st.m, kLn2, log_s);
@@ -291,23 +177,6 @@ __global__ __launch_bounds__(kBwdThreads) void logits_bwd_rows(const void* logit
   }
 }
 
-constexpr int64_t kCacheBytes = (int64_t)256 << 20;
-constexpr int64_t kMaxRows = (int64_t)1 << 31;  // the grid's x extent
-
-// Whether every row of b starts as far from a 16-byte boundary as the same row of a.
-bool same_row_offsets(const void* a, int64_t lda, const void* b, int64_t ldb, bool f32) {
-  return (((uintptr_t)a - (uintptr_t)b) & 15u) == 0 && (lda - ldb) * (f32 ? 4 : 2) % 16 == 0;
-}
-
-int check_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, float rcp_temperature) {
-  if (!logits) return SKYRL_LMHEAD_ERR_NULL;
-  if (dtype != SKYRL_LOGITS_BF16 && dtype != SKYRL_LOGITS_F32) return SKYRL_LMHEAD_ERR_ARG;
-  if (T < 1 || V < 1 || ld < V || T >= kMaxRows || V >= ((int64_t)1 << 31) || ld >= ((int64_t)1 << 40)) return SKYRL_LMHEAD_ERR_SHAPE;
-  if ((uintptr_t)logits & (dtype == SKYRL_LOGITS_F32 ? 3u : 1u)) return SKYRL_LMHEAD_ERR_ALIGN;
-  if (!(rcp_temperature > 0.f) || !std::isfinite(rcp_temperature)) return SKYRL_LMHEAD_ERR_ARG;
-  return SKYRL_LMHEAD_OK;
-}
-
 }  // namespace
 
 extern "C" {
@@ -344,13 +213,7 @@ int skyrl_logits_bwd(const void* logits, int logits_dtype, int64_t ld_logits, co
   if (ld_dlogits < V || ld_dlogits >= ((int64_t)1 << 40)) return SKYRL_LMHEAD_ERR_SHAPE;
   const bool f32 = logits_dtype == SKYRL_LOGITS_F32;
   if (((uintptr_t)dlogits & (f32 ? 3u : 1u)) || (labels && ((uintptr_t)labels & 7u))) return SKYRL_LMHEAD_ERR_ALIGN;
-  // In place, or apart: a gradient buffer that overlaps the logits in any other way would be read after it was written.
-  if (dlogits != logits || ld_dlogits != ld_logits) {
-    const char *a0 = (const char*)logits, *b0 = (const char*)dlogits;
-    const size_t es = f32 ? 4 : 2;
-    const char *a1 = a0 + ((size_t)(T - 1) * (size_t)ld_logits + (size_t)V) * es, *b1 = b0 + ((size_t)(T - 1) * (size_t)ld_dlogits + (size_t)V) * es;
-    if (a0 < b1 && b0 < a1) return SKYRL_LMHEAD_ERR_ARG;
-  }
+  if (overlaps_otherwise(logits, ld_logits, dlogits, ld_dlogits, T, V, f32)) return SKYRL_LMHEAD_ERR_ARG;
   const int vec = same_row_offsets(logits, ld_logits, dlogits, ld_dlogits, f32) ? 1 : 0;
   hipStream_t s = (hipStream_t)stream;
   const bool entgrad = dentropy != nullptr;

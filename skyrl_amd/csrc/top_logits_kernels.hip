@@ -1,0 +1,475 @@
+// Log-probability, rank and entropy of given tokens and the k best alternatives with their log-probabilities, from materialised logits
+// [T, V] in ONE pass over them; and the gradient of the logits from gradients on all of those, in one read and write pass.
+//
+//   y = z / temperature;  lse = log sum exp y;  logprob = y[label] - lse;  entropy = lse - sum softmax(y) y
+//   rank = 1 + number of columns that sort before the label;  top = the first k columns of that order, with y[column] - lse
+//   dz = ( g (1[label] - p) - q p (y - pz) + sum_j h_j (1[top_j] - p) ) / temperature,      p = exp(y - lse)
+//
+// Order of columns: the larger logit first, the lower column first among equal ones (-0 equals +0); NaN behind everything.  It is total, so that
+// the k best are one set whatever order candidates are found in.
+// A row without any logit above -inf has lse = -inf: log-probabilities -inf, entropy 0, zero gradient, columns 0 .. k - 1.
+//
+// Selection.  A candidate must reach the k-th largest of the maxima of 128 groups of lanes: those are 128 different logits of the row, so at
+// least k logits reach it, and hardly more do (128 ln 1 / (1 - k / 128): 22 for k = 20, 37 for k = 32).  The bound is formed from the
+// first 16 KiB pieces of a row before any of them is looked at, and again whenever the part of the row that has been seen doubles, so
+// that a row has about k (1 + ln(V / 16384)) candidates; a piece without one costs a comparison and a vote.  The same with the rank: only pieces that
+// reach the label's logit are counted in.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "logits_rows.hpp"
+
+namespace {
+
+using namespace logits;
+
+typedef unsigned long long key_t;
+
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kBwdThreads = 1024;
+constexpr int kInFlight = 4;  // 16-byte loads a thread has in flight
+constexpr int kMaxTop = SKYRL_LOGITS_TOP_MAX;
+constexpr int kGroups = 128;  // of four lanes, whose maxima bound the k-th largest logit from below
+constexpr int kGroupsPerWave = kGroups / kWaves;
+constexpr int kWaveList = 256;  // candidates a wave holds before it drops all but its k best
+static_assert(kMaxTop <= kGroups && kMaxTop + 64 <= kWaveList, "a bound of k groups; room for the candidates of one step behind the k best");
+
+// Bits of a float that compare as the floats do; 0 for NaN, -0 as +0.
+__device__ __forceinline__ uint32_t ordered_bits(float z) {
+  const uint32_t b = __float_as_uint(z + 0.f);
+  return z != z ? 0u : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float value_of_bits(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
+// A larger key sorts earlier.
+__device__ __forceinline__ key_t make_key(float z, int column) { return ((key_t)ordered_bits(z) << 32) | (key_t)(uint32_t)(~column); }
+__device__ __forceinline__ int key_column(key_t k) { return (int)(~(uint32_t)k); }
+__device__ __forceinline__ uint32_t key_bits(key_t k) { return (uint32_t)(k >> 32); }
+
+// LDS operations of a wave execute in order; this keeps the compiler from holding entries that another lane has rewritten.
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// The k largest of the n keys (k < n <= kWaveList) of a wave's list to its front, in any order; returns the smallest of them.  A bisection over
+// the key bits on keys held in registers.
+__device__ __noinline__ key_t keep_best(key_t* list, int n, int k) {
+  const int lane = threadIdx.x & 63;
+  constexpr int B = kWaveList / 64;
+  key_t x[B];
+#pragma unroll
+  for (int u = 0; u < B; ++u) x[u] = u * 64 + lane < n ? list[u * 64 + lane] : 0;  // 0 reaches no trial
+  key_t reach = 0;
+  for (int b = 63; b >= 0; --b) {
+    const key_t trial = reach | ((key_t)1 << b);
+    int c = 0;
+#pragma unroll
+    for (int u = 0; u < B; ++u) c += (int)__popcll(__ballot(x[u] >= trial));
+    if (c >= k) reach = trial;  // all 64 bits: `reach` ends as the k-th largest key
+  }
+  wave_fence();
+  int w = 0;
+#pragma unroll
+  for (int u = 0; u < B; ++u) {
+    const bool keep = u * 64 + lane < n && x[u] >= reach;
+    const unsigned long long mask = __ballot(keep);
+    if (keep) list[w + __popcll(mask & ((1ull << lane) - 1))] = x[u];
+    w += (int)__popcll(mask);
+  }
+  wave_fence();
+  return reach;
+}
+
+// What the waves of a workgroup share.
+struct Shared {
+  Stats stats[kWaves];
+  key_t list[kWaves][kWaveList];
+  float group_max[kGroups];
+  float bound;         // every wave's candidates reach it
+  int count[kWaves], better[kWaves];
+};
+
+// A value that at least k of the 128 groups reach, from the first 16 bits of their maxima (exact for bf16); by one wave.
+__device__ __forceinline__ float group_bound(const float* group_max, int k) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t a = ordered_bits(group_max[lane]) >> 16, b = ordered_bits(group_max[64 + lane]) >> 16;
+  uint32_t reach = 0;
+  for (int bit = 15; bit >= 0; --bit) {
+    const uint32_t trial = reach | (1u << bit);
+    if ((int)(__popcll(__ballot(a >= trial)) + __popcll(__ballot(b >= trial))) >= k) reach = trial;
+  }
+  const uint32_t bits = reach << 16;
+  return bits < 0x00800000u ? -INFINITY : value_of_bits(bits);  // NaN, or -inf: no bound yet
+}
+
+// The smallest float above z (z is not NaN; +inf gives NaN, which nothing reaches).
+__device__ __forceinline__ float next_above(float z) {
+  const int b = __float_as_int(z + 0.f);
+  return __int_as_float(b >= 0 ? b + 1 : b - 1);
+}
+
+struct TopArgs {
+  const void* logits;
+  int64_t ld;
+  const int64_t* labels;  // NULL: no log-probability and no rank wanted
+  int V, k;
+  float rcp_temp;
+  float *logprobs, *entropy, *row_lse, *row_pz;
+  int64_t* ranks;
+  float* top_logprobs;
+  int64_t* top_ids;
+};
+
+// One workgroup per row.
+template <bool F32>
+__global__ __launch_bounds__(kThreads) void logits_top_rows(const TopArgs a) {
+  constexpr int E = Piece<F32>::kElems, ES = F32 ? 4 : 2;
+  __shared__ Shared sm;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row = blockIdx.x;
+  const int V = a.V, k = a.k;
+  const char* base = (const char*)a.logits + (size_t)row * (size_t)a.ld * ES;
+  const float scale2 = a.rcp_temp * kLog2e;
+  const RowPieces rp = row_pieces<F32>(base, V, true);
+  const char* vec = base + (size_t)rp.head * ES;
+  const int pieces = rp.pieces;
+
+  int64_t label = a.labels ? a.labels[row] : (int64_t)-1;
+  const bool has_label = label >= 0 && label < (int64_t)V;
+  const float z_label = has_label ? load_one(base, (size_t)label, F32) : NAN;
+  const int y = has_label ? (int)label : -1;
+  const float above_label = next_above(z_label);  // NaN (no label, or its logit is NaN): nothing reaches it
+
+  Stats st{kLowest, 0.f, 0.f};
+  float lane_max = -INFINITY;
+  int better = 0;       // columns of this lane that sort before the label
+  int count = 0;        // candidates in the wave's list
+  key_t least = 0;      // candidates have larger keys: the worst of k that the wave has seen
+  float bound = -INFINITY;
+  key_t* const list = sm.list[wave];
+
+  auto append = [&](float z, int column, bool there) {
+    const key_t key = make_key(z, column);
+    const bool hit = there && z >= bound && key > least;
+    const unsigned long long mask = __ballot(hit);
+    if (mask == 0) return;
+    if (hit) list[count + __popcll(mask & ((1ull << lane) - 1))] = key;
+    count += (int)__popcll(mask);
+    wave_fence();
+    if (count > kWaveList - 64) {
+      least = keep_best(list, count, k);
+      count = k;
+      bound = fmaxf(bound, value_of_bits(key_bits(least)));
+    }
+  };
+  auto publish = [&]() {  // the maxima of groups of four lanes
+    float m = fmaxf(lane_max, __shfl_xor(lane_max, 1, 64));
+    m = fmaxf(m, __shfl_xor(m, 2, 64));
+    if ((lane & 3) == 0) sm.group_max[wave * kGroupsPerWave + (lane >> 2)] = m;
+  };
+  // rank: columns in front of the label's precede it with an equal logit already
+  auto count_better = [&](float z, int column) {
+    better += z >= above_label || (z == z_label && column < y) ? 1 : 0;
+  };
+
+  int step = 0;
+  for (int p0 = tid; p0 - tid < pieces; p0 += kThreads * kInFlight, ++step) {
+    Piece<F32> pc[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int p = p0 + u * kThreads;
+      pc[u].load(vec + (size_t)(p < pieces ? p : pieces - 1) * 16);
+    }
+    float mx[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      mx[u] = -INFINITY;
+      if (p0 + u * kThreads < pieces) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) mx[u] = fmaxf(mx[u], pc[u].v[i]);
+      }
+      lane_max = fmaxf(lane_max, mx[u]);
+    }
+    if (k > 0 && (step & (step + 1)) == 0) {  // steps 0, 1, 3, 7: what has been seen doubles
+      publish();
+      if (step == 0) {
+        __syncthreads();
+        if (wave == 0) {
+          const float b = group_bound(sm.group_max, k);
+          if (lane == 0) sm.bound = b;
+        }
+        __syncthreads();
+      } else if (wave == (step & (kWaves - 1))) {  // whatever the other waves have published: a bound all the same
+        wave_fence();
+        const float b = group_bound(sm.group_max, k);
+        if (lane == 0) *(volatile float*)&sm.bound = fmaxf(*(volatile float*)&sm.bound, b);
+      }
+    }
+    if (k > 0) bound = fmaxf(bound, *(volatile float*)&sm.bound);
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int p = p0 + u * kThreads;
+      const bool there = p < pieces;
+      if (__any(mx[u] * scale2 > st.m)) raise_max(st, mx[u] * scale2);
+      if (there) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) absorb<true>(st, pc[u].v[i], scale2);
+      }
+      const int c0 = rp.head + p * E;
+      if (__any(mx[u] >= z_label)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (there) count_better(pc[u].v[i], c0 + i);
+      }
+      if (k > 0 && __any(mx[u] >= bound)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) append(pc[u].v[i], c0 + i, there);
+      }
+    }
+  }
+  for (int i0 = 0; i0 < rp.single; i0 += kThreads) {
+    const int i = i0 + tid;
+    const bool there = i < rp.single;
+    const int c = single_column(rp, E, there ? i : 0);
+    const float z = load_one(base, (size_t)c, F32);
+    if (there) {
+      raise_max(st, z * scale2);
+      absorb<true>(st, z, scale2);
+      count_better(z, c);
+    }
+    if (k > 0) append(z, c, there);
+  }
+
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) better += __shfl_xor(better, o, 64);
+  if (lane == 0) sm.count[wave] = count, sm.better[wave] = better;
+  st = block_merge<kWaves>(st, sm.stats);  // a barrier: the lists and counts of all waves stand
+  const bool empty = st.s == 0.f;
+  const float log_s = empty ? -INFINITY : logf(st.s);
+  auto logprob_of = [&](float z) { return empty ? -INFINITY : fmaf(z, scale2, -st.m) * kLn2 - log_s; };
+  if (tid == 0) {
+    int before = 0;
+    for (int w = 0; w < kWaves; ++w) before += sm.better[w];
+    if (a.ranks) a.ranks[row] = has_label && z_label == z_label ? 1 + before : 0;
+    if (a.logprobs) a.logprobs[row] = has_label ? logprob_of(z_label) : 0.f;
+    if (a.entropy) a.entropy[row] = empty ? 0.f : log_s - st.e / st.s * kLn2;
+    if (a.row_lse) a.row_lse[row] = empty ? -INFINITY : fmaf(st.m, kLn2, log_s);
+    if (a.row_pz) a.row_pz[row] = empty ? 0.f : (st.e / st.s + st.m) * kLn2;
+  }
+  if (k == 0) return;
+
+  // The place of a candidate among the k best is the number of better ones: every thread takes one of all lists' candidates.
+  int total = 0;
+  for (int w = 0; w < kWaves; ++w) total += sm.count[w];
+  if (total > kThreads) {  // the same for the whole workgroup
+    __syncthreads();  // every wave has read the counts
+    if (count > k) {
+      (void)keep_best(list, count, k);
+      if (lane == 0) sm.count[wave] = k;
+    }
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < kWaves; ++w) total += sm.count[w];
+  }
+  for (int e0 = 0; e0 < total; e0 += kThreads) {
+    int e = e0 + tid, w = 0;
+    while (w < kWaves && e >= sm.count[w]) e -= sm.count[w], ++w;
+    if (w < kWaves) {
+      const key_t mine = sm.list[w][e];
+      int place = 0;
+      for (int v = 0; v < kWaves && place < k; ++v)
+        for (int i = 0; i < sm.count[v]; ++i) place += sm.list[v][i] > mine ? 1 : 0;
+      if (place < k) {
+        a.top_ids[row * (int64_t)k + place] = key_column(mine);
+        a.top_logprobs[row * (int64_t)k + place] = logprob_of(value_of_bits(key_bits(mine)));
+      }
+    }
+  }
+  // Fewer logits than k that are numbers: the first NaN columns, in order, by one wave.
+  if (total < k && wave == 0) {
+    int place = total;
+    for (int c0 = 0; c0 < V && place < k; c0 += 64) {
+      const int c = c0 + lane;
+      const float z = c < V ? load_one(base, (size_t)c, F32) : 0.f;
+      const unsigned long long mask = __ballot(z != z);
+      const int at = place + (int)__popcll(mask & ((1ull << lane) - 1));
+      if (z != z && at < k) {
+        a.top_ids[row * (int64_t)k + at] = c;
+        a.top_logprobs[row * (int64_t)k + at] = NAN;
+      }
+      place += (int)__popcll(mask);
+    }
+  }
+}
+
+// The gradient.  As logits_bwd_rows (logits_kernels.hip), with sum_j h_j in the coefficient of p, and the k + 1 columns that have a term of their
+// own written once more behind a barrier, from logits read in front of the pass (dlogits may be the logits themselves).
+struct TopBwdArgs {
+  const void* logits;
+  int64_t ld;
+  const int64_t* labels;
+  int V, k;
+  float rcp_temp;
+  int vector_ok;
+  const float *row_lse, *row_pz, *dlogprobs, *dentropy;
+  const int64_t* top_ids;
+  const float* dtop;
+  void* dlogits;
+  int64_t ldd;
+};
+
+template <bool F32, bool ENTGRAD, bool NONTEMPORAL>
+__global__ __launch_bounds__(kBwdThreads) void logits_top_bwd_rows(const TopBwdArgs a) {
+  constexpr int E = Piece<F32>::kElems, ES = F32 ? 4 : 2;
+  __shared__ float h_sum[kBwdThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = (int64_t)(gridDim.x - 1 - blockIdx.x);  // the rows that the forward read last first
+  const int V = a.V, k = a.dtop ? a.k : 0;
+  const char* src = (const char*)a.logits + (size_t)row * (size_t)a.ld * ES;
+  char* dst = (char*)a.dlogits + (size_t)row * (size_t)a.ldd * ES;
+  int64_t y = a.labels ? a.labels[row] : (int64_t)-1;
+  if (y < 0 || y >= (int64_t)V) y = -1;
+  const float g = a.dlogprobs && y >= 0 ? a.dlogprobs[row] : 0.f;
+  const float q = ENTGRAD ? a.dentropy[row] : 0.f;
+  const float lse = a.row_lse[row], lse2 = lse * kLog2e;
+  const float pz = ENTGRAD ? a.row_pz[row] : 0.f;
+  const float scale2 = a.rcp_temp * kLog2e;
+  // Thread j < k has the gradient of alternative j, thread k that of the label.  Ids that lie outside the row, which the forward does not
+  // give, have no term.
+  int64_t own = -1;
+  float own_grad = 0.f;
+  if (tid < k) {
+    own = a.top_ids[row * (int64_t)k + tid];
+    if (own < 0 || own >= (int64_t)V) own = -1;
+    own_grad = own >= 0 ? a.dtop[row * (int64_t)k + tid] : 0.f;
+  } else if (tid == k && y >= 0) {
+    own = y, own_grad = g;
+  }
+  float s = tid <= k ? own_grad : 0.f;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane == 0) h_sum[wave] = s;
+  __syncthreads();
+  float all = 0.f;
+  for (int w = 0; w * 64 <= k; ++w) all += h_sum[w];  // waves behind the k + 1 threads hold nothing
+  // A column may be both an alternative and the label, or be listed twice: the first thread that has it takes all of its terms.
+  float own_z = 0.f;
+  bool writes = own >= 0;
+  if (own >= 0) {
+    own_z = load_one(src, (size_t)own, F32);
+    for (int j = 0; j < k; ++j) {
+      const int64_t id = a.top_ids[row * (int64_t)k + j];
+      if (id != own || j == tid) continue;
+      if (j < tid) writes = false;
+      else own_grad += a.dtop[row * (int64_t)k + j];
+    }
+    if (tid < k && own == y) own_grad += g;
+  }
+  // dz = p * (c0 + c1 * z) [+ the column's own gradient / temperature],  c0 = -(g + sum h - q pz) / temperature,  c1 = -q / temperature^2
+  const float c0 = -(all - q * pz) * a.rcp_temp, c1 = -q * a.rcp_temp * a.rcp_temp;
+  const bool empty = lse == -INFINITY;  // no logit above -inf: no gradient
+  bool any = tid <= k && own_grad != 0.f;
+  const bool zero_row = empty || (__syncthreads_or((any || all != 0.f || q != 0.f) ? 1 : 0) == 0);
+  auto dz = [&](float z) {
+    const float p = __builtin_amdgcn_exp2f(fmaf(z, scale2, -lse2));
+    return ENTGRAD ? p * fmaf(c1, fmaxf(z, kMostNegativeFactor), c0) : p * c0;
+  };
+  const RowPieces rp = row_pieces<F32>(src, V, a.vector_ok != 0);
+  const char* vsrc = src + (size_t)rp.head * ES;
+  char* vdst = dst + (size_t)rp.head * ES;
+  for (int p0 = tid; p0 < rp.pieces; p0 += kBwdThreads * kInFlight) {
+    Piece<F32> pc[kInFlight];
+    if (!zero_row) {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        const int p = p0 + u * kBwdThreads;
+        pc[u].load(vsrc + (size_t)(p < rp.pieces ? p : p0) * 16);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int p = p0 + u * kBwdThreads;
+      if (p >= rp.pieces) continue;
+      float d[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) d[i] = zero_row ? 0.f : dz(pc[u].v[i]);
+      uint4 out;
+      if (F32) {
+        out = make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]), __float_as_uint(d[3]));
+      } else {
+        typedef __attribute__((ext_vector_type(4))) float f32x4;
+        typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+        const f32x4 lo4 = {d[0], d[1], d[2], d[3]}, hi4 = {d[4 % E], d[5 % E], d[6 % E], d[7 % E]};
+        const bf16x4 lo = __builtin_convertvector(lo4, bf16x4), hi = __builtin_convertvector(hi4, bf16x4);
+        const uint2 x = *(const uint2*)&lo, z = *(const uint2*)&hi;
+        out = make_uint4(x.x, x.y, z.x, z.y);
+      }
+      if constexpr (NONTEMPORAL) __builtin_nontemporal_store(*(const u32x4*)&out, (u32x4*)(vdst + (size_t)p * 16));
+      else *(uint4*)(vdst + (size_t)p * 16) = out;
+    }
+  }
+  for (int i = tid; i < rp.single; i += kBwdThreads) {
+    const int c = single_column(rp, E, i);
+    const float d = zero_row ? 0.f : dz(load_one(src, (size_t)c, F32));
+    if (F32) ((float*)dst)[c] = d;
+    else ((uint16_t*)dst)[c] = bf16_bits(d);
+  }
+  if (zero_row) return;
+  __syncthreads();  // the pass over the row is done: what is written here comes behind it
+  if (writes) {
+    const float d = fmaf(own_grad, a.rcp_temp, dz(own_z));
+    if (F32) ((float*)dst)[own] = d;
+    else ((uint16_t*)dst)[own] = bf16_bits(d);
+  }
+}
+
+int check_top(int64_t V, int64_t k) {
+  return k < 0 || k > V || k > kMaxTop ? SKYRL_LMHEAD_ERR_SHAPE : SKYRL_LMHEAD_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int skyrl_logits_top_fwd(const void* logits, int logits_dtype, int64_t ld_logits, const int64_t* labels, int64_t T, int64_t V, int64_t k,
+                         float rcp_temperature, float* logprobs, float* entropy, float* row_lse, float* row_pz, int64_t* ranks,
+                         float* top_logprobs, int64_t* top_ids, void* stream) {
+  int st = check_logits(logits, logits_dtype, ld_logits, T, V, rcp_temperature);
+  if (st) return st;
+  if ((st = check_top(V, k))) return st;
+  if ((logprobs || ranks) && !labels) return SKYRL_LMHEAD_ERR_NULL;
+  if (k > 0 && (!top_logprobs || !top_ids)) return SKYRL_LMHEAD_ERR_NULL;
+  if (k == 0 && !logprobs && !entropy && !row_lse && !row_pz && !ranks) return SKYRL_LMHEAD_ERR_NULL;
+  if (((uintptr_t)labels | (uintptr_t)ranks | (uintptr_t)top_ids) & 7u) return SKYRL_LMHEAD_ERR_ALIGN;
+  const TopArgs a{logits, ld_logits, labels, (int)V, (int)k, rcp_temperature, logprobs, entropy, row_lse, row_pz, ranks, top_logprobs, top_ids};
+  hipLaunchKernelGGL(logits_dtype == SKYRL_LOGITS_F32 ? logits_top_rows<true> : logits_top_rows<false>, dim3((unsigned)T), dim3(kThreads), 0,
+                     (hipStream_t)stream, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? SKYRL_LMHEAD_OK : (int)e;
+}
+
+int skyrl_logits_top_bwd(const void* logits, int logits_dtype, int64_t ld_logits, const int64_t* labels, const float* row_lse,
+                         const float* row_pz, const float* dlogprobs, const float* dentropy, const int64_t* top_ids, const float* dtop,
+                         int64_t T, int64_t V, int64_t k, float rcp_temperature, void* dlogits, int64_t ld_dlogits, void* stream) {
+  int st = check_logits(logits, logits_dtype, ld_logits, T, V, rcp_temperature);
+  if (st) return st;
+  if ((st = check_top(V, k))) return st;
+  if (!row_lse || !dlogits || (!dlogprobs && !dentropy && !dtop) || (dlogprobs && !labels) || (dentropy && !row_pz) || (dtop && !top_ids))
+    return SKYRL_LMHEAD_ERR_NULL;
+  if (ld_dlogits < V || ld_dlogits >= ((int64_t)1 << 40)) return SKYRL_LMHEAD_ERR_SHAPE;
+  const bool f32 = logits_dtype == SKYRL_LOGITS_F32;
+  if (((uintptr_t)dlogits & (f32 ? 3u : 1u)) || (((uintptr_t)labels | (uintptr_t)top_ids) & 7u)) return SKYRL_LMHEAD_ERR_ALIGN;
+  if (overlaps_otherwise(logits, ld_logits, dlogits, ld_dlogits, T, V, f32)) return SKYRL_LMHEAD_ERR_ARG;
+  const int vec = same_row_offsets(logits, ld_logits, dlogits, ld_dlogits, f32) ? 1 : 0;
+  const TopBwdArgs a{logits, ld_logits, labels, (int)V, (int)k, rcp_temperature, vec, row_lse, row_pz, dlogprobs, dentropy, top_ids, dtop, dlogits,
+                     ld_dlogits};
+  const bool entgrad = dentropy != nullptr, beyond = T * V * (f32 ? 4 : 2) > kCacheBytes;
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)T), dim3(kBwdThreads), 0, (hipStream_t)stream, a); };
+  if (f32 && entgrad) launch(beyond ? logits_top_bwd_rows<true, true, true> : logits_top_bwd_rows<true, true, false>);
+  else if (f32) launch(beyond ? logits_top_bwd_rows<true, false, true> : logits_top_bwd_rows<true, false, false>);
+  else if (entgrad) launch(beyond ? logits_top_bwd_rows<false, true, true> : logits_top_bwd_rows<false, true, false>);
+  else launch(beyond ? logits_top_bwd_rows<false, false, true> : logits_top_bwd_rows<false, false, false>);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? SKYRL_LMHEAD_OK : (int)e;
+}
+
+}  // extern "C"

@@ -7,6 +7,8 @@ linear layer):
   ``logprobs_from_logits_flash_attn`` -- ``skyrl/backends/skyrl_train/utils/torch_utils.py:115-177``;
 * ``chunked_entropy_from_logits(logits, requires_grad=False, attention_mask=None, chunk_size=1024)`` -- ``:58-111``;
 * ``logprobs_and_entropy_from_logits`` -- both from one pass over the logits (an extension);
+* ``top_logprobs_from_logits`` -- those two, each label's rank and the ``k`` best alternatives with their log-probabilities (an
+  extension: what a sampler answers with, and, with a gradient, a distillation loss on the policy's own alternatives);
 * ``DistributedLogprob`` / ``ChunkedDistributedLogprob`` -- the apply signatures of the logits-input autograd functions of
   ``.../distributed/megatron/model_utils.py:66-272`` on one vocabulary shard, and ``from_parallel_logits_to_logprobs`` (:487-565).
 
@@ -18,7 +20,7 @@ A sliced view such as ``logits[:, :-1]`` is walked where it lies (one launch per
 
 from __future__ import annotations
 
-from typing import Any, Optional, Tuple
+from typing import Any, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -29,7 +31,8 @@ from .ops import _require_device as _require_device_all
 __all__ = ["logprobs_from_logits", "logprobs_from_logits_v2", "logprobs_from_logits_flash_attn", "chunked_entropy_from_logits",
            "logprobs_and_entropy_from_logits", "DistributedLogprob", "ChunkedDistributedLogprob",
            "from_parallel_logits_to_logprobs", "from_parallel_logits_to_logprobs_packed_sequences", "vocab_parallel_entropy", "vocab_parallel_entropy_weighted_sum",
-           "vocab_parallel_entropy_packed_sequences", "logits_fwd", "logits_bwd", "logits_bwd_"]
+           "vocab_parallel_entropy_packed_sequences", "logits_fwd", "logits_bwd", "logits_bwd_", "TokenLogprobs", "MAX_ALTERNATIVES",
+           "top_logprobs_from_logits", "logits_top_fwd", "logits_top_bwd"]
 
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
@@ -227,6 +230,154 @@ def logprobs_and_entropy_from_logits(logits: torch.Tensor, labels: torch.Tensor,
     lp, ent = _FromLogits.apply(_flat(logits), labels.reshape(-1).to(torch.int64).contiguous(), 1.0 / float(temperature), True,
                                 bool(inplace_backward))
     return lp.reshape(shape), ent.reshape(shape)
+
+
+MAX_ALTERNATIVES = 128  # SKYRL_LOGITS_TOP_MAX
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``top_logprobs_from_logits`` returns; shapes are ``logits.shape[:-1]``, the last two with ``k`` behind it."""
+
+    logprobs: torch.Tensor       # fp32: of the label; 0 where it lies outside the vocabulary
+    entropy: torch.Tensor        # fp32
+    ranks: torch.Tensor          # int64: 1 + the number of columns that sort before the label; 0 where there is no label
+    top_logprobs: torch.Tensor   # fp32, best first
+    top_ids: torch.Tensor        # int64
+
+
+def _check_top(name: str, t: torch.Tensor, T: int, k: int, dtype: torch.dtype) -> None:
+    if t.dtype != dtype or t.shape != (T, k) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape [{T}, {k}], got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_k(k: int, V: int) -> None:
+    if not 0 <= k <= min(V, MAX_ALTERNATIVES):
+        raise ValueError(f"k must lie between 0 and min(vocabulary, {MAX_ALTERNATIVES}) = {min(V, MAX_ALTERNATIVES)}, got {k}")
+
+
+@registered_op("skyrl_amd::logits_top_fwd", mutates_args=())
+def logits_top_fwd(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int, rcp_temperature: float
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(logprobs, entropy, row_lse, row_pz, ranks, top_logprobs, top_ids)`` of ``logits [T, V] * rcp_temperature``; fp32 ``[T]``,
+    int64 ``[T]`` and ``[T, k]``.  Without ``labels`` log-probabilities and ranks are zero."""
+    T, V, pieces = _pieces(logits)
+    dev = _require_device(logits, labels)
+    _check_rows("labels", labels, T, torch.int64)
+    if T > 0:
+        _check_k(k, V)
+    f32, i64 = dict(dtype=torch.float32, device=dev), dict(dtype=torch.int64, device=dev)
+    made = torch.empty if labels is not None else torch.zeros
+    lp, ranks = made(T, **f32), made(T, **i64)
+    ent, lse, pz = torch.empty(T, **f32), torch.empty(T, **f32), torch.empty(T, **f32)
+    top, ids = torch.empty((T, k), **f32), torch.empty((T, k), **i64)
+    if T == 0:
+        return lp, ent, lse, pz, ranks, top, ids
+    lib = _lib.load()
+    with device_guard(dev):
+        stream = raw_stream(dev)
+        for view, r0 in pieces:
+            rows, _, ld = _rows(view)
+            at = lambda t, size: t.data_ptr() + size * r0  # noqa: E731
+            st = lib.skyrl_logits_top_fwd(view.data_ptr(), _DTYPES[logits.dtype], ld, None if labels is None else at(labels, 8), rows, V, k,
+                                          float(rcp_temperature), None if labels is None else at(lp, 4), at(ent, 4), at(lse, 4), at(pz, 4),
+                                          None if labels is None else at(ranks, 8), at(top, 4 * k), at(ids, 8 * k), stream)
+            _lib.check(st, "skyrl_logits_top_fwd")
+    return lp, ent, lse, pz, ranks, top, ids
+
+
+@logits_top_fwd.register_fake
+def _(logits, labels, k, rcp_temperature):
+    T = logits.numel() // max(1, logits.shape[-1])
+    f32, i64 = (lambda *s: logits.new_empty(s, dtype=torch.float32)), (lambda *s: logits.new_empty(s, dtype=torch.int64))
+    return f32(T), f32(T), f32(T), f32(T), i64(T), f32(T, k), i64(T, k)
+
+
+@registered_op("skyrl_amd::logits_top_bwd", mutates_args=())
+def logits_top_bwd(logits: torch.Tensor, labels: Optional[torch.Tensor], row_lse: torch.Tensor, row_pz: Optional[torch.Tensor],
+                   dlogprobs: Optional[torch.Tensor], dentropy: Optional[torch.Tensor], top_ids: Optional[torch.Tensor],
+                   dtop: Optional[torch.Tensor], rcp_temperature: float) -> torch.Tensor:
+    """d loss / d logits, a new tensor in the logits' dtype and shape, from gradients on log-probabilities, entropy and alternatives."""
+    T, V, pieces = _pieces(logits)
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    dev = _require_device(logits, labels, row_lse, row_pz, dlogprobs, dentropy, top_ids, dtop)
+    _check_rows("labels", labels, T, torch.int64)
+    for name, t in (("row_lse", row_lse), ("row_pz", row_pz), ("dlogprobs", dlogprobs), ("dentropy", dentropy)):
+        _check_rows(name, t, T, torch.float32)
+    if dlogprobs is None and dentropy is None and dtop is None:
+        raise ValueError("the backward needs an upstream gradient: dlogprobs, dentropy, dtop or several of them")
+    k = 0
+    if dtop is not None:
+        if top_ids is None or top_ids.dim() != 2:
+            raise ValueError("a gradient on the alternatives needs their columns, top_ids [T, k]")
+        k = int(top_ids.shape[1])
+        _check_top("top_ids", top_ids, T, k, torch.int64)
+        _check_top("dtop", dtop, T, k, torch.float32)
+    if T == 0:
+        return out
+    _check_k(k, V)
+    ptr = lambda t, r0, size: None if t is None else t.data_ptr() + size * r0  # noqa: E731
+    lib = _lib.load()
+    with device_guard(dev):
+        stream = raw_stream(dev)
+        for view, r0 in pieces:
+            n, _, ld = _rows(view)
+            dst = out.data_ptr() + r0 * V * out.element_size()  # contiguous, whatever the logits' layout is
+            st = lib.skyrl_logits_top_bwd(view.data_ptr(), _DTYPES[logits.dtype], ld, ptr(labels, r0, 8), ptr(row_lse, r0, 4), ptr(row_pz, r0, 4),
+                                          ptr(dlogprobs, r0, 4), ptr(dentropy, r0, 4), ptr(top_ids if k else None, r0, 8 * k),
+                                          ptr(dtop if k else None, r0, 4 * k), n, V, k, float(rcp_temperature), dst, V, stream)
+            _lib.check(st, "skyrl_logits_top_bwd")
+    return out
+
+
+@logits_top_bwd.register_fake
+def _(logits, labels, row_lse, row_pz, dlogprobs, dentropy, top_ids, dtop, rcp_temperature):
+    return logits.new_empty(logits.shape)
+
+
+class _TopFromLogits(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, k, rcp_temperature):
+        lp, ent, lse, pz, ranks, top, ids = call(logits_top_fwd, logits, labels, k, rcp_temperature)
+        ctx.save_for_backward(logits, labels, lse, pz, ids)
+        ctx.rcp_temperature = rcp_temperature
+        ctx.mark_non_differentiable(ranks, ids)
+        ctx.set_materialize_grads(False)
+        return lp, ent, ranks, top, ids
+
+    @staticmethod
+    def backward(ctx, dlp, dent, _dranks, dtop, _dids):
+        logits, labels, lse, pz, ids = ctx.saved_tensors
+        if labels is None:
+            dlp = None  # the log-probabilities are constants
+        if dtop is not None and dtop.shape[1] == 0:
+            dtop = None
+        if dlp is None and dent is None and dtop is None:
+            return None, None, None, None
+        f = lambda t: None if t is None else t.to(torch.float32).contiguous()  # noqa: E731
+        return call(logits_top_bwd, logits, labels, lse, pz, f(dlp), f(dent), ids, f(dtop), ctx.rcp_temperature), None, None, None
+
+
+def top_logprobs_from_logits(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int, *, temperature: float = 1.0) -> TokenLogprobs:
+    """Log-probability, rank and entropy of ``labels`` under ``softmax(logits / temperature)`` and the ``min(k, V)`` best columns with
+    their log-probabilities, from one pass over the logits ``[..., V]`` (bf16 or fp32; anything else is cast to fp32).
+
+    Equal logits sort by column, the lower first, and NaN behind everything: a label whose rank is at most ``k`` stands at
+    ``top_ids[..., rank - 1]``.  A row that a mask of ``-inf`` leaves empty has log-probabilities ``-inf``, entropy 0 and a zero gradient.
+    ``k`` is at most ``MAX_ALTERNATIVES``; 0 gives ranks without alternatives.  ``labels`` may be ``None``.  Log-probabilities,
+    alternatives' log-probabilities and entropy carry gradients to ``logits``."""
+    if not isinstance(k, int) or isinstance(k, bool) or not 0 <= k <= MAX_ALTERNATIVES:
+        raise ValueError(f"k must be an integer between 0 and {MAX_ALTERNATIVES}, got {k!r}")
+    temperature = float(temperature)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be finite and positive, got {temperature}")
+    shape, V = logits.shape[:-1], int(logits.shape[-1])
+    if labels is not None:
+        if labels.shape != shape:
+            raise ValueError(f"labels {tuple(labels.shape)} do not match logits {tuple(logits.shape)}")
+        labels = labels.reshape(-1).to(torch.int64).contiguous()
+    k = min(k, V)
+    lp, ent, ranks, top, ids = _TopFromLogits.apply(_flat(logits), labels, k, 1.0 / temperature)
+    return TokenLogprobs(lp.reshape(shape), ent.reshape(shape), ranks.reshape(shape), top.reshape(shape + (k,)), ids.reshape(shape + (k,)))
 
 
 def logprobs_from_logits(logits: torch.Tensor, labels: torch.Tensor, inplace_backward: bool = True) -> torch.Tensor:
