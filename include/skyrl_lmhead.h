@@ -466,6 +466,39 @@ int skyrl_logits_bwd(const void* logits, int logits_dtype, int64_t ld_logits, co
                      const float* row_pz, const float* dlogprobs, const float* dentropy, int64_t T, int64_t V,
                      float rcp_temperature, void* dlogits, int64_t ld_dlogits, void* stream);
 
+/* ---- the head with low-rank adapters of many requests -------------------------------------------------------------------
+ * Each token has an adapter, or none, on top of the (frozen) output weight:
+ *   z_t = hidden_t . weight^T + scaling_a ((hidden_t . A_a^T) . B_a^T),      a = adapter_ids[t]
+ * lora_a: bf16, adapter a's row r (of `rank`) at lora_a + a * a_adapter + r * a_row, H values; lora_b: bf16, adapter a's row v (of V) at lora_b +
+ * a * b_adapter + v * b_row, `rank` values; scaling fp32 [num_adapters]; adapter_ids int64 [T], in any order, a value outside [0,
+ * num_adapters): no adapter.  rank: a multiple of 8, at most SKYRL_LMHEAD_MAX_ADAPTER_RANK (an adapter of a lower rank is filled up with
+ * zeros); num_adapters at most 65535.  16-byte alignment, strides multiples of 8.
+ * The product with A is formed in fp32 and enters the matrix pipe as two bf16 terms (exact to 2^-17).  No token's result depends on the
+ * values of an adapter that it does not have, whether they are finite or not.
+ *   skyrl_lmhead_adapter_fwd     as skyrl_lmhead_fwd
+ *   skyrl_lmhead_adapter_logits  the logits themselves, logits [T, ld_logits] in bf16 or fp32 (SKYRL_LOGITS_*): decoding; temperature 1
+ *   skyrl_lmhead_adapter_bwd     as skyrl_lmhead_bwd_active_rows without d_weight.  d_lora_a [num_adapters, rank, H] and d_lora_b [num_adapters,
+ *     V, rank], bf16, contiguous, overwritten (zeros for adapters without a token that has a gradient).  d_hidden is rounded to bf16 twice: the
+ *     product with the weight, and the sum with the adapters' part.  Rows are worked on grouped by adapter, in an order that follows from
+ *     adapter_ids alone: the same bits on each call. */
+#define SKYRL_LMHEAD_MAX_ADAPTER_RANK 256
+size_t skyrl_lmhead_adapter_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t rank);
+int skyrl_lmhead_adapter_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels, const void* lora_a,
+                             int64_t a_adapter, int64_t a_row, const void* lora_b, int64_t b_adapter, int64_t b_row, const float* scaling,
+                             const int64_t* adapter_ids, int64_t num_adapters, int64_t rank, int64_t T, int64_t H, int64_t V, float rcp_temperature,
+                             float* logprobs, float* entropy, float* row_lse, float* row_pz, void* workspace, size_t workspace_bytes, void* stream);
+size_t skyrl_lmhead_adapter_logits_workspace_bytes(int64_t T, int64_t rank);
+int skyrl_lmhead_adapter_logits(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* lora_a, int64_t a_adapter,
+                                int64_t a_row, const void* lora_b, int64_t b_adapter, int64_t b_row, const float* scaling, const int64_t* adapter_ids,
+                                int64_t num_adapters, int64_t rank, int64_t T, int64_t H, int64_t V, int logits_dtype, void* logits, int64_t ld_logits,
+                                void* workspace, size_t workspace_bytes, void* stream);
+size_t skyrl_lmhead_adapter_bwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t num_adapters, int64_t rank);
+int skyrl_lmhead_adapter_bwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels, const void* lora_a,
+                             int64_t a_adapter, int64_t a_row, const void* lora_b, int64_t b_adapter, int64_t b_row, const float* scaling,
+                             const int64_t* adapter_ids, int64_t num_adapters, int64_t rank, const float* row_lse, const float* row_pz,
+                             const float* dlogprobs, const float* dentropy, int64_t T, int64_t H, int64_t V, float rcp_temperature, void* d_hidden,
+                             void* d_lora_a, void* d_lora_b, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- given tokens and the best alternatives ---------------------------------------------------------------------------
  * The statistics above and, from the same pass, each label's rank and the k columns that sort first, with their log-probabilities; no
  * counterpart in the reference's trainer.  Columns sort by logit, the larger first, equal ones (-0 equals +0) by column, the lower first,

@@ -16,6 +16,9 @@ ABI_VERSION = 20
 _c_i64 = ctypes.c_int64
 _c_p = ctypes.c_void_p
 
+# lora_a, its adapter and row strides, lora_b and its, scaling, adapter_ids, num_adapters, rank
+_ADAPTERS = [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64]
+
 # name -> (restype, argtypes); mirrors include/skyrl_lmhead.h one to one.
 SIGNATURES = {
     "skyrl_lmhead_version": (ctypes.c_int, []),
@@ -78,6 +81,19 @@ SIGNATURES = {
         [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float,
          _c_p, _c_i64, _c_p, ctypes.c_size_t, _c_p],
     ),
+    "skyrl_lmhead_adapter_fwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 4),
+    "skyrl_lmhead_adapter_fwd": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_p, _c_i64, _c_p] + _ADAPTERS + [_c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p, _c_p, _c_p, _c_p, ctypes.c_size_t, _c_p]),
+    "skyrl_lmhead_adapter_logits_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64]),
+    "skyrl_lmhead_adapter_logits": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_p, _c_i64] + _ADAPTERS + [_c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p, _c_i64, _c_p, ctypes.c_size_t, _c_p]),
+    "skyrl_lmhead_adapter_bwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 5),
+    "skyrl_lmhead_adapter_bwd": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_p, _c_i64, _c_p] + _ADAPTERS + [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p, _c_p, _c_p,
+                                                           ctypes.c_size_t, _c_p]),
     "skyrl_lmhead_topk_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "skyrl_lmhead_topk_logits": (
         ctypes.c_int,

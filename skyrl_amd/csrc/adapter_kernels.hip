@@ -1,0 +1,608 @@
+// What the head with adapters needs besides its tiles (adapters.hpp): u of every token, the label's logit, and in the backward, from the dz panel
+//     du_t = s_a B_a^T dz_t        dB_a = sum_t dz_t u_t^T        dA_a = sum_t du_t h_t^T        d_hidden_t += A_a^T du_t
+// over rows that are grouped by adapter.  All of it is bound by the panel, which two kernels read once each, or by latency.
+//
+// Operand layouts of v_mfma_f32_16x16x32_bf16 are in gemm_core.hpp.  Operands whose contraction is not their contiguous axis go through LDS
+// and the transposing read: lane (kq, s) supplies row kq * 8 + half * 4 + (s >> 2), columns (s & 3) * 4 .. + 3 of the 16, and receives column s
+// of the eight rows kq * 8 .. + 7.
+#include "adapters.hpp"
+
+namespace lmhead {
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) short i16x8;
+typedef __attribute__((address_space(3))) i16x4* lds_half_ptr;
+
+__device__ __forceinline__ f32x4 mfma(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// The transposed fragment whose 32 rows of `pitch` bytes begin at `at` (LDS), at the columns that `at` points to.
+__device__ __forceinline__ bf16x8 transposed(const char* at, int pitch) {
+  const int lane = threadIdx.x & 63, kq = lane >> 4, s = lane & 15;
+  const uint32_t addr = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)at + (uint32_t)((kq * 8 + (s >> 2)) * pitch + (s & 3) * 8);
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half_ptr)(uintptr_t)addr);
+  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half_ptr)(uintptr_t)(addr + 4u * (uint32_t)pitch));
+  const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+// x as two bf16 terms (exact to 2^-17 of it).
+struct Terms {
+  uint2 hi, lo;
+};
+__device__ __forceinline__ Terms two_terms(const f32x4& x) {
+  const bf16x4 hi = __builtin_convertvector(x, bf16x4);
+  const uint2 h = *(const uint2*)&hi;
+  const float w[4] = {__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u), __uint_as_float(h.y << 16), __uint_as_float(h.y & 0xffff0000u)};
+  f32x4 rest;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rest[i] = __builtin_isfinite(w[i]) ? x[i] - w[i] : 0.f;  // an inf stays one
+  const bf16x4 lo = __builtin_convertvector(rest, bf16x4);
+  return Terms{h, *(const uint2*)&lo};
+}
+
+__device__ __forceinline__ int tokens_in_force(int T, const int* T_dev) { return T_dev ? __builtin_amdgcn_readfirstlane(*T_dev) : T; }
+
+// ------------------------------------------------------------------------------------------------------------
+// u = s A h.  One workgroup per 16 tokens and 32 ranks; its waves share the hidden size and their sums meet in LDS.  M: rank, N: token.
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kShrinkWaves = 8;
+__global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink(const Adapters ad, const uint16_t* __restrict__ hidden, int64_t ldh,
+                                                                    const int64_t* __restrict__ ids, int T_, const int* T_dev, int H,
+                                                                    uint16_t* __restrict__ U, int* __restrict__ ids32) {
+  __shared__ f32x4 part[kShrinkWaves][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pitch = 2 * padded_rank(ad.rank), r0 = blockIdx.y * 32;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid * 8 < pitch) *(uint4*)(U + tid * 8) = make_uint4(0, 0, 0, 0);
+  const int T = tokens_in_force(T_, T_dev), t0 = blockIdx.x * 16;
+  if (t0 >= T) return;
+  const int t = t0 + lrow;
+  int id = -1;
+  if (t < T) {
+    const int64_t x = ids[t];
+    id = x >= 0 && x < (int64_t)ad.N ? (int)x : -1;
+    if (blockIdx.y == 0 && tid < 16) ids32[t] = id;
+  }
+  const uint16_t* x_row = hidden + (size_t)(t < T ? t : T - 1) * (size_t)ldh + kq * 8;
+  f32x4 u[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  unsigned left = (unsigned)__ballot(id >= 0) & 0xffffu;
+  while (left) {
+    const int a = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+    left &= ~(unsigned)__ballot(id == a);
+    const uint16_t* rows[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int r = r0 + m * 16 + lrow;
+      rows[m] = ad.A + (size_t)a * (size_t)ad.a_adapter + (size_t)(r < ad.rank ? r : ad.rank - 1) * (size_t)ad.a_row + kq * 8;
+    }
+    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 4
+    for (int k = wave * 32; k < H; k += kShrinkWaves * 32) {
+      const bf16x8 x = *(const bf16x8*)(x_row + k);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) acc[m] = mfma(*(const bf16x8*)(rows[m] + k), x, acc[m]);
+    }
+    const float s = ad.scaling[a];
+    if (id == a) u[0] = acc[0] * s, u[1] = acc[1] * s;
+  }
+#pragma unroll
+  for (int m = 0; m < 2; ++m) part[wave][m][lane] = u[m];
+  __syncthreads();
+  if (tid >= 128 || t >= T) return;
+  const int m = tid >> 6;
+  f32x4 sum = part[0][m][lane];
+#pragma unroll
+  for (int w = 1; w < kShrinkWaves; ++w) sum += part[w][m][lane];
+  const int r = r0 + m * 16 + kq * 4;
+  if (r >= ad.rank) sum = f32x4{0.f, 0.f, 0.f, 0.f};  // the rank is a multiple of 8
+  const Terms terms = two_terms(sum);
+  uint16_t* to = U + (size_t)(1 + t) * (size_t)pitch + r;
+  *(uint2*)to = terms.hi;
+  *(uint2*)(to + pitch / 2) = terms.lo;
+}
+
+// The adapter's part of the label's logit: 16 lanes a token.
+__global__ __launch_bounds__(256) void adapter_label(const Adapters ad, const uint16_t* __restrict__ U, const int* __restrict__ ids,
+                                                     const int64_t* __restrict__ labels, int T, int64_t V, float rcp_temp, float* __restrict__ logprobs) {
+  const int t = blockIdx.x * 16 + (threadIdx.x >> 4), part = threadIdx.x & 15;
+  if (t >= T) return;
+  const int a = ids[t];
+  const int64_t y = labels[t];
+  if (a < 0 || y < 0 || y >= V) return;  // the 16 lanes alike
+  const int pitch = 2 * padded_rank(ad.rank);
+  const uint16_t* b = ad.B + (size_t)a * (size_t)ad.b_adapter + (size_t)y * (size_t)ad.b_row;
+  const uint16_t* u = U + (size_t)(1 + t) * (size_t)pitch;
+  float sum = 0.f;
+  for (int r = part; r < ad.rank; r += 16) {
+    const float x = __uint_as_float((uint32_t)u[r] << 16) + __uint_as_float((uint32_t)u[pitch / 2 + r] << 16);
+    sum = fmaf(x, __uint_as_float((uint32_t)b[r] << 16), sum);
+  }
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 16);
+  if (part == 0) logprobs[t] = fmaf(sum, rcp_temp, logprobs[t]);
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Rows with a gradient, grouped by adapter (those without one last), ascending inside a group: idx, their adapters, and seg[a], the place of
+// adapter a's first row; seg[N] that of the rows without an adapter, seg[N + 1] the number of rows.  One workgroup per group: it counts the rows of
+// the groups before its own, then lists its own.  The order is a function of the inputs alone, so the sums over rows are the same bits on each call.
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kGroupThreads = 1024, kGroupTokens = 4;  // tokens per thread and step
+__global__ __launch_bounds__(kGroupThreads) void adapter_group_rows(const float* __restrict__ g, const float* __restrict__ q,
+                                                                    const int64_t* __restrict__ ids, int T, int N, int* __restrict__ idx,
+                                                                    int64_t* __restrict__ ids_c, int* __restrict__ seg) {
+  constexpr int kCounts = kGroupTokens * kGroupThreads / 64;
+  static_assert(kCounts == 64, "one lane per count");
+  __shared__ int count[2][kCounts];
+  __shared__ int before[kGroupThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mine = blockIdx.x;
+  auto group_of = [&](int t) -> int {  // -1: no gradient
+    if (t >= T) return -1;
+    const float gv = g[t], qv = q ? q[t] : 0.f;
+    const int64_t x = ids[t];
+    if (gv == 0.f && qv == 0.f) return -1;
+    return x >= 0 && x < (int64_t)N ? (int)x : N;
+  };
+  int less = 0;
+  for (int t0 = 0; t0 < T; t0 += kGroupTokens * kGroupThreads) {
+    int k[kGroupTokens];
+#pragma unroll
+    for (int j = 0; j < kGroupTokens; ++j) k[j] = group_of(t0 + j * kGroupThreads + tid);
+#pragma unroll
+    for (int j = 0; j < kGroupTokens; ++j) less += (int)__popcll(__ballot(k[j] >= 0 && k[j] < mine));
+  }
+  if (lane == 0) before[wave] = less;
+  __syncthreads();
+  int n = 0;
+  for (int w = 0; w < kGroupThreads / 64; ++w) n += before[w];
+  if (tid == 0) seg[mine] = n;
+  for (int t0 = 0, turn = 0; t0 < T; t0 += kGroupTokens * kGroupThreads, turn ^= 1) {
+    unsigned long long ballot[kGroupTokens];
+#pragma unroll
+    for (int j = 0; j < kGroupTokens; ++j) ballot[j] = __ballot(group_of(t0 + j * kGroupThreads + tid) == mine);
+#pragma unroll
+    for (int j = 0; j < kGroupTokens; ++j)
+      if (lane == 0) count[turn][j * (kGroupThreads / 64) + wave] = (int)__popcll(ballot[j]);
+    __syncthreads();
+    const int here = count[turn][lane];
+    int upto = here;
+#pragma unroll
+    for (int o = 1; o < kCounts; o <<= 1) {
+      const int below = __shfl_up(upto, o, 64);
+      upto += lane >= o ? below : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kGroupTokens; ++j) {
+      const int base = n + __shfl(upto - here, j * (kGroupThreads / 64) + wave, 64);
+      if (ballot[j] >> lane & 1) {
+        const int at = base + (int)__popcll(ballot[j] & ((1ull << lane) - 1ull));
+        idx[at] = t0 + j * kGroupThreads + tid;
+        ids_c[at] = mine < N ? mine : -1;
+      }
+    }
+    n += __shfl(upto, kCounts - 1, 64);
+  }
+  if (tid == 0 && mine == N) seg[N + 1] = n;
+}
+
+// The vocabulary row that panel column c of a chunk stands for; columns that stand for none hold zeros (VocabTail in gemm_core.hpp).
+__device__ __forceinline__ int panel_row(int vc0, int c, const VocabTail& tail) {
+  const int column = vc0 + c;
+  return tail.back > 0 && column >= tail.from ? column - tail.back : column;
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Partial sums of B_a^T dz over a range of panel columns.  One workgroup per 64 tokens, range and 64 ranks; 16 tokens a wave.  M: rank (B's rows
+// through LDS), N: token (panel rows as they lie).  B's next rows and the panel's next pieces are loaded while the present ones are multiplied.
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kDuTokens = 64, kDuColumns = 64, kDuRanks = 64;
+constexpr int kDuPitch = kDuRanks * 2 + 16;
+__global__ __launch_bounds__(256) void adapter_du_partial(const AdapterPanel p, int columns, int per_range, float* __restrict__ out, int Rp) {
+  __shared__ __attribute__((aligned(16))) char lds[2][kDuColumns * kDuPitch];
+  const int T = tokens_in_force(p.T, p.T_dev), t0 = blockIdx.x * kDuTokens;
+  if (t0 >= T) return;
+  const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r0 = blockIdx.z * kDuRanks, R = p.ad.rank;
+  const int tiles = __builtin_amdgcn_readfirstlane(((R - r0 < kDuRanks ? R - r0 : kDuRanks) + 15) / 16);
+  const int c0 = blockIdx.y * per_range, c1 = c0 + per_range < columns ? c0 + per_range : columns;
+  const int id64 = t0 + lane < T ? p.ids[t0 + lane] : -1;  // of the workgroup's tokens: alike in all waves
+  const int t = t0 + wave * 16 + lrow;
+  const int id = t < T ? p.ids[t] : -1;
+  const uint16_t* d_row = p.D + (size_t)(t < T ? t : T - 1) * (size_t)p.ldd + kq * 8;
+  f32x4 sum[4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m) sum[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  unsigned long long left = __ballot(id64 >= 0);
+  while (left) {
+    const int a = __builtin_amdgcn_readlane(id64, (int)__builtin_ctzll(left));
+    left &= ~__ballot(id64 == a);
+    const bool any = __any(id == a);
+    const uint16_t* Ba = p.ad.B + (size_t)a * (size_t)p.ad.b_adapter;
+    // 64 rows of 64 ranks: two 16-byte pieces a thread
+    u32x4 b[2];
+    bf16x8 d[2];
+    auto load = [&](int c) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int piece = j * 256 + tid, row = piece >> 3, r = r0 + (piece & 7) * 8;
+        int v = panel_row(p.vc0, c + row, p.tail);
+        v = v < p.V ? v : p.V - 1;  // a column behind the vocabulary: zeros in the panel
+        b[j] = r < R ? *(const u32x4*)(Ba + (size_t)v * (size_t)p.ad.b_row + r) : u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) d[j] = *(const bf16x8*)(d_row + c + j * 32);
+    };
+    f32x4 acc[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (c0 < c1) load(c0);
+    int turn = 0;
+    for (int c = c0; c < c1; c += kDuColumns, turn ^= 1) {
+      char* const at = lds[turn];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int piece = j * 256 + tid;
+        *(u32x4*)(at + (piece >> 3) * kDuPitch + (piece & 7) * 16) = b[j];
+      }
+      const bf16x8 d0 = d[0], d1 = d[1];
+      if (c + kDuColumns < c1) load(c + kDuColumns);
+      __syncthreads();  // the rows stand; the other buffer is written behind the next barrier's reads only
+      if (any) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          if (m < tiles) {
+            acc[m] = mfma(transposed(at + m * 32, kDuPitch), d0, acc[m]);
+            acc[m] = mfma(transposed(at + 32 * kDuPitch + m * 32, kDuPitch), d1, acc[m]);
+          }
+        }
+      }
+    }
+    __syncthreads();  // the next adapter begins with buffer 0
+    if (id == a) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) sum[m] = acc[m];
+    }
+  }
+  if (t >= T) return;
+  float* to = out + ((size_t)blockIdx.y * (size_t)p.T + (size_t)t) * (size_t)Rp + r0 + kq * 4;
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+    if (r0 + m * 16 < Rp) *(f32x4*)(to + m * 16) = sum[m];
+}
+
+// du = s * (the sum of `slots` partial sums, in order) as two bf16 terms, rows of U's form.
+__global__ __launch_bounds__(256) void adapter_du_sum(const Adapters ad, const float* __restrict__ part, int slots, int T_, const int* T_dev,
+                                                      const int* __restrict__ ids, int Rp, uint16_t* __restrict__ dU) {
+  const int T = tokens_in_force(T_, T_dev);
+  const int e = (blockIdx.x * 256 + threadIdx.x) * 4;  // Rp is a multiple of 32
+  const int t = e / Rp, r = e - t * Rp;
+  if (t >= T) return;
+  const size_t step = (size_t)T_ * (size_t)Rp;
+  const float* from = part + (size_t)t * (size_t)Rp + r;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < slots; ++s) sum += *(const f32x4*)(from + (size_t)s * step);
+  const int a = ids[t];
+  const Terms terms = two_terms(sum * (a >= 0 ? ad.scaling[a] : 0.f));
+  uint16_t* to = dU + (size_t)(1 + t) * (size_t)(2 * Rp) + r;
+  *(uint2*)to = terms.hi;
+  *(uint2*)(to + Rp) = terms.lo;
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// dB_a[v, r] = sum over adapter a's rows of dz[t, v] u[t, r].  One workgroup per 256 panel columns, adapter and 64 ranks, 64 columns a wave; M: rank,
+// N: column, both through LDS in steps of 32 rows.  u enters as its upper term alone: dz, the other factor, has been rounded to bf16 as well.
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kDbColumns = 256, kDbRows = 32, kDbRanks = 64;
+constexpr int kDbPitchD = kDbColumns * 2 + 16, kDbPitchU = kDbRanks * 2 + 16;
+__global__ __launch_bounds__(256) void adapter_db(const AdapterPanel p, const uint16_t* __restrict__ U, const int* __restrict__ seg, int row0,
+                                                  const float* sum_in, float* sum_out, uint16_t* __restrict__ dB) {
+  __shared__ __attribute__((aligned(16))) char lds_d[2][kDbRows * kDbPitchD];
+  __shared__ __attribute__((aligned(16))) char lds_u[2][kDbRows * kDbPitchU];
+  const int T = tokens_in_force(p.T, p.T_dev);
+  const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int a = blockIdx.y, r0 = blockIdx.z * kDbRanks, R = p.ad.rank, Rp = padded_rank(R);
+  const int c0 = blockIdx.x * kDbColumns;
+  auto in_block = [&](int at) { return at < row0 ? 0 : at - row0 < T ? at - row0 : T; };
+  const int begin = in_block(__builtin_amdgcn_readfirstlane(seg[a])), end = in_block(__builtin_amdgcn_readfirstlane(seg[a + 1]));
+  f32x4 acc[4][4];  // [rank tile][column tile]
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  u32x4 d[4], u;
+  const int u_row = tid >> 3, u_rank = r0 + (tid & 7) * 8;
+  auto load = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // 32 rows of 512 bytes; rows behind the last one repeat it, against zeros of u
+      const int piece = j * 256 + tid, row = t + (piece >> 5);
+      d[j] = *(const u32x4*)(p.D + (size_t)(row < end ? row : end - 1) * (size_t)p.ldd + c0 + (piece & 31) * 8);
+    }
+    u = t + u_row < end && u_rank < Rp ? *(const u32x4*)(U + (size_t)(1 + t + u_row) * (size_t)(2 * Rp) + u_rank) : u32x4{0u, 0u, 0u, 0u};
+  };
+  if (begin < end) load(begin);
+  int turn = 0;
+  for (int t = begin; t < end; t += kDbRows, turn ^= 1) {
+    char *const at_d = lds_d[turn], *const at_u = lds_u[turn];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int piece = j * 256 + tid;
+      *(u32x4*)(at_d + (piece >> 5) * kDbPitchD + (piece & 31) * 16) = d[j];
+    }
+    *(u32x4*)(at_u + u_row * kDbPitchU + (tid & 7) * 16) = u;
+    if (t + kDbRows < end) load(t + kDbRows);
+    __syncthreads();
+    bf16x8 df[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) df[n] = transposed(at_d + (wave * 64 + n * 16) * 2, kDbPitchD);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      if (r0 + m * 16 >= R) continue;
+      const bf16x8 uf = transposed(at_u + m * 32, kDbPitchU);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) acc[m][n] = mfma(uf, df[n], acc[m][n]);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int column = p.vc0 + c0 + wave * 64 + n * 16 + lrow;
+    int v = column;
+    if (p.tail.back > 0 && column >= p.tail.from) {  // the moved group: its first columns repeat the group before it
+      if (column - p.tail.from < p.tail.back || column - p.tail.from >= 2 * BK) continue;
+      v = column - p.tail.back;
+    }
+    if (v >= p.V) continue;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int r = r0 + m * 16 + kq * 4;
+      if (r >= R) continue;
+      const size_t at = ((size_t)a * (size_t)p.V + (size_t)v) * (size_t)R + r;
+      f32x4 x = acc[m][n];
+      if (sum_in) x += *(const f32x4*)(sum_in + at);
+      if (sum_out) *(f32x4*)(sum_out + at) = x;
+      if (dB) {
+        const bf16x4 b = __builtin_convertvector(x, bf16x4);
+        *(uint2*)(dB + at) = *(const uint2*)&b;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// d_hidden[row_map[t], :] += A_a^T du_t.  One workgroup per 64 tokens and 64 hidden columns, 16 tokens a wave.  M: hidden column (A's rows through
+// LDS), N: token.  d_hidden holds the product with the weight, rounded to bf16; the sum is rounded once more.
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kDhPitch = 64 * 2 + 16;
+__global__ __launch_bounds__(256) void adapter_dh_add(const Adapters ad, const uint16_t* __restrict__ dU, const int* __restrict__ ids, int T_,
+                                                      const int* T_dev, const int* __restrict__ row_map, int H, uint16_t* __restrict__ d_hidden) {
+  __shared__ __attribute__((aligned(16))) char lds[32 * kDhPitch];
+  const int T = tokens_in_force(T_, T_dev), t0 = blockIdx.x * 64, h0 = blockIdx.y * 64;
+  if (t0 >= T) return;
+  const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Rp = padded_rank(ad.rank);
+  const int id64 = t0 + lane < T ? ids[t0 + lane] : -1;
+  const int t = t0 + wave * 16 + lrow;
+  const int id = t < T ? ids[t] : -1;
+  const uint16_t* du = dU + (size_t)(1 + (t < T ? t : T - 1)) * (size_t)(2 * Rp) + kq * 8;
+  f32x4 sum[4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m) sum[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  unsigned long long left = __ballot(id64 >= 0);
+  while (left) {
+    const int a = __builtin_amdgcn_readlane(id64, (int)__builtin_ctzll(left));
+    left &= ~__ballot(id64 == a);
+    const uint16_t* Aa = ad.A + (size_t)a * (size_t)ad.a_adapter + h0;
+    f32x4 acc[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < Rp; k += 32) {
+      const int row = tid >> 3;  // 32 rows of 128 bytes
+      const uint4 x = k + row < ad.rank ? *(const uint4*)(Aa + (size_t)(k + row) * (size_t)ad.a_row + (tid & 7) * 8) : make_uint4(0, 0, 0, 0);
+      __syncthreads();
+      *(uint4*)(lds + row * kDhPitch + (tid & 7) * 16) = x;
+      __syncthreads();
+      const bf16x8 hi = *(const bf16x8*)(du + k), lo = *(const bf16x8*)(du + Rp + k);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const bf16x8 f = transposed(lds + m * 32, kDhPitch);
+        acc[m] = mfma(f, hi, acc[m]);
+        acc[m] = mfma(f, lo, acc[m]);
+      }
+    }
+    if (id == a) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) sum[m] = acc[m];
+    }
+  }
+  if (id < 0) return;
+  uint16_t* to = d_hidden + (size_t)row_map[t] * (size_t)H + h0 + kq * 4;
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const uint2 w = *(const uint2*)(to + m * 16);
+    const f32x4 x = {sum[m][0] + __uint_as_float(w.x << 16), sum[m][1] + __uint_as_float(w.x & 0xffff0000u), sum[m][2] + __uint_as_float(w.y << 16),
+                     sum[m][3] + __uint_as_float(w.y & 0xffff0000u)};
+    const bf16x4 b = __builtin_convertvector(x, bf16x4);
+    *(uint2*)(to + m * 16) = *(const uint2*)&b;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// dA_a[r, h] = sum over adapter a's rows of du[t, r] h[t, h], in pieces of at most kDaPiece rows whose sums are added in order.  Piece number p of
+// all adapters' pieces, laid end to end: its adapter and rows, or a < 0 behind the last one.
+// ------------------------------------------------------------------------------------------------------------
+struct DaPiece {
+  int a, begin, end;
+};
+__device__ __forceinline__ DaPiece da_piece(const int* seg, int N, int p) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;  // pieces of adapters in front of this step's 64
+  for (int a0 = 0; a0 < N; a0 += 64) {
+    const int a = a0 + lane;
+    const int from = a < N ? seg[a] : 0, to = a < N ? seg[a + 1] : 0, n = (to - from + kDaPiece - 1) / kDaPiece;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int below = __shfl_up(upto, o, 64);
+      upto += lane >= o ? below : 0;
+    }
+    const unsigned long long past = __ballot(before + upto > p);
+    if (past) {
+      const int l = (int)__builtin_ctzll(past);
+      const int k = p - before - __shfl(upto - n, l, 64);
+      const int begin = __shfl(from, l, 64) + k * kDaPiece, last = __shfl(to, l, 64);
+      return DaPiece{a0 + l, begin, begin + kDaPiece < last ? begin + kDaPiece : last};
+    }
+    before += __shfl(upto, 63, 64);
+  }
+  return DaPiece{-1, 0, 0};
+}
+
+// One workgroup per piece, 256 hidden columns (64 a wave) and 32 ranks.  M: hidden column, N: rank, steps of 32 rows.
+constexpr int kDaPitchH = 256 * 2 + 16, kDaPitchU = 2 * 32 * 2 + 16;
+__global__ __launch_bounds__(256) void adapter_da_partial(const Adapters ad, const uint16_t* __restrict__ hidden, int64_t ldh, const uint16_t* __restrict__ dU,
+                                                          const int* __restrict__ seg, int H, float* __restrict__ part) {
+  __shared__ __attribute__((aligned(16))) char lds_h[2][32 * kDaPitchH];
+  __shared__ __attribute__((aligned(16))) char lds_u[2][32 * kDaPitchU];
+  const DaPiece piece = da_piece(seg, ad.N, blockIdx.x);
+  if (piece.a < 0) return;
+  const int begin = __builtin_amdgcn_readfirstlane(piece.begin), end = __builtin_amdgcn_readfirstlane(piece.end);
+  const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h0 = blockIdx.y * 256, r0 = blockIdx.z * 32, Rp = padded_rank(ad.rank);
+  f32x4 acc[4][2];
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  u32x4 x[4], u;
+  const int u_row = tid >> 3, u_term = (tid >> 2) & 1, u_rank = (tid & 3) * 8;  // 32 rows of 32 upper, then 32 lower terms
+  auto load = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int p = j * 256 + tid, row = t + (p >> 5), h = h0 + (p & 31) * 8;
+      x[j] = *(const u32x4*)(hidden + (size_t)(row < end ? row : end - 1) * (size_t)ldh + (h < H ? h : H - 8));
+    }
+    u = t + u_row < end ? *(const u32x4*)(dU + (size_t)(1 + t + u_row) * (size_t)(2 * Rp) + u_term * Rp + r0 + u_rank) : u32x4{0u, 0u, 0u, 0u};
+  };
+  load(begin);
+  int turn = 0;
+  for (int t = begin; t < end; t += 32, turn ^= 1) {
+    char *const at_h = lds_h[turn], *const at_u = lds_u[turn];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int p = j * 256 + tid;
+      *(u32x4*)(at_h + (p >> 5) * kDaPitchH + (p & 31) * 16) = x[j];
+    }
+    *(u32x4*)(at_u + u_row * kDaPitchU + u_term * 64 + u_rank * 2) = u;
+    if (t + 32 < end) load(t + 32);
+    __syncthreads();
+    bf16x8 hi[2], lo[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) hi[n] = transposed(at_u + n * 32, kDaPitchU), lo[n] = transposed(at_u + 64 + n * 32, kDaPitchU);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const bf16x8 f = transposed(at_h + (wave * 64 + m * 16) * 2, kDaPitchH);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        acc[m][n] = mfma(f, hi[n], acc[m][n]);
+        acc[m][n] = mfma(f, lo[n], acc[m][n]);
+      }
+    }
+  }
+  // A lane holds four consecutive hidden columns of one rank.
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int r = r0 + n * 16 + lrow;
+    float* to = part + ((size_t)blockIdx.x * (size_t)Rp + (size_t)r) * (size_t)H;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int h = h0 + wave * 64 + m * 16 + kq * 4;
+      if (h < H) *(f32x4*)(to + h) = acc[m][n];
+    }
+  }
+}
+
+// dA of an adapter: the sum of its pieces, rounded.  One workgroup per adapter and rank.
+__global__ __launch_bounds__(256) void adapter_da_sum(const float* __restrict__ part, const int* __restrict__ seg, int H, int R, uint16_t* __restrict__ dA) {
+  const int a = blockIdx.x, r = blockIdx.y, Rp = padded_rank(R);
+  __shared__ int first_piece;
+  if (threadIdx.x < 64) {
+    int before = 0;
+    for (int b = threadIdx.x; b < a; b += 64) before += (seg[b + 1] - seg[b] + kDaPiece - 1) / kDaPiece;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) before += __shfl_xor(before, o, 64);
+    if (threadIdx.x == 0) first_piece = before;
+  }
+  __syncthreads();
+  const int n = (seg[a + 1] - seg[a] + kDaPiece - 1) / kDaPiece;
+  const float* from = part + ((size_t)first_piece * (size_t)Rp + (size_t)r) * (size_t)H;
+  uint16_t* to = dA + ((size_t)a * (size_t)R + (size_t)r) * (size_t)H;
+  for (int h = threadIdx.x * 4; h < H; h += 256 * 4) {
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < n; ++p) sum += *(const f32x4*)(from + (size_t)p * (size_t)Rp * (size_t)H + h);
+    const bf16x4 b = __builtin_convertvector(sum, bf16x4);
+    *(uint2*)(to + h) = *(const uint2*)&b;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_adapter_shrink(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const int64_t* ids, int64_t T, const int* T_dev,
+                                 int64_t H, uint16_t* U, int* ids32) {
+  hipLaunchKernelGGL(adapter_shrink, dim3((unsigned)((T + 15) / 16), (unsigned)(padded_rank(ad.rank) / 32)), dim3(kShrinkWaves * 64), 0, s, ad, hidden, ldh,
+                     ids, (int)T, T_dev, (int)H, U, ids32);
+  return hipGetLastError();
+}
+
+hipError_t launch_adapter_label(hipStream_t s, const Adapters& ad, const uint16_t* U, const int* ids32, const int64_t* labels, int64_t T, int64_t V,
+                                float rcp_temp, float* logprobs) {
+  hipLaunchKernelGGL(adapter_label, dim3((unsigned)((T + 15) / 16)), dim3(256), 0, s, ad, U, ids32, labels, (int)T, V, rcp_temp, logprobs);
+  return hipGetLastError();
+}
+
+hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float* q, const int64_t* ids, int64_t T, int N, int* idx, int64_t* ids_c, int* seg) {
+  hipLaunchKernelGGL(adapter_group_rows, dim3((unsigned)(N + 1)), dim3(kGroupThreads), 0, s, g, q, ids, (int)T, N, idx, ids_c, seg);
+  return hipGetLastError();
+}
+
+int adapter_du_ranges(int64_t T, int64_t columns, int ncu) {
+  const int64_t tiles = (T + kDuTokens - 1) / kDuTokens, wanted = (2 * (int64_t)ncu + tiles - 1) / tiles, most = (columns + 511) / 512;
+  return (int)(wanted < most ? wanted : most);
+}
+
+hipError_t launch_adapter_panel(hipStream_t s, const AdapterPanel& p, int ranges, float* du_part, const uint16_t* U, const int* seg, int row0,
+                                const float* sum_in, float* sum_out, uint16_t* dB) {
+  const int Rp = padded_rank(p.ad.rank), ranks = (Rp + 63) / 64;
+  const int per_range = ((p.columns + ranges - 1) / ranges + kDuColumns - 1) / kDuColumns * kDuColumns;
+  hipLaunchKernelGGL(adapter_du_partial, dim3((unsigned)((p.T + kDuTokens - 1) / kDuTokens), (unsigned)ranges, (unsigned)ranks), dim3(256), 0, s, p,
+                     p.columns, per_range, du_part, Rp);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(adapter_db, dim3((unsigned)(p.columns / kDbColumns), (unsigned)p.ad.N, (unsigned)ranks), dim3(256), 0, s, p, U, seg, row0, sum_in,
+                     sum_out, dB);
+  return hipGetLastError();
+}
+
+hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float* part, int slots, int64_t T, const int* T_dev, const int* ids32, uint16_t* dU) {
+  const int Rp = padded_rank(ad.rank);
+  hipLaunchKernelGGL(adapter_du_sum, dim3((unsigned)((T * (Rp / 4) + 255) / 256)), dim3(256), 0, s, ad, part, slots, (int)T, T_dev, ids32, Rp, dU);
+  return hipGetLastError();
+}
+
+hipError_t launch_adapter_finish(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const uint16_t* dU, const int* ids32, const int* seg,
+                                 int64_t T, const int* T_dev, const int* row_map, int64_t H, uint16_t* d_hidden, float* da_part, uint16_t* dA) {
+  const unsigned ranks = (unsigned)(padded_rank(ad.rank) / 32);
+  hipLaunchKernelGGL(adapter_dh_add, dim3((unsigned)((T + 63) / 64), (unsigned)(H / 64)), dim3(256), 0, s, ad, dU, ids32, (int)T, T_dev, row_map, (int)H,
+                     d_hidden);
+  hipLaunchKernelGGL(adapter_da_partial, dim3((unsigned)adapter_da_pieces(T, ad.N), (unsigned)((H + 255) / 256), ranks), dim3(256), 0, s, ad, hidden, ldh, dU,
+                     seg, (int)H, da_part);
+  hipLaunchKernelGGL(adapter_da_sum, dim3((unsigned)ad.N, (unsigned)ad.rank), dim3(256), 0, s, (const float*)da_part, seg, (int)H, ad.rank, dA);
+  return hipGetLastError();
+}
+
+}  // namespace lmhead

@@ -29,6 +29,7 @@
 
 #include "../../include/skyrl_lmhead.h"
 #include "../../include/skyrl_lmhead_bench.h"
+#include "adapters.hpp"
 #include "dh_split.hpp"
 #include "few_tokens.hpp"
 #include "gemm_core.hpp"
@@ -1178,7 +1179,8 @@ __global__ __launch_bounds__(256) void zero_f32(float* __restrict__ p, int n) {
 // tokens, in tiles or with resident dz.
 enum KernelKind {
   kFwdTiles = 0, kFwdMerge, kTranspose, kBwdChunkDz, kBwdChunkGemm, kSoftCePack, kSoftCeFwdTiles, kSoftCeFinish, kSoftCeDz,
-  kCompactRows, kSplitOperand, kTopkFilter, kTopkSelect, kTopkRows, kTopkBwdRows, kDhReduce, kBwdDwFew,
+  kCompactRows, kSplitOperand, kTopkFilter, kTopkSelect, kTopkRows, kTopkBwdRows, kDhReduce, kBwdDwFew, kAdapterRows, kAdapterPanel,
+  kAdapterFinish,
   kNumKernelKinds
 };
 const char* const kKernelNames[kNumKernelKinds] = {"lmhead_fwd_tiles", "lmhead_fwd_merge", "transpose_bf16",
@@ -1186,7 +1188,8 @@ const char* const kKernelNames[kNumKernelKinds] = {"lmhead_fwd_tiles", "lmhead_f
                                                    "softce_fwd_tiles", "softce_finish", "softce_dz_tiles",
                                                    "active_rows[compact+gather]", "split_operand_rows",
                                                    "topk_filter_tiles", "topk_select", "topk_softce_rows",
-                                                   "topk_softce_bwd_rows", "lmhead_dh_reduce", "lmhead_bwd_dw_few"};
+                                                   "topk_softce_bwd_rows", "lmhead_dh_reduce", "lmhead_bwd_dw_few",
+                                                   "adapter_rows[shrink+label+group]", "adapter_panel[du+dB]", "adapter_finish[dHidden+dA]"};
 struct Profile {
   struct Rec {
     int kind;
@@ -1369,12 +1372,25 @@ int64_t fwd_block_tokens(int64_t wanted, int64_t ld_hidden) {
   return wanted < BN ? BN : wanted;
 }
 
+// The adapters of a call, and the room for a block's rows of u.
+struct AdapterCall {
+  Adapters ad;
+  const int64_t* ids;  // [T]
+  uint16_t* U;
+  int* ids32;
+
+  AdapterTile tile(int64_t row0 = 0) const {
+    return AdapterTile{ad.B, ad.b_adapter, (int)ad.b_row, ad.rank, U + (size_t)row0 * 2 * padded_rank(ad.rank), U, ids32 + row0};
+  }
+};
+
+// call: the head's adapters, or NULL.
 int fwd_token_blocks(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels,
                      int64_t T, int64_t H, int64_t V, float rcp_temperature, float* logprobs, float* entropy, float* row_lse,
-                     float* row_pz, void* scratch, int64_t block_tokens, hipStream_t s) {
+                     float* row_pz, void* scratch, int64_t block_tokens, hipStream_t s, const AdapterCall* call = nullptr) {
   const int tiles_m = (int)((V + BM - 1) / BM);
   const size_t nparts = (size_t)tiles_m * WAVES_M;
-  const bool want_pz = entropy || row_pz;
+  const bool want_pz = entropy || row_pz || call;  // the tiles with adapters always sum it
   const uint16_t* Wp = (const uint16_t*)weight;
   for (int64_t t0 = 0; t0 < T; t0 += block_tokens) {
     const int64_t Tb = (T - t0) < block_tokens ? (T - t0) : block_tokens;
@@ -1387,12 +1403,21 @@ int fwd_token_blocks(const void* hidden, int64_t ld_hidden, const void* weight, 
     const uint16_t* Hp = (const uint16_t*)hidden + (size_t)t0 * (size_t)ld_hidden;
     const TileShapes shapes = tile_shapes(Tb, H, tiles_m, compute_units());
     const dim3 grid((unsigned)(tiles_m * tiles_n + shapes.split)), block(NTHREADS);
+    if (call) {
+      Timed timed(kAdapterRows, s);
+      const hipError_t e = launch_adapter_shrink(s, call->ad, Hp, ld_hidden, call->ids + t0, Tb, nullptr, H, call->U, call->ids32);
+      if (e != hipSuccess) return (int)e;
+    }
     {
       Timed timed(kFwdTiles, s);
       auto kernel = flagged_kernel(
           [](auto pz, auto even, auto others) { return &lmhead_fwd_tiles<pz.value, even.value, others.value>; }, want_pz, even_ktiles(H),
           shapes.used);
-      if (half)
+      if (call)
+        (void)launch_adapter_fwd_tiles(s, AdapterFwdArgs{Wp, Hp, (int)ld_weight, (int)ld_hidden, (int)Tb, (int)H, (int)V, rcp_temperature, pmax, psum,
+                                                         ppz, call->tile()},
+                                       half, even_ktiles(H), shapes.used, shapes.split, half ? tiles_m : (int)grid.x);
+      else if (half)
         launch_fwd_half_tiles(s, want_pz, Wp, (int)ld_weight, Hp, (int)ld_hidden, (int)Tb, (int)H, (int)V, rcp_temperature, pmax, psum, ppz);
       else
         hipLaunchKernelGGL(kernel, grid, block, 0, s, Wp, (int)ld_weight, Hp, (int)ld_hidden, (int)Tb, (int)H, (int)V,
@@ -1406,6 +1431,10 @@ int fwd_token_blocks(const void* hidden, int64_t ld_hidden, const void* weight, 
                        labels + t0, (int)H, (int)V, rcp_temperature, logprobs + t0, entropy ? entropy + t0 : (float*)nullptr,
                        row_lse ? row_lse + t0 : (float*)nullptr, row_pz ? row_pz + t0 : (float*)nullptr);
     if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+    if (call) {  // the merge takes the label's logit from the weight alone
+      e = launch_adapter_label(s, call->ad, call->U, call->ids32, labels + t0, Tb, V, rcp_temperature, logprobs + t0);
+      if (e != hipSuccess) return (int)e;
+    }
   }
   return SKYRL_LMHEAD_OK;
 }
@@ -1536,15 +1565,17 @@ GemmArgs dhidden_gemm(const uint16_t* D, int64_t ldd, int64_t d_rows, const uint
   return g;
 }
 
-hipError_t launch_bwd_dz(hipStream_t s, bool entgrad, DzArgs z) {
+hipError_t launch_bwd_dz(hipStream_t s, bool entgrad, DzArgs z, const AdapterTile* adapters = nullptr) {
   Timed timed(kBwdChunkDz, s);
   if (half_tile_logits(z.T)) {
     z.tiles_n = 1;
+    if (adapters) return launch_adapter_dz(s, z, *adapters, entgrad, true, true, false, z.tiles_m);
     return launch_bwd_half_dz(s, entgrad, z);
   }
   z.tiles_n = (z.T + BN - 1) / BN;
   const int tiles = z.tiles_m * z.tiles_n;
   const TileShapes shapes = z.T_dev ? tile_shapes_of_any_count(z.H, z.tiles_m, tiles, z.ncu) : tile_shapes(z.T, z.H, z.tiles_m, z.ncu);
+  if (adapters) return launch_adapter_dz(s, z, *adapters, entgrad, false, even_ktiles(z.H), shapes.used, tiles + shapes.split);
   auto kernel = flagged_kernel([](auto ent, auto even, auto others) { return &lmhead_bwd_dz<ent.value, even.value, others.value>; },
                                entgrad, even_ktiles(z.H), shapes.used);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles + shapes.split)), dim3(NTHREADS), 0, s, z);
@@ -1719,6 +1750,35 @@ size_t bwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t vocab_chunk,
   return carve_bwd(nullptr, T, H, terms * H, V, vc, compact, SIZE_MAX, false).bytes;
 }
 
+// What the backward with adapters has besides: rows grouped by adapter (row compaction is always on), their u, and the room for the sums.
+struct AdapterBwd {
+  AdapterCall call;    // U and ids32 of all rows
+  int64_t* ids_c;      // [T]
+  int* seg;            // [N + 2]
+  uint16_t* dU;        // as U
+  float *du_part, *da_part, *db_sum;  // db_sum only where there are several token blocks
+  uint16_t *dA, *dB;
+  int ranges;
+  size_t bytes;
+};
+AdapterBwd carve_adapter_bwd(void* ws, const Adapters& ad, int64_t T, int64_t H, int64_t V, int64_t vc) {
+  const int64_t Tb = bwd_block_tokens(T), Rp = padded_rank(ad.rank), chunks = (round_up(V, 256) + vc - 1) / vc;
+  Carver c(ws);
+  AdapterBwd w{};
+  w.call.ad = ad;
+  w.ranges = adapter_du_ranges(Tb, vc, compute_units());
+  w.ids_c = c.take<int64_t>((size_t)T);
+  w.call.ids32 = c.take<int>((size_t)T);
+  w.seg = c.take<int>((size_t)ad.N + 2);
+  w.call.U = c.take<uint16_t>((size_t)(T + 1) * (size_t)(2 * Rp));
+  w.dU = c.take<uint16_t>((size_t)(T + 1) * (size_t)(2 * Rp));
+  w.du_part = c.take<float>((size_t)(chunks * w.ranges) * (size_t)Tb * (size_t)Rp);
+  w.da_part = c.take<float>((size_t)adapter_da_pieces(T, ad.N) * (size_t)Rp * (size_t)H);
+  w.db_sum = bwd_num_blocks(T) > 1 ? c.take<float>((size_t)ad.N * (size_t)V * (size_t)ad.rank) : nullptr;
+  w.bytes = (size_t)round_up((int64_t)c.off, 256);
+  return w;
+}
+
 // One token block of the backward: the vocab-chunk loop.  Hk is the contraction length of the logits recompute (H, or a
 // multiple of it for stacked bf16 terms, in which case the two gradient GEMMs use the leading H columns: the hi terms).  `Tb` tokens (an upper bound when `T_dev` points at the block's
 // count in device memory and `splits_dev` at what `rated` made of it), per-token inputs and d_hidden already offset to the block.  dW of every chunk leaves the GEMM
@@ -1728,7 +1788,7 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
                     const int* T_dev, const int* splits_dev, const SplitProblem& rated, const int* row_map, int64_t H, int64_t Hk, int64_t V,
                     float rcp_temperature, uint16_t* d_hidden, bool want_dw,
                     const float* dw_in, float* dw_f32, uint16_t* dw_bf16, int64_t vc, const BwdWorkspace& w, float p_shift,
-                    hipStream_t s) {
+                    hipStream_t s, const AdapterBwd* ab = nullptr, int64_t row0 = 0, bool last_block = true) {
   const int64_t Tpad = round_up(Tb, 256), Vpad = round_up(V, 256);
   const int ncu = compute_units();
   const bool w_in_place = reads_weight_in_place(V);
@@ -1753,6 +1813,7 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
   const int64_t nchunks = (Vpad + vc - 1) / vc;
   auto chunk_width = [&](int64_t ci) { return (Vpad - ci * vc) < vc ? (Vpad - ci * vc) : vc; };  // multiple of 256
   const GemmArgs none{};
+  const AdapterTile adapters = ab ? ab->call.tile(row0) : AdapterTile{};
   for (int64_t ci = 0; ci < nchunks; ++ci) {
     // dz panel of this chunk, then the two gradient GEMMs that consume it (one launch, they are independent).
     // Carrying the next chunk's dz tiles in the GEMM launch (to fill its tail) was measured: no gain at the default chunk
@@ -1760,8 +1821,16 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
     const int64_t vc0 = ci * vc, vcw = chunk_width(ci);
     const DzArgs z{Wp, (int)ld_weight, Hp, (int)ld_hidden, (int)Tb, (int)Hk, (int)V, rcp_temperature, labels, row_lse, row_pz,
                    dlogprobs, dentropy, (int)vc0, (int)(vcw / 256), 0, tail, w.D, (int)(vcw + kLdPad), T_dev, resid, p_shift, ncu};
-    e = launch_bwd_dz(s, dentropy != nullptr, z);
+    e = launch_bwd_dz(s, dentropy != nullptr, z, ab ? &adapters : nullptr);
     if (e != hipSuccess) return (int)e;
+    if (ab) {
+      Timed timed(kAdapterPanel, s);
+      const AdapterPanel panel{ab->call.ad, w.D, (int)(vcw + kLdPad), (int)Tb, T_dev, adapters.ids, (int)vc0, (int)vcw, (int)V, tail};
+      float* const part = ab->du_part + (size_t)(ci * ab->ranges) * (size_t)Tb * (size_t)padded_rank(ab->call.ad.rank);
+      e = launch_adapter_panel(s, panel, ab->ranges, part, adapters.U, ab->seg, (int)row0, row0 > 0 ? ab->db_sum : nullptr,
+                               last_block ? nullptr : ab->db_sum, last_block ? ab->dB : nullptr);
+      if (e != hipSuccess) return (int)e;
+    }
     // dHidden[t, h] (+)= sum_v D[t, v] . weight^T[h, vc0 + v]        (A = weight^T rows at k offset vc0, B = D rows)
     // dW[vc0 + v, h]  (+)= sum_t D[t, v] . hidden^T[h, t]             (A = hidden^T rows, B = D read K-major)
     const bool first = ci == 0, last = ci == nchunks - 1;
@@ -1791,6 +1860,12 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
     if (e == hipSuccess && last) e = launch_dh_reduce(s, gh, split);
     if (e != hipSuccess) return (int)e;
   }
+  if (ab) {
+    Timed timed(kAdapterFinish, s);
+    e = launch_adapter_du_sum(s, ab->call.ad, ab->du_part, (int)(nchunks * ab->ranges), Tb, T_dev, adapters.ids,
+                              ab->dU + (size_t)row0 * 2 * padded_rank(ab->call.ad.rank));
+    if (e != hipSuccess) return (int)e;
+  }
   if (resid) {
     hipLaunchKernelGGL(label_residual_update, dim3((unsigned)Tb), dim3(256), 0, s, (const float*)resid, labels, Hp, (int)ld_hidden,
                        (int)H, Hk == 3 * H ? (int)(2 * H) : 0, (int)V, T_dev, dw_f32);
@@ -1802,7 +1877,7 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
 int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels,
               const float* row_lse, const float* row_pz, const float* dlogprobs, const float* dentropy, int64_t T, int64_t H,
               int64_t V, float rcp_temperature, void* d_hidden, void* d_weight, int dw_mode, int64_t vocab_chunk,
-              void* workspace, size_t workspace_bytes, hipStream_t s, bool compact, int64_t terms = 1) {
+              void* workspace, size_t workspace_bytes, hipStream_t s, bool compact, int64_t terms = 1, const AdapterBwd* ab = nullptr) {
   if (terms < 1 || terms > 3 || H < 1 || H > kMaxExtent / 4) return SKYRL_LMHEAD_ERR_ARG;
   // dw_mode carries one option bit next to the mode: softmax probabilities below 2^-24 count as zero in dz.
   const float p_shift = (dw_mode & SKYRL_BWD_FLUSH_TINY_DZ) ? 126.f - 24.f : 0.f;
@@ -1841,10 +1916,19 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
     Timed timed(kCompactRows, s);
     hipLaunchKernelGGL(compact_kernel(T), dim3(1), dim3(kCompactThreads), 0, s, dlogprobs, dentropy, (int)T, (int)Tb,
                        (int)nblocks, rated, w.idx, w.counts);
+    if (ab) {  // the same rows in another order
+      e = launch_adapter_group_rows(s, dlogprobs, dentropy, ab->call.ids, T, ab->call.ad.N, w.idx, ab->ids_c, ab->seg);
+      if (e != hipSuccess) return (int)e;
+    }
     hipLaunchKernelGGL(gather_active_rows, dim3((unsigned)T), dim3(256), 0, s, (const int*)w.idx, (const int*)w.counts, Hp,
                        (int)ld_hidden, (int)Hk, (int)H, labels, row_lse, row_pz, dlogprobs, dentropy, w.hidden_c, w.labels_c,
                        w.lse_c, w.pz_c, w.g_c, w.q_c, (uint16_t*)d_hidden);
     if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+  }
+  if (ab) {
+    Timed timed(kAdapterRows, s);
+    e = launch_adapter_shrink(s, ab->call.ad, w.hidden_c, H, ab->ids_c, T, w.counts, H, ab->call.U, ab->call.ids32);
+    if (e != hipSuccess) return (int)e;
   }
   if (!reads_weight_in_place(V)) {  // weight^T [H, Vpad], zero in the padding columns
     Timed timed(kTranspose, s);
@@ -1879,7 +1963,7 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
       st = bwd_token_block(w.hidden_c + (size_t)t0 * (size_t)Hk, Hk, Wp, ld_weight, w.labels_c + t0, w.lse_c + t0,
                            dentropy ? w.pz_c + t0 : nullptr, w.g_c + t0, dentropy ? w.q_c + t0 : nullptr, Tcur,
                            w.counts + 1 + b, w.counts + 1 + nblocks + b, rated, w.idx + t0, H, Hk, V, rcp_temperature, (uint16_t*)d_hidden,
-                           d_weight != nullptr, dw_in, dw_f32, dw_bf16, vc, w, p_shift, s);
+                           d_weight != nullptr, dw_in, dw_f32, dw_bf16, vc, w, p_shift, s, ab, t0, b == nblocks - 1);
     } else {
       st = bwd_token_block(Hp + (size_t)t0 * (size_t)ld_hidden, ld_hidden, Wp, ld_weight, labels + t0, row_lse + t0,
                            row_pz ? row_pz + t0 : nullptr, dlogprobs + t0, dentropy ? dentropy + t0 : nullptr, Tcur, nullptr,
@@ -1888,7 +1972,54 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
     }
     if (st) return st;
   }
+  if (ab) {
+    Timed timed(kAdapterFinish, s);
+    e = launch_adapter_finish(s, ab->call.ad, w.hidden_c, H, ab->dU, ab->call.ids32, ab->seg, T, w.counts, w.idx, H, (uint16_t*)d_hidden, ab->da_part,
+                              ab->dA);
+    if (e != hipSuccess) return (int)e;
+  }
   return SKYRL_LMHEAD_OK;
+}
+
+// The adapters of an entry point: A [N, rank, H], B [N, V, rank], scaling [N].
+constexpr int64_t kMaxAdapters = 65535;  // a grid's extent
+int check_adapters(const void* A, int64_t a_adapter, int64_t a_row, const void* B, int64_t b_adapter, int64_t b_row, const float* scaling,
+                   const int64_t* ids, int64_t N, int64_t rank, int64_t H) {
+  if (!A || !B || !scaling || !ids) return SKYRL_LMHEAD_ERR_NULL;
+  if (N < 1 || N > kMaxAdapters || rank < 8 || rank > kMaxAdapterRank || rank % 8 != 0) return SKYRL_LMHEAD_ERR_SHAPE;
+  if (a_row < H || a_row > kMaxRowPitch || b_row < rank || b_row > kMaxRowPitch || a_adapter < 0 || b_adapter < 0) return SKYRL_LMHEAD_ERR_SHAPE;
+  if (a_adapter >= ((int64_t)1 << 40) || b_adapter >= ((int64_t)1 << 40)) return SKYRL_LMHEAD_ERR_SHAPE;
+  if (!aligned16(A) || !aligned16(B) || a_row % 8 != 0 || b_row % 8 != 0 || a_adapter % 8 != 0 || b_adapter % 8 != 0) return SKYRL_LMHEAD_ERR_ALIGN;
+  if (((uintptr_t)scaling & 3u) || ((uintptr_t)ids & 7u)) return SKYRL_LMHEAD_ERR_ALIGN;
+  return SKYRL_LMHEAD_OK;
+}
+Adapters make_adapters(const void* A, int64_t a_adapter, int64_t a_row, const void* B, int64_t b_adapter, int64_t b_row, const float* scaling, int64_t N,
+                       int64_t rank) {
+  return Adapters{(const uint16_t*)A, a_adapter, a_row, (const uint16_t*)B, b_adapter, b_row, scaling, (int)N, (int)rank};
+}
+bool adapter_extents(int64_t T, int64_t H, int64_t V, int64_t N, int64_t rank) {
+  return T >= 1 && V >= 1 && H >= 1 && T <= kMaxExtent && V <= kMaxExtent && H <= kMaxRowPitch && N >= 1 && N <= kMaxAdapters && rank >= 1 &&
+         rank <= kMaxAdapterRank;
+}
+// Rows of u of one forward block, and the tokens' adapters.
+AdapterCall carve_adapter_rows(Carver& c, const Adapters& ad, const int64_t* ids, int64_t T) {
+  AdapterCall call{ad, ids, nullptr, nullptr};
+  const int64_t Tb = T < kFwdTokenBlock ? T : kFwdTokenBlock;
+  call.U = c.take<uint16_t>((size_t)(Tb + 1) * (size_t)(2 * padded_rank(ad.rank)));
+  call.ids32 = c.take<int>((size_t)Tb);
+  return call;
+}
+size_t adapter_rows_bytes(int64_t T, int64_t rank) {
+  Carver c(nullptr);
+  Adapters ad{};
+  ad.rank = (int)rank;
+  (void)carve_adapter_rows(c, ad, nullptr, T);
+  return (size_t)round_up((int64_t)c.off, 256);
+}
+// The chunk of a backward with adapters, and the bytes of scratch in front of theirs.
+int64_t adapter_bwd_chunk(int64_t T, int64_t H, int64_t V) {
+  const int64_t vc = default_vocab_chunk(bwd_block_tokens(T), H, V), Vpad = round_up(V, 256);
+  return vc < Vpad ? vc : Vpad;
 }
 
 }  // namespace
@@ -1960,6 +2091,102 @@ int skyrl_lmhead_fwd_static_scratch(const void* hidden, int64_t ld_hidden, const
 }
 
 size_t skyrl_lmhead_static_scratch_bytes(void) { return kStaticScratchBytes; }
+
+size_t skyrl_lmhead_adapter_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t rank) {
+  if (!adapter_extents(T, H, V, 1, rank)) return 0;
+  return skyrl_lmhead_fwd_workspace_bytes(T, H, V) + adapter_rows_bytes(T, rank);
+}
+
+int skyrl_lmhead_adapter_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels, const void* lora_a,
+                             int64_t a_adapter, int64_t a_row, const void* lora_b, int64_t b_adapter, int64_t b_row, const float* scaling,
+                             const int64_t* adapter_ids, int64_t num_adapters, int64_t rank, int64_t T, int64_t H, int64_t V, float rcp_temperature,
+                             float* logprobs, float* entropy, float* row_lse, float* row_pz, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_common(hidden, ld_hidden, weight, ld_weight, labels, T, H, V, rcp_temperature, true);
+  if (st) return st;
+  if ((st = check_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, adapter_ids, num_adapters, rank, H))) return st;
+  if (!logprobs) return SKYRL_LMHEAD_ERR_NULL;
+  if (!workspace || workspace_bytes < skyrl_lmhead_adapter_fwd_workspace_bytes(T, H, V, rank)) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
+  Carver c((char*)workspace + skyrl_lmhead_fwd_workspace_bytes(T, H, V));
+  const AdapterCall call =
+      carve_adapter_rows(c, make_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, num_adapters, rank), adapter_ids, T);
+  return fwd_token_blocks(hidden, ld_hidden, weight, ld_weight, labels, T, H, V, rcp_temperature, logprobs, entropy, row_lse, row_pz, workspace,
+                          fwd_block_tokens(kFwdTokenBlock, ld_hidden), (hipStream_t)stream, &call);
+}
+
+size_t skyrl_lmhead_adapter_logits_workspace_bytes(int64_t T, int64_t rank) {
+  return adapter_extents(T, 1, 1, 1, rank) ? adapter_rows_bytes(T, rank) : 0;
+}
+
+int skyrl_lmhead_adapter_logits(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* lora_a, int64_t a_adapter,
+                                int64_t a_row, const void* lora_b, int64_t b_adapter, int64_t b_row, const float* scaling, const int64_t* adapter_ids,
+                                int64_t num_adapters, int64_t rank, int64_t T, int64_t H, int64_t V, int logits_dtype, void* logits, int64_t ld_logits,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_operands(hidden, ld_hidden, weight, ld_weight, T, H, V, 1.f, true);
+  if (st) return st;
+  if ((st = check_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, adapter_ids, num_adapters, rank, H))) return st;
+  if (!logits) return SKYRL_LMHEAD_ERR_NULL;
+  if (logits_dtype != SKYRL_LOGITS_BF16 && logits_dtype != SKYRL_LOGITS_F32) return SKYRL_LMHEAD_ERR_ARG;
+  if (ld_logits < V || ld_logits >= ((int64_t)1 << 40)) return SKYRL_LMHEAD_ERR_SHAPE;
+  const bool f32 = logits_dtype == SKYRL_LOGITS_F32;
+  if ((uintptr_t)logits & (f32 ? 3u : 1u)) return SKYRL_LMHEAD_ERR_ALIGN;
+  if (!workspace || workspace_bytes < adapter_rows_bytes(T, rank)) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
+  Carver c(workspace);
+  const AdapterCall call =
+      carve_adapter_rows(c, make_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, num_adapters, rank), adapter_ids, T);
+  const int tiles_m = (int)((V + BM - 1) / BM);
+  hipStream_t s = (hipStream_t)stream;
+  for (int64_t t0 = 0; t0 < T; t0 += kFwdTokenBlock) {
+    const int64_t Tb = T - t0 < kFwdTokenBlock ? T - t0 : kFwdTokenBlock;
+    const uint16_t* Hp = (const uint16_t*)hidden + (size_t)t0 * (size_t)ld_hidden;
+    hipError_t e;
+    {
+      Timed timed(kAdapterRows, s);
+      e = launch_adapter_shrink(s, call.ad, Hp, ld_hidden, adapter_ids + t0, Tb, nullptr, H, call.U, call.ids32);
+    }
+    if (e != hipSuccess) return (int)e;
+    Timed timed(kFwdTiles, s);
+    const bool half = half_tile_logits(Tb);
+    const TileShapes shapes = tile_shapes(Tb, H, tiles_m, compute_units());
+    const int tiles = half ? tiles_m : tiles_m * (int)((Tb + BN - 1) / BN) + shapes.split;
+    e = launch_adapter_logits(s, AdapterLogitsArgs{(const uint16_t*)weight, Hp, (int)ld_weight, (int)ld_hidden, (int)Tb, (int)H, (int)V,
+                                                   (char*)logits + (size_t)t0 * (size_t)ld_logits * (f32 ? 4 : 2), ld_logits, f32 ? 1 : 0, call.tile()},
+                              half, even_ktiles(H), shapes.used, shapes.split, tiles);
+    if (e != hipSuccess) return (int)e;
+  }
+  return SKYRL_LMHEAD_OK;
+}
+
+size_t skyrl_lmhead_adapter_bwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t num_adapters, int64_t rank) {
+  if (!adapter_extents(T, H, V, num_adapters, rank)) return 0;
+  const int64_t vc = adapter_bwd_chunk(T, H, V);
+  Adapters ad{};
+  ad.N = (int)num_adapters, ad.rank = (int)rank;
+  return bwd_workspace_bytes(T, H, V, vc, true) + carve_adapter_bwd(nullptr, ad, T, H, V, vc).bytes;
+}
+
+int skyrl_lmhead_adapter_bwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels, const void* lora_a,
+                             int64_t a_adapter, int64_t a_row, const void* lora_b, int64_t b_adapter, int64_t b_row, const float* scaling,
+                             const int64_t* adapter_ids, int64_t num_adapters, int64_t rank, const float* row_lse, const float* row_pz,
+                             const float* dlogprobs, const float* dentropy, int64_t T, int64_t H, int64_t V, float rcp_temperature, void* d_hidden,
+                             void* d_lora_a, void* d_lora_b, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_common(hidden, ld_hidden, weight, ld_weight, labels, T, H, V, rcp_temperature, true);
+  if (st) return st;
+  if ((st = check_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, adapter_ids, num_adapters, rank, H))) return st;
+  if (!d_lora_a || !d_lora_b) return SKYRL_LMHEAD_ERR_NULL;
+  if (!aligned16(d_lora_a) || !aligned16(d_lora_b)) return SKYRL_LMHEAD_ERR_ALIGN;
+  const int64_t vc = adapter_bwd_chunk(T, H, V);
+  const size_t head = bwd_workspace_bytes(T, H, V, vc, true);
+  if (!workspace || workspace_bytes < skyrl_lmhead_adapter_bwd_workspace_bytes(T, H, V, num_adapters, rank)) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
+  AdapterBwd ab = carve_adapter_bwd((char*)workspace + head, make_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, num_adapters, rank), T,
+                                    H, V, vc);
+  ab.call.ids = adapter_ids;
+  ab.dA = (uint16_t*)d_lora_a, ab.dB = (uint16_t*)d_lora_b;
+  return bwd_entry(hidden, ld_hidden, weight, ld_weight, labels, row_lse, row_pz, dlogprobs, dentropy, T, H, V, rcp_temperature, d_hidden, nullptr,
+                   SKYRL_DW_FP32, vc, workspace, head, (hipStream_t)stream, true, 1, &ab);
+}
 
 int skyrl_lmhead_bwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels,
                      const float* row_lse, const float* row_pz, const float* dlogprobs, const float* dentropy, int64_t T,

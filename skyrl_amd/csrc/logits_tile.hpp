@@ -199,9 +199,11 @@ static_assert(BN % kTokenGroup == 0, "tiles begin at whole groups");
 // waves side by side along the tokens, panel columns col0 .. + 127 and twice the tokens.  product(a, b, acc) leaves the tile's products in
 // acc, with LDS free and at least NWAVES * NB * 16 * (kDzTokRow + kDzTokBytes) bytes of it, or returns false, which ends the tile; store(v, p)
 // writes one piece.
+// terms(j, acc, x), where it is given: x = the products of token block j and what is added to them (adapters.hpp).
 constexpr int kDzTokRow = WM * 2 + 16, kDzTokBytes = 24;
-template <bool ENTGRAD, int NB, bool SHORT, class Product, class Store>
-__device__ __forceinline__ void dz_tile(const DzArgs& z, int T, int col0, int t0, char* lds, Product product, Store store) {
+struct NoTerms {};
+template <bool ENTGRAD, int NB, bool SHORT, class Product, class Store, class Terms = NoTerms>
+__device__ __forceinline__ void dz_tile(const DzArgs& z, int T, int col0, int t0, char* lds, Product product, Store store, Terms terms = Terms{}) {
   constexpr int WAVE_N = NB * MT;  // tokens per wave
   const uint16_t* __restrict__ W = z.W;
   const uint16_t* __restrict__ Hd = z.Hd;
@@ -324,12 +326,17 @@ __device__ __forceinline__ void dz_tile(const DzArgs& z, int T, int col0, int t0
     constexpr bool RAGGED = decltype(ragged)::value, LABEL = decltype(label)::value;
     const float gs = gs_[j], c0 = c0_[j], c1 = c1_[j], lse2 = lse2_[j];
     const int yrel = yrel_[j];
+    constexpr bool TERMS = !std::is_same<Terms, NoTerms>::value;
+    f32x4 sums[TERMS ? TM : 1];
+    if constexpr (TERMS) terms(j, acc, sums);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       float d[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float x = acc[i][j][r];
+        float x;
+        if constexpr (TERMS) x = sums[i][r];
+        else x = acc[i][j][r];
         const float p = __builtin_amdgcn_exp2f(fmaf(x, scale2, -lse2));
         d[r] = ENTGRAD ? p * fmaf(c1, x, c0) : p * c0;
       }

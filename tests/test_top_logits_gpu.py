@@ -15,7 +15,7 @@ import math
 import pytest
 import torch
 
-from skyrl_amd import _lib, torch_utils as TU
+from skyrl_amd import torch_utils as TU
 
 pytestmark = pytest.mark.gpu
 INF = math.inf
@@ -282,25 +282,6 @@ def test_replays_from_a_graph(cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
-
-
-def test_c_entry_points_refuse_before_a_launch(cuda_device):
-    lib = _lib.load()
-    z, ids = torch.zeros(4, 64, device=cuda_device), torch.zeros(4, 8, dtype=torch.int64, device=cuda_device)
-    p, i = z.data_ptr(), ids.data_ptr()
-
-    def fwd(logits=p, dtype=1, ld=64, labels=i, T=4, V=64, k=2, rcp=1.0, ranks=i, top=p, top_ids=i):
-        return lib.skyrl_logits_top_fwd(logits, dtype, ld, labels, T, V, k, rcp, None, None, None, None, ranks, top, top_ids, None)
-
-    assert [fwd(logits=None), fwd(dtype=2), fwd(ld=63), fwd(labels=None), fwd(T=0), fwd(V=0), fwd(k=65), fwd(k=-1), fwd(V=1 << 31, ld=1 << 31),
-            fwd(rcp=0.0), fwd(rcp=math.nan), fwd(top=None), fwd(top_ids=None), fwd(top_ids=i + 4), fwd(logits=p + 2)] == \
-        [-1, -5, -2, -1, -2, -2, -2, -2, -2, -5, -5, -1, -1, -3, -3]
-
-    def bwd(lse=p, pz=p, g=p, q=None, top_ids=i, dtop=p, k=2, out=p, ldd=64, labels=i):
-        return lib.skyrl_logits_top_bwd(p, 1, 64, labels, lse, pz, g, q, top_ids, dtop, 4, 64, k, 1.0, out, ldd, None)
-
-    assert [bwd(lse=None), bwd(g=None, dtop=None), bwd(q=p, pz=None), bwd(top_ids=None), bwd(out=None), bwd(ldd=63), bwd(k=129), bwd(out=p + 256),
-            bwd(labels=None), bwd(out=p + 2)] == [-1, -1, -1, -1, -1, -2, -2, -5, -1, -3]
 
 
 def test_refusals_of_the_python_entry_point(cuda_device):
