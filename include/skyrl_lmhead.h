@@ -514,9 +514,12 @@ int skyrl_lmhead_adapter_bwd(const void* hidden, int64_t ld_hidden, const void* 
  * and dtop (fp32 [T, k]) may each be NULL, not all three; alternatives outside [0, V) have no term.  dlogits as in skyrl_logits_bwd.  Every
  * result is the same bits on each call. */
 #define SKYRL_LOGITS_TOP_MAX 128
+/* Scratch of skyrl_logits_top_fwd, 8-byte aligned: rows of a call with few of them are cut in parts whose results are joined.  0: none is needed
+ * (or an extent is out of range). */
+size_t skyrl_logits_top_workspace_bytes(int64_t T, int64_t V, int64_t k);
 int skyrl_logits_top_fwd(const void* logits, int logits_dtype, int64_t ld_logits, const int64_t* labels, int64_t T, int64_t V, int64_t k,
                          float rcp_temperature, float* logprobs, float* entropy, float* row_lse, float* row_pz, int64_t* ranks,
-                         float* top_logprobs, int64_t* top_ids, void* stream);
+                         float* top_logprobs, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
 int skyrl_logits_top_bwd(const void* logits, int logits_dtype, int64_t ld_logits, const int64_t* labels, const float* row_lse,
                          const float* row_pz, const float* dlogprobs, const float* dentropy, const int64_t* top_ids, const float* dtop,
                          int64_t T, int64_t V, int64_t k, float rcp_temperature, void* dlogits, int64_t ld_dlogits, void* stream);

@@ -119,7 +119,8 @@ SIGNATURES = {
         ctypes.c_int,
         [_c_p, ctypes.c_int, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_i64, _c_p]),
     "skyrl_logits_top_fwd": (
-        ctypes.c_int, [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float] + [_c_p] * 8),
+        ctypes.c_int, [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float] + [_c_p] * 8 + [ctypes.c_size_t, _c_p]),
+    "skyrl_logits_top_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64]),
     "skyrl_logits_top_bwd": (
         ctypes.c_int,
         [_c_p, ctypes.c_int, _c_i64] + [_c_p] * 7 + [_c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_i64, _c_p]),

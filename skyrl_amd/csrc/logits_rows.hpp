@@ -23,9 +23,8 @@ template <bool F32>
 struct Piece {
   static constexpr int kElems = F32 ? 4 : 8;
   float v[kElems];
-  __device__ __forceinline__ void load(const void* p) {
-    const uint4 raw = *(const uint4*)p;
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  __device__ __forceinline__ void load(const void* p) { widen(*(const u32x4*)p); }
+  __device__ __forceinline__ void widen(const u32x4& w) {
     if (F32) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);

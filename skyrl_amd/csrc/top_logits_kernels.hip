@@ -9,11 +9,13 @@
 // the k best are one set whatever order candidates are found in.
 // A row without any logit above -inf has lse = -inf: log-probabilities -inf, entropy 0, zero gradient, columns 0 .. k - 1.
 //
-// Selection.  A candidate must reach the k-th largest of the maxima of 128 groups of lanes: those are 128 different logits of the row, so at
-// least k logits reach it, and hardly more do (128 ln 1 / (1 - k / 128): 22 for k = 20, 37 for k = 32).  The bound is formed from the
-// first 16 KiB pieces of a row before any of them is looked at, and again whenever the part of the row that has been seen doubles, so
-// that a row has about k (1 + ln(V / 16384)) candidates; a piece without one costs a comparison and a vote.  The same with the rank: only pieces that
-// reach the label's logit are counted in.
+// Selection.  A candidate must reach the k-th largest of the maxima of 128 groups of lanes: those are 128 different logits, so at least k
+// logits reach it, and hardly more do (-128 ln(1 - k / 128): 22 for k = 20, 37 for k = 32).  The bound is formed from the first 16 KiB pieces
+// before any of them is looked at, and again whenever what has been seen doubles, so that a row has about k (1 + ln(V / 16384)) candidates.
+// The running maximum of the softmax is one value per wave, so that it, the bound and the label's logit (the rank) cost one comparison and
+// vote each per four pieces of a lane; only where a vote says so are the pieces gone through again.
+//
+// Few rows are cut in parts, a workgroup each, whose statistics and k best are joined by a second launch.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -24,7 +26,7 @@ namespace {
 
 using namespace logits;
 
-typedef unsigned long long key_t;
+typedef unsigned long long topkey_t;
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
@@ -43,24 +45,24 @@ __device__ __forceinline__ uint32_t ordered_bits(float z) {
 }
 __device__ __forceinline__ float value_of_bits(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
 // A larger key sorts earlier.
-__device__ __forceinline__ key_t make_key(float z, int column) { return ((key_t)ordered_bits(z) << 32) | (key_t)(uint32_t)(~column); }
-__device__ __forceinline__ int key_column(key_t k) { return (int)(~(uint32_t)k); }
-__device__ __forceinline__ uint32_t key_bits(key_t k) { return (uint32_t)(k >> 32); }
+__device__ __forceinline__ topkey_t make_key(float z, int column) { return ((topkey_t)ordered_bits(z) << 32) | (topkey_t)(uint32_t)(~column); }
+__device__ __forceinline__ int key_column(topkey_t k) { return (int)(~(uint32_t)k); }
+__device__ __forceinline__ uint32_t key_bits(topkey_t k) { return (uint32_t)(k >> 32); }
 
 // LDS operations of a wave execute in order; this keeps the compiler from holding entries that another lane has rewritten.
 __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // The k largest of the n keys (k < n <= kWaveList) of a wave's list to its front, in any order; returns the smallest of them.  A bisection over
 // the key bits on keys held in registers.
-__device__ __noinline__ key_t keep_best(key_t* list, int n, int k) {
+__device__ __noinline__ topkey_t keep_best(topkey_t* list, int n, int k) {
   const int lane = threadIdx.x & 63;
   constexpr int B = kWaveList / 64;
-  key_t x[B];
+  topkey_t x[B];
 #pragma unroll
   for (int u = 0; u < B; ++u) x[u] = u * 64 + lane < n ? list[u * 64 + lane] : 0;  // 0 reaches no trial
-  key_t reach = 0;
+  topkey_t reach = 0;
   for (int b = 63; b >= 0; --b) {
-    const key_t trial = reach | ((key_t)1 << b);
+    const topkey_t trial = reach | ((topkey_t)1 << b);
     int c = 0;
 #pragma unroll
     for (int u = 0; u < B; ++u) c += (int)__popcll(__ballot(x[u] >= trial));
@@ -79,13 +81,24 @@ __device__ __noinline__ key_t keep_best(key_t* list, int n, int k) {
   return reach;
 }
 
+constexpr int kMaxJoin = 2048;  // candidates that the parts of a row bring to the join
+constexpr int kMaxParts = 64;
+
 // What the waves of a workgroup share.
 struct Shared {
   Stats stats[kWaves];
-  key_t list[kWaves][kWaveList];
+  topkey_t list[kWaves][kWaveList];
+  topkey_t all[kWaves * kMaxTop];  // the candidates of all waves, side by side
   float group_max[kGroups];
-  float bound;         // every wave's candidates reach it
+  float bound;  // every wave's candidates reach it
   int count[kWaves], better[kWaves];
+};
+static_assert(kWaves * kMaxTop >= kThreads, "up to a candidate per thread without dropping any");
+
+// A part's result: its statistics, the columns that sort before the label, and how many of its k keys there are, best first.
+struct Part {
+  Stats st;
+  int better, keys;
 };
 
 // A value that at least k of the 128 groups reach, from the first 16 bits of their maxima (exact for bf16); by one wave.
@@ -117,11 +130,56 @@ struct TopArgs {
   int64_t* ranks;
   float* top_logprobs;
   int64_t* top_ids;
+  Part* part;   // [T, parts], and the keys [T, parts, k], where rows are cut
+  topkey_t* keys;
 };
 
-// One workgroup per row.
+// The results of a row from its statistics and the number of columns before the label, by one thread; logprob_of for the alternatives.
+struct RowResult {
+  bool empty;
+  float log_s, m, scale2;
+  __device__ __forceinline__ RowResult(const Stats& st, float scale2_) : empty(st.s == 0.f), m(st.m), scale2(scale2_) {
+    log_s = empty ? -INFINITY : logf(st.s);
+  }
+  __device__ __forceinline__ float logprob_of(float z) const { return empty ? -INFINITY : fmaf(z, scale2, -m) * kLn2 - log_s; }
+  __device__ __forceinline__ void write(const TopArgs& a, int64_t row, const Stats& st, bool has_label, float z_label, int before) const {
+    if (a.ranks) a.ranks[row] = has_label && z_label == z_label ? 1 + before : 0;
+    if (a.logprobs) a.logprobs[row] = has_label ? logprob_of(z_label) : 0.f;
+    if (a.entropy) a.entropy[row] = empty ? 0.f : log_s - st.e / st.s * kLn2;
+    if (a.row_lse) a.row_lse[row] = empty ? -INFINITY : fmaf(st.m, kLn2, log_s);
+    if (a.row_pz) a.row_pz[row] = empty ? 0.f : (st.e / st.s + st.m) * kLn2;
+  }
+};
+
+// Where `mine` stands among n keys of LDS.
+__device__ __forceinline__ int place_among(const topkey_t* keys, int n, topkey_t mine) {
+  int place = 0;
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) place += keys[i] > mine ? 1 : 0;
+  return place;
+}
+
+// Fewer logits than k that are numbers (`place` of them): the first NaN columns, in order, by one wave.
 template <bool F32>
-__global__ __launch_bounds__(kThreads) void logits_top_rows(const TopArgs a) {
+__device__ __noinline__ void fill_with_nan(int V, int k, int64_t* ids, float* logprobs, const char* base, int place) {
+  const int lane = threadIdx.x & 63;
+  for (int c0 = 0; c0 < V && place < k; c0 += 64) {
+    const int c = c0 + lane;
+    const float z = c < V ? load_one(base, (size_t)c, F32) : 0.f;
+    const unsigned long long mask = __ballot(z != z);
+    const int at = place + (int)__popcll(mask & ((1ull << lane) - 1));
+    if (z != z && at < k) ids[at] = c, logprobs[at] = NAN;
+    place += (int)__popcll(mask);
+  }
+}
+
+// One workgroup per row and part (PARTS: grid.y of them).
+// Bound by HBM on fp32 logits, by the vector instructions (an exponential, the comparisons, widening) on bf16: 2048 x 152064 fp32, k = 5, 228 us (5.5
+// TB/s); 4096 x 151936 bf16, k = 32, 322 us (3.9 TB/s), of which 36 are the ranks and candidates.  What brought it there from 510: one running maximum
+// a wave and votes per four pieces instead of one (437), keys formed only where a logit reaches the bound (394), no memory for
+// arguments of a call (322).  Loading a step ahead changed nothing (328 to 358): two or three workgroups a CU overlap enough.
+template <bool F32, bool PARTS>
+__global__ __launch_bounds__(kThreads, 6) void logits_top_rows(const TopArgs a) {
   constexpr int E = Piece<F32>::kElems, ES = F32 ? 4 : 2;
   __shared__ Shared sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -131,7 +189,10 @@ __global__ __launch_bounds__(kThreads) void logits_top_rows(const TopArgs a) {
   const float scale2 = a.rcp_temp * kLog2e;
   const RowPieces rp = row_pieces<F32>(base, V, true);
   const char* vec = base + (size_t)rp.head * ES;
-  const int pieces = rp.pieces;
+  const int part = PARTS ? blockIdx.y : 0, parts = PARTS ? gridDim.y : 1;
+  const int first = PARTS ? (int)((int64_t)rp.pieces * part / parts) : 0;
+  const int pieces = PARTS ? (int)((int64_t)rp.pieces * (part + 1) / parts) : rp.pieces;  // where the part ends
+  const int single = part == 0 ? rp.single : 0;
 
   int64_t label = a.labels ? a.labels[row] : (int64_t)-1;
   const bool has_label = label >= 0 && label < (int64_t)V;
@@ -139,17 +200,19 @@ __global__ __launch_bounds__(kThreads) void logits_top_rows(const TopArgs a) {
   const int y = has_label ? (int)label : -1;
   const float above_label = next_above(z_label);  // NaN (no label, or its logit is NaN): nothing reaches it
 
-  Stats st{kLowest, 0.f, 0.f};
+  Stats st{kLowest, 0.f, 0.f};  // the maximum is the wave's
   float lane_max = -INFINITY;
   int better = 0;       // columns of this lane that sort before the label
   int count = 0;        // candidates in the wave's list
-  key_t least = 0;      // candidates have larger keys: the worst of k that the wave has seen
+  topkey_t least = 0;      // candidates have larger keys: the worst of k that the wave has seen
   float bound = -INFINITY;
-  key_t* const list = sm.list[wave];
+  topkey_t* const list = sm.list[wave];
 
   auto append = [&](float z, int column, bool there) {
-    const key_t key = make_key(z, column);
-    const bool hit = there && z >= bound && key > least;
+    const bool reaches = there && z >= bound;
+    if (!__any(reaches)) return;  // by far the most often: the key is formed behind this
+    const topkey_t key = make_key(z, column);
+    const bool hit = reaches && key > least;
     const unsigned long long mask = __ballot(hit);
     if (mask == 0) return;
     if (hit) list[count + __popcll(mask & ((1ull << lane) - 1))] = key;
@@ -166,20 +229,21 @@ __global__ __launch_bounds__(kThreads) void logits_top_rows(const TopArgs a) {
     m = fmaxf(m, __shfl_xor(m, 2, 64));
     if ((lane & 3) == 0) sm.group_max[wave * kGroupsPerWave + (lane >> 2)] = m;
   };
-  // rank: columns in front of the label's precede it with an equal logit already
-  auto count_better = [&](float z, int column) {
-    better += z >= above_label || (z == z_label && column < y) ? 1 : 0;
+  auto raise_wave_max = [&](float z) {  // to the largest z of the wave
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) z = fmaxf(z, __shfl_xor(z, o, 64));
+    raise_max(st, z * scale2);
   };
 
   int step = 0;
-  for (int p0 = tid; p0 - tid < pieces; p0 += kThreads * kInFlight, ++step) {
+  for (int p0 = first + tid; p0 - tid < pieces; p0 += kThreads * kInFlight, ++step) {
     Piece<F32> pc[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       const int p = p0 + u * kThreads;
       pc[u].load(vec + (size_t)(p < pieces ? p : pieces - 1) * 16);
     }
-    float mx[kInFlight];
+    float mx[kInFlight], top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       mx[u] = -INFINITY;
@@ -187,118 +251,177 @@ __global__ __launch_bounds__(kThreads) void logits_top_rows(const TopArgs a) {
 #pragma unroll
         for (int i = 0; i < E; ++i) mx[u] = fmaxf(mx[u], pc[u].v[i]);
       }
-      lane_max = fmaxf(lane_max, mx[u]);
+      top = fmaxf(top, mx[u]);
     }
-    if (k > 0 && (step & (step + 1)) == 0) {  // steps 0, 1, 3, 7: what has been seen doubles
-      publish();
-      if (step == 0) {
-        __syncthreads();
-        if (wave == 0) {
+    lane_max = fmaxf(lane_max, top);
+    if (__any(top * scale2 > st.m)) raise_wave_max(top);
+    if (k > 0) {
+      if ((step & (step + 1)) == 0) {  // steps 0, 1, 3, 7: what has been seen doubles
+        publish();
+        if (step == 0) {
+          __syncthreads();
+          if (wave == 0) {
+            const float b = group_bound(sm.group_max, k);
+            if (lane == 0) sm.bound = b;
+          }
+          __syncthreads();
+        } else if (wave == (step & (kWaves - 1))) {  // whatever the other waves have published: a bound all the same
+          wave_fence();
           const float b = group_bound(sm.group_max, k);
-          if (lane == 0) sm.bound = b;
+          if (lane == 0) *(volatile float*)&sm.bound = fmaxf(*(volatile float*)&sm.bound, b);
         }
-        __syncthreads();
-      } else if (wave == (step & (kWaves - 1))) {  // whatever the other waves have published: a bound all the same
-        wave_fence();
-        const float b = group_bound(sm.group_max, k);
-        if (lane == 0) *(volatile float*)&sm.bound = fmaxf(*(volatile float*)&sm.bound, b);
       }
+      bound = fmaxf(bound, *(volatile float*)&sm.bound);
     }
-    if (k > 0) bound = fmaxf(bound, *(volatile float*)&sm.bound);
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      const int p = p0 + u * kThreads;
-      const bool there = p < pieces;
-      if (__any(mx[u] * scale2 > st.m)) raise_max(st, mx[u] * scale2);
-      if (there) {
+      if (p0 + u * kThreads < pieces) {
 #pragma unroll
         for (int i = 0; i < E; ++i) absorb<true>(st, pc[u].v[i], scale2);
       }
-      const int c0 = rp.head + p * E;
-      if (__any(mx[u] >= z_label)) {
+    }
+    if (__any(top >= z_label)) {
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (there) count_better(pc[u].v[i], c0 + i);
+      for (int u = 0; u < kInFlight; ++u) {
+        const int p = p0 + u * kThreads, c0 = rp.head + p * E;
+        if (p < pieces) {
+          // columns in front of the label's precede it with an equal logit already
+          const float reach = c0 + E <= y ? z_label : above_label;
+#pragma unroll
+          for (int i = 0; i < E; ++i) better += pc[u].v[i] >= reach ? 1 : 0;
+          if (c0 < y && y < c0 + E) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) better += c0 + i < y && pc[u].v[i] == z_label ? 1 : 0;
+          }
+        }
       }
-      if (k > 0 && __any(mx[u] >= bound)) {
+    }
+    if (k > 0 && __any(top >= bound)) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) append(pc[u].v[i], c0 + i, there);
+      for (int u = 0; u < kInFlight; ++u) {
+        const int p = p0 + u * kThreads;
+        if (!__any(mx[u] >= bound)) continue;
+#pragma unroll
+        for (int i = 0; i < E; ++i) append(pc[u].v[i], rp.head + p * E + i, p < pieces);
       }
     }
   }
-  for (int i0 = 0; i0 < rp.single; i0 += kThreads) {
+  for (int i0 = 0; i0 < single; i0 += kThreads) {
     const int i = i0 + tid;
-    const bool there = i < rp.single;
+    const bool there = i < single;
     const int c = single_column(rp, E, there ? i : 0);
     const float z = load_one(base, (size_t)c, F32);
+    raise_wave_max(there ? z : -INFINITY);
     if (there) {
-      raise_max(st, z * scale2);
       absorb<true>(st, z, scale2);
-      count_better(z, c);
+      better += z >= above_label || (z == z_label && c < y) ? 1 : 0;
     }
     if (k > 0) append(z, c, there);
   }
 
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) better += __shfl_xor(better, o, 64);
+  if (count > k && k > 0 && __builtin_amdgcn_readfirstlane(count) > kThreads / kWaves) {  // so that all fit behind each other
+    (void)keep_best(list, count, k);
+    count = k;
+  }
   if (lane == 0) sm.count[wave] = count, sm.better[wave] = better;
   st = block_merge<kWaves>(st, sm.stats);  // a barrier: the lists and counts of all waves stand
-  const bool empty = st.s == 0.f;
-  const float log_s = empty ? -INFINITY : logf(st.s);
-  auto logprob_of = [&](float z) { return empty ? -INFINITY : fmaf(z, scale2, -st.m) * kLn2 - log_s; };
+  const RowResult result(st, scale2);
+  int total = 0, before = 0, mine_at = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w == wave) mine_at = total;
+    total += sm.count[w], before += sm.better[w];
+  }
   if (tid == 0) {
-    int before = 0;
-    for (int w = 0; w < kWaves; ++w) before += sm.better[w];
-    if (a.ranks) a.ranks[row] = has_label && z_label == z_label ? 1 + before : 0;
-    if (a.logprobs) a.logprobs[row] = has_label ? logprob_of(z_label) : 0.f;
-    if (a.entropy) a.entropy[row] = empty ? 0.f : log_s - st.e / st.s * kLn2;
-    if (a.row_lse) a.row_lse[row] = empty ? -INFINITY : fmaf(st.m, kLn2, log_s);
-    if (a.row_pz) a.row_pz[row] = empty ? 0.f : (st.e / st.s + st.m) * kLn2;
+    if (PARTS) a.part[row * parts + part] = Part{st, before, total < k ? total : k};
+    else result.write(a, row, st, has_label, z_label, before);
   }
   if (k == 0) return;
-
-  // The place of a candidate among the k best is the number of better ones: every thread takes one of all lists' candidates.
-  int total = 0;
-  for (int w = 0; w < kWaves; ++w) total += sm.count[w];
-  if (total > kThreads) {  // the same for the whole workgroup
-    __syncthreads();  // every wave has read the counts
-    if (count > k) {
-      (void)keep_best(list, count, k);
-      if (lane == 0) sm.count[wave] = k;
-    }
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < kWaves; ++w) total += sm.count[w];
-  }
-  for (int e0 = 0; e0 < total; e0 += kThreads) {
-    int e = e0 + tid, w = 0;
-    while (w < kWaves && e >= sm.count[w]) e -= sm.count[w], ++w;
-    if (w < kWaves) {
-      const key_t mine = sm.list[w][e];
-      int place = 0;
-      for (int v = 0; v < kWaves && place < k; ++v)
-        for (int i = 0; i < sm.count[v]; ++i) place += sm.list[v][i] > mine ? 1 : 0;
-      if (place < k) {
+  for (int e = lane; e < count; e += 64) sm.all[mine_at + e] = list[e];
+  __syncthreads();
+  // The place of a candidate is the number of better ones.
+  for (int e = tid; e < total; e += kThreads) {
+    const topkey_t mine = sm.all[e];
+    const int place = place_among(sm.all, total, mine);
+    if (place < k) {
+      if (PARTS) {
+        a.keys[(row * parts + part) * (int64_t)k + place] = mine;
+      } else {
         a.top_ids[row * (int64_t)k + place] = key_column(mine);
-        a.top_logprobs[row * (int64_t)k + place] = logprob_of(value_of_bits(key_bits(mine)));
+        a.top_logprobs[row * (int64_t)k + place] = result.logprob_of(value_of_bits(key_bits(mine)));
       }
     }
   }
-  // Fewer logits than k that are numbers: the first NaN columns, in order, by one wave.
-  if (total < k && wave == 0) {
-    int place = total;
-    for (int c0 = 0; c0 < V && place < k; c0 += 64) {
-      const int c = c0 + lane;
-      const float z = c < V ? load_one(base, (size_t)c, F32) : 0.f;
-      const unsigned long long mask = __ballot(z != z);
-      const int at = place + (int)__popcll(mask & ((1ull << lane) - 1));
-      if (z != z && at < k) {
-        a.top_ids[row * (int64_t)k + at] = c;
-        a.top_logprobs[row * (int64_t)k + at] = NAN;
-      }
-      place += (int)__popcll(mask);
+  if (!PARTS && total < k && wave == 0) fill_with_nan<F32>(V, k, a.top_ids + row * (int64_t)k, a.top_logprobs + row * (int64_t)k, base, total);
+}
+
+// Joins the parts of a row.  The k best of the parts' first ceil(k / parts) keys give a bound that few keys of a row reach; those find their
+// places.
+constexpr int kJoinThreads = 256;
+template <bool F32>
+__global__ __launch_bounds__(kJoinThreads) void logits_top_join(const TopArgs a, int parts) {
+  __shared__ topkey_t keys[kMaxJoin];
+  __shared__ topkey_t firsts[kMaxTop + kMaxParts];
+  __shared__ topkey_t bound;
+  __shared__ int have[kMaxParts], kept;
+  const int tid = threadIdx.x, k = a.k;
+  const int64_t row = blockIdx.x;
+  const char* base = (const char*)a.logits + (size_t)row * (size_t)a.ld * (F32 ? 4 : 2);
+  const int each = k > 0 ? (k + parts - 1) / parts : 0;
+  // Every wave joins the statistics for itself, a part a lane.
+  const int lane = tid & 63;
+  Part q{{kLowest, 0.f, 0.f}, 0, 0};
+  if (lane < parts) q = a.part[row * parts + lane];
+  Stats st = q.st;
+  int before = q.better, found = q.keys;
+  if (tid < kMaxParts) have[tid] = q.keys;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    Stats other;
+    other.m = __shfl_xor(st.m, o, 64), other.s = __shfl_xor(st.s, o, 64), other.e = __shfl_xor(st.e, o, 64);
+    merge(st, other);
+    before += __shfl_xor(before, o, 64), found += __shfl_xor(found, o, 64);
+  }
+  // Lane 0's for all: the lanes' sums differ in their last bits, and which lane writes an alternative below is not fixed.
+  auto of_lane_0 = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
+  st = Stats{of_lane_0(st.m), of_lane_0(st.s), of_lane_0(st.e)};
+  if (tid == 0) bound = 0, kept = 0;
+  __syncthreads();
+  for (int e = tid; e < parts * each; e += kJoinThreads) {
+    const int p = e / each, i = e - p * each;
+    firsts[e] = i < have[p] ? a.keys[(row * parts + p) * (int64_t)k + i] : 0;
+  }
+  const RowResult result(st, a.rcp_temp * kLog2e);
+  if (tid == 0) {
+    const int64_t label = a.labels ? a.labels[row] : (int64_t)-1;
+    const bool has_label = label >= 0 && label < (int64_t)a.V;
+    result.write(a, row, st, has_label, has_label ? load_one(base, (size_t)label, F32) : NAN, before);
+  }
+  if (k == 0) return;
+  __syncthreads();
+  for (int e = tid; e < parts * each; e += kJoinThreads) {
+    const topkey_t mine = firsts[e];
+    if (mine != 0 && place_among(firsts, parts * each, mine) == k - 1) bound = mine;  // at most one: keys differ
+  }
+  __syncthreads();
+  const topkey_t least = bound;  // 0 where the firsts have fewer than k keys: everything is kept
+  for (int e = tid; e < parts * k; e += kJoinThreads) {
+    const int p = e / k, i = e - p * k;
+    const topkey_t key = i < have[p] ? a.keys[(row * parts + p) * (int64_t)k + i] : 0;
+    if (key != 0 && key >= least) keys[atomicAdd(&kept, 1)] = key;  // in any order: places depend on the keys alone
+  }
+  __syncthreads();
+  const int n = kept;
+  for (int e = tid; e < n; e += kJoinThreads) {
+    const topkey_t mine = keys[e];
+    const int place = place_among(keys, n, mine);
+    if (place < k) {
+      a.top_ids[row * (int64_t)k + place] = key_column(mine);
+      a.top_logprobs[row * (int64_t)k + place] = result.logprob_of(value_of_bits(key_bits(mine)));
     }
   }
+  if (found < k && tid < 64) fill_with_nan<F32>(a.V, k, a.top_ids + row * (int64_t)k, a.top_logprobs + row * (int64_t)k, base, found);
 }
 
 // The gradient.  As logits_bwd_rows (logits_kernels.hip), with sum_j h_j in the coefficient of p, and the k + 1 columns that have a term of their
@@ -426,23 +549,50 @@ int check_top(int64_t V, int64_t k) {
   return k < 0 || k > V || k > kMaxTop ? SKYRL_LMHEAD_ERR_SHAPE : SKYRL_LMHEAD_OK;
 }
 
+// Parts of a row: so many that 1024 workgroups, four a CU, share the logits, of at least 8192 logits each.
+int top_parts(int64_t T, int64_t V, int64_t k) {
+  int64_t n = 1024 / T;
+  if (n > V / 8192) n = V / 8192;
+  if (n > kMaxParts) n = kMaxParts;
+  if (k > 0 && n > kMaxJoin / k) n = kMaxJoin / k;
+  return n < 1 ? 1 : (int)n;
+}
+
 }  // namespace
 
 extern "C" {
 
+size_t skyrl_logits_top_workspace_bytes(int64_t T, int64_t V, int64_t k) {
+  if (T < 1 || V < 1 || T >= kMaxRows || V >= ((int64_t)1 << 31) || check_top(V, k)) return 0;
+  const size_t parts = (size_t)top_parts(T, V, k);
+  return parts == 1 ? 0 : (size_t)T * parts * (sizeof(Part) + (size_t)k * sizeof(topkey_t)) + 8;
+}
+
 int skyrl_logits_top_fwd(const void* logits, int logits_dtype, int64_t ld_logits, const int64_t* labels, int64_t T, int64_t V, int64_t k,
                          float rcp_temperature, float* logprobs, float* entropy, float* row_lse, float* row_pz, int64_t* ranks,
-                         float* top_logprobs, int64_t* top_ids, void* stream) {
+                         float* top_logprobs, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
   int st = check_logits(logits, logits_dtype, ld_logits, T, V, rcp_temperature);
   if (st) return st;
   if ((st = check_top(V, k))) return st;
   if ((logprobs || ranks) && !labels) return SKYRL_LMHEAD_ERR_NULL;
   if (k > 0 && (!top_logprobs || !top_ids)) return SKYRL_LMHEAD_ERR_NULL;
   if (k == 0 && !logprobs && !entropy && !row_lse && !row_pz && !ranks) return SKYRL_LMHEAD_ERR_NULL;
-  if (((uintptr_t)labels | (uintptr_t)ranks | (uintptr_t)top_ids) & 7u) return SKYRL_LMHEAD_ERR_ALIGN;
-  const TopArgs a{logits, ld_logits, labels, (int)V, (int)k, rcp_temperature, logprobs, entropy, row_lse, row_pz, ranks, top_logprobs, top_ids};
-  hipLaunchKernelGGL(logits_dtype == SKYRL_LOGITS_F32 ? logits_top_rows<true> : logits_top_rows<false>, dim3((unsigned)T), dim3(kThreads), 0,
-                     (hipStream_t)stream, a);
+  if (((uintptr_t)labels | (uintptr_t)ranks | (uintptr_t)top_ids | (uintptr_t)workspace) & 7u) return SKYRL_LMHEAD_ERR_ALIGN;
+  const size_t need = skyrl_logits_top_workspace_bytes(T, V, k);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  const int parts = top_parts(T, V, k);
+  const bool f32 = logits_dtype == SKYRL_LOGITS_F32;
+  topkey_t* const keys = (topkey_t*)workspace;
+  const TopArgs a{logits, ld_logits, labels, (int)V, (int)k, rcp_temperature, logprobs, entropy, row_lse, row_pz, ranks, top_logprobs, top_ids,
+                  (Part*)(keys + (size_t)T * (size_t)parts * (size_t)k), keys};
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)T, (unsigned)parts), block(kThreads);
+  if (parts == 1) {
+    hipLaunchKernelGGL((f32 ? logits_top_rows<true, false> : logits_top_rows<false, false>), grid, block, 0, s, a);
+  } else {
+    hipLaunchKernelGGL((f32 ? logits_top_rows<true, true> : logits_top_rows<false, true>), grid, block, 0, s, a);
+    hipLaunchKernelGGL(f32 ? logits_top_join<true> : logits_top_join<false>, dim3((unsigned)T), dim3(kJoinThreads), 0, s, a, parts);
+  }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SKYRL_LMHEAD_OK : (int)e;
 }

@@ -25,7 +25,7 @@ from typing import Any, NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from ._launch import call, device_guard, raw_stream, registered_op
+from ._launch import call, device_guard, plain_eager, raw_stream, registered_op
 from .ops import _require_device as _require_device_all
 
 __all__ = ["logprobs_from_logits", "logprobs_from_logits_v2", "logprobs_from_logits_flash_attn", "chunked_entropy_from_logits",
@@ -255,11 +255,8 @@ def _check_k(k: int, V: int) -> None:
         raise ValueError(f"k must lie between 0 and min(vocabulary, {MAX_ALTERNATIVES}) = {min(V, MAX_ALTERNATIVES)}, got {k}")
 
 
-@registered_op("skyrl_amd::logits_top_fwd", mutates_args=())
-def logits_top_fwd(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int, rcp_temperature: float
-                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(logprobs, entropy, row_lse, row_pz, ranks, top_logprobs, top_ids)`` of ``logits [T, V] * rcp_temperature``; fp32 ``[T]``,
-    int64 ``[T]`` and ``[T, k]``.  Without ``labels`` log-probabilities and ranks are zero."""
+def _top_fwd(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int, rcp_temperature: float, want_rows: bool) -> tuple:
+    """The seven results of ``logits_top_fwd``; ``row_lse`` and ``row_pz``, which only a backward needs, are ``None`` unless they are wanted."""
     T, V, pieces = _pieces(logits)
     dev = _require_device(logits, labels)
     _check_rows("labels", labels, T, torch.int64)
@@ -268,7 +265,8 @@ def logits_top_fwd(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int,
     f32, i64 = dict(dtype=torch.float32, device=dev), dict(dtype=torch.int64, device=dev)
     made = torch.empty if labels is not None else torch.zeros
     lp, ranks = made(T, **f32), made(T, **i64)
-    ent, lse, pz = torch.empty(T, **f32), torch.empty(T, **f32), torch.empty(T, **f32)
+    ent = torch.empty(T, **f32)
+    lse, pz = (torch.empty(T, **f32), torch.empty(T, **f32)) if want_rows else (None, None)
     top, ids = torch.empty((T, k), **f32), torch.empty((T, k), **i64)
     if T == 0:
         return lp, ent, lse, pz, ranks, top, ids
@@ -277,12 +275,23 @@ def logits_top_fwd(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int,
         stream = raw_stream(dev)
         for view, r0 in pieces:
             rows, _, ld = _rows(view)
-            at = lambda t, size: t.data_ptr() + size * r0  # noqa: E731
-            st = lib.skyrl_logits_top_fwd(view.data_ptr(), _DTYPES[logits.dtype], ld, None if labels is None else at(labels, 8), rows, V, k,
-                                          float(rcp_temperature), None if labels is None else at(lp, 4), at(ent, 4), at(lse, 4), at(pz, 4),
-                                          None if labels is None else at(ranks, 8), at(top, 4 * k), at(ids, 8 * k), stream)
+            at = lambda t, size: None if t is None else t.data_ptr() + size * r0  # noqa: E731
+            nbytes = lib.skyrl_logits_top_workspace_bytes(rows, V, k) if rows < 1024 else 0  # longer runs need none
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            st = lib.skyrl_logits_top_fwd(view.data_ptr(), _DTYPES[logits.dtype], ld, at(labels, 8), rows, V, k, float(rcp_temperature),
+                                          None if labels is None else at(lp, 4), at(ent, 4), at(lse, 4), at(pz, 4),
+                                          None if labels is None else at(ranks, 8), at(top, 4 * k), at(ids, 8 * k),
+                                          None if ws is None else ws.data_ptr(), nbytes, stream)
             _lib.check(st, "skyrl_logits_top_fwd")
     return lp, ent, lse, pz, ranks, top, ids
+
+
+@registered_op("skyrl_amd::logits_top_fwd", mutates_args=())
+def logits_top_fwd(logits: torch.Tensor, labels: Optional[torch.Tensor], k: int, rcp_temperature: float
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(logprobs, entropy, row_lse, row_pz, ranks, top_logprobs, top_ids)`` of ``logits [T, V] * rcp_temperature``; fp32 ``[T]``,
+    int64 ``[T]`` and ``[T, k]``.  Without ``labels`` log-probabilities and ranks are zero."""
+    return _top_fwd(logits, labels, k, rcp_temperature, True)
 
 
 @logits_top_fwd.register_fake
@@ -375,8 +384,13 @@ def top_logprobs_from_logits(logits: torch.Tensor, labels: Optional[torch.Tensor
         if labels.shape != shape:
             raise ValueError(f"labels {tuple(labels.shape)} do not match logits {tuple(logits.shape)}")
         labels = labels.reshape(-1).to(torch.int64).contiguous()
-    k = min(k, V)
-    lp, ent, ranks, top, ids = _TopFromLogits.apply(_flat(logits), labels, k, 1.0 / temperature)
+    k, flat = min(k, V), _flat(logits)
+    if torch.is_grad_enabled() and flat.requires_grad or not plain_eager() or type(flat) not in (torch.Tensor, torch.nn.Parameter):
+        lp, ent, ranks, top, ids = _TopFromLogits.apply(flat, labels, k, 1.0 / temperature)
+    else:  # nothing follows the call: without autograd's function and what only a backward reads
+        lp, ent, _, _, ranks, top, ids = _top_fwd(flat, labels, k, 1.0 / temperature, False)
+    if len(shape) == 1:
+        return TokenLogprobs(lp, ent, ranks, top, ids)
     return TokenLogprobs(lp.reshape(shape), ent.reshape(shape), ranks.reshape(shape), top.reshape(shape + (k,)), ids.reshape(shape + (k,)))
 
 

@@ -81,12 +81,18 @@ def test_other_arguments_are_checked_before_a_launch():
 def test_top_arguments_are_checked_before_a_launch():
     lib = _lib.load()
 
-    def fwd(logits=P, dtype=1, ld=64, labels=P, T=4, V=64, k=2, rcp=1.0, ranks=P, top=P, top_ids=P):
-        return lib.skyrl_logits_top_fwd(logits, dtype, ld, labels, T, V, k, rcp, None, None, None, None, ranks, top, top_ids, None)
+    def fwd(logits=P, dtype=1, ld=64, labels=P, T=4, V=64, k=2, rcp=1.0, ranks=P, top=P, top_ids=P, ws=None, nbytes=0):
+        return lib.skyrl_logits_top_fwd(logits, dtype, ld, labels, T, V, k, rcp, None, None, None, None, ranks, top, top_ids, ws, nbytes, None)
 
     assert [fwd(logits=None), fwd(dtype=2), fwd(ld=63), fwd(labels=None), fwd(T=0), fwd(V=0), fwd(k=65), fwd(k=-1), fwd(V=1 << 31, ld=1 << 31),
             fwd(rcp=0.0), fwd(rcp=math.nan), fwd(top=None), fwd(top_ids=None), fwd(top_ids=P + 4), fwd(logits=P + 2)] == \
         [NULL, ARG, SHAPE, NULL, SHAPE, SHAPE, SHAPE, SHAPE, SHAPE, ARG, ARG, NULL, NULL, ALIGN, ALIGN]
+    need = lib.skyrl_logits_top_workspace_bytes(4, 152064, 20)
+    assert 4 * 18 * 20 * 8 < need < 4 * 64 * 20 * 8 and lib.skyrl_logits_top_workspace_bytes(4096, 152064, 20) == 0
+    assert [fwd(ld=152064, V=152064, k=20), fwd(ld=152064, V=152064, k=20, ws=P, nbytes=need - 1), fwd(ld=152064, V=152064, k=20, ws=P + 4, nbytes=need)] == \
+        [WORKSPACE, WORKSPACE, ALIGN]
+    for T, V, k in ((0, 64, 2), (4, 0, 0), (4, 64, 65), (4, 64, 129), (1 << 40, 64, 2), (4, 1 << 40, 2)):
+        assert lib.skyrl_logits_top_workspace_bytes(T, V, k) == 0
 
     def bwd(lse=P, pz=P, g=P, q=None, top_ids=P, dtop=P, k=2, out=P + 4096, ldd=64, labels=P):
         return lib.skyrl_logits_top_bwd(P, 1, 64, labels, lse, pz, g, q, top_ids, dtop, 4, 64, k, 1.0, out, ldd, None)

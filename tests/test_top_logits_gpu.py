@@ -254,6 +254,12 @@ def test_same_bits_on_each_call_and_on_another_stream(cuda_device):
         again = TU.top_logprobs_from_logits(d, y, 20)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+    for T, V, dtype in ((64, 151936, torch.float32), (1500, 30000, torch.bfloat16)):
+        logits, labels, _ = make(T, V, dtype, 4)
+        d, y = logits.to(cuda_device), labels.to(cuda_device)
+        first = TU.top_logprobs_from_logits(d, y, 20)
+        for _ in range(5):
+            assert all(torch.equal(a, b) for a, b in zip(first, TU.top_logprobs_from_logits(d, y, 20)))
 
 
 def test_replays_from_a_graph(cuda_device):
