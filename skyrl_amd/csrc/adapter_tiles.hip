@@ -3,16 +3,8 @@
 #include "adapters.hpp"
 #include "half_tile.hpp"
 
-#include <type_traits>
-#include <utility>
-
 namespace lmhead {
 namespace {
-
-template <class F, int... I>
-__device__ __forceinline__ void for_each(std::integer_sequence<int, I...>, F f) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
 
 // f(shape, v0): the tile of that shape from vocabulary row v0 on, for the workgroup's tile t.
 template <bool SHAPES, class F>
@@ -29,49 +21,56 @@ __device__ __forceinline__ void tile_of_shape(const Tile& t, int T, F f) {
   f(std::integral_constant<int, kSquare>{}, t.tm * BM);
 }
 
+// tile_product() with the loads of the first adapter's rows and of the first block's u between its first copies and the mainloop, which hides
+// them: behind the mainloop they cost every tile a trip to memory.
+template <int SHAPE, bool EVEN, class Terms>
+__device__ __forceinline__ void tile_product_and_start(const Operand& a, const Operand& b, int nk, char* lds, f32x4 (&acc)[TM][wave_cols(SHAPE)],
+                                                       Terms& terms) {
+  prefetch_first_tiles<false, SHAPE>(a, b, 0, nk, lds);
+  terms.start();
+  zero_acc(acc);
+  if constexpr (SHAPE == kSquare) mainloop<false, EVEN>(a, b, 0, nk, lds, acc);
+  else mainloop_ksteps<false, SHAPE>(a, b, 0, nk, lds, acc);
+}
+
 // Statistics of a wave's sums, as fwd_epilogue() (logits_tile.hpp) makes them of its accumulators.
-template <int NB, bool HOLD>
-__device__ __forceinline__ void fwd_stats(f32x4 (&acc)[TM][NB], AdapterTerms<NB, HOLD>& terms, const AdapterFwdArgs& a, int part, int nparts) {
+template <int NB>
+__device__ __forceinline__ void fwd_stats(f32x4 (&acc)[TM][NB], AdapterTerms<NB>& terms, const AdapterFwdArgs& a, int part, int nparts) {
   const int lane = threadIdx.x & 63, lrow = lane & 15, kq = lane >> 4;
   const int vbase = part * WM;
   const float scale2 = a.rcp_temp * kLog2e;
   const int rows_kind = __builtin_amdgcn_readfirstlane(vbase + WM <= a.V ? 0 : (vbase < a.V ? 1 : 2));
-  auto token_blocks = [&](auto kind) {
-    constexpr int KIND = decltype(kind)::value;
+  for_each_int(std::make_integer_sequence<int, NB>{}, [&](auto block) {
+    constexpr int j = decltype(block)::value;
+    const int t = terms.t0 + j * MT + lrow;
+    float m = -INFINITY, s = 0.f, e = 0.f;
+    f32x4 z[TM][1];
+    {
+      f32x4 x[TM];
+      terms.block(j, acc, x);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int t = terms.t0 + j * MT + lrow;
-      float m = -INFINITY, s = 0.f, e = 0.f;
-      if constexpr (KIND < 2) {
-        f32x4 z[TM][1];
-        f32x4 x[TM];
-        terms.block(j, acc, x);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) z[i][0] = x[i];
-        fwd_tile_stats<true, KIND == 1, false>(z, 0, vbase, a.V, scale2, kq, m, s, e);
-      }
-      if (kq == 0 && t < a.T) {
-        const size_t idx = part_index(part, t, nparts);
-        a.part_max[idx] = m;
-        a.part_sum[idx] = s;
-        a.part_pz[idx] = e;
-      }
+      for (int i = 0; i < TM; ++i) z[i][0] = x[i];
     }
-  };
-  if (rows_kind == 0) token_blocks(std::integral_constant<int, 0>{});
-  else if (rows_kind == 1) token_blocks(std::integral_constant<int, 1>{});
-  else token_blocks(std::integral_constant<int, 2>{});
+    if (rows_kind == 0) fwd_tile_stats<true, false, false>(z, 0, vbase, a.V, scale2, kq, m, s, e);
+    else if (rows_kind == 1) fwd_tile_stats<true, true, false>(z, 0, vbase, a.V, scale2, kq, m, s, e);
+    if (kq == 0 && t < a.T) {
+      const size_t idx = part_index(part, t, nparts);
+      a.part_max[idx] = m;
+      a.part_sum[idx] = s;
+      a.part_pz[idx] = e;
+    }
+  });
 }
 
 // epilogue(acc, terms) of a tile of whatever shape; v0: its first vocabulary row.
 template <int SHAPE, bool EVEN, class Args, class Epilogue>
 __device__ __forceinline__ void head_tile(const Args& a, int v0, int tn, char* lds, Epilogue epilogue) {
   const int wave = threadIdx.x >> 6;
-  AdapterTerms<wave_cols(SHAPE), true> terms(a.adapters, v0 + wave / waves_n(SHAPE) * WM, a.V, tn * BN + wave % waves_n(SHAPE) * (wave_cols(SHAPE) * MT), a.T);
+  AdapterTerms<wave_cols(SHAPE)> terms(a.adapters, v0 + wave / waves_n(SHAPE) * WM, a.V, tn * BN + wave % waves_n(SHAPE) * (wave_cols(SHAPE) * MT), a.T);
   // A part behind the vocabulary (the upper half of the last tile) is made of any row and dropped behind this.
   const Operand oa{a.W, a.ldw, SHAPE == kShort && v0 >= a.V ? a.V - 1 : v0, a.V}, ob{a.Hd, a.ldh, tn * BN, a.T};
   f32x4 acc[TM][wave_cols(SHAPE)];
-  tile_product<SHAPE, EVEN>(oa, ob, a.H / BK, lds, acc);
+  tile_product_and_start<SHAPE, EVEN>(oa, ob, a.H / BK, lds, acc, terms);
   epilogue(acc, terms);
 }
 
@@ -81,9 +80,10 @@ __device__ __forceinline__ void head_half_tile(const Args& a, char* lds, Epilogu
   int tm, tn;
   tile_coords(blockIdx.x, tiles_m, tiles_n, kGroupM, tm, tn);
   const int wave = threadIdx.x >> 6, wm = wave / WAVES_N, wn = wave % WAVES_N;
-  AdapterTerms<kHalfTN, false> terms(a.adapters, tm * BM + wm * WM, a.V, tn * kHalfBN + wn * kHalfWN, a.T);
+  AdapterTerms<kHalfTN> terms(a.adapters, tm * BM + wm * WM, a.V, tn * kHalfBN + wn * kHalfWN, a.T);
   half_acc_t acc;
   half_tile_product(Operand{a.W, a.ldw, tm * BM, a.V}, Operand{a.Hd, a.ldh, tn * kHalfBN, a.T}, a.H / kHalfBK, lds, acc);
+  terms.start();
   epilogue(acc, terms);
 }
 
@@ -112,8 +112,8 @@ struct __attribute__((packed, aligned(2))) Piece16 {
   u32x4 v;
 };
 
-template <bool F32, int NB, bool HOLD>
-__device__ __forceinline__ void store_logits(f32x4 (&acc)[TM][NB], AdapterTerms<NB, HOLD>& terms, const AdapterLogitsArgs& a, char* lds) {
+template <bool F32, int NB>
+__device__ __forceinline__ void store_logits(f32x4 (&acc)[TM][NB], AdapterTerms<NB>& terms, const AdapterLogitsArgs& a, char* lds) {
   constexpr int ES = F32 ? 4 : 2, E = 16 / ES;   // elements of a piece
   constexpr int kRow = WM * ES + 16;             // of the stage: 16 bytes further into the banks per token
   constexpr int kPieces = WM / E;                // per token
@@ -122,10 +122,10 @@ __device__ __forceinline__ void store_logits(f32x4 (&acc)[TM][NB], AdapterTerms<
   const int lane = threadIdx.x & 63, lrow = lane & 15, kq = lane >> 4;
   const int rows = a.V - terms.v0 < WM ? a.V - terms.v0 : WM;  // of the wave that exist
   if (rows <= 0) return;
-  for_each(std::make_integer_sequence<int, NB>{}, [&](auto block) {
+  for_each_int(std::make_integer_sequence<int, NB>{}, [&](auto block) {
     constexpr int j = decltype(block)::value;
     f32x4 z[TM];
-    terms.template block<true>(j, acc, z);
+    terms.block(j, acc, z);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       char* at = stage + lrow * kRow + (i * MT + kq * 4) * ES;
@@ -191,11 +191,11 @@ __global__ __launch_bounds__(NTHREADS) void adapter_bwd_dz(const DzArgs z, const
     constexpr int NB = wave_cols(SHAPE);
     const int wave = threadIdx.x >> 6;
     const WaveRows rows = wave_vocab_rows(z.vc0 + col0 + wave / waves_n(SHAPE) * WM, z.V, z.tail);
-    AdapterTerms<NB, true> terms(ad, rows.v0, z.V, t.tn * BN + wave % waves_n(SHAPE) * (NB * MT), T);
+    AdapterTerms<NB> terms(ad, rows.v0, z.V, t.tn * BN + wave % waves_n(SHAPE) * (NB * MT), T);
     dz_tile<ENTGRAD, NB, SHAPE == kShort>(
         z, T, col0, t.tn * BN, lds,
         [&](Operand a, Operand b, f32x4 (&acc)[TM][NB]) {
-          tile_product<SHAPE, EVEN>(a, b, z.H / BK, lds, acc);
+          tile_product_and_start<SHAPE, EVEN>(a, b, z.H / BK, lds, acc, terms);
           return true;
         },
         [](u32x4 v, u32x4* p) { __builtin_nontemporal_store(v, p); },
@@ -213,11 +213,12 @@ __global__ __launch_bounds__(NTHREADS, 2) void adapter_bwd_half_dz(const DzArgs 
   if (!dz_tile_of<false>(z, blockIdx.x, kHalfBN, T, tile)) return;
   const int wave = threadIdx.x >> 6, wm = wave / WAVES_N, wn = wave % WAVES_N;
   const WaveRows rows = wave_vocab_rows(z.vc0 + tile.tm * BM + wm * WM, z.V, z.tail);
-  AdapterTerms<kHalfTN, false> terms(ad, rows.v0, z.V, tile.tn * kHalfBN + wn * kHalfWN, T);
+  AdapterTerms<kHalfTN> terms(ad, rows.v0, z.V, tile.tn * kHalfBN + wn * kHalfWN, T);
   dz_tile<ENTGRAD, kHalfTN, false>(
       z, T, tile.tm * BM, tile.tn * kHalfBN, lds,
       [&](const Operand& a, const Operand& b, half_acc_t& acc) {
         half_tile_product(a, b, z.H / kHalfBK, lds, acc);
+        terms.start();
         return true;
       },
       [](u32x4 v, u32x4* p) { __builtin_nontemporal_store(v, p); },

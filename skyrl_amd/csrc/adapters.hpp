@@ -32,103 +32,137 @@ struct AdapterTile {
 // What the adapters of a wave's tokens t0 .. t0 + 16 NB - 1 (of T) add to its accumulators of the vocabulary rows v0 .. v0 + 127 (of V), 16
 // tokens at a time: the epilogues, which go through the accumulators block by block, read them through block().  The accumulators
 // themselves are left alone: the mainloop holds them in fixed registers, and any loop over adapters that wrote them would have the compiler
-// move them about, past MFMAs that it does not know.  A block's sums are one assembly statement of MFMAs into vector registers, and every
-// lane, which holds one token, takes the sums of its own adapter only: an adapter's inf or NaN does not reach the tokens of others.
-// HOLD: the rows of B are kept from block to block while the adapter stays the same (ranks up to 32); the half tiles, with half of the
-// registers, take four row blocks at a time and load them again.
-template <int NB, bool HOLD>
+// move them about, past MFMAs that it does not know.  A block's products are one assembly statement of MFMAs into vector registers, once per
+// adapter that its tokens have, against zeros for the tokens of others.  The rows of B are kept from block to block while the adapter
+// stays the same (ranks up to 32).
+//
+// A token must not depend on the values of another's adapter, and 0 * inf would be NaN.  So in a block that adapters share the rows' top
+// exponent bits are looked at (set from 2.0 on, and in every inf and NaN); where one is set the values that are not finite are replaced by zero, and
+// the adapter's own tokens get the NaN.
+template <int NB>
 struct AdapterTerms {
-  static constexpr int kRows = 4;  // row blocks per statement
+  static constexpr int kNoToken = -2;
   const AdapterTile& a;
-  int v0, V, t0, id[(NB + 3) / 4];
+  int v0, V, t0, id[NB];
   int held = -1;
-  bf16x8 rows[HOLD ? TM : kRows];
+  bf16x8 rows[TM], hi_, lo_;  // hi_, lo_: u of the next block's tokens, the first 32 ranks
 
-  // In front of the mainloop: the loads of the tokens' adapters.
+  // The loads of the tokens' adapters.
   __device__ __forceinline__ AdapterTerms(const AdapterTile& a_, int v0_, int V_, int t0_, int T) : a(a_), v0(v0_), V(V_), t0(t0_) {
-    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int u = 0; u < (NB + 3) / 4; ++u) {
-      const int t = t0 + u * 64 + lane;
-      id[u] = u * 64 + lane < NB * MT && t < T ? a.ids[t] : -1;
+    for (int j = 0; j < NB; ++j) {
+      const int t = t0 + j * MT + (threadIdx.x & 15);
+      id[j] = t < T ? a.ids[t] : kNoToken;
     }
   }
 
-  __device__ __forceinline__ bf16x8 row(const uint16_t* B, int i) const {
-    const int v = v0 + i * MT + (threadIdx.x & 15);
-    return *(const bf16x8*)(B + (size_t)(v < V ? v : V - 1) * (size_t)a.ldb);
+  __device__ __forceinline__ const uint16_t* u_row(int j) const {
+    return id[j] >= 0 ? a.U + (size_t)((1 + t0 + j * MT + (threadIdx.x & 15)) * (2 * padded_rank(a.rank))) : a.zero_row;
   }
-  // Wait states in front for the writes of the operands, behind for the reads of the sums.
-  static __device__ __forceinline__ void products(f32x4& s0, f32x4& s1, f32x4& s2, f32x4& s3, const bf16x8* r, const bf16x8& hi, const bf16x8& lo) {
-    asm volatile(
-        "s_nop 7\n\t"
-        "v_mfma_f32_16x16x32_bf16 %0, %4, %8, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %5, %8, %1\n\t"
-        "v_mfma_f32_16x16x32_bf16 %2, %6, %8, %2\n\tv_mfma_f32_16x16x32_bf16 %3, %7, %8, %3\n\t"
-        "v_mfma_f32_16x16x32_bf16 %0, %4, %9, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %5, %9, %1\n\t"
-        "v_mfma_f32_16x16x32_bf16 %2, %6, %9, %2\n\tv_mfma_f32_16x16x32_bf16 %3, %7, %9, %3\n\t"
-        "s_nop 15\n\ts_nop 3"
-        : "+v"(s0), "+v"(s1), "+v"(s2), "+v"(s3)
-        : "v"(r[0]), "v"(r[1]), "v"(r[2]), "v"(r[3]), "v"(hi), "v"(lo));
+  __device__ __forceinline__ void load_u(int j, int k, bf16x8& hi, bf16x8& lo) const {
+    const uint16_t* u = u_row(j) + k;
+    hi = *(const bf16x8*)u, lo = *(const bf16x8*)(u + padded_rank(a.rank));
   }
-
-  // z = acc[.][j] + the adapters' part.  PIN: the block's accumulators come to vector registers here; left to itself the compiler brings all of
-  // them there at the mainloop's end, in front of the stores of logits (which it then spills), not in front of the other epilogues.
-  template <bool PIN = false>
-  __device__ __forceinline__ void block(int j, f32x4 (&acc)[TM][NB], f32x4 (&z)[TM]) {
-    const int lane = threadIdx.x & 63, lrow = lane & 15, kq = lane >> 4;
-    __builtin_amdgcn_sched_barrier(0);  // one block's accumulators at a time: there are no registers for the next one's
-    const int mine = __shfl(id[j / 4], (j & 3) * 16 + lrow, 64);  // the adapter of this lane's token
+  __device__ __forceinline__ void load_rows(int adapter, int k) {
+    const uint16_t* B = a.B + (size_t)adapter * (size_t)a.b_adapter + (k < a.rank ? k : 0);  // behind the rank any value does: u is zero there
+    int first = v0 + (threadIdx.x & 15);
+    asm volatile("" : "+v"(first));  // the addresses are formed here, where they are needed once in many blocks, and not in front of every block's loop
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      if constexpr (PIN) asm volatile("" : "+a"(acc[i][j]));
-      z[i] = acc[i][j];
+      const int v = first + i * MT;
+      rows[i] = *(const bf16x8*)(B + (size_t)(v < V ? v : V - 1) * (size_t)a.ldb);
+    }
+    held = adapter;
+  }
+  // The loads of the first block's u and of the first adapter's rows.
+  __device__ __forceinline__ void start() {
+    const int k = ((threadIdx.x & 63) >> 4) * 8;
+    load_u(0, k, hi_, lo_);
+    const unsigned long long any = __ballot(id[0] >= 0);
+    if (any) load_rows(__builtin_amdgcn_readlane(id[0], (int)__builtin_ctzll(any)), k);
+  }
+
+  // z += rows . (hi + lo).  Wait states in front for the writes of the operands, behind for the reads of the sums.
+  static __device__ __forceinline__ void products(f32x4 (&z)[TM], const bf16x8 (&r)[TM], const bf16x8& hi, const bf16x8& lo) {
+    asm volatile(
+        "s_nop 1\n\t"
+        "v_mfma_f32_16x16x32_bf16 %0, %8, %16, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %9, %16, %1\n\t"
+        "v_mfma_f32_16x16x32_bf16 %2, %10, %16, %2\n\tv_mfma_f32_16x16x32_bf16 %3, %11, %16, %3\n\t"
+        "v_mfma_f32_16x16x32_bf16 %4, %12, %16, %4\n\tv_mfma_f32_16x16x32_bf16 %5, %13, %16, %5\n\t"
+        "v_mfma_f32_16x16x32_bf16 %6, %14, %16, %6\n\tv_mfma_f32_16x16x32_bf16 %7, %15, %16, %7\n\t"
+        "v_mfma_f32_16x16x32_bf16 %0, %8, %17, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %9, %17, %1\n\t"
+        "v_mfma_f32_16x16x32_bf16 %2, %10, %17, %2\n\tv_mfma_f32_16x16x32_bf16 %3, %11, %17, %3\n\t"
+        "v_mfma_f32_16x16x32_bf16 %4, %12, %17, %4\n\tv_mfma_f32_16x16x32_bf16 %5, %13, %17, %5\n\t"
+        "v_mfma_f32_16x16x32_bf16 %6, %14, %17, %6\n\tv_mfma_f32_16x16x32_bf16 %7, %15, %17, %7\n\t"
+        "s_nop 12"
+        : "+v"(z[0]), "+v"(z[1]), "+v"(z[2]), "+v"(z[3]), "+v"(z[4]), "+v"(z[5]), "+v"(z[6]), "+v"(z[7])
+        : "v"(r[0]), "v"(r[1]), "v"(r[2]), "v"(r[3]), "v"(r[4]), "v"(r[5]), "v"(r[6]), "v"(r[7]), "v"(hi), "v"(lo));
+  }
+
+  // Rows of a shared block: values that are not finite become zero, and z NaN there for the adapter's own tokens.
+  __device__ __forceinline__ void make_finite(f32x4 (&z)[TM], bool own) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const u32x4 w = __builtin_bit_cast(u32x4, rows[i]);
+      bits |= w[0] | w[1] | w[2] | w[3];
+    }
+    if (!__any((bits & 0x40004000u) != 0u)) return;
+    const int kq = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      u32x4 w = __builtin_bit_cast(u32x4, rows[i]);
+      bool bad = false;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const bool low = (w[d] & 0x7f80u) == 0x7f80u, high = (w[d] & 0x7f800000u) == 0x7f800000u;
+        bad |= low || high;
+        w[d] = (low ? 0u : w[d] & 0xffffu) | (high ? 0u : w[d] & 0xffff0000u);
+      }
+      rows[i] = __builtin_bit_cast(bf16x8, w);
+      const unsigned long long lanes = __ballot(bad);
+      const unsigned in_row = (unsigned)(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) >> (kq * 4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z[i][r] = own && (in_row >> r & 1u) ? NAN : z[i][r];
+    }
+    held = -1;  // they are not the adapter's rows any more
+  }
+
+  // z = acc[.][j] + the adapters' part.  The accumulators are read by name: left to itself the compiler either brings all of them to vector
+  // registers at the mainloop's end and spills them, or works on them where they are and moves them there and back around the products.
+  __device__ __forceinline__ void block(int j, f32x4 (&acc)[TM][NB], f32x4 (&z)[TM]) {
+    __builtin_amdgcn_sched_barrier(0);  // one block's accumulators at a time: there are no registers for the next one's
+    const int mine = id[j], kq8 = ((threadIdx.x & 63) >> 4) * 8;
+    bf16x8 hi = hi_, lo = lo_;
+    if (j + 1 < NB) load_u(j + 1, kq8, hi_, lo_);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(z[i][r]) : "a"(acc[i][j][r]));
     }
     unsigned left = (unsigned)__ballot(mine >= 0) & 0xffffu;
-    if (left == 0) return;
-    const int pitch = 2 * padded_rank(a.rank);
-    const uint16_t* u = mine >= 0 ? a.U + (size_t)(1 + t0 + j * MT + lrow) * (size_t)pitch : a.zero_row;
     while (left) {
       const int first = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
-      left &= ~(unsigned)__ballot(mine == first);
-      const uint16_t* B = a.B + (size_t)first * (size_t)a.b_adapter;
-      if constexpr (HOLD) {
-        f32x4 sum[TM];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int k0 = 0; k0 < a.rank; k0 += 32) {
-          const int k = k0 + kq * 8;
-          const bf16x8 hi = *(const bf16x8*)(u + k), lo = *(const bf16x8*)(u + pitch / 2 + k);
-          if (held != first || a.rank > 32) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i) rows[i] = row(B + (k < a.rank ? k : 0), i);  // behind the rank any value does: u is zero there
-            held = first;
-          }
-          products(sum[0], sum[1], sum[2], sum[3], rows, hi, lo);
-          products(sum[4], sum[5], sum[6], sum[7], rows + kRows, hi, lo);
+      const unsigned own = (unsigned)__ballot(mine == first) & 0xffffu;
+      const bool shared = ((unsigned)__ballot(mine == first || mine == kNoToken) & 0xffffu) != 0xffffu;
+      left &= ~own;
+      for (int k0 = 0; k0 < a.rank; k0 += 32) {
+        if (k0 > 0) {
+          int k = k0 + kq8;
+          asm volatile("" : "+v"(k));  // as in load_rows()
+          load_u(j, k, hi, lo);
         }
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) z[i][r] = mine == first ? z[i][r] + sum[i][r] : z[i][r];
-      } else {
-#pragma unroll
-        for (int i0 = 0; i0 < TM; i0 += kRows) {
-          f32x4 sum[kRows];
-#pragma unroll
-          for (int i = 0; i < kRows; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-          for (int k0 = 0; k0 < a.rank; k0 += 32) {
-            const int k = k0 + kq * 8;
-            const bf16x8 hi = *(const bf16x8*)(u + k), lo = *(const bf16x8*)(u + pitch / 2 + k);
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) rows[i] = row(B + (k < a.rank ? k : 0), i0 + i);
-            products(sum[0], sum[1], sum[2], sum[3], rows, hi, lo);
-          }
-#pragma unroll
-          for (int i = 0; i < kRows; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) z[i0 + i][r] = mine == first ? z[i0 + i][r] + sum[i][r] : z[i0 + i][r];
+        if (held != first || a.rank > 32) load_rows(first, k0 + kq8);
+        bf16x8 h = hi, l = lo;
+        if (shared) {
+          const u32x4 none = {0u, 0u, 0u, 0u};
+          h = __builtin_bit_cast(bf16x8, mine == first ? __builtin_bit_cast(u32x4, hi) : none);
+          l = __builtin_bit_cast(bf16x8, mine == first ? __builtin_bit_cast(u32x4, lo) : none);
+          make_finite(z, mine == first);
         }
+        products(z, rows, h, l);
       }
+      if (left && a.rank > 32) load_u(j, kq8, hi, lo);
     }
   }
 };

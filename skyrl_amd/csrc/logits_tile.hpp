@@ -3,6 +3,9 @@
 #pragma once
 #include <math.h>
 
+#include <type_traits>
+#include <utility>
+
 #include "gemm_core.hpp"
 
 namespace lmhead {
@@ -202,6 +205,10 @@ static_assert(BN % kTokenGroup == 0, "tiles begin at whole groups");
 // terms(j, acc, x), where it is given: x = the products of token block j and what is added to them (adapters.hpp).
 constexpr int kDzTokRow = WM * 2 + 16, kDzTokBytes = 24;
 struct NoTerms {};
+template <class F, int... I>
+__device__ __forceinline__ void for_each_int(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
 template <bool ENTGRAD, int NB, bool SHORT, class Product, class Store, class Terms = NoTerms>
 __device__ __forceinline__ void dz_tile(const DzArgs& z, int T, int col0, int t0, char* lds, Product product, Store store, Terms terms = Terms{}) {
   constexpr int WAVE_N = NB * MT;  // tokens per wave
@@ -322,13 +329,12 @@ __device__ __forceinline__ void dz_tile(const DzArgs& z, int T, int col0, int t0
   // vocabulary's end (RAGGED: only the last vocab tile), a label of some token inside the wave's rows (LABEL, decided per
   // token block by a ballot), the fp32 residual of the label's value (fp32 operands only) -- is decided once outside the
   // unrolled loops: as tests inside them they cost three branches per i-step, a third of the epilogue's time.
+  constexpr bool TERMS = !std::is_same<Terms, NoTerms>::value;
+  f32x4 sums[TERMS ? TM : 1];
   auto token_block = [&](int j, auto ragged, auto label) {
     constexpr bool RAGGED = decltype(ragged)::value, LABEL = decltype(label)::value;
     const float gs = gs_[j], c0 = c0_[j], c1 = c1_[j], lse2 = lse2_[j];
     const int yrel = yrel_[j];
-    constexpr bool TERMS = !std::is_same<Terms, NoTerms>::value;
-    f32x4 sums[TERMS ? TM : 1];
-    if constexpr (TERMS) terms(j, acc, sums);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       float d[4];
@@ -364,7 +370,15 @@ __device__ __forceinline__ void dz_tile(const DzArgs& z, int T, int col0, int t0
   };
   std::true_type yes;
   std::false_type no;
-  if (__builtin_amdgcn_readfirstlane((int)full)) {
+  if constexpr (TERMS) {  // one copy of them per block, and the blocks unrolled whatever their size
+    for_each_int(std::make_integer_sequence<int, NB>{}, [&](auto block) {
+      constexpr int j = decltype(block)::value;
+      terms(j, acc, sums);
+      if (!__builtin_amdgcn_readfirstlane((int)full)) token_block(j, yes, yes);
+      else if (__any(yrel_[j] >= 0)) token_block(j, no, yes);
+      else token_block(j, no, no);
+    });
+  } else if (__builtin_amdgcn_readfirstlane((int)full)) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       if (__any(yrel_[j] >= 0)) token_block(j, no, yes);  // some token of this block has its label inside the wave's rows
