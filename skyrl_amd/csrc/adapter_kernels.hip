@@ -45,9 +45,11 @@ __device__ __forceinline__ Terms two_terms(const f32x4& x) {
 __device__ __forceinline__ int tokens_in_force(int T, const int* T_dev) { return T_dev ? __builtin_amdgcn_readfirstlane(*T_dev) : T; }
 
 // ------------------------------------------------------------------------------------------------------------
-// u = s A h.  One workgroup per 16 tokens and 32 ranks; its waves share the hidden size and their sums meet in LDS.  M: rank, N: token.
+// u = s A h.  One workgroup per 16 tokens, 32 ranks and every so many of the tokens' adapters (grid.z, so that a batch of unlike tokens does not
+// read its adapters one behind the other); its waves share the hidden size and their sums meet in LDS.  M: rank, N: token.  Bound by the
+// latency of its loads: with all adapters of 16 tokens in one workgroup of eight waves 97 us at T=16, H=3584, ten adapters.
 // ------------------------------------------------------------------------------------------------------------
-constexpr int kShrinkWaves = 8;
+constexpr int kShrinkWaves = 16;
 __global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink(const Adapters ad, const uint16_t* __restrict__ hidden, int64_t ldh,
                                                                     const int64_t* __restrict__ ids, int T_, const int* T_dev, int H,
                                                                     uint16_t* __restrict__ U, int* __restrict__ ids32) {
@@ -55,7 +57,7 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink(const Adapte
   const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int pitch = 2 * padded_rank(ad.rank), r0 = blockIdx.y * 32;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && tid * 8 < pitch) *(uint4*)(U + tid * 8) = make_uint4(0, 0, 0, 0);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && tid * 8 < pitch) *(uint4*)(U + tid * 8) = make_uint4(0, 0, 0, 0);
   const int T = tokens_in_force(T_, T_dev), t0 = blockIdx.x * 16;
   if (t0 >= T) return;
   const int t = t0 + lrow;
@@ -63,14 +65,18 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink(const Adapte
   if (t < T) {
     const int64_t x = ids[t];
     id = x >= 0 && x < (int64_t)ad.N ? (int)x : -1;
-    if (blockIdx.y == 0 && tid < 16) ids32[t] = id;
+    if (blockIdx.y == 0 && blockIdx.z == 0 && tid < 16) ids32[t] = id;
   }
   const uint16_t* x_row = hidden + (size_t)(t < T ? t : T - 1) * (size_t)ldh + kq * 8;
   f32x4 u[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  bool mine = blockIdx.z == 0 && id < 0;  // whether this workgroup writes the token's row
+  bool any = __any(mine);
   unsigned left = (unsigned)__ballot(id >= 0) & 0xffffu;
-  while (left) {
+  for (unsigned n = 0; left; ++n) {
     const int a = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
     left &= ~(unsigned)__ballot(id == a);
+    if (n % gridDim.z != blockIdx.z) continue;
+    any = true;
     const uint16_t* rows[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -78,19 +84,20 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink(const Adapte
       rows[m] = ad.A + (size_t)a * (size_t)ad.a_adapter + (size_t)(r < ad.rank ? r : ad.rank - 1) * (size_t)ad.a_row + kq * 8;
     }
     f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll 4
+#pragma unroll 8
     for (int k = wave * 32; k < H; k += kShrinkWaves * 32) {
       const bf16x8 x = *(const bf16x8*)(x_row + k);
 #pragma unroll
       for (int m = 0; m < 2; ++m) acc[m] = mfma(*(const bf16x8*)(rows[m] + k), x, acc[m]);
     }
     const float s = ad.scaling[a];
-    if (id == a) u[0] = acc[0] * s, u[1] = acc[1] * s;
+    if (id == a) u[0] = acc[0] * s, u[1] = acc[1] * s, mine = true;
   }
+  if (!any) return;  // alike in all waves
 #pragma unroll
   for (int m = 0; m < 2; ++m) part[wave][m][lane] = u[m];
   __syncthreads();
-  if (tid >= 128 || t >= T) return;
+  if (tid >= 128 || t >= T || !mine) return;
   const int m = tid >> 6;
   f32x4 sum = part[0][m][lane];
 #pragma unroll
@@ -197,7 +204,7 @@ __device__ __forceinline__ int panel_row(int vc0, int c, const VocabTail& tail) 
 // Partial sums of B_a^T dz over a range of panel columns.  One workgroup per 64 tokens, range and 64 ranks; 16 tokens a wave.  M: rank (B's rows
 // through LDS), N: token (panel rows as they lie).  B's next rows and the panel's next pieces are loaded while the present ones are multiplied.
 // ------------------------------------------------------------------------------------------------------------
-constexpr int kDuTokens = 64, kDuColumns = 64, kDuRanks = 64;
+constexpr int kDuTokens = 64, kDuColumns = 128, kDuRanks = 64;
 constexpr int kDuPitch = kDuRanks * 2 + 16;
 __global__ __launch_bounds__(256) void adapter_du_partial(const AdapterPanel p, int columns, int per_range, float* __restrict__ out, int Rp) {
   __shared__ __attribute__((aligned(16))) char lds[2][kDuColumns * kDuPitch];
@@ -221,19 +228,20 @@ __global__ __launch_bounds__(256) void adapter_du_partial(const AdapterPanel p, 
     left &= ~__ballot(id64 == a);
     const bool any = __any(id == a);
     const uint16_t* Ba = p.ad.B + (size_t)a * (size_t)p.ad.b_adapter;
-    // 64 rows of 64 ranks: two 16-byte pieces a thread
-    u32x4 b[2];
-    bf16x8 d[2];
+    // 128 rows of 64 ranks: four 16-byte pieces a thread
+    constexpr int kPieces = kDuColumns * kDuRanks / 8 / 256, kSteps = kDuColumns / 32;
+    u32x4 b[kPieces];
+    bf16x8 d[kSteps];
     auto load = [&](int c) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < kPieces; ++j) {
         const int piece = j * 256 + tid, row = piece >> 3, r = r0 + (piece & 7) * 8;
         int v = panel_row(p.vc0, c + row, p.tail);
         v = v < p.V ? v : p.V - 1;  // a column behind the vocabulary: zeros in the panel
         b[j] = r < R ? *(const u32x4*)(Ba + (size_t)v * (size_t)p.ad.b_row + r) : u32x4{0u, 0u, 0u, 0u};
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) d[j] = *(const bf16x8*)(d_row + c + j * 32);
+      for (int j = 0; j < kSteps; ++j) d[j] = *(const bf16x8*)(d_row + c + j * 32);
     };
     f32x4 acc[4];
 #pragma unroll
@@ -243,19 +251,21 @@ __global__ __launch_bounds__(256) void adapter_du_partial(const AdapterPanel p, 
     for (int c = c0; c < c1; c += kDuColumns, turn ^= 1) {
       char* const at = lds[turn];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < kPieces; ++j) {
         const int piece = j * 256 + tid;
         *(u32x4*)(at + (piece >> 3) * kDuPitch + (piece & 7) * 16) = b[j];
       }
-      const bf16x8 d0 = d[0], d1 = d[1];
+      bf16x8 now[kSteps];
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) now[j] = d[j];
       if (c + kDuColumns < c1) load(c + kDuColumns);
       __syncthreads();  // the rows stand; the other buffer is written behind the next barrier's reads only
       if (any) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           if (m < tiles) {
-            acc[m] = mfma(transposed(at + m * 32, kDuPitch), d0, acc[m]);
-            acc[m] = mfma(transposed(at + 32 * kDuPitch + m * 32, kDuPitch), d1, acc[m]);
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) acc[m] = mfma(transposed(at + j * 32 * kDuPitch + m * 32, kDuPitch), now[j], acc[m]);
           }
         }
       }
@@ -273,18 +283,27 @@ __global__ __launch_bounds__(256) void adapter_du_partial(const AdapterPanel p, 
     if (r0 + m * 16 < Rp) *(f32x4*)(to + m * 16) = sum[m];
 }
 
-// du = s * (the sum of `slots` partial sums, in order) as two bf16 terms, rows of U's form.
+// du = s * (the sum of `slots` partial sums) as two bf16 terms, rows of U's form.  Sixteen threads share the slots of four ranks of a token, in an
+// order that the number of slots alone determines.
 __global__ __launch_bounds__(256) void adapter_du_sum(const Adapters ad, const float* __restrict__ part, int slots, int T_, const int* T_dev,
                                                       const int* __restrict__ ids, int Rp, uint16_t* __restrict__ dU) {
+  __shared__ f32x4 sums[16][16];
   const int T = tokens_in_force(T_, T_dev);
-  const int e = (blockIdx.x * 256 + threadIdx.x) * 4;  // Rp is a multiple of 32
+  const int q = threadIdx.x & 15, share = threadIdx.x >> 4;
+  const int e = (blockIdx.x * 16 + q) * 4;  // Rp is a multiple of 32: the 16 quads of a workgroup lie in one or two tokens
   const int t = e / Rp, r = e - t * Rp;
-  if (t >= T) return;
   const size_t step = (size_t)T_ * (size_t)Rp;
-  const float* from = part + (size_t)t * (size_t)Rp + r;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = 0; s < slots; ++s) sum += *(const f32x4*)(from + (size_t)s * step);
+  if (t < T) {
+    const float* from = part + (size_t)t * (size_t)Rp + r;
+#pragma unroll 4
+    for (int s = share; s < slots; s += 16) sum += *(const f32x4*)(from + (size_t)s * step);
+  }
+  sums[share][q] = sum;
+  __syncthreads();
+  if (share != 0 || t >= T) return;
+#pragma unroll
+  for (int s = 1; s < 16; ++s) sum += sums[s][q];
   const int a = ids[t];
   const Terms terms = two_terms(sum * (a >= 0 ? ad.scaling[a] : 0.f));
   uint16_t* to = dU + (size_t)(1 + t) * (size_t)(2 * Rp) + r;
@@ -554,8 +573,10 @@ __global__ __launch_bounds__(256) void adapter_da_sum(const float* __restrict__ 
 
 hipError_t launch_adapter_shrink(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const int64_t* ids, int64_t T, const int* T_dev,
                                  int64_t H, uint16_t* U, int* ids32) {
-  hipLaunchKernelGGL(adapter_shrink, dim3((unsigned)((T + 15) / 16), (unsigned)(padded_rank(ad.rank) / 32)), dim3(kShrinkWaves * 64), 0, s, ad, hidden, ldh,
-                     ids, (int)T, T_dev, (int)H, U, ids32);
+  // Up to 16 workgroups share the adapters of 16 tokens; with many tokens their tiles fill the chip by themselves.
+  const int64_t tiles = (T + 15) / 16, most = tiles <= 64 ? 16 : tiles <= 256 ? 4 : 2;
+  hipLaunchKernelGGL(adapter_shrink, dim3((unsigned)tiles, (unsigned)(padded_rank(ad.rank) / 32), (unsigned)(ad.N < most ? ad.N : most)),
+                     dim3(kShrinkWaves * 64), 0, s, ad, hidden, ldh, ids, (int)T, T_dev, (int)H, U, ids32);
   return hipGetLastError();
 }
 
@@ -571,7 +592,7 @@ hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float*
 }
 
 int adapter_du_ranges(int64_t T, int64_t columns, int ncu) {
-  const int64_t tiles = (T + kDuTokens - 1) / kDuTokens, wanted = (2 * (int64_t)ncu + tiles - 1) / tiles, most = (columns + 511) / 512;
+  const int64_t tiles = (T + kDuTokens - 1) / kDuTokens, wanted = (4 * (int64_t)ncu + tiles - 1) / tiles, most = (columns + 511) / 512;
   return (int)(wanted < most ? wanted : most);
 }
 
@@ -590,7 +611,7 @@ hipError_t launch_adapter_panel(hipStream_t s, const AdapterPanel& p, int ranges
 
 hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float* part, int slots, int64_t T, const int* T_dev, const int* ids32, uint16_t* dU) {
   const int Rp = padded_rank(ad.rank);
-  hipLaunchKernelGGL(adapter_du_sum, dim3((unsigned)((T * (Rp / 4) + 255) / 256)), dim3(256), 0, s, ad, part, slots, (int)T, T_dev, ids32, Rp, dU);
+  hipLaunchKernelGGL(adapter_du_sum, dim3((unsigned)((T * (Rp / 4) + 15) / 16)), dim3(256), 0, s, ad, part, slots, (int)T, T_dev, ids32, Rp, dU);
   return hipGetLastError();
 }
 
