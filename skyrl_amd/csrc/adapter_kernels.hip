@@ -194,6 +194,38 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_group_rows(const float*
   if (tid == 0 && mine == N) seg[N + 1] = n;
 }
 
+// The rows of every adapter cut in pieces of at most SIZE, laid end to end: piece p's adapter and rows, or a < 0 behind the last one.  Of the rows
+// row0 .. row0 + T - 1 that seg counts, numbered from 0.
+struct RowPiece {
+  int a, begin, end;
+};
+template <int SIZE>
+__device__ __forceinline__ RowPiece row_piece(const int* seg, int N, int row0, int T, int p) {
+  const int lane = threadIdx.x & 63;
+  auto inside = [&](int at) { return at < row0 ? 0 : at - row0 < T ? at - row0 : T; };
+  int before = 0;  // pieces of adapters in front of this step's 64
+  for (int a0 = 0; a0 < N; a0 += 64) {
+    const int a = a0 + lane;
+    const int from = a < N ? inside(seg[a]) : 0, to = a < N ? inside(seg[a + 1]) : 0, n = (to - from + SIZE - 1) / SIZE;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int below = __shfl_up(upto, o, 64);
+      upto += lane >= o ? below : 0;
+    }
+    const unsigned long long past = __ballot(before + upto > p);
+    if (past) {
+      const int l = (int)__builtin_ctzll(past);
+      const int k = p - before - __shfl(upto - n, l, 64);
+      const int begin = __shfl(from, l, 64) + k * SIZE, last = __shfl(to, l, 64);
+      return RowPiece{__builtin_amdgcn_readfirstlane(a0 + l), __builtin_amdgcn_readfirstlane(begin),
+                      __builtin_amdgcn_readfirstlane(begin + SIZE < last ? begin + SIZE : last)};
+    }
+    before += __shfl(upto, 63, 64);
+  }
+  return RowPiece{-1, 0, 0};
+}
+
 // The vocabulary row that panel column c of a chunk stands for; columns that stand for none hold zeros (VocabTail in gemm_core.hpp).
 __device__ __forceinline__ int panel_row(int vc0, int c, const VocabTail& tail) {
   const int column = vc0 + c;
@@ -201,86 +233,94 @@ __device__ __forceinline__ int panel_row(int vc0, int c, const VocabTail& tail) 
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Partial sums of B_a^T dz over a range of panel columns.  One workgroup per 64 tokens, range and 64 ranks; 16 tokens a wave.  M: rank (B's rows
-// through LDS), N: token (panel rows as they lie).  B's next rows and the panel's next pieces are loaded while the present ones are multiplied.
+// Partial sums of B_a^T dz over a range of panel columns.  One workgroup per piece of at most 128 rows of one adapter, range and 64 ranks; 32 rows a
+// wave.  M: rank (B's rows through LDS), N: row (panel rows as they lie).  B's next rows and the panel's next pieces are loaded while the
+// present ones are multiplied.  HBM: the panel once and B once per piece, which is why pieces are not smaller (64 rows that adapters share:
+// 202 us for 1024 rows x 151936 columns of six adapters, rank 32).
 // ------------------------------------------------------------------------------------------------------------
-constexpr int kDuTokens = 64, kDuColumns = 128, kDuRanks = 64;
+constexpr int kDuColumns = 128, kDuRanks = 64;
 constexpr int kDuPitch = kDuRanks * 2 + 16;
-__global__ __launch_bounds__(256) void adapter_du_partial(const AdapterPanel p, int columns, int per_range, float* __restrict__ out, int Rp) {
+__global__ __launch_bounds__(256) void adapter_du_partial(const AdapterPanel p, const int* __restrict__ seg, int row0, int columns, int per_range,
+                                                          float* __restrict__ out, int Rp) {
   __shared__ __attribute__((aligned(16))) char lds[2][kDuColumns * kDuPitch];
-  const int T = tokens_in_force(p.T, p.T_dev), t0 = blockIdx.x * kDuTokens;
-  if (t0 >= T) return;
+  const RowPiece piece = row_piece<kDuPiece>(seg, p.ad.N, row0, tokens_in_force(p.T, p.T_dev), blockIdx.x);
+  if (piece.a < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r0 = blockIdx.z * kDuRanks, R = p.ad.rank;
   const int tiles = __builtin_amdgcn_readfirstlane(((R - r0 < kDuRanks ? R - r0 : kDuRanks) + 15) / 16);
   const int c0 = blockIdx.y * per_range, c1 = c0 + per_range < columns ? c0 + per_range : columns;
-  const int id64 = t0 + lane < T ? p.ids[t0 + lane] : -1;  // of the workgroup's tokens: alike in all waves
-  const int t = t0 + wave * 16 + lrow;
-  const int id = t < T ? p.ids[t] : -1;
-  const uint16_t* d_row = p.D + (size_t)(t < T ? t : T - 1) * (size_t)p.ldd + kq * 8;
-  f32x4 sum[4];
+  const int t0 = piece.begin + wave * 32;
+  const int blocks = piece.end - t0 > 16 ? 2 : piece.end > t0 ? 1 : 0;  // of 16 rows that this wave has
+  const uint16_t* d_row[2];
 #pragma unroll
-  for (int m = 0; m < 4; ++m) sum[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  unsigned long long left = __ballot(id64 >= 0);
-  while (left) {
-    const int a = __builtin_amdgcn_readlane(id64, (int)__builtin_ctzll(left));
-    left &= ~__ballot(id64 == a);
-    const bool any = __any(id == a);
-    const uint16_t* Ba = p.ad.B + (size_t)a * (size_t)p.ad.b_adapter;
-    // 128 rows of 64 ranks: four 16-byte pieces a thread
-    constexpr int kPieces = kDuColumns * kDuRanks / 8 / 256, kSteps = kDuColumns / 32;
-    u32x4 b[kPieces];
-    bf16x8 d[kSteps];
-    auto load = [&](int c) {
+  for (int n = 0; n < 2; ++n) {
+    const int t = t0 + n * 16 + lrow;
+    d_row[n] = p.D + (size_t)(t < piece.end ? t : piece.end - 1) * (size_t)p.ldd + kq * 8;
+  }
+  const uint16_t* Ba = p.ad.B + (size_t)piece.a * (size_t)p.ad.b_adapter;
+  // 128 rows of 64 ranks: four 16-byte pieces a thread
+  constexpr int kPieces = kDuColumns * kDuRanks / 8 / 256, kSteps = kDuColumns / 32;
+  u32x4 b[kPieces];
+  bf16x8 d[2][kSteps];
+  auto load = [&](int c) {
 #pragma unroll
-      for (int j = 0; j < kPieces; ++j) {
-        const int piece = j * 256 + tid, row = piece >> 3, r = r0 + (piece & 7) * 8;
-        int v = panel_row(p.vc0, c + row, p.tail);
-        v = v < p.V ? v : p.V - 1;  // a column behind the vocabulary: zeros in the panel
-        b[j] = r < R ? *(const u32x4*)(Ba + (size_t)v * (size_t)p.ad.b_row + r) : u32x4{0u, 0u, 0u, 0u};
-      }
+    for (int j = 0; j < kPieces; ++j) {
+      const int at = j * 256 + tid, row = at >> 3, r = r0 + (at & 7) * 8;
+      int v = panel_row(p.vc0, c + row, p.tail);
+      v = v < p.V ? v : p.V - 1;  // a column behind the vocabulary: zeros in the panel
+      b[j] = r < R ? *(const u32x4*)(Ba + (size_t)v * (size_t)p.ad.b_row + r) : u32x4{0u, 0u, 0u, 0u};
+    }
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j) d[j] = *(const bf16x8*)(d_row + c + j * 32);
-    };
-    f32x4 acc[4];
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int m = 0; m < 4; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (c0 < c1) load(c0);
-    int turn = 0;
-    for (int c = c0; c < c1; c += kDuColumns, turn ^= 1) {
-      char* const at = lds[turn];
+      for (int j = 0; j < kSteps; ++j)
+        if (n < blocks) d[n][j] = *(const bf16x8*)(d_row[n] + c + j * 32);
+  };
+  f32x4 acc[2][4];
 #pragma unroll
-      for (int j = 0; j < kPieces; ++j) {
-        const int piece = j * 256 + tid;
-        *(u32x4*)(at + (piece >> 3) * kDuPitch + (piece & 7) * 16) = b[j];
-      }
-      bf16x8 now[kSteps];
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j) now[j] = d[j];
-      if (c + kDuColumns < c1) load(c + kDuColumns);
-      __syncthreads();  // the rows stand; the other buffer is written behind the next barrier's reads only
-      if (any) {
+    for (int m = 0; m < 4; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (c0 < c1) load(c0);
+  int turn = 0;
+  for (int c = c0; c < c1; c += kDuColumns, turn ^= 1) {
+    char* const at = lds[turn];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          if (m < tiles) {
+    for (int j = 0; j < kPieces; ++j) {
+      const int e = j * 256 + tid;
+      *(u32x4*)(at + (e >> 3) * kDuPitch + (e & 7) * 16) = b[j];
+    }
+    bf16x8 now[2][kSteps];
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) acc[m] = mfma(transposed(at + j * 32 * kDuPitch + m * 32, kDuPitch), now[j], acc[m]);
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) now[n][j] = d[n][j];
+    if (c + kDuColumns < c1) load(c + kDuColumns);
+    __syncthreads();  // the rows stand; the other buffer is written behind the next barrier's reads only
+    if (blocks > 0) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        if (m < tiles) {
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j) {
+            const bf16x8 f = transposed(at + j * 32 * kDuPitch + m * 32, kDuPitch);
+            acc[0][m] = mfma(f, now[0][j], acc[0][m]);
+            if (blocks > 1) acc[1][m] = mfma(f, now[1][j], acc[1][m]);
           }
         }
       }
     }
-    __syncthreads();  // the next adapter begins with buffer 0
-    if (id == a) {
-#pragma unroll
-      for (int m = 0; m < 4; ++m) sum[m] = acc[m];
-    }
   }
-  if (t >= T) return;
-  float* to = out + ((size_t)blockIdx.y * (size_t)p.T + (size_t)t) * (size_t)Rp + r0 + kq * 4;
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
-    if (r0 + m * 16 < Rp) *(f32x4*)(to + m * 16) = sum[m];
+  for (int n = 0; n < 2; ++n) {
+    const int t = t0 + n * 16 + lrow;
+    if (t >= piece.end) continue;
+    float* to = out + ((size_t)blockIdx.y * (size_t)p.T + (size_t)t) * (size_t)Rp + r0 + kq * 4;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      if (r0 + m * 16 < Rp) *(f32x4*)(to + m * 16) = acc[n][m];
+  }
 }
 
 // du = s * (the sum of `slots` partial sums) as two bf16 terms, rows of U's form.  Sixteen threads share the slots of four ranks of a token, in an
@@ -294,7 +334,8 @@ __global__ __launch_bounds__(256) void adapter_du_sum(const Adapters ad, const f
   const int t = e / Rp, r = e - t * Rp;
   const size_t step = (size_t)T_ * (size_t)Rp;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  if (t < T) {
+  const int a = t < T ? ids[t] : -1;
+  if (a >= 0) {  // rows without an adapter have no partial sums
     const float* from = part + (size_t)t * (size_t)Rp + r;
 #pragma unroll 4
     for (int s = share; s < slots; s += 16) sum += *(const f32x4*)(from + (size_t)s * step);
@@ -304,7 +345,6 @@ __global__ __launch_bounds__(256) void adapter_du_sum(const Adapters ad, const f
   if (share != 0 || t >= T) return;
 #pragma unroll
   for (int s = 1; s < 16; ++s) sum += sums[s][q];
-  const int a = ids[t];
   const Terms terms = two_terms(sum * (a >= 0 ? ad.scaling[a] : 0.f));
   uint16_t* to = dU + (size_t)(1 + t) * (size_t)(2 * Rp) + r;
   *(uint2*)to = terms.hi;
@@ -451,45 +491,17 @@ __global__ __launch_bounds__(256) void adapter_dh_add(const Adapters ad, const u
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// dA_a[r, h] = sum over adapter a's rows of du[t, r] h[t, h], in pieces of at most kDaPiece rows whose sums are added in order.  Piece number p of
-// all adapters' pieces, laid end to end: its adapter and rows, or a < 0 behind the last one.
+// dA_a[r, h] = sum over adapter a's rows of du[t, r] h[t, h], in pieces of at most kDaPiece rows whose sums are added in order.
 // ------------------------------------------------------------------------------------------------------------
-struct DaPiece {
-  int a, begin, end;
-};
-__device__ __forceinline__ DaPiece da_piece(const int* seg, int N, int p) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;  // pieces of adapters in front of this step's 64
-  for (int a0 = 0; a0 < N; a0 += 64) {
-    const int a = a0 + lane;
-    const int from = a < N ? seg[a] : 0, to = a < N ? seg[a + 1] : 0, n = (to - from + kDaPiece - 1) / kDaPiece;
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int below = __shfl_up(upto, o, 64);
-      upto += lane >= o ? below : 0;
-    }
-    const unsigned long long past = __ballot(before + upto > p);
-    if (past) {
-      const int l = (int)__builtin_ctzll(past);
-      const int k = p - before - __shfl(upto - n, l, 64);
-      const int begin = __shfl(from, l, 64) + k * kDaPiece, last = __shfl(to, l, 64);
-      return DaPiece{a0 + l, begin, begin + kDaPiece < last ? begin + kDaPiece : last};
-    }
-    before += __shfl(upto, 63, 64);
-  }
-  return DaPiece{-1, 0, 0};
-}
-
 // One workgroup per piece, 256 hidden columns (64 a wave) and 32 ranks.  M: hidden column, N: rank, steps of 32 rows.
 constexpr int kDaPitchH = 256 * 2 + 16, kDaPitchU = 2 * 32 * 2 + 16;
 __global__ __launch_bounds__(256) void adapter_da_partial(const Adapters ad, const uint16_t* __restrict__ hidden, int64_t ldh, const uint16_t* __restrict__ dU,
                                                           const int* __restrict__ seg, int H, float* __restrict__ part) {
   __shared__ __attribute__((aligned(16))) char lds_h[2][32 * kDaPitchH];
   __shared__ __attribute__((aligned(16))) char lds_u[2][32 * kDaPitchU];
-  const DaPiece piece = da_piece(seg, ad.N, blockIdx.x);
+  const RowPiece piece = row_piece<kDaPiece>(seg, ad.N, 0, seg[ad.N], blockIdx.x);
   if (piece.a < 0) return;
-  const int begin = __builtin_amdgcn_readfirstlane(piece.begin), end = __builtin_amdgcn_readfirstlane(piece.end);
+  const int begin = piece.begin, end = piece.end;
   const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h0 = blockIdx.y * 256, r0 = blockIdx.z * 32, Rp = padded_rank(ad.rank);
@@ -592,7 +604,7 @@ hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float*
 }
 
 int adapter_du_ranges(int64_t T, int64_t columns, int ncu) {
-  const int64_t tiles = (T + kDuTokens - 1) / kDuTokens, wanted = (4 * (int64_t)ncu + tiles - 1) / tiles, most = (columns + 511) / 512;
+  const int64_t tiles = (T + kDuPiece - 1) / kDuPiece, wanted = (8 * (int64_t)ncu + tiles - 1) / tiles, most = (columns + 511) / 512;
   return (int)(wanted < most ? wanted : most);
 }
 
@@ -600,7 +612,7 @@ hipError_t launch_adapter_panel(hipStream_t s, const AdapterPanel& p, int ranges
                                 const float* sum_in, float* sum_out, uint16_t* dB) {
   const int Rp = padded_rank(p.ad.rank), ranks = (Rp + 63) / 64;
   const int per_range = ((p.columns + ranges - 1) / ranges + kDuColumns - 1) / kDuColumns * kDuColumns;
-  hipLaunchKernelGGL(adapter_du_partial, dim3((unsigned)((p.T + kDuTokens - 1) / kDuTokens), (unsigned)ranges, (unsigned)ranks), dim3(256), 0, s, p,
+  hipLaunchKernelGGL(adapter_du_partial, dim3((unsigned)row_pieces(p.T, p.ad.N, kDuPiece), (unsigned)ranges, (unsigned)ranks), dim3(256), 0, s, p, seg, row0,
                      p.columns, per_range, du_part, Rp);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;

@@ -233,7 +233,10 @@ hipError_t launch_adapter_panel(hipStream_t s, const AdapterPanel& p, int ranges
 hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float* part, int slots, int64_t T, const int* T_dev, const int* ids32, uint16_t* dU);
 
 constexpr int kDaPiece = 256;  // rows whose dA is one sum
-inline int64_t adapter_da_pieces(int64_t T, int64_t N) { return T / kDaPiece + (N < T ? N : T); }
+constexpr int kDuPiece = 128;  // rows of one adapter whose du a workgroup forms
+// Pieces of at most `size` rows that T rows of N adapters are cut in, at most.
+inline int64_t row_pieces(int64_t T, int64_t N, int64_t size) { return T / size + (N < T ? N : T); }
+inline int64_t adapter_da_pieces(int64_t T, int64_t N) { return row_pieces(T, N, kDaPiece); }
 // d_hidden += A^T du through row_map, and dA [N, rank, H]; da_part: [adapter_da_pieces][padded rank][H] fp32.
 hipError_t launch_adapter_finish(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const uint16_t* dU, const int* ids32, const int* seg,
                                  int64_t T, const int* T_dev, const int* row_map, int64_t H, uint16_t* d_hidden, float* da_part, uint16_t* dA);
