@@ -482,12 +482,12 @@ int skyrl_logits_bwd(const void* logits, int logits_dtype, int64_t ld_logits, co
  *     product with the weight, and the sum with the adapters' part.  Rows are worked on grouped by adapter, in an order that follows from
  *     adapter_ids alone: the same bits on each call. */
 #define SKYRL_LMHEAD_MAX_ADAPTER_RANK 256
-size_t skyrl_lmhead_adapter_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t rank);
+size_t skyrl_lmhead_adapter_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t num_adapters, int64_t rank);
 int skyrl_lmhead_adapter_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels, const void* lora_a,
                              int64_t a_adapter, int64_t a_row, const void* lora_b, int64_t b_adapter, int64_t b_row, const float* scaling,
                              const int64_t* adapter_ids, int64_t num_adapters, int64_t rank, int64_t T, int64_t H, int64_t V, float rcp_temperature,
                              float* logprobs, float* entropy, float* row_lse, float* row_pz, void* workspace, size_t workspace_bytes, void* stream);
-size_t skyrl_lmhead_adapter_logits_workspace_bytes(int64_t T, int64_t rank);
+size_t skyrl_lmhead_adapter_logits_workspace_bytes(int64_t T, int64_t H, int64_t num_adapters, int64_t rank);
 int skyrl_lmhead_adapter_logits(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* lora_a, int64_t a_adapter,
                                 int64_t a_row, const void* lora_b, int64_t b_adapter, int64_t b_row, const float* scaling, const int64_t* adapter_ids,
                                 int64_t num_adapters, int64_t rank, int64_t T, int64_t H, int64_t V, int logits_dtype, void* logits, int64_t ld_logits,

@@ -81,11 +81,11 @@ SIGNATURES = {
         [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float,
          _c_p, _c_i64, _c_p, ctypes.c_size_t, _c_p],
     ),
-    "skyrl_lmhead_adapter_fwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 4),
+    "skyrl_lmhead_adapter_fwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 5),
     "skyrl_lmhead_adapter_fwd": (
         ctypes.c_int,
         [_c_p, _c_i64, _c_p, _c_i64, _c_p] + _ADAPTERS + [_c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p, _c_p, _c_p, _c_p, ctypes.c_size_t, _c_p]),
-    "skyrl_lmhead_adapter_logits_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64]),
+    "skyrl_lmhead_adapter_logits_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 4),
     "skyrl_lmhead_adapter_logits": (
         ctypes.c_int,
         [_c_p, _c_i64, _c_p, _c_i64] + _ADAPTERS + [_c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p, _c_i64, _c_p, ctypes.c_size_t, _c_p]),

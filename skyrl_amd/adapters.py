@@ -78,7 +78,7 @@ def lmhead_adapter_logits(hidden: torch.Tensor, weight: torch.Tensor, lora_a: to
     if T == 0:
         return out
     lib = _lib.load()
-    ws = _workspace(lib, int(lib.skyrl_lmhead_adapter_logits_workspace_bytes(T, R)), dev, f"T={T}, rank={R}")
+    ws = _workspace(lib, int(lib.skyrl_lmhead_adapter_logits_workspace_bytes(T, H, N, R)), dev, f"T={T}, H={H}, N={N}, rank={R}")
     with device_guard(dev):
         st = lib.skyrl_lmhead_adapter_logits(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0),
                                              *_adapter_args(lora_a, lora_b, scaling, adapter_ids, N, R), T, H, V, int(fp32), out.data_ptr(), V,
@@ -105,7 +105,7 @@ def lmhead_adapter_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch
     if T == 0:
         return lp, ent, lse, pz
     lib = _lib.load()
-    ws = _workspace(lib, int(lib.skyrl_lmhead_adapter_fwd_workspace_bytes(T, H, V, R)), dev, f"T={T}, H={H}, V={V}, rank={R}")
+    ws = _workspace(lib, int(lib.skyrl_lmhead_adapter_fwd_workspace_bytes(T, H, V, N, R)), dev, f"T={T}, H={H}, V={V}, N={N}, rank={R}")
     with device_guard(dev):
         st = lib.skyrl_lmhead_adapter_fwd(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), labels.data_ptr(),
                                           *_adapter_args(lora_a, lora_b, scaling, adapter_ids, N, R), T, H, V, float(rcp_temperature), lp.data_ptr(),

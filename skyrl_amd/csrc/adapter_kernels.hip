@@ -84,11 +84,22 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink(const Adapte
       rows[m] = ad.A + (size_t)a * (size_t)ad.a_adapter + (size_t)(r < ad.rank ? r : ad.rank - 1) * (size_t)ad.a_row + kq * 8;
     }
     f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll 8
-    for (int k = wave * 32; k < H; k += kShrinkWaves * 32) {
-      const bf16x8 x = *(const bf16x8*)(x_row + k);
+    constexpr int kAhead = 8, kStep = kShrinkWaves * 32;  // loads in flight; the compiler does not unroll a loop of MFMAs by itself
+    for (int k0 = wave * 32; k0 < H; k0 += kAhead * kStep) {
+      bf16x8 x[kAhead], w[kAhead][2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) acc[m] = mfma(*(const bf16x8*)(rows[m] + k), x, acc[m]);
+      for (int i = 0; i < kAhead; ++i) {
+        const int k = k0 + i * kStep < H ? k0 + i * kStep : k0;
+        x[i] = *(const bf16x8*)(x_row + k);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) w[i][m] = *(const bf16x8*)(rows[m] + k);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (k0 + i * kStep >= H) break;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) acc[m] = mfma(w[i][m], x[i], acc[m]);
+      }
     }
     const float s = ad.scaling[a];
     if (id == a) u[0] = acc[0] * s, u[1] = acc[1] * s, mine = true;
@@ -110,29 +121,46 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink(const Adapte
   *(uint2*)(to + pitch / 2) = terms.lo;
 }
 
-// The adapter's part of the label's logit: 16 lanes a token.
+// The adapter's part of the label's logit, 16 lanes a token, and the way of grouped rows' results to their tokens.
 __global__ __launch_bounds__(256) void adapter_label(const Adapters ad, const uint16_t* __restrict__ U, const int* __restrict__ ids,
-                                                     const int64_t* __restrict__ labels, int T, int64_t V, float rcp_temp, float* __restrict__ logprobs) {
+                                                     const int64_t* __restrict__ labels, int T, int64_t V, float rcp_temp, const RowResults from,
+                                                     const int* __restrict__ row_map, const RowResults to) {
   const int t = blockIdx.x * 16 + (threadIdx.x >> 4), part = threadIdx.x & 15;
   if (t >= T) return;
   const int a = ids[t];
   const int64_t y = labels[t];
-  if (a < 0 || y < 0 || y >= V) return;  // the 16 lanes alike
-  const int pitch = 2 * padded_rank(ad.rank);
-  const uint16_t* b = ad.B + (size_t)a * (size_t)ad.b_adapter + (size_t)y * (size_t)ad.b_row;
-  const uint16_t* u = U + (size_t)(1 + t) * (size_t)pitch;
   float sum = 0.f;
-  for (int r = part; r < ad.rank; r += 16) {
-    const float x = __uint_as_float((uint32_t)u[r] << 16) + __uint_as_float((uint32_t)u[pitch / 2 + r] << 16);
-    sum = fmaf(x, __uint_as_float((uint32_t)b[r] << 16), sum);
-  }
+  if (a >= 0 && y >= 0 && y < V) {  // the 16 lanes alike
+    const int pitch = 2 * padded_rank(ad.rank);
+    const uint16_t* b = ad.B + (size_t)a * (size_t)ad.b_adapter + (size_t)y * (size_t)ad.b_row;
+    const uint16_t* u = U + (size_t)(1 + t) * (size_t)pitch;
+    for (int r = part; r < ad.rank; r += 16) {
+      const float x = __uint_as_float((uint32_t)u[r] << 16) + __uint_as_float((uint32_t)u[pitch / 2 + r] << 16);
+      sum = fmaf(x, __uint_as_float((uint32_t)b[r] << 16), sum);
+    }
 #pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 16);
-  if (part == 0) logprobs[t] = fmaf(sum, rcp_temp, logprobs[t]);
+    for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 16);
+  }
+  const int row = row_map ? row_map[t] : t;
+  if (part == 0) to.logprobs[row] = a >= 0 ? fmaf(sum, rcp_temp, from.logprobs[t]) : from.logprobs[t];
+  if (!row_map) return;
+  if (part == 1 && to.entropy) to.entropy[row] = from.entropy[t];
+  if (part == 2 && to.row_lse) to.row_lse[row] = from.row_lse[t];
+  if (part == 3 && to.row_pz) to.row_pz[row] = from.row_pz[t];
+}
+
+// Rows of the hidden states (and labels) in the order of idx.
+__global__ __launch_bounds__(256) void adapter_gather_rows(const int* __restrict__ idx, const uint16_t* __restrict__ hidden, int64_t ldh, int H,
+                                                           const int64_t* __restrict__ labels, uint16_t* __restrict__ hidden_c, int64_t* __restrict__ labels_c) {
+  const int r = blockIdx.x, t = idx[r];
+  const uint16_t* src = hidden + (size_t)t * (size_t)ldh;
+  uint16_t* dst = hidden_c + (size_t)r * (size_t)H;
+  for (int c = threadIdx.x * 8; c < H; c += 256 * 8) *(uint4*)(dst + c) = *(const uint4*)(src + c);
+  if (labels && threadIdx.x == 0) labels_c[r] = labels[t];
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Rows with a gradient, grouped by adapter (those without one last), ascending inside a group: idx, their adapters, and seg[a], the place of
+// Rows with a gradient (all of them without g), grouped by adapter (those without one last), ascending inside a group: idx, their adapters, and seg[a], the place of
 // adapter a's first row; seg[N] that of the rows without an adapter, seg[N + 1] the number of rows.  One workgroup per group: it counts the rows of
 // the groups before its own, then lists its own.  The order is a function of the inputs alone, so the sums over rows are the same bits on each call.
 // ------------------------------------------------------------------------------------------------------------
@@ -147,7 +175,7 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_group_rows(const float*
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mine = blockIdx.x;
   auto group_of = [&](int t) -> int {  // -1: no gradient
     if (t >= T) return -1;
-    const float gv = g[t], qv = q ? q[t] : 0.f;
+    const float gv = g ? g[t] : 1.f, qv = q ? q[t] : 0.f;
     const int64_t x = ids[t];
     if (gv == 0.f && qv == 0.f) return -1;
     return x >= 0 && x < (int64_t)N ? (int)x : N;
@@ -593,8 +621,14 @@ hipError_t launch_adapter_shrink(hipStream_t s, const Adapters& ad, const uint16
 }
 
 hipError_t launch_adapter_label(hipStream_t s, const Adapters& ad, const uint16_t* U, const int* ids32, const int64_t* labels, int64_t T, int64_t V,
-                                float rcp_temp, float* logprobs) {
-  hipLaunchKernelGGL(adapter_label, dim3((unsigned)((T + 15) / 16)), dim3(256), 0, s, ad, U, ids32, labels, (int)T, V, rcp_temp, logprobs);
+                                float rcp_temp, const RowResults& from, const int* row_map, const RowResults& to) {
+  hipLaunchKernelGGL(adapter_label, dim3((unsigned)((T + 15) / 16)), dim3(256), 0, s, ad, U, ids32, labels, (int)T, V, rcp_temp, from, row_map, to);
+  return hipGetLastError();
+}
+
+hipError_t launch_adapter_gather_rows(hipStream_t s, const int* idx, const uint16_t* hidden, int64_t ldh, int64_t T, int64_t H, const int64_t* labels,
+                                      uint16_t* hidden_c, int64_t* labels_c) {
+  hipLaunchKernelGGL(adapter_gather_rows, dim3((unsigned)T), dim3(256), 0, s, idx, hidden, ldh, (int)H, labels, hidden_c, labels_c);
   return hipGetLastError();
 }
 

@@ -124,6 +124,8 @@ __device__ __forceinline__ void store_logits(f32x4 (&acc)[TM][NB], AdapterTerms<
   if (rows <= 0) return;
   for_each_int(std::make_integer_sequence<int, NB>{}, [&](auto block) {
     constexpr int j = decltype(block)::value;
+    const int here = terms.t0 + j * MT + lrow;
+    const int out_row = a.row_map ? a.row_map[here < a.T ? here : a.T - 1] : here;
     f32x4 z[TM];
     terms.block(j, acc, z);
 #pragma unroll
@@ -140,10 +142,11 @@ __device__ __forceinline__ void store_logits(f32x4 (&acc)[TM][NB], AdapterTerms<
     const int at = lane % kPieces * E;
     int t = terms.t0 + j * MT + lane / kPieces;
     const char* from = stage + lane / kPieces * kRow + at * ES;
-    char* to = (char*)a.out + ((size_t)t * (size_t)a.ldo + (size_t)(terms.v0 + at)) * ES;
 #pragma unroll 2
     for (int it = 0; it < MT * kPieces / 64; ++it) {
+      const int row = __shfl(out_row, it * (64 / kPieces) + lane / kPieces, 64);
       if (t < a.T) {
+        char* to = (char*)a.out + ((size_t)row * (size_t)a.ldo + (size_t)(terms.v0 + at)) * ES;
         if (at + E <= rows) {
           ((Piece16*)to)->v = *(const u32x4*)from;
         } else {
@@ -153,7 +156,7 @@ __device__ __forceinline__ void store_logits(f32x4 (&acc)[TM][NB], AdapterTerms<
           }
         }
       }
-      t += 64 / kPieces, from += 64 / kPieces * kRow, to += (size_t)(64 / kPieces) * (size_t)a.ldo * ES;
+      t += 64 / kPieces, from += 64 / kPieces * kRow;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   });

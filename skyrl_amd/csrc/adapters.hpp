@@ -185,6 +185,7 @@ struct AdapterLogitsArgs {
   void* out;
   int64_t ldo;
   int out_f32;
+  const int* row_map;  // NULL, or the row of `out` that a token's logits go to
   AdapterTile adapters;
 };
 hipError_t launch_adapter_logits(hipStream_t s, const AdapterLogitsArgs& a, bool half, bool even, bool shapes, int split, int workgroups);
@@ -207,11 +208,19 @@ struct Adapters {
 // only that many tokens.
 hipError_t launch_adapter_shrink(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const int64_t* ids, int64_t T, const int* T_dev,
                                  int64_t H, uint16_t* U, int* ids32);
-// logprobs[t] += u_t . B_a[label_t] * rcp_temp: the adapter's part of the label's logit.
+// The results of rows; entropy, row_lse and row_pz may be NULL.
+struct RowResults {
+  float *logprobs, *entropy, *row_lse, *row_pz;
+};
+// to.logprobs = from.logprobs + u_t . B_a[label_t] * rcp_temp, the adapter's part of the label's logit.  With row_map all results of row t go to row
+// row_map[t] of `to`.
 hipError_t launch_adapter_label(hipStream_t s, const Adapters& ad, const uint16_t* U, const int* ids32, const int64_t* labels, int64_t T, int64_t V,
-                                float rcp_temp, float* logprobs);
-// The T rows whose g or q is not zero, grouped by adapter: idx, their ids and the groups' places, seg [N + 2].
+                                float rcp_temp, const RowResults& from, const int* row_map, const RowResults& to);
+// The T rows whose g or q is not zero (all without g), grouped by adapter: idx, their ids and the groups' places, seg [N + 2].
 hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float* q, const int64_t* ids, int64_t T, int N, int* idx, int64_t* ids_c, int* seg);
+// hidden_c [T, H] and labels_c (both or neither of the labels' pointers): the rows that idx names.
+hipError_t launch_adapter_gather_rows(hipStream_t s, const int* idx, const uint16_t* hidden, int64_t ldh, int64_t T, int64_t H, const int64_t* labels,
+                                      uint16_t* hidden_c, int64_t* labels_c);
 
 // A chunk's dz panel, of rows grouped by adapter.
 struct AdapterPanel {

@@ -1378,6 +1378,9 @@ struct AdapterCall {
   const int64_t* ids;  // [T]
   uint16_t* U;
   int* ids32;
+  // Rows grouped by adapter: the tokens that they are, and where their results go.
+  const int* row_map;
+  RowResults results;
 
   AdapterTile tile(int64_t row0 = 0) const {
     return AdapterTile{ad.B, ad.b_adapter, (int)ad.b_row, ad.rank, U + (size_t)row0 * 2 * padded_rank(ad.rank), U, ids32 + row0};
@@ -1432,7 +1435,10 @@ int fwd_token_blocks(const void* hidden, int64_t ld_hidden, const void* weight, 
                        row_lse ? row_lse + t0 : (float*)nullptr, row_pz ? row_pz + t0 : (float*)nullptr);
     if ((e = hipGetLastError()) != hipSuccess) return (int)e;
     if (call) {  // the merge takes the label's logit from the weight alone
-      e = launch_adapter_label(s, call->ad, call->U, call->ids32, labels + t0, Tb, V, rcp_temperature, logprobs + t0);
+      const RowResults here{logprobs + t0, entropy ? entropy + t0 : nullptr, row_lse ? row_lse + t0 : nullptr, row_pz ? row_pz + t0 : nullptr};
+      Timed timed_label(kAdapterRows, s);
+      e = launch_adapter_label(s, call->ad, call->U, call->ids32, labels + t0, Tb, V, rcp_temperature, here, call->row_map ? call->row_map + t0 : nullptr,
+                               call->row_map ? call->results : here);
       if (e != hipSuccess) return (int)e;
     }
   }
@@ -2001,20 +2007,57 @@ bool adapter_extents(int64_t T, int64_t H, int64_t V, int64_t N, int64_t rank) {
   return T >= 1 && V >= 1 && H >= 1 && T <= kMaxExtent && V <= kMaxExtent && H <= kMaxRowPitch && N >= 1 && N <= kMaxAdapters && rank >= 1 &&
          rank <= kMaxAdapterRank;
 }
-// Rows of u of one forward block, and the tokens' adapters.
-AdapterCall carve_adapter_rows(Carver& c, const Adapters& ad, const int64_t* ids, int64_t T) {
-  AdapterCall call{ad, ids, nullptr, nullptr};
+// Whether the forward works on rows grouped by adapter: a block of 16 tokens costs a trip to memory and its products per adapter that it has, and
+// tokens may come in any order.  Tokens in order, a decoding step of 128 tokens of 48 adapters and its grouping: see adapters.hpp.
+constexpr int64_t kGroupFromTokens = 17;
+inline bool group_rows(int64_t T, int64_t N) { return N > 1 && T >= kGroupFromTokens; }
+
+// The room of a forward: u of one block and the tokens' adapters, and, where rows are grouped, those rows.
+struct AdapterForward {
+  AdapterCall call;
+  int64_t *ids_c, *labels_c;
+  uint16_t* hidden_c;
+  int *idx, *seg;
+  RowResults results;
+  size_t bytes;
+};
+AdapterForward carve_adapter_fwd(void* ws, const Adapters& ad, const int64_t* ids, int64_t T, int64_t H, bool statistics) {
+  Carver c(ws);
+  AdapterForward w{};
+  w.call.ad = ad, w.call.ids = ids;
   const int64_t Tb = T < kFwdTokenBlock ? T : kFwdTokenBlock;
-  call.U = c.take<uint16_t>((size_t)(Tb + 1) * (size_t)(2 * padded_rank(ad.rank)));
-  call.ids32 = c.take<int>((size_t)Tb);
-  return call;
+  w.call.U = c.take<uint16_t>((size_t)(Tb + 1) * (size_t)(2 * padded_rank(ad.rank)));
+  w.call.ids32 = c.take<int>((size_t)Tb);
+  if (group_rows(T, ad.N)) {
+    w.ids_c = c.take<int64_t>((size_t)T);
+    w.idx = c.take<int>((size_t)T);
+    w.seg = c.take<int>((size_t)ad.N + 2);
+    w.hidden_c = c.take<uint16_t>((size_t)T * (size_t)H);
+    if (statistics) {
+      w.labels_c = c.take<int64_t>((size_t)T);
+      w.results.logprobs = c.take<float>((size_t)T), w.results.entropy = c.take<float>((size_t)T);
+      w.results.row_lse = c.take<float>((size_t)T), w.results.row_pz = c.take<float>((size_t)T);
+    }
+  }
+  w.bytes = (size_t)round_up((int64_t)c.off, 256);
+  return w;
 }
-size_t adapter_rows_bytes(int64_t T, int64_t rank) {
-  Carver c(nullptr);
+size_t adapter_fwd_bytes(int64_t T, int64_t H, int64_t N, int64_t rank, bool statistics) {
   Adapters ad{};
-  ad.rank = (int)rank;
-  (void)carve_adapter_rows(c, ad, nullptr, T);
-  return (size_t)round_up((int64_t)c.off, 256);
+  ad.N = (int)N, ad.rank = (int)rank;
+  return carve_adapter_fwd(nullptr, ad, nullptr, T, H, statistics).bytes;
+}
+// Groups the rows of a forward; hidden, its pitch and labels become those of the grouped rows.
+hipError_t group_forward(hipStream_t s, AdapterForward& w, const void*& hidden, int64_t& ld_hidden, const int64_t** labels, int64_t T, int64_t H) {
+  if (!group_rows(T, w.call.ad.N)) return hipSuccess;
+  Timed timed(kAdapterRows, s);
+  hipError_t e = launch_adapter_group_rows(s, nullptr, nullptr, w.call.ids, T, w.call.ad.N, w.idx, w.ids_c, w.seg);
+  if (e != hipSuccess) return e;
+  e = launch_adapter_gather_rows(s, w.idx, (const uint16_t*)hidden, ld_hidden, T, H, labels ? *labels : nullptr, w.hidden_c, w.labels_c);
+  hidden = w.hidden_c, ld_hidden = H;
+  if (labels) *labels = w.labels_c;
+  w.call.ids = w.ids_c, w.call.row_map = w.idx;
+  return e;
 }
 // The chunk of a backward with adapters, and the bytes of scratch in front of theirs.
 int64_t adapter_bwd_chunk(int64_t T, int64_t H, int64_t V) {
@@ -2092,9 +2135,9 @@ int skyrl_lmhead_fwd_static_scratch(const void* hidden, int64_t ld_hidden, const
 
 size_t skyrl_lmhead_static_scratch_bytes(void) { return kStaticScratchBytes; }
 
-size_t skyrl_lmhead_adapter_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t rank) {
-  if (!adapter_extents(T, H, V, 1, rank)) return 0;
-  return skyrl_lmhead_fwd_workspace_bytes(T, H, V) + adapter_rows_bytes(T, rank);
+size_t skyrl_lmhead_adapter_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t num_adapters, int64_t rank) {
+  if (!adapter_extents(T, H, V, num_adapters, rank)) return 0;
+  return skyrl_lmhead_fwd_workspace_bytes(T, H, V) + adapter_fwd_bytes(T, H, num_adapters, rank, true);
 }
 
 int skyrl_lmhead_adapter_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels, const void* lora_a,
@@ -2105,17 +2148,24 @@ int skyrl_lmhead_adapter_fwd(const void* hidden, int64_t ld_hidden, const void* 
   if (st) return st;
   if ((st = check_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, adapter_ids, num_adapters, rank, H))) return st;
   if (!logprobs) return SKYRL_LMHEAD_ERR_NULL;
-  if (!workspace || workspace_bytes < skyrl_lmhead_adapter_fwd_workspace_bytes(T, H, V, rank)) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < skyrl_lmhead_adapter_fwd_workspace_bytes(T, H, V, num_adapters, rank)) return SKYRL_LMHEAD_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
-  Carver c((char*)workspace + skyrl_lmhead_fwd_workspace_bytes(T, H, V));
-  const AdapterCall call =
-      carve_adapter_rows(c, make_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, num_adapters, rank), adapter_ids, T);
-  return fwd_token_blocks(hidden, ld_hidden, weight, ld_weight, labels, T, H, V, rcp_temperature, logprobs, entropy, row_lse, row_pz, workspace,
-                          fwd_block_tokens(kFwdTokenBlock, ld_hidden), (hipStream_t)stream, &call);
+  AdapterForward w =
+      carve_adapter_fwd((char*)workspace + skyrl_lmhead_fwd_workspace_bytes(T, H, V),
+                        make_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, num_adapters, rank), adapter_ids, T, H, true);
+  const hipError_t e = group_forward((hipStream_t)stream, w, hidden, ld_hidden, &labels, T, H);
+  if (e != hipSuccess) return (int)e;
+  RowResults out{logprobs, entropy, row_lse, row_pz};
+  if (w.call.row_map) {  // the statistics of grouped rows, of those that are wanted, on the way to their tokens
+    w.call.results = out;
+    out = RowResults{w.results.logprobs, entropy ? w.results.entropy : nullptr, row_lse ? w.results.row_lse : nullptr, row_pz ? w.results.row_pz : nullptr};
+  }
+  return fwd_token_blocks(hidden, ld_hidden, weight, ld_weight, labels, T, H, V, rcp_temperature, out.logprobs, out.entropy, out.row_lse, out.row_pz,
+                          workspace, fwd_block_tokens(kFwdTokenBlock, ld_hidden), (hipStream_t)stream, &w.call);
 }
 
-size_t skyrl_lmhead_adapter_logits_workspace_bytes(int64_t T, int64_t rank) {
-  return adapter_extents(T, 1, 1, 1, rank) ? adapter_rows_bytes(T, rank) : 0;
+size_t skyrl_lmhead_adapter_logits_workspace_bytes(int64_t T, int64_t H, int64_t num_adapters, int64_t rank) {
+  return adapter_extents(T, H, 1, num_adapters, rank) ? adapter_fwd_bytes(T, H, num_adapters, rank, false) : 0;
 }
 
 int skyrl_lmhead_adapter_logits(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* lora_a, int64_t a_adapter,
@@ -2130,20 +2180,22 @@ int skyrl_lmhead_adapter_logits(const void* hidden, int64_t ld_hidden, const voi
   if (ld_logits < V || ld_logits >= ((int64_t)1 << 40)) return SKYRL_LMHEAD_ERR_SHAPE;
   const bool f32 = logits_dtype == SKYRL_LOGITS_F32;
   if ((uintptr_t)logits & (f32 ? 3u : 1u)) return SKYRL_LMHEAD_ERR_ALIGN;
-  if (!workspace || workspace_bytes < adapter_rows_bytes(T, rank)) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < adapter_fwd_bytes(T, H, num_adapters, rank, false)) return SKYRL_LMHEAD_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
-  Carver c(workspace);
-  const AdapterCall call =
-      carve_adapter_rows(c, make_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, num_adapters, rank), adapter_ids, T);
+  AdapterForward w = carve_adapter_fwd(workspace, make_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, num_adapters, rank),
+                                       adapter_ids, T, H, false);
   const int tiles_m = (int)((V + BM - 1) / BM);
   hipStream_t s = (hipStream_t)stream;
+  const hipError_t grouped = group_forward(s, w, hidden, ld_hidden, nullptr, T, H);
+  if (grouped != hipSuccess) return (int)grouped;
+  const AdapterCall& call = w.call;
   for (int64_t t0 = 0; t0 < T; t0 += kFwdTokenBlock) {
     const int64_t Tb = T - t0 < kFwdTokenBlock ? T - t0 : kFwdTokenBlock;
     const uint16_t* Hp = (const uint16_t*)hidden + (size_t)t0 * (size_t)ld_hidden;
     hipError_t e;
     {
       Timed timed(kAdapterRows, s);
-      e = launch_adapter_shrink(s, call.ad, Hp, ld_hidden, adapter_ids + t0, Tb, nullptr, H, call.U, call.ids32);
+      e = launch_adapter_shrink(s, call.ad, Hp, ld_hidden, call.ids + t0, Tb, nullptr, H, call.U, call.ids32);
     }
     if (e != hipSuccess) return (int)e;
     Timed timed(kFwdTiles, s);
@@ -2151,7 +2203,8 @@ int skyrl_lmhead_adapter_logits(const void* hidden, int64_t ld_hidden, const voi
     const TileShapes shapes = tile_shapes(Tb, H, tiles_m, compute_units());
     const int tiles = half ? tiles_m : tiles_m * (int)((Tb + BN - 1) / BN) + shapes.split;
     e = launch_adapter_logits(s, AdapterLogitsArgs{(const uint16_t*)weight, Hp, (int)ld_weight, (int)ld_hidden, (int)Tb, (int)H, (int)V,
-                                                   (char*)logits + (size_t)t0 * (size_t)ld_logits * (f32 ? 4 : 2), ld_logits, f32 ? 1 : 0, call.tile()},
+                                                   call.row_map ? logits : (char*)logits + (size_t)t0 * (size_t)ld_logits * (f32 ? 4 : 2), ld_logits,
+                                                   f32 ? 1 : 0, call.row_map ? call.row_map + t0 : nullptr, call.tile()},
                               half, even_ktiles(H), shapes.used, shapes.split, tiles);
     if (e != hipSuccess) return (int)e;
   }

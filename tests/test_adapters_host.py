@@ -20,16 +20,18 @@ P = 0x10000
 def test_workspaces():
     lib = _lib.load()
     rows = lambda T, Rp: 4 * (T + 1) * Rp + 4 * T  # noqa: E731
-    assert rows(300, 32) <= lib.skyrl_lmhead_adapter_logits_workspace_bytes(300, 24) <= rows(300, 32) + 1024
+    assert rows(300, 32) <= lib.skyrl_lmhead_adapter_logits_workspace_bytes(300, 896, 1, 24) <= rows(300, 32) + 1024
+    grouped = rows(300, 32) + 300 * (8 + 4 + 2 * 896)   # rows of several adapters are brought together
+    assert grouped <= lib.skyrl_lmhead_adapter_logits_workspace_bytes(300, 896, 5, 24) <= grouped + 2048
     head = lib.skyrl_lmhead_fwd_workspace_bytes(300, 896, 5000)
-    assert head + rows(300, 64) <= lib.skyrl_lmhead_adapter_fwd_workspace_bytes(300, 896, 5000, 64) <= head + rows(300, 64) + 1024
+    assert head + rows(300, 64) <= lib.skyrl_lmhead_adapter_fwd_workspace_bytes(300, 896, 5000, 1, 64) <= head + rows(300, 64) + 1024
     small, large = (lib.skyrl_lmhead_adapter_bwd_workspace_bytes(300, 896, 5000, n, 16) for n in (1, 64))
     assert lib.skyrl_lmhead_bwd_active_rows_workspace_bytes(300, 896, 5000, 0) < small < large
     # what does not fit any call has no workspace
     for T, H, V, N, R in ((0, 64, 8, 1, 8), (8, 64, 0, 1, 8), (8, 64, 8, 0, 8), (8, 64, 8, 65536, 8), (8, 64, 8, 1, 257), (1 << 31, 64, 8, 1, 8)):
         assert lib.skyrl_lmhead_adapter_bwd_workspace_bytes(T, H, V, N, R) == 0
     for T, R in ((0, 8), (1 << 40, 8), (8, 0), (8, 264)):
-        assert lib.skyrl_lmhead_adapter_logits_workspace_bytes(T, R) == 0
+        assert lib.skyrl_lmhead_adapter_logits_workspace_bytes(T, 64, 1, R) == 0
     big = (1, 300, 1 << 20, (1 << 31) - 1, 1 << 40)
     for T, V, N in itertools.product(big, (5, 152064, 1 << 40), (1, 65535, 1 << 40)):
         lib.skyrl_lmhead_adapter_bwd_workspace_bytes(T, 3584, V, N, 256)
