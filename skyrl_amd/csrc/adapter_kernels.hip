@@ -10,23 +10,6 @@
 namespace lmhead {
 namespace {
 
-typedef __attribute__((ext_vector_type(8))) short i16x8;
-typedef __attribute__((address_space(3))) i16x4* lds_half_ptr;
-
-__device__ __forceinline__ f32x4 mfma(const bf16x8& a, const bf16x8& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-// The transposed fragment whose 32 rows of `pitch` bytes begin at `at` (LDS), at the columns that `at` points to.
-__device__ __forceinline__ bf16x8 transposed(const char* at, int pitch) {
-  const int lane = threadIdx.x & 63, kq = lane >> 4, s = lane & 15;
-  const uint32_t addr = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)at + (uint32_t)((kq * 8 + (s >> 2)) * pitch + (s & 3) * 8);
-  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half_ptr)(uintptr_t)addr);
-  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half_ptr)(uintptr_t)(addr + 4u * (uint32_t)pitch));
-  const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  return __builtin_bit_cast(bf16x8, v);
-}
-
 // x as two bf16 terms (exact to 2^-17 of it).
 struct Terms {
   uint2 hi, lo;
@@ -381,14 +364,14 @@ __global__ __launch_bounds__(256) void adapter_du_sum(const Adapters ad, const f
 
 // ------------------------------------------------------------------------------------------------------------
 // dB_a[v, r] = sum over adapter a's rows of dz[t, v] u[t, r].  One workgroup per 256 panel columns, adapter and 64 ranks, 64 columns a wave; M: rank,
-// N: column, both through LDS in steps of 32 rows.  u enters as its upper term alone: dz, the other factor, has been rounded to bf16 as well.
+// N: column, both through LDS in steps of 32 rows.  HBM: the panel once, 5.3 TB/s at 8192 rows x 76032 columns (235 us).
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kDbColumns = 256, kDbRows = 32, kDbRanks = 64;
 constexpr int kDbPitchD = kDbColumns * 2 + 16, kDbPitchU = kDbRanks * 2 + 16;
 __global__ __launch_bounds__(256) void adapter_db(const AdapterPanel p, const uint16_t* __restrict__ U, const int* __restrict__ seg, int row0,
                                                   const float* sum_in, float* sum_out, uint16_t* __restrict__ dB) {
   __shared__ __attribute__((aligned(16))) char lds_d[2][kDbRows * kDbPitchD];
-  __shared__ __attribute__((aligned(16))) char lds_u[2][kDbRows * kDbPitchU];
+  __shared__ __attribute__((aligned(16))) char lds_u[2][2 * kDbRows * kDbPitchU];  // the upper terms' rows, then the lower ones'
   const int T = tokens_in_force(p.T, p.T_dev);
   const int tid = threadIdx.x, lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -401,7 +384,7 @@ __global__ __launch_bounds__(256) void adapter_db(const AdapterPanel p, const ui
   for (int m = 0; m < 4; ++m)
 #pragma unroll
     for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  u32x4 d[4], u;
+  u32x4 d[4], u[2];
   const int u_row = tid >> 3, u_rank = r0 + (tid & 7) * 8;
   auto load = [&](int t) {
 #pragma unroll
@@ -409,7 +392,10 @@ __global__ __launch_bounds__(256) void adapter_db(const AdapterPanel p, const ui
       const int piece = j * 256 + tid, row = t + (piece >> 5);
       d[j] = *(const u32x4*)(p.D + (size_t)(row < end ? row : end - 1) * (size_t)p.ldd + c0 + (piece & 31) * 8);
     }
-    u = t + u_row < end && u_rank < Rp ? *(const u32x4*)(U + (size_t)(1 + t + u_row) * (size_t)(2 * Rp) + u_rank) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int term = 0; term < 2; ++term)
+      u[term] = t + u_row < end && u_rank < Rp ? *(const u32x4*)(U + (size_t)(1 + t + u_row) * (size_t)(2 * Rp) + term * Rp + u_rank)
+                                               : u32x4{0u, 0u, 0u, 0u};
   };
   if (begin < end) load(begin);
   int turn = 0;
@@ -420,7 +406,8 @@ __global__ __launch_bounds__(256) void adapter_db(const AdapterPanel p, const ui
       const int piece = j * 256 + tid;
       *(u32x4*)(at_d + (piece >> 5) * kDbPitchD + (piece & 31) * 16) = d[j];
     }
-    *(u32x4*)(at_u + u_row * kDbPitchU + (tid & 7) * 16) = u;
+#pragma unroll
+    for (int term = 0; term < 2; ++term) *(u32x4*)(at_u + (term * kDbRows + u_row) * kDbPitchU + (tid & 7) * 16) = u[term];
     if (t + kDbRows < end) load(t + kDbRows);
     __syncthreads();
     bf16x8 df[4];
@@ -429,9 +416,12 @@ __global__ __launch_bounds__(256) void adapter_db(const AdapterPanel p, const ui
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       if (r0 + m * 16 >= R) continue;
-      const bf16x8 uf = transposed(at_u + m * 32, kDbPitchU);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) acc[m][n] = mfma(uf, df[n], acc[m][n]);
+      for (int term = 0; term < 2; ++term) {
+        const bf16x8 uf = transposed(at_u + term * kDbRows * kDbPitchU + m * 32, kDbPitchU);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[m][n] = mfma(uf, df[n], acc[m][n]);
+      }
     }
   }
 #pragma unroll
@@ -461,7 +451,8 @@ __global__ __launch_bounds__(256) void adapter_db(const AdapterPanel p, const ui
 
 // ------------------------------------------------------------------------------------------------------------
 // d_hidden[row_map[t], :] += A_a^T du_t.  One workgroup per 64 tokens and 64 hidden columns, 16 tokens a wave.  M: hidden column (A's rows through
-// LDS), N: token.  d_hidden holds the product with the weight, rounded to bf16; the sum is rounded once more.
+// LDS), N: token.  d_hidden holds the product with the weight, rounded to bf16; the sum is rounded once more.  Only for the small vocabularies whose
+// weight is transposed (reads_weight_in_place); elsewhere lmhead_dh_reduce adds the adapters' part in fp32.
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kDhPitch = 64 * 2 + 16;
 __global__ __launch_bounds__(256) void adapter_dh_add(const Adapters ad, const uint16_t* __restrict__ dU, const int* __restrict__ ids, int T_,
@@ -664,7 +655,7 @@ hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float*
 hipError_t launch_adapter_finish(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const uint16_t* dU, const int* ids32, const int* seg,
                                  int64_t T, const int* T_dev, const int* row_map, int64_t H, uint16_t* d_hidden, float* da_part, uint16_t* dA) {
   const unsigned ranks = (unsigned)(padded_rank(ad.rank) / 32);
-  hipLaunchKernelGGL(adapter_dh_add, dim3((unsigned)((T + 63) / 64), (unsigned)(H / 64)), dim3(256), 0, s, ad, dU, ids32, (int)T, T_dev, row_map, (int)H,
+  if (d_hidden) hipLaunchKernelGGL(adapter_dh_add, dim3((unsigned)((T + 63) / 64), (unsigned)(H / 64)), dim3(256), 0, s, ad, dU, ids32, (int)T, T_dev, row_map, (int)H,
                      d_hidden);
   hipLaunchKernelGGL(adapter_da_partial, dim3((unsigned)adapter_da_pieces(T, ad.N), (unsigned)((H + 255) / 256), ranks), dim3(256), 0, s, ad, hidden, ldh, dU,
                      seg, (int)H, da_part);

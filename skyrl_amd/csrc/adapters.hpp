@@ -167,6 +167,23 @@ struct AdapterTerms {
   }
 };
 
+typedef __attribute__((ext_vector_type(8))) short i16x8;
+typedef __attribute__((address_space(3))) i16x4* lds_half_ptr;
+
+__device__ __forceinline__ f32x4 mfma(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// The transposed fragment whose 32 rows of `pitch` bytes begin at `at` (LDS), at the columns that `at` points to.
+__device__ __forceinline__ bf16x8 transposed(const char* at, int pitch) {
+  const int lane = threadIdx.x & 63, kq = lane >> 4, s = lane & 15;
+  const uint32_t addr = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)at + (uint32_t)((kq * 8 + (s >> 2)) * pitch + (s & 3) * 8);
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half_ptr)(uintptr_t)addr);
+  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_half_ptr)(uintptr_t)(addr + 4u * (uint32_t)pitch));
+  const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(bf16x8, v);
+}
+
 // ---- launches (adapter_tiles.hip) ----
 
 struct AdapterFwdArgs {
@@ -246,7 +263,7 @@ constexpr int kDuPiece = 128;  // rows of one adapter whose du a workgroup forms
 // Pieces of at most `size` rows that T rows of N adapters are cut in, at most.
 inline int64_t row_pieces(int64_t T, int64_t N, int64_t size) { return T / size + (N < T ? N : T); }
 inline int64_t adapter_da_pieces(int64_t T, int64_t N) { return row_pieces(T, N, kDaPiece); }
-// d_hidden += A^T du through row_map, and dA [N, rank, H]; da_part: [adapter_da_pieces][padded rank][H] fp32.
+// d_hidden (when not NULL) += A^T du through row_map, and dA [N, rank, H]; da_part: [adapter_da_pieces][padded rank][H] fp32.
 hipError_t launch_adapter_finish(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const uint16_t* dU, const int* ids32, const int* seg,
                                  int64_t T, const int* T_dev, const int* row_map, int64_t H, uint16_t* d_hidden, float* da_part, uint16_t* dA);
 

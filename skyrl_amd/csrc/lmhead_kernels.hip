@@ -833,17 +833,21 @@ struct DhReduceArgs {
   const int *T_dev, *splits_dev, *row_map;  // as in GemmArgs
   uint16_t* C;
   int ldc;
+  // The adapters' part (adapters.hpp): A^T du is added to every sum, of one slab too, before it is rounded.
+  Adapters ad;
+  const uint16_t* dU;
+  const int* ids;
 };
 constexpr int kReduceGroups = NWAVES * TM;  // workgroups per tile
 
-template <bool SHARES>
+template <bool SHARES, bool ADAPTERS = false>
 __global__ __launch_bounds__(256) void lmhead_dh_reduce(const DhReduceArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t rows[MT][WN + 8];
   const int splits = a.splits_dev ? *a.splits_dev : a.splits;
   const int M = a.T_dev ? *a.T_dev : a.M;
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (a.H + BN - 1) / BN, tiles = tiles_m * tiles_n;
   const int tile = blockIdx.x / kReduceGroups, wave = blockIdx.x / TM % NWAVES, i = blockIdx.x % TM;
-  if (splits < 2 || tile >= tiles) return;  // without splits the GEMM epilogue has written C
+  if ((!ADAPTERS && splits < 2) || tile >= tiles) return;  // without splits the GEMM epilogue has written C
   // Splits: the slabs of a tile stand `tiles` apart, in row order; shares: `groups` apart, in the launch's order.
   int tm = tile / tiles_n, tn = tile % tiles_n, count = splits, step = tiles, slot = tile;
   if (SHARES && splits >= 256) {
@@ -851,7 +855,7 @@ __global__ __launch_bounds__(256) void lmhead_dh_reduce(const DhReduceArgs a) {
     const int in_group = tile / sh.groups, g = tile - in_group * sh.groups, bg = sh.tiles_of(g, tiles), first = sh.first_workgroup(in_group, bg);
     count = __builtin_amdgcn_readfirstlane(sh.last_workgroup(in_group, bg) - first + 1), step = __builtin_amdgcn_readfirstlane(sh.groups);
     slot = __builtin_amdgcn_readfirstlane(sh.slot(g, in_group, first));
-    if (count < 2) return;  // one workgroup made the tile, and its epilogue has written C
+    if (!ADAPTERS && count < 2) return;  // one workgroup made the tile, and its epilogue has written C
     banded_tile(tile, tiles_m, tiles_n, kGroupM, tm, tn);
   }
   const int m0 = tm * BM + wave / WAVES_N * WM + i * MT;
@@ -867,6 +871,47 @@ __global__ __launch_bounds__(256) void lmhead_dh_reduce(const DhReduceArgs a) {
     sum[1] += *(const f32x4*)(part + (size_t)s * slab + 1024);
   }
   const int lane = tid & 63, lrow = lane & 15, kq = lane >> 4;
+  if constexpr (ADAPTERS) {
+    // M: the 16 tokens, N: hidden column (A's rows through LDS); the accumulator layout is that of the slabs.
+    constexpr int kPitch = WN * 2 + 16;
+    __shared__ __attribute__((aligned(16))) char lds[32 * kPitch];
+    const int Rp = padded_rank(a.ad.rank), t = m0 + lrow;
+    const int id = t < M ? a.ids[t] : -1;
+    const uint16_t* du = a.dU + (size_t)(1 + (t < M ? t : M - 1)) * (size_t)(2 * Rp) + kq * 8;
+    int id_of[4];  // of the tokens whose sums this lane holds
+#pragma unroll
+    for (int r = 0; r < 4; ++r) id_of[r] = __shfl(id, kq * 4 + r, 64);
+    unsigned left = (unsigned)__ballot(id >= 0) & 0xffffu;  // alike in all waves
+    while (left) {
+      const int one = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+      left &= ~(unsigned)__ballot(id == one);
+      const uint16_t* Aa = a.ad.A + (size_t)one * (size_t)a.ad.a_adapter;
+      f32x4 more[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      for (int k = 0; k < Rp; k += 32) {
+        u32x4 x[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {  // 32 rows of 256 bytes
+          const int e = j * 256 + tid, row = k + (e >> 4), h = n0 + (e & 15) * 8;
+          x[j] = row < a.ad.rank && h < a.H ? *(const u32x4*)(Aa + (size_t)row * (size_t)a.ad.a_row + h) : u32x4{0u, 0u, 0u, 0u};
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) *(u32x4*)(lds + ((j * 256 + tid) >> 4) * kPitch + (tid & 15) * 16) = x[j];
+        __syncthreads();
+        const bf16x8 hi = *(const bf16x8*)(du + k), lo = *(const bf16x8*)(du + Rp + k);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bf16x8 f = transposed(lds + (u * 4 + (tid >> 6)) * MT * 2, kPitch);
+          more[u] = mfma(hi, f, more[u]);
+          more[u] = mfma(lo, f, more[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[u][r] = id_of[r] == one ? sum[u][r] + more[u][r] : sum[u][r];
+    }
+  }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const bf16x4 b4 = __builtin_convertvector(sum[u], bf16x4);
@@ -1617,14 +1662,22 @@ inline bool few_token_dw(bool want_dw, bool adds, int64_t T, int64_t H, int64_t 
 }
 
 // The sum over the slabs of a split dHidden contraction; g is the GEMM of the last chunk, split the problem that its splits are chosen with.
-hipError_t launch_dh_reduce(hipStream_t s, const GemmArgs& g, const SplitProblem& split) {
+// adapters: with their part, from the slabs of whatever launch that left all of its sums there.
+hipError_t launch_dh_reduce(hipStream_t s, const GemmArgs& g, const SplitProblem& split, const DhReduceArgs* adapters = nullptr) {
+  if (adapters) {
+    Timed timed(kDhReduce, s);
+    DhReduceArgs a{g.P, g.M, g.N, g.splits, g.T_dev, g.splits_dev, g.row_map, g.Cb, g.ldc, adapters->ad, adapters->dU, adapters->ids};
+    hipLaunchKernelGGL((split.shares ? lmhead_dh_reduce<true, true> : lmhead_dh_reduce<false, true>), dim3((unsigned)(gemm_tiles(g) * kReduceGroups)),
+                       dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
   if (!g.splits_dev && g.splits < 2) return hipSuccess;
   // a problem with more tiles than slots is never split, and without shares none with more than half as many
   const int64_t tiles = gemm_tiles(g), slots = split.shares ? split.slots : split.slots / 2, most = g.splits_dev && slots < tiles ? slots : tiles;
   if (most < 1) return hipSuccess;
   Timed timed(kDhReduce, s);
-  hipLaunchKernelGGL(split.shares ? lmhead_dh_reduce<true> : lmhead_dh_reduce<false>, dim3((unsigned)(most * kReduceGroups)), dim3(256), 0, s,
-                     DhReduceArgs{g.P, g.M, g.N, g.splits, g.T_dev, g.splits_dev, g.row_map, g.Cb, g.ldc});
+  hipLaunchKernelGGL((split.shares ? lmhead_dh_reduce<true, false> : lmhead_dh_reduce<false, false>), dim3((unsigned)(most * kReduceGroups)), dim3(256), 0, s,
+                     DhReduceArgs{g.P, g.M, g.N, g.splits, g.T_dev, g.splits_dev, g.row_map, g.Cb, g.ldc, Adapters{}, nullptr, nullptr});
   return hipGetLastError();
 }
 
@@ -1862,14 +1915,22 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
                                          moved ? gw.n_tail : 0x7fffffff, gw.n_back, cf, cb, ncu});
       if (e != hipSuccess) return (int)e;
     }
+    if (ab && w_in_place) gh.p_last = 0;  // every sum stays in its slab: the adapters' part is added before the rounding
     e = launch_bwd_gemm(s, gh, gw, split);
-    if (e == hipSuccess && last) e = launch_dh_reduce(s, gh, split);
-    if (e != hipSuccess) return (int)e;
-  }
-  if (ab) {
-    Timed timed(kAdapterFinish, s);
-    e = launch_adapter_du_sum(s, ab->call.ad, ab->du_part, (int)(nchunks * ab->ranges), Tb, T_dev, adapters.ids,
-                              ab->dU + (size_t)row0 * 2 * padded_rank(ab->call.ad.rank));
+    if (ab && last && e == hipSuccess) {
+      uint16_t* const dU = ab->dU + (size_t)row0 * 2 * padded_rank(ab->call.ad.rank);
+      {
+        Timed timed(kAdapterFinish, s);
+        e = launch_adapter_du_sum(s, ab->call.ad, ab->du_part, (int)(nchunks * ab->ranges), Tb, T_dev, adapters.ids, dU);
+      }
+      if (e == hipSuccess && w_in_place) {
+        DhReduceArgs part{};
+        part.ad = ab->call.ad, part.dU = dU, part.ids = adapters.ids;
+        e = launch_dh_reduce(s, gh, split, &part);
+      }
+    } else if (e == hipSuccess && last) {
+      e = launch_dh_reduce(s, gh, split);
+    }
     if (e != hipSuccess) return (int)e;
   }
   if (resid) {
@@ -1980,8 +2041,8 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
   }
   if (ab) {
     Timed timed(kAdapterFinish, s);
-    e = launch_adapter_finish(s, ab->call.ad, w.hidden_c, H, ab->dU, ab->call.ids32, ab->seg, T, w.counts, w.idx, H, (uint16_t*)d_hidden, ab->da_part,
-                              ab->dA);
+    e = launch_adapter_finish(s, ab->call.ad, w.hidden_c, H, ab->dU, ab->call.ids32, ab->seg, T, w.counts, w.idx, H,
+                              reads_weight_in_place(V) ? nullptr : (uint16_t*)d_hidden, ab->da_part, ab->dA);
     if (e != hipSuccess) return (int)e;
   }
   return SKYRL_LMHEAD_OK;
