@@ -6,6 +6,7 @@
 // and the transposing read: lane (kq, s) supplies row kq * 8 + half * 4 + (s >> 2), columns (s & 3) * 4 .. + 3 of the 16, and receives column s
 // of the eight rows kq * 8 .. + 7.
 #include "adapters.hpp"
+#include "dh_reduce.hpp"
 
 namespace lmhead {
 namespace {
@@ -649,6 +650,11 @@ hipError_t launch_adapter_panel(hipStream_t s, const AdapterPanel& p, int ranges
 hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float* part, int slots, int64_t T, const int* T_dev, const int* ids32, uint16_t* dU) {
   const int Rp = padded_rank(ad.rank);
   hipLaunchKernelGGL(adapter_du_sum, dim3((unsigned)((T * (Rp / 4) + 15) / 16)), dim3(256), 0, s, ad, part, slots, (int)T, T_dev, ids32, Rp, dU);
+  return hipGetLastError();
+}
+
+hipError_t launch_adapter_dh_reduce(hipStream_t s, const DhReduceArgs& a, bool shares, int tiles) {
+  hipLaunchKernelGGL((shares ? lmhead_dh_reduce<true, true> : lmhead_dh_reduce<false, true>), dim3((unsigned)(tiles * kReduceGroups)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
