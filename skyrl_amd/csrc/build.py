@@ -6,6 +6,7 @@ Usage: ``python -m skyrl_amd.csrc.build`` (or ``build()`` from Python).  The lib
 
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -43,16 +44,28 @@ def build(verbose: bool = False, extra_flags=(), out: str | None = None) -> str:
     if not os.path.exists(hipcc):
         raise RuntimeError("hipcc not found: the fused LM-head library can only be built with the ROCm toolchain")
     out = out or lib_path()
-    # Compile into a temporary name and rename, so a failed build never leaves a half-written library behind.
-    fd, tmp = tempfile.mkstemp(suffix=".so", dir=os.path.dirname(out) or ".")
-    os.close(fd)
-    cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, "-o", tmp, *[os.path.join(HERE, s) for s in SOURCES]]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        os.unlink(tmp)
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    # The sources side by side into a temporary folder, and the library under a temporary name that is renamed, so a failed build never leaves a
+    # half-written one behind.
+    flags = [f for f in (*HIPCC_FLAGS, *extra_flags) if f != "-shared"]
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+
+    with tempfile.TemporaryDirectory() as objects:
+        targets = [os.path.join(objects, s + ".o") for s in SOURCES]
+        with concurrent.futures.ThreadPoolExecutor(8) as pool:
+            list(pool.map(run, [[hipcc, *flags, "-c", "-o", o, os.path.join(HERE, s)] for s, o in zip(SOURCES, targets)]))
+        fd, tmp = tempfile.mkstemp(suffix=".so", dir=os.path.dirname(out) or ".")
+        os.close(fd)
+        try:
+            run([hipcc, *flags, "-shared", "-o", tmp, *targets])
+        except RuntimeError:
+            os.unlink(tmp)
+            raise
     os.replace(tmp, out)
     os.chmod(out, 0o755)
     return out
