@@ -133,6 +133,64 @@ __global__ __launch_bounds__(256) void adapter_label(const Adapters ad, const ui
   if (part == 3 && to.row_pz) to.row_pz[row] = from.row_pz[t];
 }
 
+// A token's dz is of order g in its label's column and of order g p elsewhere, so what the rounding to bf16 takes from that one value is most of the
+// error of its gradients: 2.3e-3 to 2.5e-3 of dB's norm, where rounding the result alone takes 1.7e-3, which is what this leaves.  dz is linear in
+// (g, q): both are multiplied by the factor, within 2^-8 of 1, that makes the label's value a bf16 number, and what is formed from the row is divided by
+// it: du and d_hidden in fp32 (`back`), dB through the two terms of U_back.  Rows without an adapter stay as they are and get the bits that the head
+// without adapters gives.  The label's value is formed anew, one wave a token, from a row of the weight and one of B: latency, 3 us of 446 at 96 tokens.
+__global__ __launch_bounds__(256) void adapter_fit_rows(const Adapters ad, const uint16_t* __restrict__ hidden, const uint16_t* __restrict__ weight, int64_t ldw,
+                                                        const int64_t* __restrict__ labels, const int* __restrict__ ids, const float* __restrict__ lse,
+                                                        const float* __restrict__ pz, int T_, const int* __restrict__ T_dev, int H, int V, float rcp_temp,
+                                                        const uint16_t* __restrict__ U, float* __restrict__ g, float* __restrict__ q,
+                                                        float* __restrict__ back, uint16_t* __restrict__ U_back) {
+  const int T = tokens_in_force(T_, T_dev), lane = threadIdx.x & 63;
+  const int t = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (t >= T) return;
+  const int Rp = padded_rank(ad.rank), a = ids[t];
+  const int64_t y = labels[t];
+  const uint16_t* u = U + (size_t)(1 + t) * (size_t)(2 * Rp);
+  auto wide = [](uint16_t x) { return __uint_as_float((uint32_t)x << 16); };
+  float inverse = 1.f;
+  if (a >= 0 && y >= 0 && y < V) {
+    const uint16_t *w = weight + (size_t)y * (size_t)ldw, *h = hidden + (size_t)t * (size_t)H;
+    float z = 0.f;
+    for (int c = lane * 8; c < H; c += 64 * 8) {
+      const u32x4 x = *(const u32x4*)(w + c), v = *(const u32x4*)(h + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        z = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(v[i] << 16), z);
+        z = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(v[i] & 0xffff0000u), z);
+      }
+    }
+    const uint16_t* b = ad.B + (size_t)a * (size_t)ad.b_adapter + (size_t)y * (size_t)ad.b_row;
+    for (int r = lane; r < ad.rank; r += 64) z = fmaf(wide(u[r]) + wide(u[Rp + r]), wide(b[r]), z);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o, 64);
+    const float gt = g[t], qt = q ? q[t] : 0.f;
+    const float p = __builtin_amdgcn_exp2f((z * rcp_temp - lse[t]) * kLog2e);
+    const float c0 = -(gt - (q ? qt * pz[t] : 0.f)) * rcp_temp, c1 = -qt * rcp_temp * rcp_temp;
+    const float d = fmaf(p, fmaf(c1, z, c0), gt * rcp_temp);
+    if (fabsf(d) > 0x1p-100f && fabsf(d) < 0x1p100f) {  // neither NaN nor infinite, and so is what follows
+      const float fit = (float)(__bf16)d;
+      inverse = d / fit;
+      if (lane == 0) {
+        g[t] = gt * (fit / d);
+        if (q) q[t] = qt * (fit / d);
+      }
+    }
+  }
+  if (lane == 0) back[t] = inverse;
+  uint16_t* to = U_back + (size_t)(1 + t) * (size_t)(2 * Rp);
+  for (int r = lane * 4; r < Rp; r += 64 * 4) {
+    const uint2 hi = *(const uint2*)(u + r), lo = *(const uint2*)(u + Rp + r);
+    const f32x4 x = {__uint_as_float(hi.x << 16) + __uint_as_float(lo.x << 16), __uint_as_float(hi.x & 0xffff0000u) + __uint_as_float(lo.x & 0xffff0000u),
+                     __uint_as_float(hi.y << 16) + __uint_as_float(lo.y << 16), __uint_as_float(hi.y & 0xffff0000u) + __uint_as_float(lo.y & 0xffff0000u)};
+    const Terms terms = two_terms(x * inverse);
+    *(uint2*)(to + r) = terms.hi;
+    *(uint2*)(to + Rp + r) = terms.lo;
+  }
+}
+
 // Rows of the hidden states (and labels) in the order of idx.
 __global__ __launch_bounds__(256) void adapter_gather_rows(const int* __restrict__ idx, const uint16_t* __restrict__ hidden, int64_t ldh, int H,
                                                            const int64_t* __restrict__ labels, uint16_t* __restrict__ hidden_c, int64_t* __restrict__ labels_c) {
@@ -335,10 +393,10 @@ __global__ __launch_bounds__(256) void adapter_du_partial(const AdapterPanel p, 
   }
 }
 
-// du = s * (the sum of `slots` partial sums) as two bf16 terms, rows of U's form.  Sixteen threads share the slots of four ranks of a token, in an
+// du = s * back * (the sum of `slots` partial sums) as two bf16 terms, rows of U's form.  Sixteen threads share the slots of four ranks of a token, in an
 // order that the number of slots alone determines.
 __global__ __launch_bounds__(256) void adapter_du_sum(const Adapters ad, const float* __restrict__ part, int slots, int T_, const int* T_dev,
-                                                      const int* __restrict__ ids, int Rp, uint16_t* __restrict__ dU) {
+                                                      const int* __restrict__ ids, const float* __restrict__ back, int Rp, uint16_t* __restrict__ dU) {
   __shared__ f32x4 sums[16][16];
   const int T = tokens_in_force(T_, T_dev);
   const int q = threadIdx.x & 15, share = threadIdx.x >> 4;
@@ -357,7 +415,7 @@ __global__ __launch_bounds__(256) void adapter_du_sum(const Adapters ad, const f
   if (share != 0 || t >= T) return;
 #pragma unroll
   for (int s = 1; s < 16; ++s) sum += sums[s][q];
-  const Terms terms = two_terms(sum * (a >= 0 ? ad.scaling[a] : 0.f));
+  const Terms terms = two_terms(sum * (a >= 0 ? ad.scaling[a] * back[t] : 0.f));
   uint16_t* to = dU + (size_t)(1 + t) * (size_t)(2 * Rp) + r;
   *(uint2*)to = terms.hi;
   *(uint2*)(to + Rp) = terms.lo;
@@ -451,13 +509,14 @@ __global__ __launch_bounds__(256) void adapter_db(const AdapterPanel p, const ui
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// d_hidden[row_map[t], :] += A_a^T du_t.  One workgroup per 64 tokens and 64 hidden columns, 16 tokens a wave.  M: hidden column (A's rows through
+// d_hidden[row_map[t], :] = back_t d_hidden[row_map[t], :] + A_a^T du_t.  One workgroup per 64 tokens and 64 hidden columns, 16 tokens a wave.  M: hidden column (A's rows through
 // LDS), N: token.  d_hidden holds the product with the weight, rounded to bf16; the sum is rounded once more.  Only for the small vocabularies whose
 // weight is transposed (reads_weight_in_place); elsewhere lmhead_dh_reduce adds the adapters' part in fp32.
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kDhPitch = 64 * 2 + 16;
 __global__ __launch_bounds__(256) void adapter_dh_add(const Adapters ad, const uint16_t* __restrict__ dU, const int* __restrict__ ids, int T_,
-                                                      const int* T_dev, const int* __restrict__ row_map, int H, uint16_t* __restrict__ d_hidden) {
+                                                      const int* T_dev, const int* __restrict__ row_map, const float* __restrict__ back, int H,
+                                                      uint16_t* __restrict__ d_hidden) {
   __shared__ __attribute__((aligned(16))) char lds[32 * kDhPitch];
   const int T = tokens_in_force(T_, T_dev), t0 = blockIdx.x * 64, h0 = blockIdx.y * 64;
   if (t0 >= T) return;
@@ -498,13 +557,14 @@ __global__ __launch_bounds__(256) void adapter_dh_add(const Adapters ad, const u
       for (int m = 0; m < 4; ++m) sum[m] = acc[m];
     }
   }
-  if (id < 0) return;
+  if (t >= T) return;
+  const float by = back[t];
   uint16_t* to = d_hidden + (size_t)row_map[t] * (size_t)H + h0 + kq * 4;
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     const uint2 w = *(const uint2*)(to + m * 16);
-    const f32x4 x = {sum[m][0] + __uint_as_float(w.x << 16), sum[m][1] + __uint_as_float(w.x & 0xffff0000u), sum[m][2] + __uint_as_float(w.y << 16),
-                     sum[m][3] + __uint_as_float(w.y & 0xffff0000u)};
+    const f32x4 x = {fmaf(by, __uint_as_float(w.x << 16), sum[m][0]), fmaf(by, __uint_as_float(w.x & 0xffff0000u), sum[m][1]),
+                     fmaf(by, __uint_as_float(w.y << 16), sum[m][2]), fmaf(by, __uint_as_float(w.y & 0xffff0000u), sum[m][3])};
     const bf16x4 b = __builtin_convertvector(x, bf16x4);
     *(uint2*)(to + m * 16) = *(const uint2*)&b;
   }
@@ -618,6 +678,14 @@ hipError_t launch_adapter_label(hipStream_t s, const Adapters& ad, const uint16_
   return hipGetLastError();
 }
 
+hipError_t launch_adapter_fit_rows(hipStream_t s, const Adapters& ad, const uint16_t* hidden, const uint16_t* weight, int64_t ldw, const int64_t* labels,
+                                   const int* ids32, const float* lse, const float* pz, int64_t T, const int* T_dev, int64_t H, int64_t V, float rcp_temp,
+                                   const uint16_t* U, float* g, float* q, float* back, uint16_t* U_back) {
+  hipLaunchKernelGGL(adapter_fit_rows, dim3((unsigned)((T + 3) / 4)), dim3(256), 0, s, ad, hidden, weight, ldw, labels, ids32, lse, pz, (int)T, T_dev, (int)H,
+                     (int)V, rcp_temp, U, g, q, back, U_back);
+  return hipGetLastError();
+}
+
 hipError_t launch_adapter_gather_rows(hipStream_t s, const int* idx, const uint16_t* hidden, int64_t ldh, int64_t T, int64_t H, const int64_t* labels,
                                       uint16_t* hidden_c, int64_t* labels_c) {
   hipLaunchKernelGGL(adapter_gather_rows, dim3((unsigned)T), dim3(256), 0, s, idx, hidden, ldh, (int)H, labels, hidden_c, labels_c);
@@ -647,9 +715,10 @@ hipError_t launch_adapter_panel(hipStream_t s, const AdapterPanel& p, int ranges
   return hipGetLastError();
 }
 
-hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float* part, int slots, int64_t T, const int* T_dev, const int* ids32, uint16_t* dU) {
+hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float* part, int slots, int64_t T, const int* T_dev, const int* ids32,
+                                 const float* back, uint16_t* dU) {
   const int Rp = padded_rank(ad.rank);
-  hipLaunchKernelGGL(adapter_du_sum, dim3((unsigned)((T * (Rp / 4) + 15) / 16)), dim3(256), 0, s, ad, part, slots, (int)T, T_dev, ids32, Rp, dU);
+  hipLaunchKernelGGL(adapter_du_sum, dim3((unsigned)((T * (Rp / 4) + 15) / 16)), dim3(256), 0, s, ad, part, slots, (int)T, T_dev, ids32, back, Rp, dU);
   return hipGetLastError();
 }
 
@@ -659,10 +728,10 @@ hipError_t launch_adapter_dh_reduce(hipStream_t s, const DhReduceArgs& a, bool s
 }
 
 hipError_t launch_adapter_finish(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const uint16_t* dU, const int* ids32, const int* seg,
-                                 int64_t T, const int* T_dev, const int* row_map, int64_t H, uint16_t* d_hidden, float* da_part, uint16_t* dA) {
+                                 int64_t T, const int* T_dev, const int* row_map, const float* back, int64_t H, uint16_t* d_hidden, float* da_part, uint16_t* dA) {
   const unsigned ranks = (unsigned)(padded_rank(ad.rank) / 32);
-  if (d_hidden) hipLaunchKernelGGL(adapter_dh_add, dim3((unsigned)((T + 63) / 64), (unsigned)(H / 64)), dim3(256), 0, s, ad, dU, ids32, (int)T, T_dev, row_map, (int)H,
-                     d_hidden);
+  if (d_hidden) hipLaunchKernelGGL(adapter_dh_add, dim3((unsigned)((T + 63) / 64), (unsigned)(H / 64)), dim3(256), 0, s, ad, dU, ids32, (int)T, T_dev, row_map,
+                     back, (int)H, d_hidden);
   hipLaunchKernelGGL(adapter_da_partial, dim3((unsigned)adapter_da_pieces(T, ad.N), (unsigned)((H + 255) / 256), ranks), dim3(256), 0, s, ad, hidden, ldh, dU,
                      seg, (int)H, da_part);
   hipLaunchKernelGGL(adapter_da_sum, dim3((unsigned)ad.N, (unsigned)ad.rank), dim3(256), 0, s, (const float*)da_part, seg, (int)H, ad.rank, dA);

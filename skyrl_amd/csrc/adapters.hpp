@@ -239,6 +239,11 @@ hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float*
 hipError_t launch_adapter_gather_rows(hipStream_t s, const int* idx, const uint16_t* hidden, int64_t ldh, int64_t T, int64_t H, const int64_t* labels,
                                       uint16_t* hidden_c, int64_t* labels_c);
 
+// g and q (or NULL) of rows in place, times what makes the label's dz value a bf16 number; its inverse, and U times that in U's form.
+hipError_t launch_adapter_fit_rows(hipStream_t s, const Adapters& ad, const uint16_t* hidden, const uint16_t* weight, int64_t ldw, const int64_t* labels,
+                                   const int* ids32, const float* lse, const float* pz, int64_t T, const int* T_dev, int64_t H, int64_t V, float rcp_temp,
+                                   const uint16_t* U, float* g, float* q, float* back, uint16_t* U_back);
+
 // A chunk's dz panel, of rows grouped by adapter.
 struct AdapterPanel {
   Adapters ad;
@@ -256,15 +261,16 @@ int adapter_du_ranges(int64_t T, int64_t columns, int ncu);
 // panel's rows; row0: the place of the panel's first row among all rows that seg counts.
 hipError_t launch_adapter_panel(hipStream_t s, const AdapterPanel& p, int ranges, float* du_part, const uint16_t* U, const int* seg, int row0,
                                 const float* sum_in, float* sum_out, uint16_t* dB);
-hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float* part, int slots, int64_t T, const int* T_dev, const int* ids32, uint16_t* dU);
+hipError_t launch_adapter_du_sum(hipStream_t s, const Adapters& ad, const float* part, int slots, int64_t T, const int* T_dev, const int* ids32,
+                                 const float* back, uint16_t* dU);
 
 constexpr int kDaPiece = 256;  // rows whose dA is one sum
 constexpr int kDuPiece = 128;  // rows of one adapter whose du a workgroup forms
 // Pieces of at most `size` rows that T rows of N adapters are cut in, at most.
 inline int64_t row_pieces(int64_t T, int64_t N, int64_t size) { return T / size + (N < T ? N : T); }
 inline int64_t adapter_da_pieces(int64_t T, int64_t N) { return row_pieces(T, N, kDaPiece); }
-// d_hidden (when not NULL) += A^T du through row_map, and dA [N, rank, H]; da_part: [adapter_da_pieces][padded rank][H] fp32.
+// d_hidden (when not NULL) = back * d_hidden + A^T du through row_map, and dA [N, rank, H]; da_part: [adapter_da_pieces][padded rank][H] fp32.
 hipError_t launch_adapter_finish(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const uint16_t* dU, const int* ids32, const int* seg,
-                                 int64_t T, const int* T_dev, const int* row_map, int64_t H, uint16_t* d_hidden, float* da_part, uint16_t* dA);
+                                 int64_t T, const int* T_dev, const int* row_map, const float* back, int64_t H, uint16_t* d_hidden, float* da_part, uint16_t* dA);
 
 }  // namespace lmhead

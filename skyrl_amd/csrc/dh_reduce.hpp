@@ -23,10 +23,11 @@ struct DhReduceArgs {
   const int *T_dev, *splits_dev, *row_map;  // as in GemmArgs
   uint16_t* C;
   int ldc;
-  // The adapters' part (adapters.hpp): A^T du is added to every sum, of one slab too, before it is rounded.
+  // The adapters' part (adapters.hpp): every sum, of one slab too, is multiplied by back[token], and A^T du is added to it, before it is rounded.
   Adapters ad;
   const uint16_t* dU;
   const int* ids;
+  const float* back;
 };
 constexpr int kReduceGroups = NWAVES * TM;  // workgroups per tile
 
@@ -68,9 +69,15 @@ __global__ __launch_bounds__(256) void lmhead_dh_reduce(const DhReduceArgs a) {
     const int Rp = padded_rank(a.ad.rank), t = m0 + lrow;
     const int id = t < M ? a.ids[t] : -1;
     const uint16_t* du = a.dU + (size_t)(1 + (t < M ? t : M - 1)) * (size_t)(2 * Rp) + kq * 8;
+    const float by = a.back[t < M ? t : M - 1];
     int id_of[4];  // of the tokens whose sums this lane holds
 #pragma unroll
-    for (int r = 0; r < 4; ++r) id_of[r] = __shfl(id, kq * 4 + r, 64);
+    for (int r = 0; r < 4; ++r) {
+      id_of[r] = __shfl(id, kq * 4 + r, 64);
+      const float by_r = __shfl(by, kq * 4 + r, 64);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) sum[u][r] *= by_r;
+    }
     unsigned left = (unsigned)__ballot(id >= 0) & 0xffffu;  // alike in all waves
     while (left) {
       const int one = __builtin_amdgcn_readlane(id, __builtin_ctz(left));

@@ -1563,7 +1563,7 @@ hipError_t launch_dh_reduce(hipStream_t s, const GemmArgs& g, const SplitProblem
   if (adapters) {
     Timed timed(kDhReduce, s);
     return launch_adapter_dh_reduce(s, DhReduceArgs{g.P, g.M, g.N, g.splits, g.T_dev, g.splits_dev, g.row_map, g.Cb, g.ldc, adapters->ad, adapters->dU,
-                                                    adapters->ids},
+                                                    adapters->ids, adapters->back},
                                     split.shares != 0, (int)gemm_tiles(g));
   }
   if (!g.splits_dev && g.splits < 2) return hipSuccess;
@@ -1710,6 +1710,8 @@ struct AdapterBwd {
   int64_t* ids_c;      // [T]
   int* seg;            // [N + 2]
   uint16_t* dU;        // as U
+  uint16_t* U_back;    // as U, times back
+  float* back;         // [T], see adapter_fit_rows
   float *du_part, *da_part, *db_sum;  // db_sum only where there are several token blocks
   uint16_t *dA, *dB;
   int ranges;
@@ -1726,6 +1728,8 @@ AdapterBwd carve_adapter_bwd(void* ws, const Adapters& ad, int64_t T, int64_t H,
   w.seg = c.take<int>((size_t)ad.N + 2);
   w.call.U = c.take<uint16_t>((size_t)(T + 1) * (size_t)(2 * Rp));
   w.dU = c.take<uint16_t>((size_t)(T + 1) * (size_t)(2 * Rp));
+  w.U_back = c.take<uint16_t>((size_t)(T + 1) * (size_t)(2 * Rp));
+  w.back = c.take<float>((size_t)T);
   w.du_part = c.take<float>((size_t)(chunks * w.ranges) * (size_t)Tb * (size_t)Rp);
   w.da_part = c.take<float>((size_t)adapter_da_pieces(T, ad.N) * (size_t)Rp * (size_t)H);
   w.db_sum = bwd_num_blocks(T) > 1 ? c.take<float>((size_t)ad.N * (size_t)V * (size_t)ad.rank) : nullptr;
@@ -1781,7 +1785,7 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
       Timed timed(kAdapterPanel, s);
       const AdapterPanel panel{ab->call.ad, w.D, (int)(vcw + kLdPad), (int)Tb, T_dev, adapters.ids, (int)vc0, (int)vcw, (int)V, tail};
       float* const part = ab->du_part + (size_t)(ci * ab->ranges) * (size_t)Tb * (size_t)padded_rank(ab->call.ad.rank);
-      e = launch_adapter_panel(s, panel, ab->ranges, part, adapters.U, ab->seg, (int)row0, row0 > 0 ? ab->db_sum : nullptr,
+      e = launch_adapter_panel(s, panel, ab->ranges, part, ab->U_back + (size_t)row0 * 2 * padded_rank(ab->call.ad.rank), ab->seg, (int)row0, row0 > 0 ? ab->db_sum : nullptr,
                                last_block ? nullptr : ab->db_sum, last_block ? ab->dB : nullptr);
       if (e != hipSuccess) return (int)e;
     }
@@ -1816,11 +1820,11 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
       uint16_t* const dU = ab->dU + (size_t)row0 * 2 * padded_rank(ab->call.ad.rank);
       {
         Timed timed(kAdapterFinish, s);
-        e = launch_adapter_du_sum(s, ab->call.ad, ab->du_part, (int)(nchunks * ab->ranges), Tb, T_dev, adapters.ids, dU);
+        e = launch_adapter_du_sum(s, ab->call.ad, ab->du_part, (int)(nchunks * ab->ranges), Tb, T_dev, adapters.ids, ab->back + row0, dU);
       }
       if (e == hipSuccess && w_in_place) {
         DhReduceArgs part{};
-        part.ad = ab->call.ad, part.dU = dU, part.ids = adapters.ids;
+        part.ad = ab->call.ad, part.dU = dU, part.ids = adapters.ids, part.back = ab->back + row0;
         e = launch_dh_reduce(s, gh, split, &part);
       }
     } else if (e == hipSuccess && last) {
@@ -1891,6 +1895,9 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
     Timed timed(kAdapterRows, s);
     e = launch_adapter_shrink(s, ab->call.ad, w.hidden_c, H, ab->ids_c, T, w.counts, H, ab->call.U, ab->call.ids32);
     if (e != hipSuccess) return (int)e;
+    e = launch_adapter_fit_rows(s, ab->call.ad, w.hidden_c, Wp, ld_weight, w.labels_c, ab->call.ids32, w.lse_c, dentropy ? w.pz_c : nullptr, T, w.counts, H, V,
+                                rcp_temperature, ab->call.U, w.g_c, dentropy ? w.q_c : nullptr, ab->back, ab->U_back);
+    if (e != hipSuccess) return (int)e;
   }
   if (!reads_weight_in_place(V)) {  // weight^T [H, Vpad], zero in the padding columns
     Timed timed(kTranspose, s);
@@ -1936,7 +1943,7 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
   }
   if (ab) {
     Timed timed(kAdapterFinish, s);
-    e = launch_adapter_finish(s, ab->call.ad, w.hidden_c, H, ab->dU, ab->call.ids32, ab->seg, T, w.counts, w.idx, H,
+    e = launch_adapter_finish(s, ab->call.ad, w.hidden_c, H, ab->dU, ab->call.ids32, ab->seg, T, w.counts, w.idx, ab->back, H,
                               reads_weight_in_place(V) ? nullptr : (uint16_t*)d_hidden, ab->da_part, ab->dA);
     if (e != hipSuccess) return (int)e;
   }

@@ -377,3 +377,37 @@ def test_refusals_of_the_python_entry_points(cuda_device):
         AD.adapter_logits(*x)
     with pytest.raises(ValueError):
         AD.stack_adapters([], [])
+
+
+@pytest.mark.parametrize("V", [300, 2049])  # d_hidden of a transposed weight, and of one that is read in place
+@pytest.mark.parametrize("entropy_grad", [False, True])
+def test_the_labels_part_of_the_gradients_is_not_rounded_before_the_result(V, entropy_grad, cuda_device):
+    """One token per adapter.  The label's value makes up nearly all of a token's gradients, so its rounding would scale them, by up to e.  The scale
+    of a result is its projection on the true one: the roundings of its n elements are independent and at most e each (rms e / sqrt 3), so the
+    projection is off by 6 * 0.58 e / sqrt(n) at most, n >= 128, twice that variance where d_hidden is rounded twice (n = 256): 0.31 e.  The other
+    columns' roundings add at most e * |p| (the norm of a token's probabilities, below 0.1 for 300 columns): 0.1 e."""
+    T, H, R = 40, 256, 128
+    *x, gen = make(T, H, V, T, R, seed=V, b_scale=0.02)
+    x[1] = (x[1].float() / 4).to(torch.bfloat16)  # logits of about 0.5: p is flat
+    x[5] = torch.arange(T)
+    labels, g = torch.randperm(V, generator=gen)[:T], torch.randn(T, generator=gen)
+    q = 0.1 * torch.randn(T, generator=gen) if entropy_grad else None
+    leaves = [t.double().requires_grad_() for t in (x[0], x[2], x[3])]
+    z = plain_logits(leaves[0], x[1], leaves[1], leaves[2], x[4], x[5])
+    lps = torch.log_softmax(z, dim=1)
+    loss = (lps[torch.arange(T), labels] * g.double()).sum()
+    if entropy_grad:
+        loss = loss - (lps.exp() * lps).sum(1) @ q.double()
+    want = torch.autograd.grad(loss, leaves)
+    assert float(lps.exp().norm(dim=1).max()) < 0.1
+    d, y = on(cuda_device, *x), labels.to(cuda_device)
+    _, _, lse, pz = AD.lmhead_adapter_fwd(d[0], d[1], y, *d[2:], 1.0)
+    got = AD.lmhead_adapter_bwd(d[0], d[1], y, *d[2:], lse, pz, g.to(cuda_device), None if q is None else q.to(cuda_device), 1.0)
+    rows = torch.arange(T)
+    for mine, true in zip(got, want):
+        mine, true = mine.cpu().double(), true
+        if mine.shape[1] == V:  # dB: the label's row
+            mine, true = mine[rows, labels], true[rows, labels]
+        mine, true = mine.flatten(1), true.flatten(1)
+        scale = (mine * true).sum(1) / (true * true).sum(1)
+        assert float((scale - 1).abs().max()) <= 0.41 * E, float((scale - 1).abs().max() / E)
