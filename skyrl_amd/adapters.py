@@ -30,6 +30,7 @@ __all__ = ["MAX_RANK", "stack_adapters", "adapter_logits", "adapter_logprobs_fro
            "lmhead_adapter_bwd"]
 
 MAX_RANK = 256  # SKYRL_LMHEAD_MAX_ADAPTER_RANK
+_MAX_PITCH = 1 << 22  # elements between rows that the kernels can walk
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
@@ -58,8 +59,13 @@ def _check(hidden, weight, lora_a, lora_b, scaling, adapter_ids) -> Tuple[int, i
 
 
 def _adapter_args(lora_a, lora_b, scaling, adapter_ids, N: int, R: int):
-    return (lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1), lora_b.data_ptr(), lora_b.stride(0), lora_b.stride(1), scaling.data_ptr(),
-            adapter_ids.data_ptr(), N, R)
+    V, H = lora_b.shape[1], lora_a.shape[2]  # the stride of a dimension of one may be anything
+    return (lora_a.data_ptr(), lora_a.stride(0) if N > 1 else R * H, lora_a.stride(1), lora_b.data_ptr(), lora_b.stride(0) if N > 1 else V * R,
+            _pitch(lora_b[0]), scaling.data_ptr(), adapter_ids.data_ptr(), N, R)
+
+
+def _pitch(rows: torch.Tensor) -> int:
+    return int(rows.stride(0) if rows.shape[0] > 1 else rows.shape[1])
 
 
 def _workspace(lib, nbytes: int, dev: torch.device, what: str) -> torch.Tensor:
@@ -80,7 +86,7 @@ def lmhead_adapter_logits(hidden: torch.Tensor, weight: torch.Tensor, lora_a: to
     lib = _lib.load()
     ws = _workspace(lib, int(lib.skyrl_lmhead_adapter_logits_workspace_bytes(T, H, N, R)), dev, f"T={T}, H={H}, N={N}, rank={R}")
     with device_guard(dev):
-        st = lib.skyrl_lmhead_adapter_logits(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0),
+        st = lib.skyrl_lmhead_adapter_logits(hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight),
                                              *_adapter_args(lora_a, lora_b, scaling, adapter_ids, N, R), T, H, V, int(fp32), out.data_ptr(), V,
                                              ws.data_ptr(), ws.numel(), raw_stream(dev))
     _lib.check(st, "skyrl_lmhead_adapter_logits")
@@ -107,7 +113,7 @@ def lmhead_adapter_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch
     lib = _lib.load()
     ws = _workspace(lib, int(lib.skyrl_lmhead_adapter_fwd_workspace_bytes(T, H, V, N, R)), dev, f"T={T}, H={H}, V={V}, N={N}, rank={R}")
     with device_guard(dev):
-        st = lib.skyrl_lmhead_adapter_fwd(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), labels.data_ptr(),
+        st = lib.skyrl_lmhead_adapter_fwd(hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), labels.data_ptr(),
                                           *_adapter_args(lora_a, lora_b, scaling, adapter_ids, N, R), T, H, V, float(rcp_temperature), lp.data_ptr(),
                                           ent.data_ptr(), lse.data_ptr(), pz.data_ptr(), ws.data_ptr(), ws.numel(), raw_stream(dev))
     _lib.check(st, "skyrl_lmhead_adapter_fwd")
@@ -142,7 +148,7 @@ def lmhead_adapter_bwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch
     lib = _lib.load()
     ws = _workspace(lib, int(lib.skyrl_lmhead_adapter_bwd_workspace_bytes(T, H, V, N, R)), dev, f"T={T}, H={H}, V={V}, N={N}, rank={R}")
     with device_guard(dev):
-        st = lib.skyrl_lmhead_adapter_bwd(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), labels.data_ptr(),
+        st = lib.skyrl_lmhead_adapter_bwd(hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), labels.data_ptr(),
                                           *_adapter_args(lora_a, lora_b, scaling, adapter_ids, N, R), row_lse.data_ptr(), _ptr(row_pz),
                                           dlogprobs.data_ptr(), _ptr(dentropy), T, H, V, float(rcp_temperature), dh.data_ptr(), da.data_ptr(),
                                           db.data_ptr(), ws.data_ptr(), ws.numel(), raw_stream(dev))
@@ -179,7 +185,12 @@ class _AdapterLogprobs(torch.autograd.Function):
 def _rows(hidden: torch.Tensor, adapter_ids: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if adapter_ids.shape != hidden.shape[:-1]:
         raise ValueError(f"adapter_ids {tuple(adapter_ids.shape)} do not match hidden {tuple(hidden.shape)}")
-    return hidden.reshape(-1, hidden.shape[-1]), adapter_ids.reshape(-1).to(torch.int64).contiguous()
+    if adapter_ids.dtype.is_floating_point:
+        raise TypeError(f"adapter_ids must be integers, got {adapter_ids.dtype}")
+    rows = hidden.reshape(-1, hidden.shape[-1])
+    if not rows.shape[1] <= _pitch(rows) <= _MAX_PITCH:  # the last position of each long sequence, or one row repeated
+        rows = rows.contiguous()
+    return rows, adapter_ids.reshape(-1).to(torch.int64).contiguous()
 
 
 def adapter_logits(hidden: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: torch.Tensor,

@@ -174,7 +174,7 @@ __device__ __noinline__ void fill_with_nan(int V, int k, int64_t* ids, float* lo
 }
 
 // One workgroup per row and part (PARTS: grid.y of them).
-// Bound by HBM on fp32 logits, by the vector instructions (an exponential, the comparisons, widening) on bf16: 2048 x 152064 fp32, k = 5, 228 us (5.5
+// Bound by HBM on fp32 logits, by the vector instructions (an exponential, the comparisons, widening) on bf16: 2048 x 152064 fp32, k = 5, 217 us (5.7
 // TB/s); 4096 x 151936 bf16, k = 32, 322 us (3.9 TB/s), of which 36 are the ranks and candidates.  What brought it there from 510: one running maximum
 // a wave and votes per four pieces instead of one (437), keys formed only where a logit reaches the bound (394), no memory for
 // arguments of a call (322).  Loading a step ahead changed nothing (328 to 358): two or three workgroups a CU overlap enough.

@@ -411,3 +411,26 @@ def test_the_labels_part_of_the_gradients_is_not_rounded_before_the_result(V, en
         mine, true = mine.flatten(1), true.flatten(1)
         scale = (mine * true).sum(1) / (true * true).sum(1)
         assert float((scale - 1).abs().max()) <= 0.41 * E, float((scale - 1).abs().max() / E)
+
+
+def test_last_positions_of_long_sequences_and_dimensions_of_one(cuda_device):
+    """Rows further apart than the kernels walk, one row repeated, and strides that mean nothing."""
+    *x, gen = make(2, 128, 300, 1, 8, "one", seed=8)
+    h, w, a, b, s, ids = on(cuda_device, *x)
+    y = torch.randint(0, 300, (2,), generator=gen).to(cuda_device)
+    want = AD.adapter_logits(h, w, a, b, s, ids)
+    long = torch.zeros((2, 40000, 128), dtype=torch.bfloat16, device=cuda_device)
+    long[:, -1] = h
+    assert torch.equal(AD.adapter_logits(long[:, -1], w, a, b, s, ids), want)
+    assert torch.equal(AD.adapter_logits(long[:1, -1], w, a, b, s, ids[:1]), want[:1])
+    odd = lambda t: t.as_strided(t.shape, (3,) + t.stride()[1:])  # noqa: E731  a first dimension of one
+    assert torch.equal(AD.adapter_logits(odd(h[:1]), w, odd(a), odd(b), s, ids[:1]), want[:1])
+    one = AD.adapter_logits(h, odd(w[:1]), a, b[:, :1].as_strided((1, 1, 8), (8, 3, 1)), s, ids)
+    assert float((one.float() - want[:, :1].float()).abs().max()) <= 2 * E * float(want[:, :1].abs().max()) + 1e-3
+    row = h[:1].clone().requires_grad_()
+    rows = h[:1].expand(2, 128).contiguous().requires_grad_()
+    for leaf, use in ((row, lambda: row.expand(2, 128)), (rows, lambda: rows)):
+        AD.adapter_logprobs_from_hidden(use(), w, y, a, b, s, ids)[0].sum().backward()
+    assert float((row.grad.float() - rows.grad.float().sum(0)).abs().max()) <= E * float(rows.grad.abs().float().sum(0).max())
+    with pytest.raises(TypeError):
+        AD.adapter_logits(h, w, a, b, s, ids.float())
