@@ -549,9 +549,11 @@ int check_top(int64_t V, int64_t k) {
   return k < 0 || k > V || k > kMaxTop ? SKYRL_LMHEAD_ERR_SHAPE : SKYRL_LMHEAD_OK;
 }
 
-// Parts of a row: so many that 1024 workgroups, four a CU, share the logits, of at least 8192 logits each.
+// Parts of a row: so many that 512 workgroups share the logits, of at least 8192 logits each, and none for rows so short that the second launch costs
+// what the parts save.  Without / with parts, both launches, bf16, k = 20: 8 x 151936 27.5 / 13.1 us, 64 rows 29.8 / 17.6, 255 rows 34.1 / 33.4, 512 rows 43.5 / 49
+// (two parts); 8 x 32001 11.8 / 13.1, 255 x 32001 12.9 / 16.0.  With 1024 workgroups 64 rows take 20.5 us, with 2048 22.1.
 int top_parts(int64_t T, int64_t V, int64_t k) {
-  int64_t n = 1024 / T;
+  int64_t n = V < 6 * 8192 ? 1 : 512 / T;
   if (n > V / 8192) n = V / 8192;
   if (n > kMaxParts) n = kMaxParts;
   if (k > 0 && n > kMaxJoin / k) n = kMaxJoin / k;

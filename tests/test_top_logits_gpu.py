@@ -91,7 +91,7 @@ SIZES = [
     (1, 1, 1, torch.float32), (1, 1, 5, torch.bfloat16), (3, 2, 0, torch.bfloat16), (64, 7, 7, torch.float32), (5, 129, 128, torch.bfloat16),
     (3, 511, 20, torch.float32), (4, 4095, 64, torch.bfloat16), (2, 16384, 33, torch.bfloat16), (2, 16385, 1, torch.float32),
     (17, 20011, 20, torch.bfloat16), (1, 151936, 20, torch.bfloat16), (9, 152064, 128, torch.float32), (300, 32001, 5, torch.bfloat16),
-    (1, 600000, 40, torch.bfloat16),
+    (1, 600000, 40, torch.bfloat16), (40, 50021, 128, torch.bfloat16), (255, 49152, 3, torch.float32), (257, 49999, 20, torch.bfloat16),
 ]
 
 
@@ -108,8 +108,9 @@ def test_against_64_bits(T, V, k, dtype, cuda_device):
 @pytest.mark.parametrize("k", [1, 20, 128])
 @pytest.mark.parametrize("kind", ["constant", "ascending", "descending", "few values", "zeros of both signs", "all but one masked", "masked",
                                   "fewer than k", "empty", "nan", "nan and masked", "all nan", "huge", "one huge"])
-def test_rows_that_select_badly(kind, k, cuda_device):
-    T, V = 6, 33001
+@pytest.mark.parametrize("V", [33001, 66001])  # a workgroup for a row; eight of them, and their join
+def test_rows_that_select_badly(kind, k, V, cuda_device):
+    T = 6
     logits, labels, gen = make(T, V, torch.float32, 5)
     ramp = torch.arange(V, dtype=torch.float32) / 1000
     if kind == "constant":
@@ -262,9 +263,10 @@ def test_same_bits_on_each_call_and_on_another_stream(cuda_device):
             assert all(torch.equal(a, b) for a, b in zip(first, TU.top_logprobs_from_logits(d, y, 20)))
 
 
-def test_replays_from_a_graph(cuda_device):
+@pytest.mark.parametrize("V", [30001, 70001])
+def test_replays_from_a_graph(V, cuda_device):
     gen = torch.Generator().manual_seed(9)
-    d = torch.zeros(5, 30001, dtype=torch.bfloat16, device=cuda_device)
+    d = torch.zeros(5, V, dtype=torch.bfloat16, device=cuda_device)
     y = torch.zeros(5, dtype=torch.int64, device=cuda_device)
     h = torch.rand(5, 7, generator=gen).to(cuda_device)
 
@@ -282,7 +284,7 @@ def test_replays_from_a_graph(cuda_device):
     with torch.cuda.graph(graph):
         out = step()
     for i in range(4):
-        logits, labels, _ = make(5, 30001, torch.bfloat16, 100 + i)
+        logits, labels, _ = make(5, V, torch.bfloat16, 100 + i)
         d.copy_(logits)
         y.copy_(labels)
         graph.replay()
