@@ -479,7 +479,8 @@ int skyrl_logits_bwd(const void* logits, int logits_dtype, int64_t ld_logits, co
  *   skyrl_lmhead_adapter_logits  the logits themselves, logits [T, ld_logits] in bf16 or fp32 (SKYRL_LOGITS_*): decoding; temperature 1
  *   skyrl_lmhead_adapter_bwd     as skyrl_lmhead_bwd_active_rows without d_weight.  d_lora_a [num_adapters, rank, H] and d_lora_b [num_adapters,
  *     V, rank], bf16, contiguous, overwritten (zeros for adapters without a token that has a gradient).  dz is rounded to bf16 once, as
- *     without adapters, and every result once (d_hidden of a vocabulary below 1024 that is not a multiple of 128 twice).  Rows are worked on grouped by adapter, in an order that follows from
+ *     without adapters, but for the label's value of a token with an adapter, which is exact; every result is rounded once (d_hidden of a
+ *     vocabulary below 1024 that is not a multiple of 128 twice).  Rows are worked on grouped by adapter, in an order that follows from
  *     adapter_ids alone: the same bits on each call. */
 #define SKYRL_LMHEAD_MAX_ADAPTER_RANK 256
 size_t skyrl_lmhead_adapter_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t num_adapters, int64_t rank);

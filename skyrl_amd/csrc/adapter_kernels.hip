@@ -136,8 +136,8 @@ __global__ __launch_bounds__(256) void adapter_label(const Adapters ad, const ui
 // A token's dz is of order g in its label's column and of order g p elsewhere, so what the rounding to bf16 takes from that one value is most of the
 // error of its gradients: 2.3e-3 to 2.5e-3 of dB's norm, where rounding the result alone takes 1.7e-3, which is what this leaves.  dz is linear in
 // (g, q): both are multiplied by the factor, within 2^-8 of 1, that makes the label's value a bf16 number, and what is formed from the row is divided by
-// it: du and d_hidden in fp32 (`back`), dB through the two terms of U_back.  Rows without an adapter stay as they are and get the bits that the head
-// without adapters gives.  The label's value is formed anew, one wave a token, from a row of the weight and one of B: latency, 3 us of 446 at 96 tokens.
+// it: du and d_hidden in fp32 (`back`), dB through the two terms of U_back.  Rows without an adapter stay as they are, as in the head
+// without adapters.  The label's value is formed anew, one wave a token, from a row of the weight and one of B: latency, 3 us of 446 at 96 tokens.
 __global__ __launch_bounds__(256) void adapter_fit_rows(const Adapters ad, const uint16_t* __restrict__ hidden, const uint16_t* __restrict__ weight, int64_t ldw,
                                                         const int64_t* __restrict__ labels, const int* __restrict__ ids, const float* __restrict__ lse,
                                                         const float* __restrict__ pz, int T_, const int* __restrict__ T_dev, int H, int V, float rcp_temp,

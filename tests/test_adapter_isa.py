@@ -83,7 +83,7 @@ def faults(lines):
     return found
 
 
-def test_the_checker_finds_what_it_looks_for():
+def test_hazards_are_found_where_they_are():
     mfma = "v_mfma_f32_16x16x32_bf16 v[0:3], v[8:11], v[16:19], v[0:3]"
     assert not faults([mfma, mfma, "s_nop 10", "v_add_f32_e32 v9, v3, v4"]) and faults([mfma, "s_nop 9", "v_add_f32_e32 v9, v3, v4"])
     assert faults(["v_mov_b32_e32 v8, 0", "s_nop 0", mfma]) and not faults(["v_mov_b32_e32 v8, 0", "s_nop 1", mfma])
