@@ -10,8 +10,9 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
-__all__ = ["registered_op", "plain_eager", "call", "device_guard", "raw_stream"]
+__all__ = ["registered_op", "plain_eager", "direct", "has_tangent", "call", "device_guard", "raw_stream"]
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _NO_GUARD = contextlib.nullcontext()
@@ -48,20 +49,32 @@ def plain_eager() -> bool:
     return not (dispatch_modes() > 0 or function_modes() > 0 or transform() is not None or tracing() or profiling())
 
 
-def call(op, *args):
-    """``op(*args)``: the registered function itself in a plain eager call on real tensors, without a gradient to record.  Tensor
-    subclasses, tensors on the meta device and those whose memory is not their value (negative views, such as the imaginary part of a
-    conjugate, and autograd's zero tensors, which have none) go through the op, whose dispatcher layers know what to do with them.  So
-    does what autograd would record, also in a backward that is recorded itself (``create_graph=True``): the op knows its formula, or
-    that it has none and a second derivative must raise."""
+def direct(*args) -> bool:
+    """Whether a registered function may be given these arguments itself: a plain eager call on real tensors, without a gradient to
+    record.  Not so for tensor subclasses, tensors on the meta device and those whose memory is not their value (negative views, such
+    as the imaginary part of a conjugate, and autograd's zero tensors, which have none)."""
     if not plain_eager():
-        return op(*args)
+        return False
     grad = torch.is_grad_enabled()
     for a in args:
         if isinstance(a, torch.Tensor) and (type(a) not in _PLAIN or a.is_meta or (grad and a.requires_grad) or a.is_neg()
                                             or a._is_zerotensor()):
-            return op(*args)
-    return op.eager(*args)
+            return False
+    return True
+
+
+def has_tangent(*args) -> bool:
+    """Whether one of the tensors carries a tangent of forward-mode differentiation."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(isinstance(a, torch.Tensor) and forward_ad.unpack_dual(a).tangent is not None for a in args)
+
+
+def call(op, *args):
+    """``op(*args)``: the registered function itself where that is all there is to it (``direct``).  Everything else goes through the
+    op, whose dispatcher layers know what to do with it.  So does what autograd would record, also in a backward that is recorded
+    itself (``create_graph=True``): the op knows its formula, or that it has none and a second derivative must raise."""
+    return op.eager(*args) if direct(*args) else op(*args)
 
 
 def device_guard(dev: torch.device):

@@ -25,7 +25,7 @@ from typing import Any, NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from ._launch import call, device_guard, plain_eager, raw_stream, registered_op
+from ._launch import call, device_guard, direct, has_tangent, raw_stream, registered_op
 from .ops import _require_device as _require_device_all
 
 __all__ = ["logprobs_from_logits", "logprobs_from_logits_v2", "logprobs_from_logits_flash_attn", "chunked_entropy_from_logits",
@@ -385,10 +385,10 @@ def top_logprobs_from_logits(logits: torch.Tensor, labels: Optional[torch.Tensor
             raise ValueError(f"labels {tuple(labels.shape)} do not match logits {tuple(logits.shape)}")
         labels = labels.reshape(-1).to(torch.int64).contiguous()
     k, flat = min(k, V), _flat(logits)
-    if torch.is_grad_enabled() and flat.requires_grad or not plain_eager() or type(flat) not in (torch.Tensor, torch.nn.Parameter):
-        lp, ent, ranks, top, ids = _TopFromLogits.apply(flat, labels, k, 1.0 / temperature)
-    else:  # nothing follows the call: without autograd's function and what only a backward reads
+    if direct(flat, labels) and not has_tangent(flat):  # nothing follows the call: without autograd's function and what only a backward reads
         lp, ent, _, _, ranks, top, ids = _top_fwd(flat, labels, k, 1.0 / temperature, False)
+    else:
+        lp, ent, ranks, top, ids = _TopFromLogits.apply(flat, labels, k, 1.0 / temperature)
     if len(shape) == 1:
         return TokenLogprobs(lp, ent, ranks, top, ids)
     return TokenLogprobs(lp.reshape(shape), ent.reshape(shape), ranks.reshape(shape), top.reshape(shape + (k,)), ids.reshape(shape + (k,)))
