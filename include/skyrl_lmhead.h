@@ -477,7 +477,9 @@ int skyrl_logits_bwd(const void* logits, int logits_dtype, int64_t ld_logits, co
  * values of an adapter that it does not have, whether they are finite or not.
  *   skyrl_lmhead_adapter_fwd     as skyrl_lmhead_fwd
  *   skyrl_lmhead_adapter_logits  the logits themselves, logits [T, ld_logits] in bf16 or fp32 (SKYRL_LOGITS_*): decoding; temperature 1
- *   skyrl_lmhead_adapter_bwd     as skyrl_lmhead_bwd_active_rows without d_weight.  d_lora_a [num_adapters, rank, H] and d_lora_b [num_adapters,
+ *   skyrl_lmhead_adapter_bwd     as skyrl_lmhead_bwd_active_rows without d_weight, but that a label outside [0, V), whose log-probability is the
+ *     constant 0, takes no gradient from dlogprobs (the head without adapters, which may hold a shard of the vocabulary, keeps the softmax's
+ *     part there).  d_lora_a [num_adapters, rank, H] and d_lora_b [num_adapters,
  *     V, rank], bf16, contiguous, overwritten (zeros for adapters without a token that has a gradient).  dz is rounded to bf16 once, as
  *     without adapters, but for the label's value of a token with an adapter, which is exact; every result is rounded once (d_hidden of a
  *     vocabulary below 1024 that is not a multiple of 128 twice).  Rows are worked on grouped by adapter, in an order that follows from

@@ -208,8 +208,8 @@ def adapter_logits(hidden: torch.Tensor, weight: torch.Tensor, lora_a: torch.Ten
 def adapter_logprobs_from_hidden(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                                  scaling: torch.Tensor, adapter_ids: torch.Tensor, *, temperature: float = 1.0
                                  ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``(logprobs, entropy)``, fp32 ``hidden.shape[:-1]``, of ``labels`` (outside ``[0, V)``: log-probability 0) under ``softmax(z /
-    temperature)``.  Both carry gradients to ``hidden``, ``lora_a`` and ``lora_b`` (bf16); ``weight`` and ``scaling`` take none, and either that
+    """``(logprobs, entropy)``, fp32 ``hidden.shape[:-1]``, of ``labels`` (outside ``[0, V)``: log-probability 0, without a gradient) under
+    ``softmax(z / temperature)``.  Both carry gradients to ``hidden``, ``lora_a`` and ``lora_b`` (bf16); ``weight`` and ``scaling`` take none, and either that
     asks for one is refused."""
     temperature = float(temperature)
     if not 0.0 < temperature < float("inf"):

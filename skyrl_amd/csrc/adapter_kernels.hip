@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256) void adapter_gather_rows(const int* __restrict
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kGroupThreads = 1024, kGroupTokens = 4;  // tokens per thread and step
 __global__ __launch_bounds__(kGroupThreads) void adapter_group_rows(const float* __restrict__ g, const float* __restrict__ q,
-                                                                    const int64_t* __restrict__ ids, int T, int N, int* __restrict__ idx,
+                                                                    const int64_t* __restrict__ labels, int64_t V, const int64_t* __restrict__ ids, int T, int N, int* __restrict__ idx,
                                                                     int64_t* __restrict__ ids_c, int* __restrict__ seg) {
   constexpr int kCounts = kGroupTokens * kGroupThreads / 64;
   static_assert(kCounts == 64, "one lane per count");
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_group_rows(const float*
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mine = blockIdx.x;
   auto group_of = [&](int t) -> int {  // -1: no gradient
     if (t >= T) return -1;
-    const float gv = g ? g[t] : 1.f, qv = q ? q[t] : 0.f;
+    const float gv = g ? target_grad(g, labels, V, t) : 1.f, qv = q ? q[t] : 0.f;
     const int64_t x = ids[t];
     if (gv == 0.f && qv == 0.f) return -1;
     return x >= 0 && x < (int64_t)N ? (int)x : N;
@@ -692,8 +692,9 @@ hipError_t launch_adapter_gather_rows(hipStream_t s, const int* idx, const uint1
   return hipGetLastError();
 }
 
-hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float* q, const int64_t* ids, int64_t T, int N, int* idx, int64_t* ids_c, int* seg) {
-  hipLaunchKernelGGL(adapter_group_rows, dim3((unsigned)(N + 1)), dim3(kGroupThreads), 0, s, g, q, ids, (int)T, N, idx, ids_c, seg);
+hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float* q, const int64_t* labels, int64_t V, const int64_t* ids, int64_t T, int N,
+                                     int* idx, int64_t* ids_c, int* seg) {
+  hipLaunchKernelGGL(adapter_group_rows, dim3((unsigned)(N + 1)), dim3(kGroupThreads), 0, s, g, q, labels, V, ids, (int)T, N, idx, ids_c, seg);
   return hipGetLastError();
 }
 

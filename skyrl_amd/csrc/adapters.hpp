@@ -188,6 +188,12 @@ __device__ __forceinline__ bf16x8 transposed(const char* at, int pitch) {
   return __builtin_bit_cast(bf16x8, v);
 }
 
+// The gradient on token t's log-probability.  labels, where it is not NULL: 0 for a label outside [0, V), whose log-probability is the constant 0.
+__device__ __forceinline__ float target_grad(const float* g, const int64_t* labels, int64_t V, int t) {
+  if (labels && (labels[t] < 0 || labels[t] >= V)) return 0.f;
+  return g[t];
+}
+
 // ---- launches (adapter_tiles.hip) ----
 
 struct AdapterFwdArgs {
@@ -237,8 +243,9 @@ struct RowResults {
 // row_map[t] of `to`.
 hipError_t launch_adapter_label(hipStream_t s, const Adapters& ad, const uint16_t* U, const int* ids32, const int64_t* labels, int64_t T, int64_t V,
                                 float rcp_temp, const RowResults& from, const int* row_map, const RowResults& to);
-// The T rows whose g or q is not zero (all without g), grouped by adapter: idx, their ids and the groups' places, seg [N + 2].
-hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float* q, const int64_t* ids, int64_t T, int N, int* idx, int64_t* ids_c, int* seg);
+// The T rows whose g (by target_grad) or q is not zero (all without g), grouped by adapter: idx, their ids and the groups' places, seg [N + 2].
+hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float* q, const int64_t* labels, int64_t V, const int64_t* ids, int64_t T, int N,
+                                     int* idx, int64_t* ids_c, int* seg);
 // hidden_c [T, H] and labels_c (both or neither of the labels' pointers): the rows that idx names.
 hipError_t launch_adapter_gather_rows(hipStream_t s, const int* idx, const uint16_t* hidden, int64_t ldh, int64_t T, int64_t H, const int64_t* labels,
                                       uint16_t* hidden_c, int64_t* labels_c);

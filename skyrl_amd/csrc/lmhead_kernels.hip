@@ -977,7 +977,8 @@ __global__ __launch_bounds__(256) void split_operand_rows(const void* __restrict
 // dW and its dHidden row is zero.  In RL micro-batches those are the prompt and padding tokens the loss mask removes, often
 // more than half of the batch.  Two small kernels let the backward run on the remaining rows without the host ever
 // learning how many there are (no synchronisation, so the call can be captured in a HIP graph):
-//   compact_active_rows   one workgroup: idx[i] = i-th token with g != 0 or q != 0 (ascending), counts[0] = their number n,
+//   compact_active_rows   one workgroup: idx[i] = i-th token with g != 0 or q != 0 (ascending), counts[0] = their number n; with labels a g whose
+//                         label lies outside [0, V) counts as 0 (target_grad in adapters.hpp);
 //                         counts[1 + b] = how many of them fall into block b of `block` compacted rows,
 //                         counts[1 + nblocks + b] = how that block's dHidden contraction is cut: the number of splits, or, where
 //                         SplitProblem::shares admits it, a code of Shares, which only lmhead_bwd_dh_shares and lmhead_dh_reduce read
@@ -989,8 +990,9 @@ constexpr int kCompactThreads = 1024;
 
 template <int TOKENS>  // per thread and step
 __global__ __launch_bounds__(kCompactThreads) void compact_active_rows(const float* __restrict__ g, const float* __restrict__ q,
-                                                                       int T, int block, int nblocks, SplitProblem split,
-                                                                       int* __restrict__ idx, int* __restrict__ counts) {
+                                                                       const int64_t* __restrict__ labels, int64_t V, int T, int block,
+                                                                       int nblocks, SplitProblem split, int* __restrict__ idx,
+                                                                       int* __restrict__ counts) {
   // A step takes four tokens per thread: their loads travel together, and every wave scans the 64 counts of the step by itself, so that one
   // barrier stands between the counts and the list.  What bounds it is that chain: with a token per thread and the counts added up by one thread
   // 12.1 -> 7.7 us at T=8192, 6.7 -> 5.4 at 4096, 6.6 -> 5.2 at 2100.  Up to 1024 tokens, where it is the code that has to be fetched first, a
@@ -1006,7 +1008,7 @@ __global__ __launch_bounds__(kCompactThreads) void compact_active_rows(const flo
     for (int k = 0; k < TOKENS; ++k) {
       const int t = t0 + k * kCompactThreads + tid;
       const int tc = t < T ? t : T - 1;
-      const float gv = g[tc], qv = q ? q[tc] : 0.f;
+      const float gv = target_grad(g, labels, V, tc), qv = q ? q[tc] : 0.f;
       ballot[k] = __ballot(t < T && (gv != 0.f || qv != 0.f));
     }
 #pragma unroll
@@ -1058,11 +1060,13 @@ __global__ __launch_bounds__(kCompactThreads) void compact_active_rows(const flo
 inline auto compact_kernel(int64_t T) { return T <= kCompactThreads ? compact_active_rows<1> : compact_active_rows<4>; }
 
 // One workgroup per row r < T: as compacted row r (when r < n) it copies the inputs of token idx[r]; as token r it clears
-// d_hidden[r] -- active tokens get their row from the dHidden GEMM (or the sum over its splits) afterwards.
+// d_hidden[r] -- active tokens get their row from the dHidden GEMM (or the sum over its splits) afterwards.  targets: V, where labels outside
+// [0, V) take g's place away as in compact_active_rows; 0: g as it is.
 __global__ __launch_bounds__(256) void gather_active_rows(const int* __restrict__ idx, const int* __restrict__ counts,
                                                           const uint16_t* __restrict__ hidden, int ldh, int Hk, int H,
-                                                          const int64_t* __restrict__ labels, const float* __restrict__ lse,
-                                                          const float* __restrict__ pz, const float* __restrict__ g,
+                                                          const int64_t* __restrict__ labels, int64_t targets,
+                                                          const float* __restrict__ lse, const float* __restrict__ pz,
+                                                          const float* __restrict__ g,
                                                           const float* __restrict__ q, uint16_t* __restrict__ hidden_c,
                                                           int64_t* __restrict__ labels_c, float* __restrict__ lse_c,
                                                           float* __restrict__ pz_c, float* __restrict__ g_c,
@@ -1078,7 +1082,7 @@ __global__ __launch_bounds__(256) void gather_active_rows(const int* __restrict_
   if (threadIdx.x == 0) {
     labels_c[r] = labels[t];
     lse_c[r] = lse[t];
-    g_c[r] = g[t];
+    g_c[r] = target_grad(g, targets > 0 ? labels : nullptr, targets, t);
     if (q) q_c[r] = q[t], pz_c[r] = pz[t];
   }
 }
@@ -1880,14 +1884,16 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
   const SplitProblem rated = split_problem(Tb, H, vc, dw_in_gemm, w.slots, compute_units());
   if (compact) {
     Timed timed(kCompactRows, s);
-    hipLaunchKernelGGL(compact_kernel(T), dim3(1), dim3(kCompactThreads), 0, s, dlogprobs, dentropy, (int)T, (int)Tb,
+    // With adapters no shard of a vocabulary is meant: a label outside it is a constant log-probability, which has no gradient.
+    const int64_t* const targets = ab ? labels : nullptr;
+    hipLaunchKernelGGL(compact_kernel(T), dim3(1), dim3(kCompactThreads), 0, s, dlogprobs, dentropy, targets, V, (int)T, (int)Tb,
                        (int)nblocks, rated, w.idx, w.counts);
     if (ab) {  // the same rows in another order
-      e = launch_adapter_group_rows(s, dlogprobs, dentropy, ab->call.ids, T, ab->call.ad.N, w.idx, ab->ids_c, ab->seg);
+      e = launch_adapter_group_rows(s, dlogprobs, dentropy, targets, V, ab->call.ids, T, ab->call.ad.N, w.idx, ab->ids_c, ab->seg);
       if (e != hipSuccess) return (int)e;
     }
     hipLaunchKernelGGL(gather_active_rows, dim3((unsigned)T), dim3(256), 0, s, (const int*)w.idx, (const int*)w.counts, Hp,
-                       (int)ld_hidden, (int)Hk, (int)H, labels, row_lse, row_pz, dlogprobs, dentropy, w.hidden_c, w.labels_c,
+                       (int)ld_hidden, (int)Hk, (int)H, labels, ab ? V : (int64_t)0, row_lse, row_pz, dlogprobs, dentropy, w.hidden_c, w.labels_c,
                        w.lse_c, w.pz_c, w.g_c, w.q_c, (uint16_t*)d_hidden);
     if ((e = hipGetLastError()) != hipSuccess) return (int)e;
   }
@@ -2015,7 +2021,7 @@ size_t adapter_fwd_bytes(int64_t T, int64_t H, int64_t N, int64_t rank, bool sta
 hipError_t group_forward(hipStream_t s, AdapterForward& w, const void*& hidden, int64_t& ld_hidden, const int64_t** labels, int64_t T, int64_t H) {
   if (!group_rows(T, w.call.ad.N)) return hipSuccess;
   Timed timed(kAdapterRows, s);
-  hipError_t e = launch_adapter_group_rows(s, nullptr, nullptr, w.call.ids, T, w.call.ad.N, w.idx, w.ids_c, w.seg);
+  hipError_t e = launch_adapter_group_rows(s, nullptr, nullptr, nullptr, 0, w.call.ids, T, w.call.ad.N, w.idx, w.ids_c, w.seg);
   if (e != hipSuccess) return e;
   e = launch_adapter_gather_rows(s, w.idx, (const uint16_t*)hidden, ld_hidden, T, H, labels ? *labels : nullptr, w.hidden_c, w.labels_c);
   hidden = w.hidden_c, ld_hidden = H;
@@ -2353,7 +2359,7 @@ int skyrl_softce_bwd(const void* student_hidden, int64_t ld_student, const void*
   const SplitProblem split = split_problem(T, H, vc, false, w.slots, ncu);
   {  // tokens without an upstream gradient (what the supervision mask removes) have a zero row and take no part
     Timed timed(kCompactRows, s);
-    hipLaunchKernelGGL(compact_kernel(T), dim3(1), dim3(kCompactThreads), 0, s, dloss, (const float*)nullptr, (int)T, (int)T, 1,
+    hipLaunchKernelGGL(compact_kernel(T), dim3(1), dim3(kCompactThreads), 0, s, dloss, (const float*)nullptr, (const int64_t*)nullptr, (int64_t)0, (int)T, (int)T, 1,
                        split, w.idx, w.counts);
   }
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
