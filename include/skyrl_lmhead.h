@@ -510,7 +510,8 @@ int skyrl_lmhead_adapter_bwd(const void* hidden, int64_t ld_hidden, const void* 
  *     label among the alternatives stands at place rank - 1.
  *   top_ids int64 [T, k], top_logprobs fp32 [T, k], contiguous: best first.  0 <= k <= min(V, SKYRL_LOGITS_TOP_MAX).
  * A row without any logit above -inf has log-probabilities -inf (row_lse too), entropy and row_pz 0 and columns 0 .. k - 1; its gradient is
- * zero.  Any of logprobs, entropy, row_lse, row_pz and ranks may be NULL, top_ids and top_logprobs with k = 0.
+ * zero.  Finite logits of any size are logits: a row full of the type's lowest value is uniform.  row_lse and row_pz are then the nearest fp32
+ * values; the backward, where |row_lse| is 4096 and more, forms the row's statistics anew from the logits.  Any of logprobs, entropy, row_lse, row_pz and ranks may be NULL, top_ids and top_logprobs with k = 0.
  * skyrl_logits_top_bwd writes
  *   dlogits = ( g (onehot[label] - p) - dentropy p (y - row_pz) + sum_j dtop_j (onehot[top_ids_j] - p) ) * rcp_temperature
  * with g = dlogprobs where the label lies in [0, V) and 0 elsewhere (the log-probability is the constant 0 there).  dlogprobs, dentropy

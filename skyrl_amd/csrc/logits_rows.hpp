@@ -124,6 +124,58 @@ __device__ __forceinline__ Stats block_merge(Stats st, Stats* sm) {
   return all;
 }
 
+// Statistics keep y2 = z * log2e / temperature in fp32, whose step at m is up to |m| * 2^-24: from |m| = 2^24 on the largest logit's own
+// 2^(y2 - m) is anything, from about 2^31 on 0 or infinite, and y2 itself overflows for logits beyond 2.3e38 * temperature.  The row's logits
+// may be ordinary but for a mask of -1e10 that one wave has seen nothing else of: an infinite sum shows that.
+constexpr float kFar = 0x1p24f;
+__device__ __forceinline__ bool is_far(const Stats& st) { return !(fabsf(st.m) < kFar && st.s < INFINITY); }
+
+// Such a row's statistics from differences of logits, which do not overflow where it matters: m is the largest LOGIT, t = (z - m) * scale2, s = sum 2^t,
+// e = sum t 2^t.  By a whole workgroup in two passes; sm: 2 * WAVES floats of LDS that nothing else is in.  -inf, 0, 0 where no logit is above -inf.
+__device__ __forceinline__ float far_origin(float top) { return top > -INFINITY ? top : 0.f; }  // (-inf) minus it is -inf
+
+template <bool F32, int WAVES>
+__device__ __noinline__ Stats far_row(const char* base, int V, float scale2, float* sm) {
+  constexpr int E = Piece<F32>::kElems;
+  const RowPieces rp = row_pieces<F32>(base, V, true);
+  const char* vec = base + (size_t)rp.head * (F32 ? 4 : 2);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto each = [&](auto f) {
+    for (int p = tid; p < rp.pieces; p += WAVES * 64) {
+      Piece<F32> pc;
+      pc.load(vec + (size_t)p * 16);
+#pragma unroll
+      for (int i = 0; i < E; ++i) f(pc.v[i]);
+    }
+    for (int i = tid; i < rp.single; i += WAVES * 64) f(load_one(base, (size_t)single_column(rp, E, i), F32));
+  };
+  float top = -INFINITY, s = 0.f, e = 0.f;
+  each([&](float z) { top = fmaxf(top, z); });
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  __syncthreads();
+  if (lane == 0) sm[wave] = top;
+  __syncthreads();
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w]);
+  const float from = far_origin(top);
+  each([&](float z) {
+    const float t = (z - from) * scale2, p = __builtin_amdgcn_exp2f(t);
+    s += p;
+    e = fmaf(fmaxf(t, kMostNegativeFactor), p, e);
+  });
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64), e += __shfl_xor(e, o, 64);
+  __syncthreads();
+  if (lane == 0) sm[wave] = s, sm[WAVES + wave] = e;
+  __syncthreads();
+  s = e = 0.f;
+  for (int w = 0; w < WAVES; ++w) s += sm[w], e += sm[WAVES + w];
+  return Stats{top, s, e};
+}
+
+// The nearest finite value of a log-sum-exp or mean that may have left fp32.
+__device__ __forceinline__ float finite(float x) { return x == INFINITY ? 3.402823466e38f : x == -INFINITY ? -3.402823466e38f : x; }
+
 constexpr int64_t kCacheBytes = (int64_t)256 << 20;
 constexpr int64_t kMaxRows = (int64_t)1 << 31;  // the grid's x extent
 

@@ -95,6 +95,9 @@ struct Shared {
 };
 static_assert(kWaves * kMaxTop >= kThreads, "up to a candidate per thread without dropping any");
 
+// The maximum of a part whose logits all lie below kLowest: only where there is no logit above -inf it stays kLowest itself.
+constexpr float kFarPart = -2.9e38f;
+
 // A part's result: its statistics, the columns that sort before the label, and how many of its k keys there are, best first.
 struct Part {
   Stats st;
@@ -134,20 +137,33 @@ struct TopArgs {
   topkey_t* keys;
 };
 
-// The results of a row from its statistics and the number of columns before the label, by one thread; logprob_of for the alternatives.
+// The results of a row from its statistics (far: those of far_row) and the number of columns before the label, by one thread; logprob_of for
+// the alternatives.
 struct RowResult {
-  bool empty;
-  float log_s, m, scale2;
-  __device__ __forceinline__ RowResult(const Stats& st, float scale2_) : empty(st.s == 0.f), m(st.m), scale2(scale2_) {
+  bool empty, far;
+  float log_s, m, scale2, rcp_temp;
+  __device__ __forceinline__ RowResult(const Stats& st, float rcp_temp_, bool far_)
+      : empty(!far_ && st.s == 0.f), far(far_), m(st.m), scale2(rcp_temp_ * kLog2e), rcp_temp(rcp_temp_) {
     log_s = empty ? -INFINITY : logf(st.s);
   }
-  __device__ __forceinline__ float logprob_of(float z) const { return empty ? -INFINITY : fmaf(z, scale2, -m) * kLn2 - log_s; }
+  __device__ __forceinline__ float logprob_of(float z) const {
+    if (empty) return -INFINITY;
+    const bool finite_z = fabsf(z) < INFINITY;
+    if (far) {
+      const float d = z - m;
+      return (finite_z && fabsf(d) == INFINITY ? z * rcp_temp - m * rcp_temp : d * rcp_temp) - log_s;
+    }
+    const float t = fmaf(z, scale2, -m);
+    if (finite_z && fabsf(t) == INFINITY) return z * rcp_temp - fmaf(m, kLn2, log_s);  // y in base 2 overflows before y does
+    return t * kLn2 - log_s;
+  }
   __device__ __forceinline__ void write(const TopArgs& a, int64_t row, const Stats& st, bool has_label, float z_label, int before) const {
     if (a.ranks) a.ranks[row] = has_label && z_label == z_label ? 1 + before : 0;
     if (a.logprobs) a.logprobs[row] = has_label ? logprob_of(z_label) : 0.f;
     if (a.entropy) a.entropy[row] = empty ? 0.f : log_s - st.e / st.s * kLn2;
-    if (a.row_lse) a.row_lse[row] = empty ? -INFINITY : fmaf(st.m, kLn2, log_s);
-    if (a.row_pz) a.row_pz[row] = empty ? 0.f : (st.e / st.s + st.m) * kLn2;
+    const float mean = st.e / st.s;
+    if (a.row_lse) a.row_lse[row] = empty ? -INFINITY : far ? finite(fmaf(m, rcp_temp, log_s)) : fmaf(m, kLn2, log_s);
+    if (a.row_pz) a.row_pz[row] = empty ? 0.f : far ? finite(fmaf(m, rcp_temp, mean * kLn2)) : (mean + m) * kLn2;
   }
 };
 
@@ -232,7 +248,9 @@ __global__ __launch_bounds__(kThreads, 6) void logits_top_rows(const TopArgs a) 
   auto raise_wave_max = [&](float z) {  // to the largest z of the wave
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) z = fmaxf(z, __shfl_xor(z, o, 64));
-    raise_max(st, z * scale2);
+    const float y2 = z * scale2;
+    // Where a row is far, above its logits: a wave that has seen nothing but a mask of -1e10 must not bring an infinite sum to the others' logits.
+    raise_max(st, fabsf(y2) < kFar ? y2 : fmaf(fabsf(y2), 0x1p-22f, y2));
   };
 
   int step = 0;
@@ -313,6 +331,7 @@ __global__ __launch_bounds__(kThreads, 6) void logits_top_rows(const TopArgs a) 
     const float z = load_one(base, (size_t)c, F32);
     raise_wave_max(there ? z : -INFINITY);
     if (there) {
+      lane_max = fmaxf(lane_max, z);
       absorb<true>(st, z, scale2);
       better += z >= above_label || (z == z_label && c < y) ? 1 : 0;
     }
@@ -327,7 +346,12 @@ __global__ __launch_bounds__(kThreads, 6) void logits_top_rows(const TopArgs a) 
   }
   if (lane == 0) sm.count[wave] = count, sm.better[wave] = better;
   st = block_merge<kWaves>(st, sm.stats);  // a barrier: the lists and counts of all waves stand
-  const RowResult result(st, scale2);
+  const bool far = is_far(st) && __syncthreads_or(lane_max > -INFINITY ? 1 : 0) != 0;  // else it is empty, or its logits are NaN and -inf
+  if (far) {
+    if (!PARTS) st = far_row<F32, kWaves>(base, V, scale2, (float*)sm.stats);
+    else if (st.m == kLowest) st.m = kFarPart;
+  }
+  const RowResult result(st, a.rcp_temp, far);
   int total = 0, before = 0, mine_at = 0;
   for (int w = 0; w < kWaves; ++w) {
     if (w == wave) mine_at = total;
@@ -365,6 +389,7 @@ __global__ __launch_bounds__(kJoinThreads) void logits_top_join(const TopArgs a,
   __shared__ topkey_t firsts[kMaxTop + kMaxParts];
   __shared__ topkey_t bound;
   __shared__ int have[kMaxParts], kept;
+  __shared__ float far_sums[2 * kJoinThreads / 64];
   const int tid = threadIdx.x, k = a.k;
   const int64_t row = blockIdx.x;
   const char* base = (const char*)a.logits + (size_t)row * (size_t)a.ld * (F32 ? 4 : 2);
@@ -392,7 +417,9 @@ __global__ __launch_bounds__(kJoinThreads) void logits_top_join(const TopArgs a,
     const int p = e / each, i = e - p * each;
     firsts[e] = i < have[p] ? a.keys[(row * parts + p) * (int64_t)k + i] : 0;
   }
-  const RowResult result(st, a.rcp_temp * kLog2e);
+  const bool far = is_far(st) && !(st.m == kLowest && st.s == 0.f);
+  if (far) st = far_row<F32, kJoinThreads / 64>(base, a.V, a.rcp_temp * kLog2e, far_sums);
+  const RowResult result(st, a.rcp_temp, far);
   if (tid == 0) {
     const int64_t label = a.labels ? a.labels[row] : (int64_t)-1;
     const bool has_label = label >= 0 && label < (int64_t)a.V;
@@ -440,10 +467,14 @@ struct TopBwdArgs {
   int64_t ldd;
 };
 
+// From this size on the fp32 log-sum-exp costs p more than 2^-12 of its value (the rounding of lse, and of lse in base 2): such a row's statistics are
+// formed anew, and its gradient from differences of logits.  No model's row, but a row that a mask of finite values has all of.
+constexpr float kFarLse = 4096.f;
+
 template <bool F32, bool ENTGRAD, bool NONTEMPORAL>
 __global__ __launch_bounds__(kBwdThreads) void logits_top_bwd_rows(const TopBwdArgs a) {
   constexpr int E = Piece<F32>::kElems, ES = F32 ? 4 : 2;
-  __shared__ float h_sum[kBwdThreads / 64];
+  __shared__ float h_sum[kBwdThreads / 64], far_sums[2 * kBwdThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = (int64_t)(gridDim.x - 1 - blockIdx.x);  // the rows that the forward read last first
   const int V = a.V, k = a.dtop ? a.k : 0;
@@ -492,6 +523,22 @@ __global__ __launch_bounds__(kBwdThreads) void logits_top_bwd_rows(const TopBwdA
   const bool empty = lse == -INFINITY;  // no logit above -inf: no gradient
   bool any = tid <= k && own_grad != 0.f;
   const bool zero_row = empty || (__syncthreads_or((any || all != 0.f || q != 0.f) ? 1 : 0) == 0);
+  if (!zero_row && fabsf(lse) >= kFarLse) {
+    const Stats st = far_row<F32, kBwdThreads / 64>(src, V, scale2, far_sums);
+    const float from = far_origin(st.m), rcp_s = st.s == 0.f ? 0.f : 1.f / st.s, mean = st.s == 0.f ? 0.f : st.e / st.s;
+    auto dz = [&](float z) {
+      const float t = (z - from) * scale2, p = __builtin_amdgcn_exp2f(t) * rcp_s;
+      return p * (-all - q * ((fmaxf(t, kMostNegativeFactor) - mean) * kLn2)) * a.rcp_temp;
+    };
+    auto write = [&](int64_t c, float d) {
+      if (F32) ((float*)dst)[c] = d;
+      else ((uint16_t*)dst)[c] = bf16_bits(d);
+    };
+    for (int c = tid; c < V; c += kBwdThreads) write(c, dz(load_one(src, (size_t)c, F32)));
+    __syncthreads();
+    if (writes && st.s != 0.f) write(own, fmaf(own_grad, a.rcp_temp, dz(own_z)));
+    return;
+  }
   auto dz = [&](float z) {
     const float p = __builtin_amdgcn_exp2f(fmaf(z, scale2, -lse2));
     return ENTGRAD ? p * fmaf(c1, fmaxf(z, kMostNegativeFactor), c0) : p * c0;

@@ -371,7 +371,8 @@ def top_logprobs_from_logits(logits: torch.Tensor, labels: Optional[torch.Tensor
     their log-probabilities, from one pass over the logits ``[..., V]`` (bf16 or fp32; anything else is cast to fp32).
 
     Equal logits sort by column, the lower first, and NaN behind everything: a label whose rank is at most ``k`` stands at
-    ``top_ids[..., rank - 1]``.  A row that a mask of ``-inf`` leaves empty has log-probabilities ``-inf``, entropy 0 and a zero gradient.
+    ``top_ids[..., rank - 1]``.  A row that a mask of ``-inf`` leaves empty has log-probabilities ``-inf``, entropy 0 and a zero gradient;
+    finite logits of any size, such as a mask of the type's lowest value, are taken as logits.
     ``k`` is at most ``MAX_ALTERNATIVES``; 0 gives ranks without alternatives.  ``labels`` may be ``None``.  Log-probabilities,
     alternatives' log-probabilities and entropy carry gradients to ``logits``."""
     if not isinstance(k, int) or isinstance(k, bool) or not 0 <= k <= MAX_ALTERNATIVES:
