@@ -23,7 +23,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._launch import call, device_guard, raw_stream, registered_op
+from ._launch import call, device_guard, has_tangent, raw_stream, registered_op
 from .ops import _ptr, _require_device
 
 __all__ = ["MAX_RANK", "stack_adapters", "adapter_logits", "adapter_logprobs_from_hidden", "lmhead_adapter_logits", "lmhead_adapter_fwd",
@@ -196,9 +196,13 @@ def _rows(hidden: torch.Tensor, adapter_ids: torch.Tensor) -> Tuple[torch.Tensor
 def adapter_logits(hidden: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: torch.Tensor,
                    adapter_ids: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """Logits ``hidden.shape[:-1] + (V,)`` in ``dtype`` (bf16 or fp32) of ``hidden [..., H]`` with the adapters of ``adapter_ids [...]``.
-    Not differentiable: for training see ``adapter_logprobs_from_hidden``."""
+    Not differentiable: operands that ask for a gradient are refused outside ``torch.no_grad()``, and those with a tangent; for training see
+    ``adapter_logprobs_from_hidden``."""
     if dtype not in _DTYPES:
         raise TypeError(f"logits are torch.bfloat16 or torch.float32, got {dtype}")
+    operands = (hidden, weight, lora_a, lora_b, scaling)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in operands) or has_tangent(*operands):
+        raise ValueError("adapter_logits has no gradient: call it under torch.no_grad(), or adapter_logprobs_from_hidden for training")
     rows, ids = _rows(hidden, adapter_ids)
     with torch.no_grad():
         out = call(lmhead_adapter_logits, rows, weight, lora_a, lora_b, scaling, ids, dtype == torch.float32)
