@@ -1449,7 +1449,8 @@ inline int64_t bwd_num_blocks(int64_t T) { return (T + kBwdTokenBlock - 1) / kBw
 
 // vc: chunk width for a block of bwd_block_tokens(T) tokens.  compact: the buffers of the row-compacting entry point.
 // Hk: length of the logits contraction, a multiple of H when the operands are stacked bf16 terms of fp32 values.
-BwdWorkspace lay_out_bwd(void* ws, int64_t T, int64_t H, int64_t Hk, int64_t V, int64_t vc, bool compact, int64_t slab_floats) {
+// sums_dw: room for dW summed over blocks; without it the call makes no dW.
+BwdWorkspace lay_out_bwd(void* ws, int64_t T, int64_t H, int64_t Hk, int64_t V, int64_t vc, bool compact, bool sums_dw, int64_t slab_floats) {
   const int64_t Tb = bwd_block_tokens(T), Tpad = round_up(Tb, 256), Vpad = round_up(V, 256);
   Carver c(ws);
   BwdWorkspace w{};
@@ -1459,7 +1460,7 @@ BwdWorkspace lay_out_bwd(void* ws, int64_t T, int64_t H, int64_t Hk, int64_t V, 
   w.dHacc = c.take<float>((size_t)slab_floats);  // dHidden partial sums in accumulator order, whole tiles
   w.D = c.take<uint16_t>((size_t)Tpad * (vc + kLdPad));
   // Several blocks and a bf16 dW: the sum over the blocks is kept in fp32 here and rounded once, by the last block.
-  w.dWsum = bwd_num_blocks(T) > 1 ? c.take<float>((size_t)V * (size_t)H) : nullptr;
+  w.dWsum = sums_dw && bwd_num_blocks(T) > 1 ? c.take<float>((size_t)V * (size_t)H) : nullptr;
   w.label_resid = Hk > H ? c.take<float>((size_t)Tpad) : nullptr;  // stacked terms: fp32 operands
   if (compact) {
     w.hidden_c = c.take<uint16_t>((size_t)T * (size_t)Hk);
@@ -1478,12 +1479,12 @@ BwdWorkspace lay_out_bwd(void* ws, int64_t T, int64_t H, int64_t Hk, int64_t V, 
 // The row-compacting entry point has more room for slabs: its token count, and with it the number of tiles, may be far below T.
 // A result whose `bytes` exceed ws_bytes does not fit.  own_chunk: the library's choice of vc, which leaves a caller nothing to size by
 // but a query, for this call or a longer one; the latter's has at least 1 MiB more, and less than that of slabs stays as it is.
-BwdWorkspace carve_bwd(void* ws, int64_t T, int64_t H, int64_t Hk, int64_t V, int64_t vc, bool compact, size_t ws_bytes, bool own_chunk) {
+BwdWorkspace carve_bwd(void* ws, int64_t T, int64_t H, int64_t Hk, int64_t V, int64_t vc, bool compact, bool sums_dw, size_t ws_bytes, bool own_chunk) {
   const int64_t Tb = bwd_block_tokens(T), more = compact ? T * H / 2 : 0;
   const int64_t wanted = slab_slots(Tb, H, vc) * kSlabTileFloats + more, least = dh_tiles(Tb, H) * kSlabTileFloats + more;
-  const BwdWorkspace w = lay_out_bwd(ws, T, H, Hk, V, vc, compact, wanted);
+  const BwdWorkspace w = lay_out_bwd(ws, T, H, Hk, V, vc, compact, sums_dw, wanted);
   if (w.bytes <= ws_bytes || (own_chunk && wanted - least < 4 * kSlabTileFloats)) return w;
-  return lay_out_bwd(ws, T, H, Hk, V, vc, compact, fitting_slabs(wanted, least, w.bytes - ws_bytes));
+  return lay_out_bwd(ws, T, H, Hk, V, vc, compact, sums_dw, fitting_slabs(wanted, least, w.bytes - ws_bytes));
 }
 
 GemmArgs make_gemm(const uint16_t* A, int64_t lda, int64_t a_rows, const uint16_t* B, int64_t ldb, int64_t b_rows, bool b_kmajor,
@@ -1700,12 +1701,12 @@ TopkWorkspace carve_topk(void* ws, int64_t T, int64_t V, int64_t k, size_t ws_by
   return w;
 }
 
-size_t bwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t vocab_chunk, bool compact, int64_t terms = 1) {
+size_t bwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t vocab_chunk, bool compact, int64_t terms = 1, bool sums_dw = true) {
   if (T < 1 || V < 1 || H < 1 || vocab_chunk < 0 || vocab_chunk % 256 != 0 || terms < 1 || terms > 3) return 0;
   if (T > kMaxExtent || V > kMaxExtent || H > kMaxExtent / 4 || vocab_chunk > kMaxExtent) return 0;
   int64_t vc = vocab_chunk ? vocab_chunk : default_vocab_chunk(bwd_block_tokens(T), H, V);
   if (vc > round_up(V, 256)) vc = round_up(V, 256);
-  return carve_bwd(nullptr, T, H, terms * H, V, vc, compact, SIZE_MAX, false).bytes;
+  return carve_bwd(nullptr, T, H, terms * H, V, vc, compact, sums_dw, SIZE_MAX, false).bytes;
 }
 
 // What the backward with adapters has besides: rows grouped by adapter (row compaction is always on), their u, and the room for the sums.
@@ -1868,9 +1869,9 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
   // Row pitches of the scratch matrices (weight^T, hidden^T, the dz panel) under the copy plan's limit; Hk <= ld_hidden is.
   if ((!reads_weight_in_place(V) && Vpad + kLdPad > kMaxRowPitch) || Tbpad + kLdPad > kMaxRowPitch || vc + kLdPad > kMaxRowPitch)
     return SKYRL_LMHEAD_ERR_SHAPE;
-  const size_t full = bwd_workspace_bytes(T, H, V, vc, compact, terms);
+  const size_t full = bwd_workspace_bytes(T, H, V, vc, compact, terms, !ab);
   if (!vocab_chunk && workspace_bytes < full) vc = fitting_chunk(vc, Tbpad, V, full - workspace_bytes);
-  const BwdWorkspace w = carve_bwd(workspace, T, H, Hk, V, vc, compact, workspace_bytes, !vocab_chunk);
+  const BwdWorkspace w = carve_bwd(workspace, T, H, Hk, V, vc, compact, !ab, workspace_bytes, !vocab_chunk);
   if (!workspace || workspace_bytes < w.bytes) return SKYRL_LMHEAD_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
 
@@ -2186,7 +2187,7 @@ size_t skyrl_lmhead_adapter_bwd_workspace_bytes(int64_t T, int64_t H, int64_t V,
   const int64_t vc = adapter_bwd_chunk(T, H, V);
   Adapters ad{};
   ad.N = (int)num_adapters, ad.rank = (int)rank;
-  return bwd_workspace_bytes(T, H, V, vc, true) + carve_adapter_bwd(nullptr, ad, T, H, V, vc).bytes;
+  return bwd_workspace_bytes(T, H, V, vc, true, 1, false) + carve_adapter_bwd(nullptr, ad, T, H, V, vc).bytes;
 }
 
 int skyrl_lmhead_adapter_bwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels, const void* lora_a,
@@ -2200,7 +2201,7 @@ int skyrl_lmhead_adapter_bwd(const void* hidden, int64_t ld_hidden, const void* 
   if (!d_lora_a || !d_lora_b) return SKYRL_LMHEAD_ERR_NULL;
   if (!aligned16(d_lora_a) || !aligned16(d_lora_b)) return SKYRL_LMHEAD_ERR_ALIGN;
   const int64_t vc = adapter_bwd_chunk(T, H, V);
-  const size_t head = bwd_workspace_bytes(T, H, V, vc, true);
+  const size_t head = bwd_workspace_bytes(T, H, V, vc, true, 1, false);
   if (!workspace || workspace_bytes < skyrl_lmhead_adapter_bwd_workspace_bytes(T, H, V, num_adapters, rank)) return SKYRL_LMHEAD_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
   AdapterBwd ab = carve_adapter_bwd((char*)workspace + head, make_adapters(lora_a, a_adapter, a_row, lora_b, b_adapter, b_row, scaling, num_adapters, rank), T,

@@ -7,6 +7,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
+from skyrl_amd import _lib
 from skyrl_amd import adapters as AD
 
 NAMES = ("hidden", "weight", "lora_a", "lora_b", "scaling")
@@ -49,3 +50,13 @@ def test_a_tangent_is_refused(name):
 def test_a_frozen_batch_gets_logits():
     with FakeTensorMode(allow_non_fake_inputs=True):
         assert AD.adapter_logits(**operands()).shape == (3, 50)
+
+
+@pytest.mark.parametrize("H,V", [(896, 151936), (3584, 152064)])
+def test_no_room_is_taken_for_a_gradient_of_the_weight(H, V):
+    """From the second block of 32768 tokens on the head keeps dW's sum, V H fp32; with adapters there is no dW, only dB's sum, N V R fp32."""
+    lib = _lib.load()
+    head = [lib.skyrl_lmhead_bwd_active_rows_workspace_bytes(T, H, V, 0) for T in (32768, 32769)]
+    ours = [lib.skyrl_lmhead_adapter_bwd_workspace_bytes(T, H, V, 1, 8) for T in (32768, 32769)]
+    assert head[1] - head[0] >= 4 * V * H
+    assert 4 * V * 8 <= ours[1] - ours[0] <= 4 * V * 8 + (1 << 20)
