@@ -54,7 +54,8 @@ __device__ __forceinline__ Stats row_stats(const void* logits, int64_t ld, int64
         float mx = pc[u].v[0];
 #pragma unroll
         for (int i = 1; i < E; ++i) mx = fmaxf(mx, pc[u].v[i]);
-        if (__any(mx * scale2 > st.m)) raise_max(st, mx * scale2);
+        const float to = max_from(mx, scale2);
+        if (__any(to > st.m)) raise_max(st, to);
 #pragma unroll
         for (int i = 0; i < E; ++i) absorb<ENT>(st, pc[u].v[i], scale2);
       }
@@ -62,7 +63,7 @@ __device__ __forceinline__ Stats row_stats(const void* logits, int64_t ld, int64
   }
   for (int i = threadIdx.x; i < rp.single; i += kThreads) {
     const float z = load_one(base, (size_t)single_column(rp, E, i), F32);
-    raise_max(st, z * scale2);
+    raise_max(st, max_from(z, scale2));
     absorb<ENT>(st, z, scale2);
   }
   return st;

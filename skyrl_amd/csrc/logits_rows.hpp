@@ -87,11 +87,17 @@ __device__ __forceinline__ void rebase(float& s, float& e, float from, float to)
   s *= c;
 }
 
-// Raise the running maximum to at least `cand` (a value of y2).
-__device__ __forceinline__ void raise_max(Stats& st, float cand) {
-  if (cand > st.m) {
-    rebase(st.s, st.e, st.m, cand);
-    st.m = cand;
+// A running maximum for sums over logits up to z: z * scale2.  That product's rounding is what absorb() will see of z itself: +440 for a mask of -1e10, whose
+// sum would be infinite, and NaN beside a larger maximum.  There it is a little above z, and the sum 0.
+__device__ __forceinline__ float max_from(float z, float scale2) {
+  const float y2 = z * scale2;
+  return fmaf(z, scale2, -y2) > 64.f ? fmaf(fabsf(y2), 0x1p-22f, y2) : y2;
+}
+// Raise the running maximum to at least `to`, of max_from().
+__device__ __forceinline__ void raise_max(Stats& st, float to) {
+  if (to > st.m) {
+    rebase(st.s, st.e, st.m, to);
+    st.m = to;
   }
 }
 

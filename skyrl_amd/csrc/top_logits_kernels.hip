@@ -248,9 +248,7 @@ __global__ __launch_bounds__(kThreads, 6) void logits_top_rows(const TopArgs a) 
   auto raise_wave_max = [&](float z) {  // to the largest z of the wave
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) z = fmaxf(z, __shfl_xor(z, o, 64));
-    const float y2 = z * scale2;
-    // Where a row is far, above its logits: a wave that has seen nothing but a mask of -1e10 must not bring an infinite sum to the others' logits.
-    raise_max(st, fabsf(y2) < kFar ? y2 : fmaf(fabsf(y2), 0x1p-22f, y2));
+    raise_max(st, max_from(z, scale2));
   };
 
   int step = 0;
