@@ -202,11 +202,12 @@ __global__ __launch_bounds__(256) void adapter_gather_rows(const int* __restrict
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// Rows with a gradient (all of them without g), grouped by adapter (those without one last), ascending inside a group: idx, their adapters, and seg[a], the place of
+// Rows with a gradient (without GRADS all of them), grouped by adapter (those without one last), ascending inside a group: idx, their adapters, and seg[a], the place of
 // adapter a's first row; seg[N] that of the rows without an adapter, seg[N + 1] the number of rows.  One workgroup per group: it counts the rows of
 // the groups before its own, then lists its own.  The order is a function of the inputs alone, so the sums over rows are the same bits on each call.
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kGroupThreads = 1024, kGroupTokens = 4;  // tokens per thread and step
+template <bool GRADS>
 __global__ __launch_bounds__(kGroupThreads) void adapter_group_rows(const float* __restrict__ g, const float* __restrict__ q,
                                                                     const int64_t* __restrict__ labels, int64_t V, const int64_t* __restrict__ ids, int T, int N, int* __restrict__ idx,
                                                                     int64_t* __restrict__ ids_c, int* __restrict__ seg) {
@@ -217,9 +218,11 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_group_rows(const float*
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mine = blockIdx.x;
   auto group_of = [&](int t) -> int {  // -1: no gradient
     if (t >= T) return -1;
-    const float gv = g ? target_grad(g, labels, V, t) : 1.f, qv = q ? q[t] : 0.f;
     const int64_t x = ids[t];
-    if (gv == 0.f && qv == 0.f) return -1;
+    if constexpr (GRADS) {
+      const float gv = target_grad<true>(g, labels, V, t), qv = q ? q[t] : 0.f;
+      if (gv == 0.f && qv == 0.f) return -1;
+    }
     return x >= 0 && x < (int64_t)N ? (int)x : N;
   };
   int less = 0;
@@ -665,7 +668,10 @@ __global__ __launch_bounds__(256) void adapter_da_sum(const float* __restrict__ 
 
 hipError_t launch_adapter_shrink(hipStream_t s, const Adapters& ad, const uint16_t* hidden, int64_t ldh, const int64_t* ids, int64_t T, const int* T_dev,
                                  int64_t H, uint16_t* U, int* ids32) {
-  // Up to 16 workgroups share the adapters of 16 tokens; with many tokens their tiles fill the chip by themselves.
+  // Up to 16 workgroups share the adapters of 16 tokens; with many tokens their tiles fill the chip by themselves, and workgroups without an adapter
+  // only cost.  us with 16 / 4 / 2 / 1 of them, rank 32, mixed: T=16, H=3584, 48 adapters 12.9 / 38.4 / 65.6 / 147; T=256 12.4 / 20.9 / 30.1 / 56.6; T=1024 12.4 / 12.4
+  // / 12.4 / 21.6; T=2048, H=896 12.2 / 6.7 / 6.4 / 10.6, H=3584 16.8 / 13.0 / 13.2 / 21.6; T=4096, H=896 19.6 / 9.7 / 9.5 / 11.0, eight adapters 13.0 / 8.0 / 8.9 / 9.0;
+  // T=8192, H=896 20.2 / 14.6 / 13.4 / 12.9, H=3584 32.6 / 32.3 / 31.8 / 31.2.
   const int64_t tiles = (T + 15) / 16, most = tiles <= 64 ? 16 : tiles <= 256 ? 4 : 2;
   hipLaunchKernelGGL(adapter_shrink, dim3((unsigned)tiles, (unsigned)(padded_rank(ad.rank) / 32), (unsigned)(ad.N < most ? ad.N : most)),
                      dim3(kShrinkWaves * 64), 0, s, ad, hidden, ldh, ids, (int)T, T_dev, (int)H, U, ids32);
@@ -694,7 +700,7 @@ hipError_t launch_adapter_gather_rows(hipStream_t s, const int* idx, const uint1
 
 hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float* q, const int64_t* labels, int64_t V, const int64_t* ids, int64_t T, int N,
                                      int* idx, int64_t* ids_c, int* seg) {
-  hipLaunchKernelGGL(adapter_group_rows, dim3((unsigned)(N + 1)), dim3(kGroupThreads), 0, s, g, q, labels, V, ids, (int)T, N, idx, ids_c, seg);
+  hipLaunchKernelGGL((g ? adapter_group_rows<true> : adapter_group_rows<false>), dim3((unsigned)(N + 1)), dim3(kGroupThreads), 0, s, g, q, labels, V, ids, (int)T, N, idx, ids_c, seg);
   return hipGetLastError();
 }
 

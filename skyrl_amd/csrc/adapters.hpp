@@ -188,10 +188,13 @@ __device__ __forceinline__ bf16x8 transposed(const char* at, int pitch) {
   return __builtin_bit_cast(bf16x8, v);
 }
 
-// The gradient on token t's log-probability.  labels, where it is not NULL: 0 for a label outside [0, V), whose log-probability is the constant 0.
+// The gradient on token t's log-probability.  TARGETS: 0 for a label outside [0, V), whose log-probability is the constant 0.
+template <bool TARGETS>
 __device__ __forceinline__ float target_grad(const float* g, const int64_t* labels, int64_t V, int t) {
-  if (labels && (labels[t] < 0 || labels[t] >= V)) return 0.f;
-  return g[t];
+  const float gv = g[t];
+  if constexpr (!TARGETS) return gv;
+  const int64_t y = labels[t];
+  return y >= 0 && y < V ? gv : 0.f;
 }
 
 // ---- launches (adapter_tiles.hip) ----
@@ -243,7 +246,8 @@ struct RowResults {
 // row_map[t] of `to`.
 hipError_t launch_adapter_label(hipStream_t s, const Adapters& ad, const uint16_t* U, const int* ids32, const int64_t* labels, int64_t T, int64_t V,
                                 float rcp_temp, const RowResults& from, const int* row_map, const RowResults& to);
-// The T rows whose g (by target_grad) or q is not zero (all without g), grouped by adapter: idx, their ids and the groups' places, seg [N + 2].
+// The T rows whose g (of a label in [0, V)) or q is not zero (without g all, and no labels), grouped by adapter: idx, their ids and the groups'
+// places, seg [N + 2].
 hipError_t launch_adapter_group_rows(hipStream_t s, const float* g, const float* q, const int64_t* labels, int64_t V, const int64_t* ids, int64_t T, int N,
                                      int* idx, int64_t* ids_c, int* seg);
 // hidden_c [T, H] and labels_c (both or neither of the labels' pointers): the rows that idx names.
@@ -261,7 +265,6 @@ struct AdapterPanel {
   const uint16_t* D;
   int ldd, T;
   const int* T_dev;
-  const int* ids;      // of the panel's rows
   int vc0, columns;    // the chunk's first column; panel columns that hold values, a multiple of 256
   int V;
   VocabTail tail;

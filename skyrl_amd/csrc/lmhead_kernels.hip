@@ -977,7 +977,7 @@ __global__ __launch_bounds__(256) void split_operand_rows(const void* __restrict
 // dW and its dHidden row is zero.  In RL micro-batches those are the prompt and padding tokens the loss mask removes, often
 // more than half of the batch.  Two small kernels let the backward run on the remaining rows without the host ever
 // learning how many there are (no synchronisation, so the call can be captured in a HIP graph):
-//   compact_active_rows   one workgroup: idx[i] = i-th token with g != 0 or q != 0 (ascending), counts[0] = their number n; with labels a g whose
+//   compact_active_rows   one workgroup: idx[i] = i-th token with g != 0 or q != 0 (ascending), counts[0] = their number n; with TARGETS a g whose
 //                         label lies outside [0, V) counts as 0 (target_grad in adapters.hpp);
 //                         counts[1 + b] = how many of them fall into block b of `block` compacted rows,
 //                         counts[1 + nblocks + b] = how that block's dHidden contraction is cut: the number of splits, or, where
@@ -988,7 +988,7 @@ __global__ __launch_bounds__(256) void split_operand_rows(const void* __restrict
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kCompactThreads = 1024;
 
-template <int TOKENS>  // per thread and step
+template <int TOKENS, bool TARGETS>  // tokens per thread and step
 __global__ __launch_bounds__(kCompactThreads) void compact_active_rows(const float* __restrict__ g, const float* __restrict__ q,
                                                                        const int64_t* __restrict__ labels, int64_t V, int T, int block,
                                                                        int nblocks, SplitProblem split, int* __restrict__ idx,
@@ -1008,7 +1008,7 @@ __global__ __launch_bounds__(kCompactThreads) void compact_active_rows(const flo
     for (int k = 0; k < TOKENS; ++k) {
       const int t = t0 + k * kCompactThreads + tid;
       const int tc = t < T ? t : T - 1;
-      const float gv = target_grad(g, labels, V, tc), qv = q ? q[tc] : 0.f;
+      const float gv = target_grad<TARGETS>(g, labels, V, tc), qv = q ? q[tc] : 0.f;
       ballot[k] = __ballot(t < T && (gv != 0.f || qv != 0.f));
     }
 #pragma unroll
@@ -1057,7 +1057,8 @@ __global__ __launch_bounds__(kCompactThreads) void compact_active_rows(const flo
   }
 }
 
-inline auto compact_kernel(int64_t T) { return T <= kCompactThreads ? compact_active_rows<1> : compact_active_rows<4>; }
+template <bool TARGETS>
+inline auto compact_kernel(int64_t T) { return T <= kCompactThreads ? compact_active_rows<1, TARGETS> : compact_active_rows<4, TARGETS>; }
 
 // One workgroup per row r < T: as compacted row r (when r < n) it copies the inputs of token idx[r]; as token r it clears
 // d_hidden[r] -- active tokens get their row from the dHidden GEMM (or the sum over its splits) afterwards.  targets: V, where labels outside
@@ -1082,7 +1083,7 @@ __global__ __launch_bounds__(256) void gather_active_rows(const int* __restrict_
   if (threadIdx.x == 0) {
     labels_c[r] = labels[t];
     lse_c[r] = lse[t];
-    g_c[r] = target_grad(g, targets > 0 ? labels : nullptr, targets, t);
+    g_c[r] = targets > 0 ? target_grad<true>(g, labels, targets, t) : g[t];
     if (q) q_c[r] = q[t], pz_c[r] = pz[t];
   }
 }
@@ -1788,7 +1789,7 @@ int bwd_token_block(const uint16_t* Hp, int64_t ld_hidden, const uint16_t* Wp, i
     if (e != hipSuccess) return (int)e;
     if (ab) {
       Timed timed(kAdapterPanel, s);
-      const AdapterPanel panel{ab->call.ad, w.D, (int)(vcw + kLdPad), (int)Tb, T_dev, adapters.ids, (int)vc0, (int)vcw, (int)V, tail};
+      const AdapterPanel panel{ab->call.ad, w.D, (int)(vcw + kLdPad), (int)Tb, T_dev, (int)vc0, (int)vcw, (int)V, tail};
       float* const part = ab->du_part + (size_t)(ci * ab->ranges) * (size_t)Tb * (size_t)padded_rank(ab->call.ad.rank);
       e = launch_adapter_panel(s, panel, ab->ranges, part, ab->U_back + (size_t)row0 * 2 * padded_rank(ab->call.ad.rank), ab->seg, (int)row0, row0 > 0 ? ab->db_sum : nullptr,
                                last_block ? nullptr : ab->db_sum, last_block ? ab->dB : nullptr);
@@ -1886,11 +1887,10 @@ int bwd_entry(const void* hidden, int64_t ld_hidden, const void* weight, int64_t
   if (compact) {
     Timed timed(kCompactRows, s);
     // With adapters no shard of a vocabulary is meant: a label outside it is a constant log-probability, which has no gradient.
-    const int64_t* const targets = ab ? labels : nullptr;
-    hipLaunchKernelGGL(compact_kernel(T), dim3(1), dim3(kCompactThreads), 0, s, dlogprobs, dentropy, targets, V, (int)T, (int)Tb,
+    hipLaunchKernelGGL((ab ? compact_kernel<true>(T) : compact_kernel<false>(T)), dim3(1), dim3(kCompactThreads), 0, s, dlogprobs, dentropy, labels, V, (int)T, (int)Tb,
                        (int)nblocks, rated, w.idx, w.counts);
     if (ab) {  // the same rows in another order
-      e = launch_adapter_group_rows(s, dlogprobs, dentropy, targets, V, ab->call.ids, T, ab->call.ad.N, w.idx, ab->ids_c, ab->seg);
+      e = launch_adapter_group_rows(s, dlogprobs, dentropy, labels, V, ab->call.ids, T, ab->call.ad.N, w.idx, ab->ids_c, ab->seg);
       if (e != hipSuccess) return (int)e;
     }
     hipLaunchKernelGGL(gather_active_rows, dim3((unsigned)T), dim3(256), 0, s, (const int*)w.idx, (const int*)w.counts, Hp,
@@ -2360,7 +2360,7 @@ int skyrl_softce_bwd(const void* student_hidden, int64_t ld_student, const void*
   const SplitProblem split = split_problem(T, H, vc, false, w.slots, ncu);
   {  // tokens without an upstream gradient (what the supervision mask removes) have a zero row and take no part
     Timed timed(kCompactRows, s);
-    hipLaunchKernelGGL(compact_kernel(T), dim3(1), dim3(kCompactThreads), 0, s, dloss, (const float*)nullptr, (const int64_t*)nullptr, (int64_t)0, (int)T, (int)T, 1,
+    hipLaunchKernelGGL(compact_kernel<false>(T), dim3(1), dim3(kCompactThreads), 0, s, dloss, (const float*)nullptr, (const int64_t*)nullptr, (int64_t)0, (int)T, (int)T, 1,
                        split, w.idx, w.counts);
   }
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
