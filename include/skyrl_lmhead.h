@@ -483,7 +483,10 @@ int skyrl_logits_bwd(const void* logits, int logits_dtype, int64_t ld_logits, co
  *     V, rank], bf16, contiguous, overwritten (zeros for adapters without a token that has a gradient).  dz is rounded to bf16 once, as
  *     without adapters, but for the label's value of a token with an adapter, which is exact; every result is rounded once (d_hidden of a
  *     vocabulary below 1024 that is not a multiple of 128 twice).  Rows are worked on grouped by adapter, in an order that follows from
- *     adapter_ids alone: the same bits on each call. */
+ *     adapter_ids alone: the same bits on each call.
+ * The backward's workspace is that of skyrl_lmhead_bwd_active_rows without its sum of dW, and fp32 sums: of dA, (T / 256 + min(num_adapters, T)) *
+ * rank * H (0.8 GB at T=8192, 64 adapters of rank 256, H=8192); of du, at most 1 MiB * rank for every chunk of the vocabulary; with more than 32768
+ * tokens of dB, num_adapters * V * rank. */
 #define SKYRL_LMHEAD_MAX_ADAPTER_RANK 256
 size_t skyrl_lmhead_adapter_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V, int64_t num_adapters, int64_t rank);
 int skyrl_lmhead_adapter_fwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels, const void* lora_a,

@@ -7,8 +7,8 @@
 // lie.  A wave walks the distinct adapters of its tokens, whatever their order is; a batch of sequences one behind the other has one or two.
 //
 // What that costs a tile is a trip to memory per 16 tokens' adapter, hidden for the first one behind the mainloop, and its products, 2 of H / 32 per 32 ranks.
-// Forward tiles without / with adapters: T=2048, H=896, V=151936, six adapters of rank 32, 435 / 527 us; T=8192, H=3584, V=152064, four, 5.65 / 6.04 ms
-// (power). Logits of 16 tokens, H=3584, eight of rank 16: 253 us, 4.5 TB/s of weight, B and logits.
+// Forwards without / with adapters, all kernels: T=2048, H=896, V=151936, six adapters of rank 32, 446 / 580 us; T=8192, H=3584, V=152064, four, 5.63 / 6.08 ms
+// (power). Logits of 16 tokens, H=3584, eight of rank 16: 250 us, 4.5 TB/s of weight, B and logits; rank 64 275 us, 128 314 us.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -10,8 +10,9 @@
 // A row without any logit above -inf has lse = -inf: log-probabilities -inf, entropy 0, zero gradient, columns 0 .. k - 1.
 //
 // Selection.  A candidate must reach the k-th largest of the maxima of 128 groups of lanes: those are 128 different logits, so at least k
-// logits reach it, and hardly more do (-128 ln(1 - k / 128): 22 for k = 20, 37 for k = 32).  The bound is formed from the first 16 KiB pieces
-// before any of them is looked at, and again whenever what has been seen doubles, so that a row has about k (1 + ln(V / 16384)) candidates.
+// logits reach it, and hardly more do (-128 ln(1 - k / 128): 22 for k = 20, 37 for k = 32).  The bound is formed from a workgroup's first 32 KiB (n =
+// 16384 bf16 or 8192 fp32 logits) before any of them is looked at, and again whenever what has been seen doubles, so that a workgroup that walks v
+// logits has about k (1 + ln(v / n)) candidates.
 // The running maximum of the softmax is one value per wave, so that it, the bound and the label's logit (the rank) cost one comparison and
 // vote each per four pieces of a lane; only where a vote says so are the pieces gone through again.
 //
@@ -191,7 +192,7 @@ __device__ __noinline__ void fill_with_nan(int V, int k, int64_t* ids, float* lo
 
 // One workgroup per row and part (PARTS: grid.y of them).
 // Bound by HBM on fp32 logits, by the vector instructions (an exponential, the comparisons, widening) on bf16: 2048 x 152064 fp32, k = 5, 217 us (5.7
-// TB/s); 4096 x 151936 bf16, k = 32, 322 us (3.9 TB/s), of which 36 are the ranks and candidates.  What brought it there from 510: one running maximum
+// TB/s); 4096 x 151936 bf16, k = 32, 316 us (3.9 TB/s; in a graph of two calls 277), of which 36 are the ranks and candidates.  What brought it there from 510: one running maximum
 // a wave and votes per four pieces instead of one (437), keys formed only where a logit reaches the bound (394), no memory for
 // arguments of a call (322).  Loading a step ahead changed nothing (328 to 358): two or three workgroups a CU overlap enough.
 template <bool F32, bool PARTS>
@@ -595,8 +596,17 @@ int check_top(int64_t V, int64_t k) {
 }
 
 // Parts of a row: so many that 512 workgroups share the logits, of at least 8192 logits each, and none for rows so short that the second launch costs
-// what the parts save.  Without / with parts, both launches, bf16, k = 20: 8 x 151936 27.5 / 13.1 us, 64 rows 29.8 / 17.6, 255 rows 34.1 / 33.4, 512 rows 43.5 / 49
-// (two parts); 8 x 32001 11.8 / 13.1, 255 x 32001 12.9 / 16.0.  With 1024 workgroups 64 rows take 20.5 us, with 2048 22.1.
+// what the parts save.  us in a graph, both launches, k = 20, one workgroup a row / parts for 256, 512 and 1024 workgroups:
+//             8 rows                  64 rows                      128 rows                     255 rows
+//   bf16 32001  13.2 / 14.4           13.6 / 15.0                  14.4 / 16.3, 17.3, 17.2      15.4 / -, 19.3, 20.0
+//        40000  14.3 / 13.7           15.1 / 14.6, 14.4, 14.3      16.0 / 18.0, 16.9, 16.9      17.0 / -, 21.3, 23.3
+//        49152  15.7 / 13.5           16.5 / 14.6, 15.6, 15.6      17.8 / 19.1, 17.8, 18.5      18.3 / -, 22.2, 24.3
+//        80000  19.9 / 13.9           22.1 / 17.9, 17.0, 18.6      22.3 / 22.1, 21.0, 23.1      23.4 / -, 26.1, 29.6
+//       151936  29.9 / 14.5           32.3 / 21.8, 21.2, 23.6      33.1 / 27.9, 25.5, 29.1      36.6 / -, 35.1, 38.2
+//   fp32 32001  15.7 / 16.3           17.0 / 17.7                  17.9 / 19.3, 19.8, 20.0      19.0 / -, 21.6, 22.9
+//        49152  18.6 / 13.9           20.4 / 18.2, 17.3, 17.2      21.0 / 21.3, 20.2, 19.7      22.2 / -, 24.6, 28.2
+//       151936  36.2 / 15.7           41.5 / 25.2, 23.3, 27.9      45.2 / 36.3, 30.2, 33.9      49.3 / -, 45.6, 50.1
+// What one limit for all costs: two parts a row (171 to 256 rows) lose 2 to 4 us below some 100000 bf16 or 70000 fp32 columns.
 int top_parts(int64_t T, int64_t V, int64_t k) {
   int64_t n = V < 6 * 8192 ? 1 : 512 / T;
   if (n > V / 8192) n = V / 8192;
