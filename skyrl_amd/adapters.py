@@ -188,8 +188,8 @@ def _rows(hidden: torch.Tensor, adapter_ids: torch.Tensor) -> Tuple[torch.Tensor
     if adapter_ids.dtype.is_floating_point:
         raise TypeError(f"adapter_ids must be integers, got {adapter_ids.dtype}")
     rows = hidden.reshape(-1, hidden.shape[-1])
-    if not rows.shape[1] <= _pitch(rows) <= _MAX_PITCH:  # the last position of each long sequence, or one row repeated
-        rows = rows.contiguous()
+    if not rows.shape[1] <= _pitch(rows) <= _MAX_PITCH or _pitch(rows) % 8 != 0:
+        rows = rows.contiguous()  # the last position of each long sequence, one row repeated, rows that do not begin on 16 bytes
     return rows, adapter_ids.reshape(-1).to(torch.int64).contiguous()
 
 
