@@ -531,6 +531,20 @@ int skyrl_logits_top_bwd(const void* logits, int logits_dtype, int64_t ld_logits
                          const float* row_pz, const float* dlogprobs, const float* dentropy, const int64_t* top_ids, const float* dtop,
                          int64_t T, int64_t V, int64_t k, float rcp_temperature, void* dlogits, int64_t ld_dlogits, void* stream);
 
+/* ---- the embedding ------------------------------------------------------------------------------------------------------
+ * out[t] = scale * table[ids[t]], zeros where the id lies outside [0, V); the gradient of the table, dtable[v] = scale * the sum of dout[t] over the
+ * tokens with ids[t] = v, none of them where v is `padding` (a value outside [0, V): no such row).  dtype (SKYRL_LOGITS_*): of table and
+ * out, of dout and dtable.  Rows of any pitch (of dout also 0, one row for all tokens) and alignment.  Sums are fp32, in an order that the ids
+ * fix: the same bits on each call.  accumulate: 0, dtable [V, H] is overwritten, zeros where no token names a row; 1, dtable is fp32 whatever
+ * dtype is, and is added to in the rows that tokens name.  dtable must not overlap dout.  T at most 2^24, H at most 2^22, and as many
+ * windows of 16 tokens by slices of a row as one grid holds (T H at most 2^34 is always fine); the query answers 0 beyond.
+ * The workspace (256-byte aligned) holds the sorted ids and, for each 16 tokens, two fp32 rows: T * (16 + H / 2) bytes. */
+int skyrl_lmhead_embedding_fwd(const void* table, int dtype, int64_t ld_table, const int64_t* ids, int64_t T, int64_t H, int64_t V, float scale, void* out,
+                               void* stream);
+size_t skyrl_lmhead_embedding_bwd_workspace_bytes(int64_t T, int64_t H, int64_t V);
+int skyrl_lmhead_embedding_bwd(const void* dout, int dtype, int64_t ld_dout, const int64_t* ids, int64_t padding, int64_t T, int64_t H, int64_t V,
+                               float scale, int accumulate, void* dtable, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

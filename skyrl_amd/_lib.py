@@ -11,7 +11,7 @@ import os
 import threading
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "libskyrl_lmhead.so")
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 _c_i64 = ctypes.c_int64
 _c_p = ctypes.c_void_p
@@ -124,6 +124,12 @@ SIGNATURES = {
     "skyrl_logits_top_bwd": (
         ctypes.c_int,
         [_c_p, ctypes.c_int, _c_i64] + [_c_p] * 7 + [_c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_i64, _c_p]),
+    "skyrl_lmhead_embedding_fwd": (
+        ctypes.c_int, [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p]),
+    "skyrl_lmhead_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 3),
+    "skyrl_lmhead_embedding_bwd": (
+        ctypes.c_int,
+        [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_int, _c_p, _c_p, ctypes.c_size_t, _c_p]),
     "skyrl_logprob_diff_metrics": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p]),
     "skyrl_lmhead_mfma_probe": (ctypes.c_int, [_c_p, ctypes.c_int, ctypes.c_int, _c_p, _c_p]),
     "skyrl_lmhead_atomic_floor_probe": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p]),

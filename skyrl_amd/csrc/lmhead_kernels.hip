@@ -2040,7 +2040,7 @@ int64_t adapter_bwd_chunk(int64_t T, int64_t H, int64_t V) {
 
 extern "C" {
 
-int skyrl_lmhead_version(void) { return 20; }
+int skyrl_lmhead_version(void) { return 21; }
 
 const char* skyrl_lmhead_strerror(int status) {
   switch (status) {
