@@ -545,6 +545,31 @@ size_t skyrl_lmhead_embedding_bwd_workspace_bytes(int64_t T, int64_t H, int64_t 
 int skyrl_lmhead_embedding_bwd(const void* dout, int dtype, int64_t ld_dout, const int64_t* ids, int64_t padding, int64_t T, int64_t H, int64_t V,
                                float scale, int accumulate, void* dtable, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- beam search ---------------------------------------------------------------------------------------------------------
+ * skyrl_logits_beam_select: of each item's beams x V candidates the k with the largest total = score + log-softmax(logits * rcp_temperature), best
+ * first: out_scores fp32, parents (the beam) and tokens (the column) int64, each [items, k].  Among equal totals the lower beam and then the
+ * lower column comes first; a beam offers its k largest logits, the lower column first among equal ones.  Totals are formed in 64 bits from a sum of
+ * exponentials in 64 bits, so that the order of candidates of different beams is that of the exact totals but where they differ by less than some
+ * 1e-7.  A beam whose score is -inf, or that has no logit above -inf, offers columns 0 .. with total -inf; one with a NaN or +inf among its logits, or whose
+ * score is NaN or +inf, the same columns with NaN, behind those.  Parents and tokens are valid in every case.
+ * logits: bf16 or fp32, item i's beam b at logits + i * ld_item + b * ld_beam elements (either may be 0: rows that beams share); scores fp32 [items, beams].
+ * 1 <= k <= min(beams * V, SKYRL_LOGITS_TOP_MAX), beams <= SKYRL_LOGITS_BEAMS_MAX, items * beams <= 2^22.  workspace: 8-byte aligned.
+ *
+ * skyrl_logits_beam_reorder: row j of item i (of beams_out) of each of `count` tensors becomes row parents[i, j] of that item (of beams_in); zeros where
+ * the parent lies outside [0, beams_in).  A row is `segments` pieces of `bytes` contiguous bytes: tensor t's at from[t] + (i * beams_in + parent) *
+ * from_row + s * from_segment, written to to[t] + (i * beams_out + j) * to_row + s * to_segment; strides in bytes.  from and to are host arrays of
+ * at most SKYRL_LOGITS_STATES_MAX device pointers, read before the call returns.  In place, to[t] == from[t] for every t with the same strides
+ * and beams_in == beams_out <= SKYRL_LOGITS_BEAMS_MAX, rows that keep their place are neither read nor written for that; otherwise the two must not overlap. */
+#define SKYRL_LOGITS_BEAMS_MAX 128
+#define SKYRL_LOGITS_STATES_MAX 200
+size_t skyrl_logits_beam_select_workspace_bytes(int64_t items, int64_t beams, int64_t V, int64_t k);
+int skyrl_logits_beam_select(const void* logits, int logits_dtype, int64_t ld_item, int64_t ld_beam, const float* scores, int64_t items, int64_t beams,
+                             int64_t V, int64_t k, double rcp_temperature, float* out_scores, int64_t* parents, int64_t* tokens, void* workspace,
+                             size_t workspace_bytes, void* stream);
+int skyrl_logits_beam_reorder(const void* const* from, void* const* to, int64_t count, int64_t from_row, int64_t from_segment, int64_t to_row,
+                              int64_t to_segment, int64_t segments, int64_t bytes, const int64_t* parents, int64_t items, int64_t beams_in, int64_t beams_out,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

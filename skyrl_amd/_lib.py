@@ -130,6 +130,12 @@ SIGNATURES = {
     "skyrl_lmhead_embedding_bwd": (
         ctypes.c_int,
         [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_int, _c_p, _c_p, ctypes.c_size_t, _c_p]),
+    "skyrl_logits_beam_select_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 4),
+    "skyrl_logits_beam_select": (
+        ctypes.c_int,
+        [_c_p, ctypes.c_int, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_double, _c_p, _c_p, _c_p, _c_p, ctypes.c_size_t, _c_p]),
+    "skyrl_logits_beam_reorder": (
+        ctypes.c_int, [ctypes.POINTER(_c_p), ctypes.POINTER(_c_p)] + [_c_i64] * 7 + [_c_p, _c_i64, _c_i64, _c_i64, _c_p]),
     "skyrl_logprob_diff_metrics": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p]),
     "skyrl_lmhead_mfma_probe": (ctypes.c_int, [_c_p, ctypes.c_int, ctypes.c_int, _c_p, _c_p]),
     "skyrl_lmhead_atomic_floor_probe": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p]),

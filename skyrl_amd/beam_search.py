@@ -1,0 +1,198 @@
+"""One step of beam search: the best continuations of each prompt's beams, and the beams' states brought to their order.
+
+    total[n, b, v] = scores[n, b] + log_softmax(logits[n, b] / temperature)[v]
+
+* ``beam_select`` -- the ``k`` largest totals of each prompt over beams and vocabulary, with the beam (``parents``) and the token of each;
+* ``beam_reorder`` -- key / value caches and whatever else a beam carries follow their parents, into other buffers or in place, all tensors of a
+  layout in one launch.
+
+Among equal totals the lower beam and then the lower token comes first.  Totals are formed in 64 bits, so that candidates of different
+beams come in the order of their exact totals but where those differ by less than some 1e-7.  Neither waits for the GPU, and both may be
+captured in a HIP graph.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import List, NamedTuple, Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from ._launch import call, device_guard, has_tangent, raw_stream, registered_op
+from .ops import _require_device
+
+__all__ = ["MAX_CANDIDATES", "MAX_BEAMS", "BeamSelection", "beam_select", "beam_reorder", "logits_beam_select"]
+
+MAX_CANDIDATES = 128  # SKYRL_LOGITS_TOP_MAX
+MAX_BEAMS = 128       # SKYRL_LOGITS_BEAMS_MAX
+_MAX_STATES = 200     # SKYRL_LOGITS_STATES_MAX
+_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+
+
+class BeamSelection(NamedTuple):
+    scores: torch.Tensor   # [N, k] fp32, best first
+    parents: torch.Tensor  # [N, k] int64, the beam that a candidate continues
+    tokens: torch.Tensor   # [N, k] int64
+
+
+def _check_select(logits: torch.Tensor, scores: torch.Tensor, k: int) -> Tuple[int, int, int]:
+    if logits.dim() != 3:
+        raise ValueError(f"expected logits [N, B, V], got {tuple(logits.shape)}")
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"logits must be torch.bfloat16 or torch.float32, got {logits.dtype}")
+    N, B, V = (int(x) for x in logits.shape)
+    if tuple(scores.shape) != (N, B):
+        raise ValueError(f"scores {tuple(scores.shape)} do not match logits {tuple(logits.shape)}")
+    if scores.dtype != torch.float32:
+        raise TypeError(f"scores must be torch.float32, got {scores.dtype}")
+    if not 1 <= B <= MAX_BEAMS or not 1 <= k <= min(B * V, MAX_CANDIDATES):
+        raise ValueError(f"need 1 to {MAX_BEAMS} beams and k from 1 to the candidates of a prompt and at most {MAX_CANDIDATES}, got {B} beams, V={V} and k={k}")
+    return N, B, V
+
+
+@registered_op("skyrl_amd::logits_beam_select", mutates_args=())
+def logits_beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, rcp_temperature: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(scores, parents, tokens)``, each ``[N, k]``, of ``logits [N, B, V]`` with unit stride along ``V`` and contiguous ``scores [N, B]``."""
+    N, B, V = _check_select(logits, scores, k)
+    if V > 1 and logits.stride(2) != 1 or not scores.is_contiguous():
+        raise ValueError("logits must have unit stride in the last dimension and scores must be contiguous")
+    dev = _require_device(logits, scores)
+    best = torch.empty((N, k), dtype=torch.float32, device=dev)
+    parents, tokens = (torch.empty((N, k), dtype=torch.int64, device=dev) for _ in range(2))
+    if N == 0:
+        return best, parents, tokens
+    lib = _lib.load()
+    nbytes = int(lib.skyrl_logits_beam_select_workspace_bytes(N, B, V, k))
+    if nbytes == 0:
+        raise ValueError(f"no workspace for N={N}, B={B}, V={V}, k={k}: an extent is out of range")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with device_guard(dev):
+        st = lib.skyrl_logits_beam_select(logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), logits.stride(1), scores.data_ptr(), N, B, V, k,
+                                          float(rcp_temperature), best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes, raw_stream(dev))
+    _lib.check(st, "skyrl_logits_beam_select")
+    return best, parents, tokens
+
+
+@logits_beam_select.register_fake
+def _(logits, scores, k, rcp_temperature):
+    N = logits.shape[0]
+    return scores.new_empty((N, k)), scores.new_empty((N, k), dtype=torch.int64), scores.new_empty((N, k), dtype=torch.int64)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, temperature: float = 1.0) -> BeamSelection:
+    """The ``k`` best candidates of each prompt, best first, of ``logits [N, B, V]`` (bf16 or fp32; rows of any pitch, shared by beams where the tensor is
+    expanded) and the beams' ``scores [N, B]`` (fp32, the sums of their log-probabilities so far).
+
+    ``k`` is at most 128 and may exceed the number of beams, as it has to where ended beams are set aside.  A beam of score -inf has ended; it, and one
+    with no logit above -inf, offers tokens 0, 1, ... with a total of -inf.  One with a NaN or +inf among its logits, or whose score is NaN or +inf,
+    offers the same with NaN, behind those.  Not differentiable: operands that ask for a gradient are refused outside ``torch.no_grad()``."""
+    k, temperature = int(k), float(temperature)
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"temperature must be finite and positive, got {temperature}")
+    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad) or has_tangent(logits, scores):
+        raise ValueError("beam_select has no gradient: call it under torch.no_grad()")
+    _, _, V = _check_select(logits, scores, k)
+    rows = logits if V <= 1 or logits.stride(2) == 1 else logits.contiguous()
+    with torch.no_grad():
+        return BeamSelection(*call(logits_beam_select, rows, scores.contiguous(), k, 1.0 / temperature))
+
+
+def _segments(t: torch.Tensor, u: torch.Tensor) -> List[Tuple[torch.Tensor, torch.Tensor, int, int, int, int]]:
+    """``(from, to, segments, bytes, from_segment, to_segment)`` of two tensors of one shape, rows along dimension 0: what a row is in both, one run of
+    equally spaced contiguous pieces.  Tensors with more dimensions that do not join are taken apart along the first of them."""
+    size = t.element_size()
+    shape, a, b = list(t.shape[1:]), list(t.stride()[1:]), list(u.stride()[1:])
+    dims: List[List[int]] = []  # [extent, stride of t, stride of u], outer first, neighbours joined
+    for n, x, y in zip(shape, a, b):
+        if n == 1:
+            continue
+        if dims and dims[-1][1] == n * x and dims[-1][2] == n * y:
+            dims[-1] = [dims[-1][0] * n, x, y]
+        else:
+            dims.append([n, x, y])
+    inner = dims.pop()[0] if dims and dims[-1][1] == dims[-1][2] == 1 else 1
+    if len(dims) > 1:
+        axis = next(i for i, n in enumerate(shape) if n != 1) + 1
+        return [s for i in range(shape[axis - 1]) for s in _segments(t.select(axis, i), u.select(axis, i))]
+    n, x, y = dims[0] if dims else (1, 0, 0)
+    return [(t, u, n, inner * size, x * size, y * size)]
+
+
+def _check_states(states: Sequence[torch.Tensor], parents: torch.Tensor, out: Optional[Sequence[torch.Tensor]]) -> Tuple[int, int, int]:
+    """``(items, beams_in, beams_out)``."""
+    if parents.dim() != 2:
+        raise ValueError(f"expected parents [N, B], got {tuple(parents.shape)}")
+    if parents.dtype != torch.int64:
+        raise TypeError(f"parents must be int64, got {parents.dtype}")
+    N, B_out = (int(x) for x in parents.shape)
+    if len(states) == 0:
+        return N, 0, B_out
+    rows = int(states[0].shape[0]) if states[0].dim() > 0 else 0
+    for t in states:
+        if t.dim() < 1 or int(t.shape[0]) != rows:
+            raise ValueError("every state must have the beams of all prompts, N * B of them, along its first dimension; got "
+                             + ", ".join(str(tuple(s.shape)) for s in states))
+    if N == 0 and rows or N and rows % N:
+        raise ValueError(f"{rows} rows of states do not divide among {N} prompts")
+    if out is not None:
+        if len(out) != len(states):
+            raise ValueError(f"{len(out)} results for {len(states)} states")
+        for t, u in zip(states, out):
+            if u.shape != (N * B_out,) + t.shape[1:] or u.dtype != t.dtype:
+                raise ValueError(f"a result must be {(N * B_out,) + tuple(t.shape[1:])} {t.dtype}, got {tuple(u.shape)} {u.dtype}")
+            if any(n > 1 and s == 0 for n, s in zip(u.shape, u.stride())):
+                raise ValueError("a result must not be expanded: its elements would be written more than once")
+    return N, rows // N if N else 0, B_out
+
+
+def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
+    """Row ``n * B_out + j`` of each result is row ``n * B_in + parents[n, j]`` of its state, for states ``[N * B_in, ...]`` of any types and strides
+    (the used part of a cache, say) and ``parents [N, B_out]`` int64; zeros where a parent lies outside ``[0, B_in)``.
+
+    ``out``: tensors to write, new ones without it.  ``out=states`` reorders in place (``B_out == B_in``, at most 128 beams): rows that keep their place
+    are not moved.  A result is otherwise in memory of its own; one that shares a storage with a state is refused.  Not differentiable."""
+    states = list(states)
+    N, B_in, B_out = _check_states(states, parents, out)
+    if any(torch.is_grad_enabled() and t.requires_grad for t in [*states, *(out or [])]) or has_tangent(*states):
+        raise ValueError("beam_reorder has no gradient: call it under torch.no_grad()")
+    if out is None:
+        results = [t.new_empty((N * B_out,) + tuple(t.shape[1:])) for t in states]
+    else:
+        results = list(out)
+    if not states or N * B_out == 0 or all(t.numel() == 0 for t in results):
+        return results
+    dev = _require_device(parents, *states, *results)
+    if B_in == 0:  # no row to take
+        return [u.zero_() for u in results]
+    kept = {t.untyped_storage().data_ptr() for t in states} if out is not None else ()
+    groups: dict = {}
+    seen = set()
+    for t, u in zip(states, results):
+        if u.numel() == 0:
+            continue
+        in_place = t.data_ptr() == u.data_ptr() and t.shape == u.shape and t.stride() == u.stride()
+        if out is not None:
+            if u.data_ptr() in seen:
+                raise ValueError("a result is given twice")
+            seen.add(u.data_ptr())
+            if not in_place and u.untyped_storage().data_ptr() in kept:
+                raise ValueError("a result shares its storage with a state and is not that state: it would be read after it was written")
+            if in_place and B_in > MAX_BEAMS:
+                raise ValueError(f"at most {MAX_BEAMS} beams are reordered in place, got {B_in}")
+        size = t.element_size()
+        for x, y, n, nbytes, from_segment, to_segment in _segments(t, u):
+            layout = (in_place, x.stride(0) * size if x.shape[0] > 1 else 0, from_segment, y.stride(0) * size if y.shape[0] > 1 else 0, to_segment, n, nbytes)
+            groups.setdefault(layout, []).append((x.data_ptr(), y.data_ptr()))
+    lib, parents = _lib.load(), parents.contiguous()
+    with device_guard(dev):
+        stream = raw_stream(dev)
+        for (_, *layout), pairs in groups.items():
+            for at in range(0, len(pairs), _MAX_STATES):
+                some = pairs[at:at + _MAX_STATES]
+                array = ctypes.c_void_p * len(some)
+                st = lib.skyrl_logits_beam_reorder(array(*[p for p, _ in some]), array(*[p for _, p in some]), len(some), *layout, parents.data_ptr(), N, B_in,
+                                                   B_out, stream)
+                _lib.check(st, "skyrl_logits_beam_reorder")
+    return results

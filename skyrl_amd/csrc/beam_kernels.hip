@@ -1,0 +1,487 @@
+// One step of beam search from materialised logits: of each item's beams x vocabulary the k candidates with the largest total, and the beams'
+// states brought to the candidates' order.
+//
+//   y[b, v] = z[b, v] / temperature;   total[b, v] = score_b + y[b, v] - log sum_v exp y[b, v]
+//
+// Order: the larger total first, the lower beam and then the lower column first among equal ones.  A beam offers its k largest logits (the lower
+// column first among equal ones), so that is the order of a beam's candidates too.  Which of two candidates of different beams comes first hangs on
+// the last bits of their totals: those, the row's sum of exponentials and its logarithm are formed in 64 bits, from exponentials in 32 bits that
+// are relative to the row's largest logit and have no common error (the factor 1 / (temperature ln 2) enters as two floats).
+// A beam whose score is -inf, or that has no logit above -inf, offers columns 0 .. k - 1 with a total of -inf; one with NaN among its logits, a
+// logit of +inf, or a score that is NaN or +inf offers the same columns with NaN, which sorts behind -inf.
+//
+// beam_rows   a workgroup per beam and part of its row: one pass for the largest logit, the sum and the k best (as logits_top_rows,
+//             top_logits_kernels.hip).  Bound by HBM and, for few beams, by the way through a workgroup.
+// beam_join   a workgroup per item: joins the parts' sums; finds the k best of all parts' sorted lists.  Entry j of a list whose head r heads
+//             precede can only be among the k best if j + r < k, and must reach the k-th head: few entries are left, and each counts those before it.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "top_keys.hpp"
+
+namespace {
+
+using namespace logits;
+
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kInFlight = 4;  // 16-byte loads a thread has in flight
+constexpr int kMaxTop = SKYRL_LOGITS_TOP_MAX;
+constexpr int kMaxBeams = SKYRL_LOGITS_BEAMS_MAX;
+constexpr int kMaxLists = 512;  // of an item: beams * parts
+constexpr int kMaxParts = 64;
+constexpr int kGroupsPerWave = kGroups / kWaves;
+constexpr int kJoinThreads = 512;
+static_assert(kMaxTop <= kGroups && kMaxTop + 64 <= kWaveList && kMaxBeams <= kMaxLists && kMaxParts <= 64, "as in top_logits_kernels.hip; a part a lane");
+
+// Of one part of a row: its largest logit, sum 2^((z - top) * scale2), how many keys it has found.
+struct PartSum {
+  double sum;
+  float top;
+  int keys;
+};
+
+struct BeamArgs {
+  const void* logits;
+  int64_t ld_item, ld_beam;  // elements between items and between an item's beams
+  const float* scores;       // [items, beams]
+  int beams, V, k, each;     // each: keys of a list, min(k, V)
+  double rcp_temp;
+  float scale_hi, scale_lo;  // log2(e) / temperature
+  PartSum* part;             // [rows, parts]
+  topkey_t* keys;            // [rows, parts, each], best first
+  float* out_scores;         // [items, k]
+  int64_t *parents, *tokens;
+};
+
+struct Shared {
+  double sum[kWaves];
+  float top[kWaves];
+  int count[kWaves];
+  float bound;  // every wave's candidates reach it
+  float group_max[kGroups];
+  topkey_t list[kWaves][kWaveList];
+  topkey_t all[kWaves * kMaxTop];
+};
+
+__device__ __forceinline__ float difference(float z, float top) { return z - (top > -INFINITY ? top : 0.f); }  // -inf for -inf, never NaN of them
+
+template <bool F32>
+__global__ __launch_bounds__(kThreads, 6) void beam_rows(const BeamArgs a) {
+  constexpr int E = Piece<F32>::kElems, ES = F32 ? 4 : 2;
+  __shared__ Shared sm;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row = blockIdx.x, item = row / a.beams;
+  const int V = a.V, k = a.each, part = blockIdx.y, parts = gridDim.y;
+  const char* base = (const char*)a.logits + ((size_t)item * (size_t)a.ld_item + (size_t)(row - item * a.beams) * (size_t)a.ld_beam) * ES;
+  // Pieces begin at column 0 wherever the row does: beams of the same logits have the same sum, bit for bit, and their totals are equal.
+  struct __attribute__((packed, aligned(ES))) Unaligned {
+    u32x4 v;
+  };
+  const int all_pieces = V / E;
+  const int first = (int)((int64_t)all_pieces * part / parts), pieces = (int)((int64_t)all_pieces * (part + 1) / parts);
+  const int single = part == parts - 1 ? V - all_pieces * E : 0;
+
+  float wave_top = -INFINITY;  // the largest logit of the wave so far
+  double sum = 0.0;            // of this lane, relative to it
+  float lane_max = -INFINITY;
+  int count = 0;               // candidates in the wave's list
+  topkey_t least = 0;          // candidates have larger keys
+  float bound = -INFINITY;
+  topkey_t* const list = sm.list[wave];
+
+  auto term = [&](float z) {
+    const float d = difference(z, wave_top);
+    return __builtin_amdgcn_exp2f(fmaf(d, a.scale_hi, fmaxf(d, kMostNegativeFactor) * a.scale_lo));
+  };
+  auto raise = [&](float z) {  // the wave's largest logit, to the largest z of its lanes
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) z = fmaxf(z, __shfl_xor(z, o, 64));
+    if (z > wave_top) {
+      if (wave_top > -INFINITY) sum *= exp2((double)(wave_top - z) * ((double)a.scale_hi + (double)a.scale_lo));
+      wave_top = z;
+    }
+  };
+  auto append = [&](float z, int column, bool there) {
+    const bool reaches = there && z >= bound;
+    if (!__any(reaches)) return;
+    const topkey_t key = make_key(z, column);
+    const bool hit = reaches && key > least;
+    const unsigned long long mask = __ballot(hit);
+    if (mask == 0) return;
+    if (hit) list[count + __popcll(mask & ((1ull << lane) - 1))] = key;
+    count += (int)__popcll(mask);
+    wave_fence();
+    if (count > kWaveList - 64) {
+      least = keep_best(list, count, k);
+      count = k;
+      bound = fmaxf(bound, value_of_bits(key_bits(least)));
+    }
+  };
+
+  int step = 0;
+  for (int p0 = first + tid; p0 - tid < pieces; p0 += kThreads * kInFlight, ++step) {
+    Piece<F32> pc[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int p = p0 + u * kThreads;
+      pc[u].widen(((const Unaligned*)(base + (size_t)(p < pieces ? p : pieces - 1) * 16))->v);
+    }
+    float mx[kInFlight], top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      mx[u] = -INFINITY;
+      if (p0 + u * kThreads < pieces) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) mx[u] = fmaxf(mx[u], pc[u].v[i]);
+      }
+      top = fmaxf(top, mx[u]);
+    }
+    lane_max = fmaxf(lane_max, top);
+    if (__any(top > wave_top)) raise(top);
+    if ((step & (step + 1)) == 0) {  // steps 0, 1, 3, 7: what has been seen doubles
+      float m = fmaxf(lane_max, __shfl_xor(lane_max, 1, 64));
+      m = fmaxf(m, __shfl_xor(m, 2, 64));
+      if ((lane & 3) == 0) sm.group_max[wave * kGroupsPerWave + (lane >> 2)] = m;
+      if (step == 0) {
+        __syncthreads();
+        if (wave == 0) {
+          const float b = group_bound(sm.group_max, k);
+          if (lane == 0) sm.bound = b;
+        }
+        __syncthreads();
+      } else if (wave == (step & (kWaves - 1))) {  // whatever the other waves have published: a bound all the same
+        wave_fence();
+        const float b = group_bound(sm.group_max, k);
+        if (lane == 0) *(volatile float*)&sm.bound = fmaxf(*(volatile float*)&sm.bound, b);
+      }
+    }
+    bound = fmaxf(bound, *(volatile float*)&sm.bound);
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      if (p0 + u * kThreads < pieces) {
+        float s = 0.f;  // of one piece; pieces are added up in 64 bits
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += term(pc[u].v[i]);
+        sum += (double)s;
+      }
+    }
+    if (__any(top >= bound)) {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        const int p = p0 + u * kThreads;
+        if (!__any(mx[u] >= bound)) continue;
+#pragma unroll
+        for (int i = 0; i < E; ++i) append(pc[u].v[i], p * E + i, p < pieces);
+      }
+    }
+  }
+  if (single > 0) {  // fewer than a piece
+    const bool there = tid < single;
+    const int c = all_pieces * E + (there ? tid : 0);
+    const float z = load_one(base, (size_t)c, F32);
+    raise(there ? z : -INFINITY);
+    if (there) sum += (double)term(z);
+    append(z, c, there);
+  }
+  if (count > k && __builtin_amdgcn_readfirstlane(count) > kThreads / kWaves) {  // so that all fit behind each other
+    (void)keep_best(list, count, k);
+    count = k;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) sm.count[wave] = count, sm.sum[wave] = sum, sm.top[wave] = wave_top;
+  __syncthreads();
+  int total = 0, mine_at = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w == wave) mine_at = total;
+    total += sm.count[w];
+  }
+  if (tid == 0) {
+    float top = -INFINITY;
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sm.top[w]);
+    double s = 0.0;
+    for (int w = 0; w < kWaves; ++w) {
+      const double d = (double)difference(sm.top[w], top) * ((double)a.scale_hi + (double)a.scale_lo);
+      s += sm.top[w] == top ? sm.sum[w] : sm.top[w] > -INFINITY ? sm.sum[w] * exp2(d) : sm.sum[w];  // without a logit: 0, or NaN
+    }
+    a.part[row * parts + part] = PartSum{s, top, total < k ? total : k};
+  }
+  for (int e = lane; e < count; e += 64) sm.all[mine_at + e] = list[e];
+  __syncthreads();
+  for (int e = tid; e < total; e += kThreads) {
+    const topkey_t mine = sm.all[e];
+    const int place = place_among(sm.all, total, mine);
+    if (place < k) a.keys[(row * parts + part) * (int64_t)k + place] = mine;
+  }
+}
+
+// A candidate: a larger `total` first, a lower place among equal ones.  total: bits that compare as the 64-bit floats do; 1 for NaN, 0 for none.
+struct Candidate {
+  unsigned long long total, place;
+};
+__device__ __forceinline__ bool precedes(const Candidate& a, const Candidate& b) { return a.total > b.total || (a.total == b.total && a.place < b.place); }
+__device__ __forceinline__ unsigned long long ordered_total(double x) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(x + 0.0);
+  return x != x ? 1ull : b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
+}
+__device__ __forceinline__ double value_of_total(unsigned long long t) {
+  return t == 1ull ? (double)NAN : __longlong_as_double((long long)(t ^ ((t >> 63) ? 0x8000000000000000ull : ~0ull)));
+}
+
+__global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int parts) {
+  extern __shared__ __attribute__((aligned(16))) char dynamic[];
+  __shared__ Candidate heads[kMaxLists];
+  __shared__ double offset[kMaxBeams];  // score - log-sum-exp; not finite: the beam's total whatever the column
+  __shared__ int have[kMaxLists], rank[kMaxLists];
+  __shared__ Candidate bound;
+  __shared__ int kept;
+  Candidate* const left = (Candidate*)dynamic;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t item = blockIdx.x, row0 = item * a.beams;
+  const int lists = a.beams * parts, each = a.each, k = a.k;
+  for (int b = wave; b < a.beams; b += kJoinThreads / 64) {
+    PartSum p{0.0, -INFINITY, 0};
+    if (lane < parts) p = a.part[(row0 + b) * parts + lane];
+    float top = p.top;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    double s = p.sum;
+    if (p.top > -INFINITY && p.top != top) s *= exp2((double)(p.top - top) * ((double)a.scale_hi + (double)a.scale_lo));
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    const float score = a.scores[row0 + b];
+    // No logit above -inf: s is 0, and its logarithm -inf; NaN comes in with s.
+    double off = (double)score - ((double)(top > -INFINITY ? top : 0.f) * a.rcp_temp + log(s));
+    if (!(score < INFINITY) || s != s || top == INFINITY) off = (double)NAN;
+    else if (s == 0.0 || score == -INFINITY) off = -(double)INFINITY;
+    if (lane < parts) have[b * parts + lane] = off - off == 0.0 ? p.keys : lane == 0 ? each : 0;
+    if (lane == 0) offset[b] = off;
+  }
+  if (tid == 0) kept = 0, bound = Candidate{0, ~0ull};
+  __syncthreads();
+  auto candidate = [&](int list, int j) {
+    const int b = list / parts;
+    const double off = offset[b];
+    if (!(off - off == 0.0)) return Candidate{ordered_total(off), ((unsigned long long)b << 32) | (unsigned)j};
+    const topkey_t key = a.keys[(row0 * parts + list) * (int64_t)each + j];
+    const double total = off + (double)value_of_bits(key_bits(key)) * a.rcp_temp;
+    return Candidate{ordered_total(total), ((unsigned long long)b << 32) | (unsigned)key_column(key)};
+  };
+  for (int l = tid; l < lists; l += kJoinThreads) heads[l] = have[l] > 0 ? candidate(l, 0) : Candidate{0, ~0ull};
+  __syncthreads();
+  for (int l = tid; l < lists; l += kJoinThreads) {
+    const Candidate mine = heads[l];
+    int r = 0;
+    for (int i = 0; i < lists; ++i) r += precedes(heads[i], mine) ? 1 : 0;
+    rank[l] = have[l] > 0 ? r : kMaxTop;
+    if (r == k - 1 && have[l] > 0) bound = mine;  // at most one: places differ
+  }
+  __syncthreads();
+  const Candidate least = bound;
+  for (int e = tid; e < lists * each; e += kJoinThreads) {
+    const int l = e / each, j = e - l * each;
+    if (j + rank[l] >= k || j >= have[l]) continue;
+    const Candidate c = candidate(l, j);
+    if (!precedes(least, c)) left[atomicAdd(&kept, 1)] = c;  // in any order: places depend on the candidates alone
+  }
+  __syncthreads();
+  const int n = kept;
+  for (int e = tid; e < n; e += kJoinThreads) {
+    const Candidate mine = left[e];
+    int place = 0;
+    for (int i = 0; i < n; ++i) place += precedes(left[i], mine) ? 1 : 0;
+    if (place < k) {
+      const int64_t at = item * k + place;
+      a.out_scores[at] = (float)value_of_total(mine.total);
+      a.parents[at] = (int64_t)(mine.place >> 32);
+      a.tokens[at] = (int64_t)(mine.place & 0xffffffffull);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// The states of the beams, rows [items * beams] of `segments` pieces of `bytes` contiguous bytes each: row j of an item becomes its row
+// parents[j].  One launch for all tensors of a layout.  Bound by HBM; rows that several beams take are read from the caches.
+// ------------------------------------------------------------------------------------------------------------
+constexpr int kStates = SKYRL_LOGITS_STATES_MAX;
+constexpr int kCopyThreads = 256, kCopyPieces = 4;  // pieces that a thread has in flight
+
+struct ReorderArgs {
+  const char* from[kStates];
+  char* to[kStates];
+  int64_t from_row, from_segment, to_row, to_segment;  // bytes
+  const int64_t* parents;  // [items, beams_out]
+  int beams_in, beams_out;
+  uint32_t segments, pieces;  // of a row, of a segment
+  uint32_t blocks;            // workgroups of a segment
+};
+
+template <class Unit>
+__device__ __forceinline__ Unit nothing() {
+  if constexpr (sizeof(Unit) == 16) return Unit{0, 0, 0, 0};
+  else return Unit{0};
+}
+
+template <class Unit>
+__global__ __launch_bounds__(kCopyThreads) void beam_copy(const ReorderArgs a) {
+  const uint32_t in_row = a.segments * a.blocks, row = blockIdx.x / in_row, rest = blockIdx.x - row * in_row;
+  const uint32_t segment = rest / a.blocks, block = rest - segment * a.blocks;
+  const uint32_t item = row / (uint32_t)a.beams_out;
+  const int64_t parent = a.parents[row];
+  const bool has = parent >= 0 && parent < a.beams_in;
+  const Unit* from = (const Unit*)(a.from[blockIdx.y] + ((int64_t)item * a.beams_in + (has ? parent : 0)) * a.from_row + (int64_t)segment * a.from_segment);
+  Unit* to = (Unit*)(a.to[blockIdx.y] + (int64_t)row * a.to_row + (int64_t)segment * a.to_segment);
+  const uint32_t p0 = block * (kCopyThreads * kCopyPieces) + threadIdx.x;
+  Unit w[kCopyPieces];
+#pragma unroll
+  for (int u = 0; u < kCopyPieces; ++u) {
+    const uint32_t p = p0 + u * kCopyThreads;
+    w[u] = nothing<Unit>();
+    if (has && p < a.pieces) w[u] = from[p];
+  }
+#pragma unroll
+  for (int u = 0; u < kCopyPieces; ++u)
+    if (p0 + u * kCopyThreads < a.pieces) to[p0 + u * kCopyThreads] = w[u];
+}
+
+// In place: a thread reads one piece of all beams of an item into LDS before it writes any.  Rows that stay are not written, and those that no
+// other beam takes not read.
+template <class Unit>
+__global__ __launch_bounds__(kCopyThreads) void beam_permute(const ReorderArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char dynamic[];
+  __shared__ int parent[kMaxBeams];
+  __shared__ int wanted[kMaxBeams];
+  const uint32_t in_row = a.segments * a.blocks, item = blockIdx.x / in_row, rest = blockIdx.x - item * in_row;
+  const uint32_t segment = rest / a.blocks, block = rest - segment * a.blocks;
+  const int beams = a.beams_in;
+  for (int b = threadIdx.x; b < beams; b += blockDim.x) wanted[b] = 0;
+  __syncthreads();
+  for (int b = threadIdx.x; b < beams; b += blockDim.x) {
+    const int64_t p = a.parents[(int64_t)item * beams + b];
+    parent[b] = p >= 0 && p < beams ? (int)p : -1;
+    if (p >= 0 && p < beams && p != b) wanted[p] = 1;  // the same value from whichever beam
+  }
+  __syncthreads();
+  const uint32_t p = block * blockDim.x + threadIdx.x;
+  if (p >= a.pieces) return;
+  char* const base = a.to[blockIdx.y] + (int64_t)item * beams * a.to_row + (int64_t)segment * a.to_segment + (int64_t)p * (int64_t)sizeof(Unit);
+  Unit* const mine = (Unit*)dynamic + threadIdx.x;
+#pragma unroll 4
+  for (int b = 0; b < beams; ++b)
+    if (wanted[b]) mine[b * blockDim.x] = *(const Unit*)(base + (int64_t)b * a.to_row);
+#pragma unroll 4
+  for (int b = 0; b < beams; ++b) {
+    const int from = parent[b];
+    if (from == b) continue;
+    *(Unit*)(base + (int64_t)b * a.to_row) = from < 0 ? nothing<Unit>() : mine[from * blockDim.x];
+  }
+}
+
+// Entries that can be left of `lists` lists of `each`: sum over the heads' ranks r of what j + r < k allows.
+size_t most_left(int lists, int each, int k) {
+  size_t n = 0;
+  for (int r = 0; r < lists && r < k; ++r) n += (size_t)(each < k - r ? each : k - r);
+  return n;
+}
+
+// Parts of a row: so many that 512 workgroups share the logits, of at least 8192 logits each.
+int beam_parts(int64_t rows, int64_t beams, int64_t V) {
+  int64_t n = 512 / rows;
+  if (n > V / 8192) n = V / 8192;
+  if (n > kMaxParts) n = kMaxParts;
+  if (n > kMaxLists / beams) n = kMaxLists / beams;
+  return n < 1 ? 1 : (int)n;
+}
+
+bool beam_extents(int64_t items, int64_t beams, int64_t V, int64_t k) {
+  return items >= 1 && beams >= 1 && beams <= kMaxBeams && items <= ((int64_t)1 << 22) / beams && V >= 1 && V < ((int64_t)1 << 31) && k >= 1 && k <= kMaxTop &&
+         k <= beams * V;
+}
+
+template <class Unit>
+int launch_reorder(hipStream_t s, ReorderArgs& a, int64_t items, int64_t bytes, int count, bool in_place) {
+  const int64_t pieces = bytes / (int64_t)sizeof(Unit);
+  int threads = kCopyThreads;
+  if (in_place)
+    while (threads > 64 && (size_t)a.beams_in * threads * sizeof(Unit) > 65536) threads /= 2;  // two workgroups a CU, but for 128 beams
+  const int64_t each = in_place ? threads : kCopyThreads * kCopyPieces, blocks = (pieces + each - 1) / each;
+  const int64_t rows = in_place ? items : items * a.beams_out;
+  // In floats, which the products of what a caller passes cannot overflow.
+  if (pieces >= ((int64_t)1 << 31) || (double)blocks * (double)a.segments * (double)rows * threads >= 4294967296.0) return SKYRL_LMHEAD_ERR_SHAPE;
+  a.pieces = (uint32_t)pieces, a.blocks = (uint32_t)blocks;
+  const dim3 grid((unsigned)(blocks * a.segments * rows), (unsigned)count);
+  if (in_place) hipLaunchKernelGGL(beam_permute<Unit>, grid, dim3((unsigned)threads), (size_t)a.beams_in * threads * sizeof(Unit), s, a);
+  else hipLaunchKernelGGL(beam_copy<Unit>, grid, dim3(kCopyThreads), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? SKYRL_LMHEAD_OK : (int)e;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t skyrl_logits_beam_select_workspace_bytes(int64_t items, int64_t beams, int64_t V, int64_t k) {
+  if (!beam_extents(items, beams, V, k)) return 0;
+  const int64_t rows = items * beams;
+  return (size_t)rows * (size_t)beam_parts(rows, beams, V) * (sizeof(PartSum) + (size_t)(k < V ? k : V) * sizeof(topkey_t));
+}
+
+int skyrl_logits_beam_select(const void* logits, int logits_dtype, int64_t ld_item, int64_t ld_beam, const float* scores, int64_t items, int64_t beams,
+                             int64_t V, int64_t k, double rcp_temperature, float* out_scores, int64_t* parents, int64_t* tokens, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  if (!logits || !scores || !out_scores || !parents || !tokens) return SKYRL_LMHEAD_ERR_NULL;
+  if (logits_dtype != SKYRL_LOGITS_BF16 && logits_dtype != SKYRL_LOGITS_F32) return SKYRL_LMHEAD_ERR_ARG;
+  if (!beam_extents(items, beams, V, k) || ld_item < 0 || ld_beam < 0 || ld_item >= ((int64_t)1 << 40) || ld_beam >= ((int64_t)1 << 40))
+    return SKYRL_LMHEAD_ERR_SHAPE;
+  const bool f32 = logits_dtype == SKYRL_LOGITS_F32;
+  if (((uintptr_t)logits & (f32 ? 3u : 1u)) || (((uintptr_t)scores | (uintptr_t)out_scores) & 3u) ||
+      (((uintptr_t)parents | (uintptr_t)tokens | (uintptr_t)workspace) & 7u))
+    return SKYRL_LMHEAD_ERR_ALIGN;
+  const double scale2 = rcp_temperature * 1.4426950408889634074;
+  const float scale_hi = (float)scale2;
+  if (!(rcp_temperature > 0.0) || !std::isfinite(scale_hi) || !(scale_hi >= 0x1p-100f)) return SKYRL_LMHEAD_ERR_ARG;
+  if (!workspace || workspace_bytes < skyrl_logits_beam_select_workspace_bytes(items, beams, V, k)) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  const int64_t rows = items * beams;
+  const int parts = beam_parts(rows, beams, V), each = (int)(k < V ? k : V);
+  topkey_t* const keys = (topkey_t*)workspace;
+  const BeamArgs a{logits, ld_item, ld_beam, scores, (int)beams, (int)V, (int)k, each, rcp_temperature, scale_hi, (float)(scale2 - (double)scale_hi),
+                   (PartSum*)(keys + (size_t)rows * (size_t)parts * (size_t)each), keys, out_scores, parents, tokens};
+  hipStream_t s = (hipStream_t)stream;
+  hipLaunchKernelGGL(f32 ? beam_rows<true> : beam_rows<false>, dim3((unsigned)rows, (unsigned)parts), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(beam_join, dim3((unsigned)items), dim3(kJoinThreads), most_left((int)beams * parts, each, (int)k) * sizeof(Candidate), s, a, parts);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? SKYRL_LMHEAD_OK : (int)e;
+}
+
+int skyrl_logits_beam_reorder(const void* const* from, void* const* to, int64_t count, int64_t from_row, int64_t from_segment, int64_t to_row,
+                              int64_t to_segment, int64_t segments, int64_t bytes, const int64_t* parents, int64_t items, int64_t beams_in, int64_t beams_out,
+                              void* stream) {
+  if (!from || !to || !parents) return SKYRL_LMHEAD_ERR_NULL;
+  const int64_t most = (int64_t)1 << 40;
+  if (count < 1 || count > kStates || segments < 1 || segments >= ((int64_t)1 << 31) || bytes < 1 || bytes >= most || items < 1 || beams_in < 1 || beams_out < 1 ||
+      items >= ((int64_t)1 << 31) || beams_in >= ((int64_t)1 << 31) || beams_out >= ((int64_t)1 << 31) || items * beams_out >= ((int64_t)1 << 31) ||
+      items * beams_in >= ((int64_t)1 << 31) || from_row < 0 || from_segment < 0 || to_row < 0 || to_segment < 0 || from_row >= most || from_segment >= most ||
+      to_row >= most || to_segment >= most)
+    return SKYRL_LMHEAD_ERR_SHAPE;
+  if ((uintptr_t)parents & 7u) return SKYRL_LMHEAD_ERR_ALIGN;
+  const bool in_place = from[0] == to[0];
+  if (in_place && (beams_in != beams_out || beams_in > kMaxBeams || from_row != to_row || from_segment != to_segment)) return SKYRL_LMHEAD_ERR_ARG;
+  ReorderArgs a{};
+  uintptr_t all = (uintptr_t)bytes | (uintptr_t)from_row | (uintptr_t)from_segment | (uintptr_t)to_row | (uintptr_t)to_segment;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!from[i] || !to[i]) return SKYRL_LMHEAD_ERR_NULL;
+    if ((from[i] == to[i]) != in_place) return SKYRL_LMHEAD_ERR_ARG;
+    a.from[i] = (const char*)from[i], a.to[i] = (char*)to[i];
+    all |= (uintptr_t)from[i] | (uintptr_t)to[i];
+  }
+  a.from_row = from_row, a.from_segment = from_segment, a.to_row = to_row, a.to_segment = to_segment;
+  a.parents = parents, a.beams_in = (int)beams_in, a.beams_out = (int)beams_out, a.segments = (uint32_t)segments;
+  hipStream_t s = (hipStream_t)stream;
+  if (all % 16 == 0) return launch_reorder<u32x4>(s, a, items, bytes, (int)count, in_place);
+  if (all % 4 == 0) return launch_reorder<uint32_t>(s, a, items, bytes, (int)count, in_place);
+  return launch_reorder<uint8_t>(s, a, items, bytes, (int)count, in_place);
+}
+
+}  // extern "C"
