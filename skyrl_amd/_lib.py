@@ -124,6 +124,15 @@ SIGNATURES = {
     "skyrl_logits_top_bwd": (
         ctypes.c_int,
         [_c_p, ctypes.c_int, _c_i64] + [_c_p] * 7 + [_c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_i64, _c_p]),
+    "skyrl_lmhead_int8_rows": (ctypes.c_int, [_c_p, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p]),
+    "skyrl_lmhead_int8_fwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 3),
+    "skyrl_lmhead_int8_fwd": (
+        ctypes.c_int,
+        [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p, _c_p, ctypes.c_size_t, _c_p]),
+    "skyrl_lmhead_int8_logits_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 2),
+    "skyrl_lmhead_int8_logits": (
+        ctypes.c_int,
+        [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p, _c_i64, _c_p, ctypes.c_size_t, _c_p]),
     "skyrl_lmhead_embedding_fwd": (
         ctypes.c_int, [_c_p, ctypes.c_int, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p]),
     "skyrl_lmhead_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 3),

@@ -120,31 +120,56 @@ def _segments(t: torch.Tensor, u: torch.Tensor) -> List[Tuple[torch.Tensor, torc
     return [(t, u, n, inner * size, x * size, y * size)]
 
 
-def _check_states(states: Sequence[torch.Tensor], parents: torch.Tensor, out: Optional[Sequence[torch.Tensor]]) -> Tuple[int, int, int]:
-    """``(items, beams_in, beams_out)``."""
-    if parents.dim() != 2:
-        raise ValueError(f"expected parents [N, B], got {tuple(parents.shape)}")
-    if parents.dtype != torch.int64:
-        raise TypeError(f"parents must be int64, got {parents.dtype}")
-    N, B_out = (int(x) for x in parents.shape)
-    if len(states) == 0:
-        return N, 0, B_out
-    rows = int(states[0].shape[0]) if states[0].dim() > 0 else 0
-    for t in states:
-        if t.dim() < 1 or int(t.shape[0]) != rows:
-            raise ValueError("every state must have the beams of all prompts, N * B of them, along its first dimension; got "
-                             + ", ".join(str(tuple(s.shape)) for s in states))
-    if N == 0 and rows or N and rows % N:
-        raise ValueError(f"{rows} rows of states do not divide among {N} prompts")
-    if out is not None:
-        if len(out) != len(states):
-            raise ValueError(f"{len(out)} results for {len(states)} states")
-        for t, u in zip(states, out):
-            if u.shape != (N * B_out,) + t.shape[1:] or u.dtype != t.dtype:
-                raise ValueError(f"a result must be {(N * B_out,) + tuple(t.shape[1:])} {t.dtype}, got {tuple(u.shape)} {u.dtype}")
-            if any(n > 1 and s == 0 for n, s in zip(u.shape, u.stride())):
-                raise ValueError("a result must not be expanded: its elements would be written more than once")
-    return N, rows // N if N else 0, B_out
+class _Layout:
+    """Pairs of a state and its result that have the same type, shape and strides."""
+
+    def __init__(self, t: torch.Tensor, u: torch.Tensor, items: int, beams_out: int, given: bool):
+        self.dtype, self.shape, self.strides, self.to_strides = t.dtype, t.shape, t.stride(), u.stride()
+        if t.dim() < 1:
+            raise ValueError("a state has the beams of all prompts along its first dimension, got a scalar")
+        rows = int(t.shape[0])
+        if items == 0 and rows or items and rows % items:
+            raise ValueError(f"{rows} rows of a state {tuple(t.shape)} do not divide among {items} prompts")
+        self.beams_in = rows // items if items else 0
+        if given and any(n > 1 and s == 0 for n, s in zip(u.shape, u.stride())):
+            raise ValueError("a result must not be expanded: its elements would be written more than once")
+        self.to_shape = torch.Size((items * beams_out,) + tuple(t.shape[1:]))
+        size = t.element_size()
+        extent = lambda x: size * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) if x.numel() else 0  # noqa: E731
+        self.extent, self.to_extent = extent(t), extent(u)
+        self.pairs: List[Tuple[int, int]] = []
+        self.first = (t, u)
+
+    def launches(self) -> List[Tuple[Tuple[int, ...], List[Tuple[int, int]]]]:
+        """For each kind of segment its sizes and strides in bytes and the two addresses of its first row in each pair; pairs in place apart from the others."""
+        t, u = self.first
+        size, t0, u0 = t.element_size(), t.data_ptr(), u.data_ptr()
+        row = t.stride(0) * size if t.shape[0] > 1 else 0
+        to_row = u.stride(0) * size if u.shape[0] > 1 else 0
+        found: dict = {}
+        for x, y, n, nbytes, step, to_step in _segments(t, u):
+            dx, dy = x.data_ptr() - t0, y.data_ptr() - u0
+            found.setdefault((row, step, to_row, to_step, n, nbytes), []).extend([(p + dx, q + dy) for p, q in self.pairs])
+        kinds = []
+        for sizes, pairs in found.items():
+            inside = [pair for pair in pairs if pair[0] == pair[1]]
+            kinds += [(sizes, some) for some in (([pair for pair in pairs if pair[0] != pair[1]], inside) if inside else (pairs,)) if some]
+        return kinds
+
+
+def _overlap(states: Sequence[Tuple[int, int]], results: Sequence[Tuple[int, int]]) -> bool:
+    """Whether one of the results' ranges of addresses meets one of the states'."""
+    if max(b for _, b in states) <= min(a for a, _ in results) or max(b for _, b in results) <= min(a for a, _ in states):
+        return False
+    end_of_state = end_of_result = 0
+    for start, end, is_result in sorted([(a, b, False) for a, b in states] + [(a, b, True) for a, b in results]):
+        if start < (end_of_state if is_result else end_of_result):
+            return True
+        if is_result:
+            end_of_result = max(end_of_result, end)
+        else:
+            end_of_state = max(end_of_state, end)
+    return False
 
 
 def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
@@ -152,47 +177,72 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
     (the used part of a cache, say) and ``parents [N, B_out]`` int64; zeros where a parent lies outside ``[0, B_in)``.
 
     ``out``: tensors to write, new ones without it.  ``out=states`` reorders in place (``B_out == B_in``, at most 128 beams): rows that keep their place
-    are not moved.  A result is otherwise in memory of its own; one that shares a storage with a state is refused.  Not differentiable."""
+    are not moved.  A result is otherwise in memory of its own: one whose range of addresses meets a state's is refused.  Not differentiable."""
     states = list(states)
-    N, B_in, B_out = _check_states(states, parents, out)
-    if any(torch.is_grad_enabled() and t.requires_grad for t in [*states, *(out or [])]) or has_tangent(*states):
-        raise ValueError("beam_reorder has no gradient: call it under torch.no_grad()")
-    if out is None:
-        results = [t.new_empty((N * B_out,) + tuple(t.shape[1:])) for t in states]
-    else:
+    if parents.dim() != 2:
+        raise ValueError(f"expected parents [N, B], got {tuple(parents.shape)}")
+    if parents.dtype != torch.int64:
+        raise TypeError(f"parents must be int64, got {parents.dtype}")
+    N, B_out = (int(x) for x in parents.shape)
+    given = out is not None
+    if given:
         results = list(out)
-    if not states or N * B_out == 0 or all(t.numel() == 0 for t in results):
+        if len(results) != len(states):
+            raise ValueError(f"{len(results)} results for {len(states)} states")
+    else:
+        results = [t.new_empty((N * B_out,) + tuple(t.shape[1:])) for t in states]
+    if not states:
         return results
-    dev = _require_device(parents, *states, *results)
-    if B_in == 0:  # no row to take
+    if torch.is_grad_enabled() and any([t.requires_grad for t in states + results]) or has_tangent(*states):
+        raise ValueError("beam_reorder has no gradient: call it under torch.no_grad()")
+    # What depends on the layout alone is looked at once for each: a model has many states and few layouts.
+    kinds = list(zip([t.shape for t in states], [t.stride() for t in states], [u.stride() for u in results], [t.dtype for t in states]))
+    groups = {kinds[0]: (states, results)}
+    if kinds.count(kinds[0]) < len(kinds):
+        groups = {}
+        for kind, t, u in zip(kinds, states, results):
+            some = groups.setdefault(kind, ([], []))
+            some[0].append(t), some[1].append(u)
+    layouts = [_Layout(ts[0], us[0], N, B_out, given) for ts, us in groups.values()]
+    beams_in = layouts[0].beams_in
+    if any(layout.beams_in != beams_in for layout in layouts):
+        raise ValueError(f"states of unlike numbers of beams a prompt: {sorted({layout.beams_in for layout in layouts})}")
+    for layout, (ts, us) in zip(layouts, groups.values()):
+        if given and ([u.shape for u in us].count(layout.to_shape) < len(us) or [u.dtype for u in us].count(layout.dtype) < len(us)):
+            raise ValueError(f"a result must be {tuple(layout.to_shape)} {layout.dtype}, got " + ", ".join(f"{tuple(u.shape)} {u.dtype}" for u in us))
+        layout.pairs = list(zip([t.data_ptr() for t in ts], [u.data_ptr() for u in us]))
+    used = [layout for layout in layouts if layout.to_extent > 0]
+    if not used:
+        return results
+    device = parents.get_device()
+    if device < 0 or [t.get_device() for t in states + results].count(device) < 2 * len(states):
+        _require_device(parents, *states, *results)
+    if given:
+        apart = []  # the ranges of addresses of results that are not their states
+        for layout in used:
+            if layout.strides == layout.to_strides and layout.beams_in == B_out:
+                some = [q for p, q in layout.pairs if p != q]
+                if len(some) < len(layout.pairs) and B_out > MAX_BEAMS:
+                    raise ValueError(f"at most {MAX_BEAMS} beams are reordered in place, got {B_out}")
+            else:
+                some = [q for _, q in layout.pairs]
+            apart += [(q, q + layout.to_extent) for q in some]
+        to = [q for layout in used for _, q in layout.pairs]
+        if len(set(to)) < len(to):
+            raise ValueError("a result is given twice")
+        if apart and _overlap([(p, p + layout.extent) for layout in used for p, _ in layout.pairs], apart):
+            raise ValueError("a result overlaps a state and is not that state: it would be read after it was written")
+    dev = _require_device(parents, states[0])
+    if beams_in == 0:  # no row to take
         return [u.zero_() for u in results]
-    kept = {t.untyped_storage().data_ptr() for t in states} if out is not None else ()
-    groups: dict = {}
-    seen = set()
-    for t, u in zip(states, results):
-        if u.numel() == 0:
-            continue
-        in_place = t.data_ptr() == u.data_ptr() and t.shape == u.shape and t.stride() == u.stride()
-        if out is not None:
-            if u.data_ptr() in seen:
-                raise ValueError("a result is given twice")
-            seen.add(u.data_ptr())
-            if not in_place and u.untyped_storage().data_ptr() in kept:
-                raise ValueError("a result shares its storage with a state and is not that state: it would be read after it was written")
-            if in_place and B_in > MAX_BEAMS:
-                raise ValueError(f"at most {MAX_BEAMS} beams are reordered in place, got {B_in}")
-        size = t.element_size()
-        for x, y, n, nbytes, from_segment, to_segment in _segments(t, u):
-            layout = (in_place, x.stride(0) * size if x.shape[0] > 1 else 0, from_segment, y.stride(0) * size if y.shape[0] > 1 else 0, to_segment, n, nbytes)
-            groups.setdefault(layout, []).append((x.data_ptr(), y.data_ptr()))
     lib, parents = _lib.load(), parents.contiguous()
     with device_guard(dev):
         stream = raw_stream(dev)
-        for (_, *layout), pairs in groups.items():
-            for at in range(0, len(pairs), _MAX_STATES):
-                some = pairs[at:at + _MAX_STATES]
-                array = ctypes.c_void_p * len(some)
-                st = lib.skyrl_logits_beam_reorder(array(*[p for p, _ in some]), array(*[p for _, p in some]), len(some), *layout, parents.data_ptr(), N, B_in,
-                                                   B_out, stream)
-                _lib.check(st, "skyrl_logits_beam_reorder")
+        for layout in used:
+            for sizes, pairs in layout.launches():
+                for at in range(0, len(pairs), _MAX_STATES):
+                    from_, to = zip(*pairs[at:at + _MAX_STATES])
+                    array = ctypes.c_void_p * len(from_)
+                    st = lib.skyrl_logits_beam_reorder(array(*from_), array(*to), len(from_), *sizes, parents.data_ptr(), N, beams_in, B_out, stream)
+                    _lib.check(st, "skyrl_logits_beam_reorder")
     return results

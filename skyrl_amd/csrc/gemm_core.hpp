@@ -167,6 +167,14 @@ __device__ __forceinline__ void mfma_16x16x32(f32x4& c, const bf16x8& a, const b
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
+// The same on 8-bit integers (I8): a 16-byte chunk is sixteen of them instead of eight bf16 values, the instruction takes 64 k in the time of 32, and an
+// accumulator register holds a 32-bit integer.  Slots, copies, fragments and schedules count bytes and are the same.
+template <bool I8>
+__device__ __forceinline__ void mfma_step(f32x4& c, const bf16x8& a, const bf16x8& b) {
+  if constexpr (I8) asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else mfma_16x16x32(c, a, b);
+}
+
 template <int N>
 __device__ __forceinline__ void zero_acc(f32x4 (&acc)[TM][N]) {
 #pragma unroll
@@ -319,7 +327,7 @@ __device__ __forceinline__ void prefetch_first_tiles(const Operand& a, const Ope
 // V=151936, all tiles square -> the last one narrow: 132 -> 114 us at T=300, H=896, 252 -> 221 at T=384, H=2048, 468 -> 432 at T=1100, H=1536;
 // training pass 958 -> 925 at T=611, H=1536.  Medium, square -> medium: 84 -> 75 us at T=137, H=896, 461 -> 445 at T=1200, H=1536, training
 // pass 778 -> 751 at T=440, H=2048, V=100000.
-template <bool BKM = false, int SHAPE = kSquare>
+template <bool BKM = false, int SHAPE = kSquare, bool I8 = false>
 __device__ __forceinline__ void mainloop_ksteps(const Operand& a, const Operand& b, int k_begin, int nk, char* lds,
                                                 f32x4 (&acc)[TM][wave_cols(SHAPE)]) {
   constexpr int N = wave_cols(SHAPE);
@@ -444,7 +452,7 @@ __device__ __forceinline__ void mainloop_ksteps(const Operand& a, const Operand&
 #pragma unroll
       for (int x = 0; x < kMfmas; ++x) {
         const int i = mfma_row<N>(x), j = mfma_col<N>(x);
-        mfma_16x16x32(acc[i][j], af[ks][i], b_frag(ks, j));
+        mfma_step<I8>(acc[i][j], af[ks][i], b_frag(ks, j));
         __builtin_amdgcn_sched_barrier(0);
         if (x % 2 == 0 && x < 2 * READS_PER_STEP) {
           if (ks == 0) read_one(ra1, rb1, 1, x / 2);
@@ -532,7 +540,7 @@ constexpr QuadPlan kQuadPlan[2][4] = {
     {{0, 0, 0, 0, 1, 1, 0, 1}, {0, 1, 0, 1, 0, 1, 0, 1}, {1, 1, 1, 1, 0, 1, 1, 0}, {1, 0, 1, 0, 1, 0, 1, 1}},
     {{1, 0, 0, 1, 1, 1, 0, 0}, {1, 1, 0, 0, 0, 0, 0, 1}, {0, 1, 1, 0, 0, 0, 1, 0}, {0, 0, 1, 1, 1, 0, 1, 0}}};
 
-template <bool BKM = false>
+template <bool BKM = false, bool I8 = false>
 __device__ __forceinline__ void mainloop_pairs(const Operand& a, const Operand& b, int k_begin, int nk, char* lds, acc_t& acc) {
   CopyPlan p;
   make_plan<BKM>(p, a, b, k_begin);
@@ -634,7 +642,7 @@ __device__ __forceinline__ void mainloop_pairs(const Operand& a, const Operand& 
       for (int pos = 0; pos < 32; ++pos) {
         const int pr = pos / 2, ks = pos % 2;
         const int r = quad_row(pr), c = quad_col(pr);
-        mfma_16x16x32(acc[pl.a_half * 4 + r][pl.b_half * 4 + c], sa[pl.a_slot][r * 2 + ks], b_frag(pl.b_slot, c * 2 + ks));
+        mfma_step<I8>(acc[pl.a_half * 4 + r][pl.b_half * 4 + c], sa[pl.a_slot][r * 2 + ks], b_frag(pl.b_slot, c * 2 + ks));
         __builtin_amdgcn_sched_barrier(0);
         if (!(LMHEAD_ABLATE & 32) && do_load && pos % 2 == 0 && pos / 2 < nreads) {
           if (pl.ld_is_b) read_b(pl.ld_next ? nxt : cur, pl.ld_half, pl.ld_slot, pos / 2);
@@ -688,19 +696,19 @@ __device__ __forceinline__ void mainloop_pairs(const Operand& a, const Operand& 
 
 // The mainloop of a tile: EVEN_NK (the caller guarantees an even number of k-tiles, at least two) takes the
 // accumulator-stationary order, anything else the k-step order.  Both leave identical accumulators.
-template <bool BKM = false, bool EVEN_NK = false>
+template <bool BKM = false, bool EVEN_NK = false, bool I8 = false>
 __device__ __forceinline__ void mainloop(const Operand& a, const Operand& b, int k_begin, int nk, char* lds, acc_t& acc) {
-  if constexpr (EVEN_NK) mainloop_pairs<BKM>(a, b, k_begin, nk, lds, acc);
-  else mainloop_ksteps<BKM>(a, b, k_begin, nk, lds, acc);
+  if constexpr (EVEN_NK) mainloop_pairs<BKM, I8>(a, b, k_begin, nk, lds, acc);
+  else mainloop_ksteps<BKM, kSquare, I8>(a, b, k_begin, nk, lds, acc);
 }
 
 // acc = the product of a tile of K-contiguous operands over the whole contraction, of nk k-tiles.
-template <int SHAPE, bool EVEN_NK>
+template <int SHAPE, bool EVEN_NK, bool I8 = false>
 __device__ __forceinline__ void tile_product(const Operand& a, const Operand& b, int nk, char* lds, f32x4 (&acc)[TM][wave_cols(SHAPE)]) {
   prefetch_first_tiles<false, SHAPE>(a, b, 0, nk, lds);  // the first copies travel while the accumulators are cleared
   zero_acc(acc);
-  if constexpr (SHAPE == kSquare) mainloop<false, EVEN_NK>(a, b, 0, nk, lds, acc);
-  else mainloop_ksteps<false, SHAPE>(a, b, 0, nk, lds, acc);
+  if constexpr (SHAPE == kSquare) mainloop<false, EVEN_NK, I8>(a, b, 0, nk, lds, acc);
+  else mainloop_ksteps<false, SHAPE, I8>(a, b, 0, nk, lds, acc);
 }
 
 // Work item id -> tile coordinates.

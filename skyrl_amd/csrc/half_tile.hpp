@@ -44,6 +44,7 @@ __device__ __forceinline__ void half_copy(const char* g, uint32_t src, uint32_t 
 
 // acc = A[a.row0 : +256, 0 : 32 * steps] * B[b.row0 : +128, same k]^T.  steps >= 2.  Every thread of the workgroup calls this with the
 // same arguments; on return no copy is in flight, every wave has left the ring, and the accumulators may be read.
+template <bool I8 = false>
 __device__ __forceinline__ void half_tile_product(const Operand& a, const Operand& b, int steps, char* lds, half_acc_t& acc) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -111,7 +112,7 @@ __device__ __forceinline__ void half_tile_product(const Operand& a, const Operan
 #pragma unroll
       for (int j = 0; j < kHalfTN; ++j) {
         const int jj = (i & 1) ? kHalfTN - 1 - j : j;  // consecutive MFMAs share one operand
-        mfma_16x16x32(acc[i][jj], af[i], bfr[jj]);
+        mfma_step<I8>(acc[i][jj], af[i], bfr[jj]);
       }
     const uint32_t t = s0;
     s0 = s1, s1 = s2, s2 = t;

@@ -1,0 +1,271 @@
+// The head in 8-bit integers: hidden rows and weight rows as int8 values with one fp32 scale each,
+//
+//   z[t, v] = s_t c_v sum_i q[t, i] w[v, i]
+//
+// The sum is exact (32-bit integers); it is multiplied by the two scales in fp32.  The tiles are those of the bf16 head (gemm_core.hpp,
+// half_tile.hpp): a 16-byte chunk holds sixteen values instead of eight, the matrix instruction takes twice the k in the same time, so that
+// slots, copies and schedules stay as they are and a k-tile is 128 k long.
+#include "int8.hpp"
+
+#include "head_tiles.hpp"
+
+namespace lmhead {
+namespace {
+
+constexpr int kRowThreads = 256;
+
+// A workgroup per row: the largest magnitude m, then the values, the second time from the caches.
+// Quotients 127 x / m are rounded as if they were exact.  With significands X and M of p bits, 127 x / m is 127 X / (M 2^d), d >= 0: what is not exactly between
+// two integers is at least 1 / (M 2^(d + 1)) away from it, 2^-(p + 8) of the quotient or more.  In fp32 (p = 24) a 64-bit division, off by 2^-53,
+// stays on its side, and is exact where the quotient lies exactly between.  In bf16 (p = 8) x times the 64-bit 127 / m, rounded to fp32, is off by 2^-24, and where the
+// quotient is exactly between, a number of 9 bits, the rounding to fp32 leads back to it.
+template <bool F32>
+__global__ __launch_bounds__(kRowThreads) void int8_rows(const char* __restrict__ src, int64_t ld_src, int H, int8_t* __restrict__ values, int64_t ld,
+                                                         int K, float* __restrict__ scale) {
+  constexpr int ES = F32 ? 4 : 2, E = 8;
+  struct __attribute__((packed, aligned(ES))) Piece {
+    u32x4 v;
+  };
+  __shared__ uint32_t most[kRowThreads / 64];
+  const int64_t row = blockIdx.x;
+  const char* from = src + (size_t)row * (size_t)ld_src * ES;
+  auto load = [&](int e0, float (&x)[E]) {  // elements e0 .. e0 + 7, zeros behind the row
+    if (e0 + E <= H) {
+      const u32x4 a = ((const Piece*)(from + (size_t)e0 * ES))[0].v;
+      if constexpr (F32) {
+        const u32x4 b = ((const Piece*)(from + (size_t)e0 * ES))[1].v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(a[i]), x[4 + i] = __uint_as_float(b[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(a[i] << 16), x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        x[i] = 0.f;
+        if (e0 + i < H) {
+          if constexpr (F32) x[i] = ((const float*)from)[e0 + i];
+          else x[i] = __uint_as_float((uint32_t)((const uint16_t*)from)[e0 + i] << 16);
+        }
+      }
+    }
+  };
+  // Magnitudes as integers compare as they do as floats, and NaN is the largest.
+  uint32_t m = 0;
+  for (int e0 = threadIdx.x * E; e0 < H; e0 += kRowThreads * E) {
+    float x[E];
+    load(e0, x);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
+      m = m > b ? m : b;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const uint32_t b = (uint32_t)__shfl_xor((int)m, o, 64);
+    m = m > b ? m : b;
+  }
+  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = 0;
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 64; ++w) m = m > most[w] ? m : most[w];
+  const bool odd = m >= 0x7f800000u;  // NaN or an infinity
+  const float top = __uint_as_float(m);
+  if (threadIdx.x == 0) scale[row] = odd ? NAN : top / 127.f;
+  const double per = odd || m == 0 ? 0.0 : 127.0 / (double)top;
+  int8_t* const to = values + (size_t)row * (size_t)ld;
+  for (int e0 = threadIdx.x * E; e0 < K; e0 += kRowThreads * E) {
+    float x[E];
+    load(e0, x);
+    uint32_t packed[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      float q;
+      if constexpr (F32) q = per == 0.0 ? 0.f : (float)rint((double)x[i] * 127.0 / (double)top);
+      else q = per == 0.0 ? 0.f : rintf((float)((double)x[i] * per));
+      packed[i / 4] |= ((uint32_t)(int)q & 0xffu) << (8 * (i % 4));
+    }
+    *(uint2*)(to + e0) = make_uint2(packed[0], packed[1]);
+  }
+}
+
+__device__ __forceinline__ Operand bytes_of(const Int8Rows& r, int row0, int rows) { return Operand{(const uint16_t*)r.values, (int)(r.ld / 2), row0, rows}; }
+
+// The sums of a wave's token block j times the scales of its vocabulary rows.
+struct RowScales {
+  f32x4 c[TM];  // of rows vbase + i * 16 + (lane >> 4) * 4 .. + 3
+  __device__ __forceinline__ RowScales(const float* __restrict__ scale, int vbase, int V) {
+    struct __attribute__((packed, aligned(4))) Four {
+      f32x4 v;
+    };
+    const int v0 = vbase + ((threadIdx.x & 63) >> 4) * 4;
+    if (vbase + WM <= V) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) c[i] = ((const Four*)(scale + v0 + i * MT))->v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[i][r] = scale[v0 + i * MT + r < V ? v0 + i * MT + r : V - 1];
+    }
+  }
+  template <int NB>
+  __device__ __forceinline__ void apply(const f32x4 (&acc)[TM][NB], int j, float s, f32x4 (&z)[TM]) const {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z[i][r] = (float)__float_as_int(acc[i][j][r]) * c[i][r] * s;
+  }
+};
+
+// Statistics of a wave's logits, as fwd_epilogue() (logits_tile.hpp) makes them; the token's scale enters with the temperature.
+template <bool ENTROPY, int NB>
+__device__ __forceinline__ void int8_stats(const f32x4 (&acc)[TM][NB], const Int8FwdArgs& a, int part, int nparts, int t0) {
+  const int lane = threadIdx.x & 63, lrow = lane & 15, kq = lane >> 4;
+  const int vbase = part * WM;
+  const int rows_kind = __builtin_amdgcn_readfirstlane(vbase + WM <= a.V ? 0 : (vbase < a.V ? 1 : 2));
+  const RowScales scales(a.W.scale, vbase, a.V);
+  float s_t[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int t = t0 + j * MT + lrow;
+    s_t[j] = a.Hd.scale[t < a.T ? t : a.T - 1] * a.rcp_temp * kLog2e;
+  }
+  for_each_int(std::make_integer_sequence<int, NB>{}, [&](auto index) {
+    constexpr int j = decltype(index)::value;
+    const int t = t0 + j * MT + lrow;
+    float m = -INFINITY, s = 0.f, e = 0.f;
+    f32x4 z[TM][1];
+    {
+      f32x4 x[TM];
+      scales.apply(acc, j, 1.f, x);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) z[i][0] = x[i];
+    }
+    if (rows_kind == 0) fwd_tile_stats<ENTROPY, false, false>(z, 0, vbase, a.V, s_t[j], kq, m, s, e);
+    else if (rows_kind == 1) fwd_tile_stats<ENTROPY, true, false>(z, 0, vbase, a.V, s_t[j], kq, m, s, e);
+    if (kq == 0 && t < a.T) {
+      const size_t idx = part_index(part, t, nparts);
+      a.part_max[idx] = m;
+      a.part_sum[idx] = s;
+      if (ENTROPY) a.part_pz[idx] = e;
+    }
+  });
+}
+
+// epilogue(acc, first vocabulary row of the wave, first token of the wave) of a tile of whatever shape; v0: its first vocabulary row.
+template <int SHAPE, bool EVEN, class Args, class Epilogue>
+__device__ __forceinline__ void int8_tile(const Args& a, int v0, int tn, char* lds, Epilogue epilogue) {
+  const int wave = threadIdx.x >> 6;
+  // A part behind the vocabulary (the upper half of the last tile) is made of any row and dropped behind this.
+  const Operand oa = bytes_of(a.W, SHAPE == kShort && v0 >= a.V ? a.V - 1 : v0, a.V), ob = bytes_of(a.Hd, tn * BN, a.T);
+  f32x4 acc[TM][wave_cols(SHAPE)];
+  tile_product<SHAPE, EVEN, true>(oa, ob, a.K / kInt8K, lds, acc);
+  epilogue(acc, v0 + wave / waves_n(SHAPE) * WM, tn * BN + wave % waves_n(SHAPE) * (wave_cols(SHAPE) * MT));
+}
+
+template <class Args, class Epilogue>
+__device__ __forceinline__ void int8_half_tile(const Args& a, char* lds, Epilogue epilogue) {
+  const int tiles_m = (a.V + BM - 1) / BM, tiles_n = (a.T + kHalfBN - 1) / kHalfBN;
+  int tm, tn;
+  tile_coords(blockIdx.x, tiles_m, tiles_n, kGroupM, tm, tn);
+  const int wave = threadIdx.x >> 6;
+  half_acc_t acc;
+  half_tile_product<true>(bytes_of(a.W, tm * BM, a.V), bytes_of(a.Hd, tn * kHalfBN, a.T), a.K / kHalfRowBytes, lds, acc);
+  epilogue(acc, tm * BM + wave / WAVES_N * WM, tn * kHalfBN + wave % WAVES_N * kHalfWN);
+}
+
+template <bool ENTROPY, bool EVEN, bool SHAPES>
+__global__ __launch_bounds__(NTHREADS) void int8_fwd_tiles(const Int8FwdArgs a, int split) {
+  __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES];
+  const int tiles_m = (a.V + BM - 1) / BM, tiles_n = (a.T + BN - 1) / BN;
+  const Tile t = tile_of<false, SHAPES>(blockIdx.x, tiles_m, tiles_n, kGroupM, split);
+  tile_of_shape<SHAPES>(t, a.T, [&](auto shape, int v0) {
+    constexpr int SHAPE = decltype(shape)::value;
+    int8_tile<SHAPE, EVEN>(a, v0, t.tn, lds, [&](auto& acc, int vbase, int t0) { int8_stats<ENTROPY>(acc, a, vbase / WM, tiles_m * WAVES_M, t0); });
+  });
+}
+
+template <bool ENTROPY>
+__global__ __launch_bounds__(NTHREADS, 2) void int8_fwd_half_tiles(const Int8FwdArgs a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kHalfLdsBytes];
+  int8_half_tile(a, lds, [&](auto& acc, int vbase, int t0) { int8_stats<ENTROPY>(acc, a, vbase / WM, (a.V + BM - 1) / BM * WAVES_M, t0); });
+}
+
+template <bool F32, int NB>
+__device__ __forceinline__ void int8_store(const f32x4 (&acc)[TM][NB], const Int8LogitsArgs& a, int v0, int t0, char* lds) {
+  const RowScales scales(a.W.scale, v0, a.V);
+  const int lrow = threadIdx.x & 15;
+  float s_t[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int t = t0 + j * MT + lrow;
+    s_t[j] = a.Hd.scale[t < a.T ? t : a.T - 1];
+  }
+  store_logits_tile<F32, NB>(a.out, a.ldo, nullptr, a.T, a.V, v0, t0, lds, [&](int j, f32x4 (&z)[TM]) { scales.apply(acc, j, s_t[j], z); });
+}
+
+template <bool F32, bool EVEN, bool SHAPES>
+__global__ __launch_bounds__(NTHREADS) void int8_logits_tiles(const Int8LogitsArgs a, int split) {
+  __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES];
+  const int tiles_m = (a.V + BM - 1) / BM, tiles_n = (a.T + BN - 1) / BN;
+  const Tile t = tile_of<false, SHAPES>(blockIdx.x, tiles_m, tiles_n, kGroupM, split);
+  tile_of_shape<SHAPES>(t, a.T, [&](auto shape, int v0) {
+    constexpr int SHAPE = decltype(shape)::value;
+    int8_tile<SHAPE, EVEN>(a, v0, t.tn, lds, [&](auto& acc, int vbase, int t0) { int8_store<F32>(acc, a, vbase, t0, lds); });
+  });
+}
+
+template <bool F32>
+__global__ __launch_bounds__(NTHREADS, 2) void int8_logits_half_tiles(const Int8LogitsArgs a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kHalfLdsBytes];
+  int8_half_tile(a, lds, [&](auto& acc, int vbase, int t0) { int8_store<F32>(acc, a, vbase, t0, lds); });
+}
+
+// pick(x, y, z) for the three flags as compile-time constants.
+template <class Pick>
+auto flagged(Pick pick, bool x, bool y, bool z) {
+  const std::true_type t;
+  const std::false_type f;
+  if (x) return y ? (z ? pick(t, t, t) : pick(t, t, f)) : (z ? pick(t, f, t) : pick(t, f, f));
+  return y ? (z ? pick(f, t, t) : pick(f, t, f)) : (z ? pick(f, f, t) : pick(f, f, f));
+}
+
+bool even_ktiles(int K) { return K / kInt8K % 2 == 0; }
+
+}  // namespace
+
+hipError_t launch_int8_rows(hipStream_t s, const void* src, bool f32, int64_t ld_src, int64_t rows, int64_t H, int8_t* values, int64_t ld, float* scale) {
+  hipLaunchKernelGGL(f32 ? int8_rows<true> : int8_rows<false>, dim3((unsigned)rows), dim3(kRowThreads), 0, s, (const char*)src, ld_src, (int)H, values, ld,
+                     (int)((H + kInt8K - 1) / kInt8K * kInt8K), scale);
+  return hipGetLastError();
+}
+
+hipError_t launch_int8_fwd_tiles(hipStream_t s, const Int8FwdArgs& a, bool half, bool shapes, int split, int workgroups) {
+  const dim3 grid((unsigned)workgroups), block(NTHREADS);
+  if (half) {
+    hipLaunchKernelGGL(a.part_pz ? int8_fwd_half_tiles<true> : int8_fwd_half_tiles<false>, grid, block, 0, s, a);
+  } else {
+    auto kernel = flagged([](auto pz, auto even, auto others) { return &int8_fwd_tiles<pz.value, even.value, others.value>; }, a.part_pz != nullptr,
+                          even_ktiles(a.K), shapes);
+    hipLaunchKernelGGL(kernel, grid, block, 0, s, a, split);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_int8_logits(hipStream_t s, const Int8LogitsArgs& a, bool half, bool shapes, int split, int workgroups) {
+  const dim3 grid((unsigned)workgroups), block(NTHREADS);
+  if (half) {
+    hipLaunchKernelGGL(a.out_f32 ? int8_logits_half_tiles<true> : int8_logits_half_tiles<false>, grid, block, 0, s, a);
+  } else {
+    auto kernel = flagged([](auto f32, auto even, auto others) { return &int8_logits_tiles<f32.value, even.value, others.value>; }, a.out_f32 != 0,
+                          even_ktiles(a.K), shapes);
+    hipLaunchKernelGGL(kernel, grid, block, 0, s, a, split);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace lmhead

@@ -34,6 +34,7 @@
 #include "dh_split.hpp"
 #include "few_tokens.hpp"
 #include "gemm_core.hpp"
+#include "int8.hpp"
 #include "logits_tile.hpp"
 #include "topk_kernels.hpp"
 
@@ -202,15 +203,13 @@ __device__ __forceinline__ void merge_lanes(float& M, float& S, float& E, int o)
   merge_partials<RELATIVE>(M, S, E, m, s, e);
 }
 
-template <bool RELATIVE, int BATCH>
-__global__ __launch_bounds__(kMergeThreads) void lmhead_fwd_merge(const float* __restrict__ part_max,
-                                                                  const float* __restrict__ part_sum,
-                                                                  const float* __restrict__ part_pz, int nparts, int T,
-                                                                  const uint16_t* __restrict__ Hd, int ldh,
-                                                                  const uint16_t* __restrict__ W, int ldw,
-                                                                  const int64_t* __restrict__ labels, int H, int V, float rcp_temp,
-                                                                  float* __restrict__ logprobs, float* __restrict__ entropy,
-                                                                  float* __restrict__ row_lse, float* __restrict__ row_pz) {
+// label_dot(t, y): this lane's share of the logit of label y of token t.
+template <bool RELATIVE, int BATCH, class LabelDot>
+__device__ __forceinline__ void fwd_merge(const float* __restrict__ part_max, const float* __restrict__ part_sum,
+                                          const float* __restrict__ part_pz, int nparts, int T,
+                                          const int64_t* __restrict__ labels, int V, float rcp_temp,
+                                          float* __restrict__ logprobs, float* __restrict__ entropy,
+                                          float* __restrict__ row_lse, float* __restrict__ row_pz, LabelDot label_dot) {
   __shared__ float sm_m[kMergeWaves][kMergeTokens], sm_s[kMergeWaves][kMergeTokens], sm_e[kMergeWaves][kMergeTokens];
   __shared__ float sm_dot[kMergeTokens];
   __shared__ int sm_has_label[kMergeTokens];
@@ -236,22 +235,7 @@ __global__ __launch_bounds__(kMergeThreads) void lmhead_fwd_merge(const float* _
   // Label logit: 16-byte loads, fp32 accumulation.  Its two rows travel together with the first batch of the partials.
   float dot = 0.f;
   const bool has_label = y >= 0 && y < (int64_t)V;
-  if (has_label) {
-    const uint16_t* hp = Hd + (size_t)(t0 + wave) * (size_t)ldh;
-    const uint16_t* wp = W + (size_t)y * (size_t)ldw;
-#pragma unroll 4
-    for (int c = lane * 8; c < H; c += 64 * 8) {
-      const uint4 hv = *(const uint4*)(hp + c);
-      const uint4 wv = *(const uint4*)(wp + c);
-      const uint32_t hh[4] = {hv.x, hv.y, hv.z, hv.w};
-      const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        dot = fmaf(__uint_as_float(hh[k] << 16), __uint_as_float(ww[k] << 16), dot);
-        dot = fmaf(__uint_as_float(hh[k] & 0xffff0000u), __uint_as_float(ww[k] & 0xffff0000u), dot);
-      }
-    }
-  }
+  if (has_label) dot = label_dot(t0 + wave, y);
   {
     float M = -INFINITY, S = 0.f, E = 0.f;
     for (int p0 = first; p0 < nparts;) {
@@ -293,14 +277,73 @@ __global__ __launch_bounds__(kMergeThreads) void lmhead_fwd_merge(const float* _
   if (row_pz) row_pz[t] = RELATIVE ? lse - third : third;
 }
 
+template <bool RELATIVE, int BATCH>
+__global__ __launch_bounds__(kMergeThreads) void lmhead_fwd_merge(const float* __restrict__ part_max,
+                                                                  const float* __restrict__ part_sum,
+                                                                  const float* __restrict__ part_pz, int nparts, int T,
+                                                                  const uint16_t* __restrict__ Hd, int ldh,
+                                                                  const uint16_t* __restrict__ W, int ldw,
+                                                                  const int64_t* __restrict__ labels, int H, int V, float rcp_temp,
+                                                                  float* __restrict__ logprobs, float* __restrict__ entropy,
+                                                                  float* __restrict__ row_lse, float* __restrict__ row_pz) {
+  fwd_merge<RELATIVE, BATCH>(part_max, part_sum, part_pz, nparts, T, labels, V, rcp_temp, logprobs, entropy, row_lse, row_pz, [&](int t, int64_t y) {
+    float dot = 0.f;
+    const int lane = threadIdx.x & 63;
+    const uint16_t* hp = Hd + (size_t)t * (size_t)ldh;
+    const uint16_t* wp = W + (size_t)y * (size_t)ldw;
+#pragma unroll 4
+    for (int c = lane * 8; c < H; c += 64 * 8) {
+      const uint4 hv = *(const uint4*)(hp + c);
+      const uint4 wv = *(const uint4*)(wp + c);
+      const uint32_t hh[4] = {hv.x, hv.y, hv.z, hv.w};
+      const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        dot = fmaf(__uint_as_float(hh[k] << 16), __uint_as_float(ww[k] << 16), dot);
+        dot = fmaf(__uint_as_float(hh[k] & 0xffff0000u), __uint_as_float(ww[k] & 0xffff0000u), dot);
+      }
+    }
+    return dot;
+  });
+}
+
+// The same for rows in 8-bit integers: a lane's share of the sum is exact, and all are below 2^31.  Its logit is one lane's share.
+template <bool RELATIVE, int BATCH>
+__global__ __launch_bounds__(kMergeThreads) void int8_fwd_merge(const float* __restrict__ part_max, const float* __restrict__ part_sum,
+                                                                const float* __restrict__ part_pz, int nparts, int T, const Int8Rows Hd, const Int8Rows W,
+                                                                const int64_t* __restrict__ labels, int K, int V, float rcp_temp,
+                                                                float* __restrict__ logprobs, float* __restrict__ entropy) {
+  fwd_merge<RELATIVE, BATCH>(part_max, part_sum, part_pz, nparts, T, labels, V, rcp_temp, logprobs, entropy, nullptr, nullptr, [&](int t, int64_t y) {
+    const int lane = threadIdx.x & 63;
+    const int8_t* hp = Hd.values + (size_t)t * (size_t)Hd.ld;
+    const int8_t* wp = W.values + (size_t)y * (size_t)W.ld;
+    const float c = W.scale[y], s = Hd.scale[t];
+    int dot = 0;
+#pragma unroll 4
+    for (int k = lane * 16; k < K; k += 64 * 16) {
+      const int4 hv = *(const int4*)(hp + k), wv = *(const int4*)(wp + k);
+      dot = __builtin_amdgcn_sdot4(hv.x, wv.x, dot, false);
+      dot = __builtin_amdgcn_sdot4(hv.y, wv.y, dot, false);
+      dot = __builtin_amdgcn_sdot4(hv.z, wv.z, dot, false);
+      dot = __builtin_amdgcn_sdot4(hv.w, wv.w, dot, false);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o, 64);
+    return lane == 0 ? (float)dot * c * s : 0.f;  // the caller adds the lanes' shares
+  });
+}
+
 // Ten parts a step where that saves the first or the second of the steps that eight take (lanes without a part of their own load and drop
 // one): with ten instead of eight 8.5 -> 7.7 us at 137 tokens of V=80000 (ten parts per stream), 11.5 -> 10.6 at V=151936 (19), but 8.5 -> 9.2
 // at V=100000 (13), 10.2 -> 10.8 at V=200064 (25), and 29 -> 38 at 32768 tokens of V=32000 (4).  The same for every number of tokens, so that
 // a token's sums do not depend on it.
+inline bool merge_by_ten(int64_t nparts) {
+  const int64_t n = (nparts + kMergeStreams - 1) / kMergeStreams;
+  return n <= 20 && (n + 9) / 10 < (n + 7) / 8;
+}
 template <bool RELATIVE>
 auto merge_kernel(int64_t nparts) {
-  const int64_t n = (nparts + kMergeStreams - 1) / kMergeStreams;
-  return n <= 20 && (n + 9) / 10 < (n + 7) / 8 ? &lmhead_fwd_merge<RELATIVE, 10> : &lmhead_fwd_merge<RELATIVE, 8>;
+  return merge_by_ten(nparts) ? &lmhead_fwd_merge<RELATIVE, 10> : &lmhead_fwd_merge<RELATIVE, 8>;
 }
 
 // The dz tiles (logits_tile.hpp) on products of any shape.
@@ -1391,6 +1434,39 @@ int fwd_token_blocks(const void* hidden, int64_t ld_hidden, const void* weight, 
   return SKYRL_LMHEAD_OK;
 }
 
+// ---- the head in 8-bit integers ----
+// Both walk the tokens in blocks, whose hidden rows are brought to integers in the workspace.
+struct Int8Workspace {
+  int8_t* values;
+  float* scale;
+  char* partials;
+  size_t bytes;
+};
+Int8Workspace carve_int8(void* workspace, int64_t T, int64_t H, int64_t V, bool statistics) {
+  const int64_t block = T < kFwdTokenBlock ? T : kFwdTokenBlock;
+  Carver c(workspace);
+  Int8Workspace w;
+  w.values = c.take<int8_t>((size_t)block * (size_t)round_up(H, kInt8K));
+  w.scale = c.take<float>((size_t)block);
+  const size_t partials = statistics ? fwd_partials_bytes(block, V) : 0;
+  w.partials = c.take<char>(partials);
+  w.bytes = (size_t)round_up((int64_t)c.off, 256);
+  return w;
+}
+bool int8_extents(int64_t T, int64_t H, int64_t V) {
+  return T >= 1 && V >= 1 && H >= 1 && T <= kMaxExtent && V <= kMaxExtent && H <= kInt8MostHidden;
+}
+int check_int8(const void* hidden, int hidden_dtype, int64_t ld_hidden, const int8_t* values, int64_t ld_values, const float* scale, int64_t T, int64_t H,
+               int64_t V) {
+  if (!hidden || !values || !scale) return SKYRL_LMHEAD_ERR_NULL;
+  if (hidden_dtype != SKYRL_LOGITS_BF16 && hidden_dtype != SKYRL_LOGITS_F32) return SKYRL_LMHEAD_ERR_ARG;
+  if (!int8_extents(T, H, V) || ld_hidden < H || ld_hidden >= ((int64_t)1 << 40) || ld_values < round_up(H, kInt8K) || ld_values > 2 * kMaxRowPitch)
+    return SKYRL_LMHEAD_ERR_SHAPE;
+  if (((uintptr_t)hidden & (hidden_dtype == SKYRL_LOGITS_F32 ? 3u : 1u)) || !aligned16(values) || ld_values % 16 != 0 || ((uintptr_t)scale & 3u))
+    return SKYRL_LMHEAD_ERR_ALIGN;
+  return SKYRL_LMHEAD_OK;
+}
+
 // Address of this device's copy of the static scratch array.  Every device holds its own copy of a __device__ array at
 // its own address, so the address is looked up once per device, with that device current, and kept.
 constexpr int kMaxDevices = 64;
@@ -2210,6 +2286,89 @@ int skyrl_lmhead_adapter_bwd(const void* hidden, int64_t ld_hidden, const void* 
   ab.dA = (uint16_t*)d_lora_a, ab.dB = (uint16_t*)d_lora_b;
   return bwd_entry(hidden, ld_hidden, weight, ld_weight, labels, row_lse, row_pz, dlogprobs, dentropy, T, H, V, rcp_temperature, d_hidden, nullptr,
                    SKYRL_DW_FP32, vc, workspace, head, (hipStream_t)stream, true, 1, &ab);
+}
+
+int skyrl_lmhead_int8_rows(const void* src, int src_dtype, int64_t ld_src, int64_t rows, int64_t H, int8_t* values, int64_t ld_values, float* scale,
+                           void* stream) {
+  int st = check_int8(src, src_dtype, ld_src, values, ld_values, scale, rows, H, 1);
+  if (st) return st;
+  if (rows > ((int64_t)1 << 23)) return SKYRL_LMHEAD_ERR_SHAPE;  // of one grid
+  const hipError_t e = launch_int8_rows((hipStream_t)stream, src, src_dtype == SKYRL_LOGITS_F32, ld_src, rows, H, values, ld_values, scale);
+  return e == hipSuccess ? SKYRL_LMHEAD_OK : (int)e;
+}
+
+size_t skyrl_lmhead_int8_fwd_workspace_bytes(int64_t T, int64_t H, int64_t V) { return int8_extents(T, H, V) ? carve_int8(nullptr, T, H, V, true).bytes : 0; }
+
+int skyrl_lmhead_int8_fwd(const void* hidden, int hidden_dtype, int64_t ld_hidden, const int8_t* values, int64_t ld_values, const float* scale,
+                          const int64_t* labels, int64_t T, int64_t H, int64_t V, float rcp_temperature, float* logprobs, float* entropy, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  const int st = check_int8(hidden, hidden_dtype, ld_hidden, values, ld_values, scale, T, H, V);
+  if (st) return st;
+  if (!labels || !logprobs) return SKYRL_LMHEAD_ERR_NULL;
+  if ((uintptr_t)labels & 7u) return SKYRL_LMHEAD_ERR_ALIGN;
+  if (!(rcp_temperature > 0.f) || !isfinite(rcp_temperature)) return SKYRL_LMHEAD_ERR_ARG;
+  const Int8Workspace w = carve_int8(workspace, T, H, V, true);
+  if (!workspace || workspace_bytes < w.bytes) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  const bool f32 = hidden_dtype == SKYRL_LOGITS_F32;
+  const int64_t K = round_up(H, kInt8K);
+  const int tiles_m = (int)((V + BM - 1) / BM);
+  const size_t nparts = (size_t)tiles_m * WAVES_M;
+  const Int8Rows W{values, ld_values, scale}, Hd{w.values, K, w.scale};
+  for (int64_t t0 = 0; t0 < T; t0 += kFwdTokenBlock) {
+    const int64_t Tb = T - t0 < kFwdTokenBlock ? T - t0 : kFwdTokenBlock;
+    Carver c(w.partials);
+    float* pmax = c.take<float>(part_elems(nparts, Tb));
+    float* psum = c.take<float>(part_elems(nparts, Tb));
+    float* ppz = c.take<float>(part_elems(nparts, Tb));
+    hipError_t e = launch_int8_rows(s, (const char*)hidden + (size_t)t0 * (size_t)ld_hidden * (f32 ? 4 : 2), f32, ld_hidden, Tb, H, w.values, K, w.scale);
+    if (e != hipSuccess) return (int)e;
+    const bool half = half_tile_logits(Tb);
+    const TileShapes shapes = tile_shapes(Tb, K / 2, tiles_m, compute_units());
+    const int tiles = half ? tiles_m : tiles_m * (int)((Tb + BN - 1) / BN) + shapes.split;
+    e = launch_int8_fwd_tiles(s, Int8FwdArgs{W, Hd, (int)Tb, (int)K, (int)V, rcp_temperature, pmax, psum, entropy ? ppz : nullptr}, half, shapes.used,
+                              shapes.split, tiles);
+    if (e != hipSuccess) return (int)e;
+    hipLaunchKernelGGL((merge_by_ten(nparts) ? &int8_fwd_merge<true, 10> : &int8_fwd_merge<true, 8>), dim3((unsigned)((Tb + kMergeTokens - 1) / kMergeTokens)),
+                       dim3(kMergeThreads), 0, s, pmax, psum, entropy ? ppz : (float*)nullptr, (int)nparts, (int)Tb, Hd, W, labels + t0, (int)K, (int)V,
+                       rcp_temperature, logprobs + t0, entropy ? entropy + t0 : (float*)nullptr);
+    if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+  }
+  return SKYRL_LMHEAD_OK;
+}
+
+size_t skyrl_lmhead_int8_logits_workspace_bytes(int64_t T, int64_t H) { return int8_extents(T, H, 1) ? carve_int8(nullptr, T, H, 1, false).bytes : 0; }
+
+int skyrl_lmhead_int8_logits(const void* hidden, int hidden_dtype, int64_t ld_hidden, const int8_t* values, int64_t ld_values, const float* scale, int64_t T,
+                             int64_t H, int64_t V, int logits_dtype, void* logits, int64_t ld_logits, void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = check_int8(hidden, hidden_dtype, ld_hidden, values, ld_values, scale, T, H, V);
+  if (st) return st;
+  if (!logits) return SKYRL_LMHEAD_ERR_NULL;
+  if (logits_dtype != SKYRL_LOGITS_BF16 && logits_dtype != SKYRL_LOGITS_F32) return SKYRL_LMHEAD_ERR_ARG;
+  if (ld_logits < V || ld_logits >= ((int64_t)1 << 40)) return SKYRL_LMHEAD_ERR_SHAPE;
+  const bool f32 = hidden_dtype == SKYRL_LOGITS_F32, out_f32 = logits_dtype == SKYRL_LOGITS_F32;
+  if ((uintptr_t)logits & (out_f32 ? 3u : 1u)) return SKYRL_LMHEAD_ERR_ALIGN;
+  const Int8Workspace w = carve_int8(workspace, T, H, V, false);
+  if (!workspace || workspace_bytes < w.bytes) return SKYRL_LMHEAD_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t K = round_up(H, kInt8K);
+  const int tiles_m = (int)((V + BM - 1) / BM);
+  const Int8Rows W{values, ld_values, scale}, Hd{w.values, K, w.scale};
+  for (int64_t t0 = 0; t0 < T; t0 += kFwdTokenBlock) {
+    const int64_t Tb = T - t0 < kFwdTokenBlock ? T - t0 : kFwdTokenBlock;
+    hipError_t e = launch_int8_rows(s, (const char*)hidden + (size_t)t0 * (size_t)ld_hidden * (f32 ? 4 : 2), f32, ld_hidden, Tb, H, w.values, K, w.scale);
+    if (e != hipSuccess) return (int)e;
+    const bool half = half_tile_logits(Tb);
+    const TileShapes shapes = tile_shapes(Tb, K / 2, tiles_m, compute_units());
+    const int tiles = half ? tiles_m : tiles_m * (int)((Tb + BN - 1) / BN) + shapes.split;
+    e = launch_int8_logits(s, Int8LogitsArgs{W, Hd, (int)Tb, (int)K, (int)V, (char*)logits + (size_t)t0 * (size_t)ld_logits * (out_f32 ? 4 : 2), ld_logits,
+                                             out_f32 ? 1 : 0},
+                           half, shapes.used, shapes.split, tiles);
+    if (e != hipSuccess) return (int)e;
+  }
+  return SKYRL_LMHEAD_OK;
 }
 
 int skyrl_lmhead_bwd(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const int64_t* labels,

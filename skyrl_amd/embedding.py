@@ -175,7 +175,7 @@ def embedding_backward_accumulate(d_out: torch.Tensor, ids: torch.Tensor, d_weig
     flat, scale, padding_idx = _flat_ids(ids), _scale_of(scale), _padding_of(padding_idx, int(d_weight_accum.shape[0]))
     if torch.is_grad_enabled() and d_weight_accum.requires_grad:
         raise ValueError("d_weight_accum is written in place and takes no gradient itself")
-    rows = _walkable(d_out.detach().reshape(-1, d_weight_accum.shape[1]))
+    rows = _walkable(d_out.detach().reshape(flat.shape[0], d_weight_accum.shape[1]))
     _check_gradient(rows, flat)
     _require_device(rows, flat, d_weight_accum)
     if rows.numel() and d_weight_accum.numel():
