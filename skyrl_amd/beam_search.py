@@ -14,6 +14,7 @@ captured in a HIP graph.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
@@ -42,8 +43,8 @@ def _check_select(logits: torch.Tensor, scores: torch.Tensor, k: int) -> Tuple[i
         raise ValueError(f"expected logits [N, B, V], got {tuple(logits.shape)}")
     if logits.dtype not in _DTYPES:
         raise TypeError(f"logits must be torch.bfloat16 or torch.float32, got {logits.dtype}")
-    N, B, V = (int(x) for x in logits.shape)
-    if tuple(scores.shape) != (N, B):
+    N, B, V = logits.shape
+    if scores.shape != (N, B):
         raise ValueError(f"scores {tuple(scores.shape)} do not match logits {tuple(logits.shape)}")
     if scores.dtype != torch.float32:
         raise TypeError(f"scores must be torch.float32, got {scores.dtype}")
@@ -93,19 +94,17 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, temperatu
         raise ValueError(f"temperature must be finite and positive, got {temperature}")
     if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad) or has_tangent(logits, scores):
         raise ValueError("beam_select has no gradient: call it under torch.no_grad()")
-    _, _, V = _check_select(logits, scores, k)
-    rows = logits if V <= 1 or logits.stride(2) == 1 else logits.contiguous()
+    rows = logits if logits.dim() != 3 or logits.shape[2] <= 1 or logits.stride(2) == 1 else logits.contiguous()
+    scores = scores if scores.is_contiguous() else scores.contiguous()
     with torch.no_grad():
-        return BeamSelection(*call(logits_beam_select, rows, scores.contiguous(), k, 1.0 / temperature))
+        return BeamSelection(*call(logits_beam_select, rows, scores, k, 1.0 / temperature))
 
 
-def _segments(t: torch.Tensor, u: torch.Tensor) -> List[Tuple[torch.Tensor, torch.Tensor, int, int, int, int]]:
-    """``(from, to, segments, bytes, from_segment, to_segment)`` of two tensors of one shape, rows along dimension 0: what a row is in both, one run of
-    equally spaced contiguous pieces.  Tensors with more dimensions that do not join are taken apart along the first of them."""
-    size = t.element_size()
-    shape, a, b = list(t.shape[1:]), list(t.stride()[1:]), list(u.stride()[1:])
-    dims: List[List[int]] = []  # [extent, stride of t, stride of u], outer first, neighbours joined
-    for n, x, y in zip(shape, a, b):
+def _segments(shape: Tuple[int, ...], strides: Tuple[int, ...], to_strides: Tuple[int, ...], size: int) -> List[Tuple[int, int, int, int, int, int]]:
+    """``(place, place in the result, segments, bytes, from_segment, to_segment)``, in bytes, of a row of that shape: what it is in both, one run of
+    equally spaced contiguous pieces.  Rows with more dimensions that do not join are taken apart along the first of them."""
+    dims: List[List[int]] = []  # [extent, stride, stride in the result], outer first, neighbours joined
+    for n, x, y in zip(shape, strides, to_strides):
         if n == 1:
             continue
         if dims and dims[-1][1] == n * x and dims[-1][2] == n * y:
@@ -114,47 +113,46 @@ def _segments(t: torch.Tensor, u: torch.Tensor) -> List[Tuple[torch.Tensor, torc
             dims.append([n, x, y])
     inner = dims.pop()[0] if dims and dims[-1][1] == dims[-1][2] == 1 else 1
     if len(dims) > 1:
-        axis = next(i for i, n in enumerate(shape) if n != 1) + 1
-        return [s for i in range(shape[axis - 1]) for s in _segments(t.select(axis, i), u.select(axis, i))]
+        axis = next(i for i, n in enumerate(shape) if n != 1)
+        rest = _segments(shape[axis + 1:], strides[axis + 1:], to_strides[axis + 1:], size)
+        return [(i * strides[axis] * size + at, i * to_strides[axis] * size + to_at, *more) for i in range(shape[axis]) for at, to_at, *more in rest]
     n, x, y = dims[0] if dims else (1, 0, 0)
-    return [(t, u, n, inner * size, x * size, y * size)]
+    return [(0, 0, n, inner * size, x * size, y * size)]
 
 
-class _Layout:
-    """Pairs of a state and its result that have the same type, shape and strides."""
+class _Layout(NamedTuple):
+    """What states of one type, shape and strides and their results have in common."""
 
-    def __init__(self, t: torch.Tensor, u: torch.Tensor, items: int, beams_out: int, given: bool):
-        self.dtype, self.shape, self.strides, self.to_strides = t.dtype, t.shape, t.stride(), u.stride()
-        if t.dim() < 1:
-            raise ValueError("a state has the beams of all prompts along its first dimension, got a scalar")
-        rows = int(t.shape[0])
-        if items == 0 and rows or items and rows % items:
-            raise ValueError(f"{rows} rows of a state {tuple(t.shape)} do not divide among {items} prompts")
-        self.beams_in = rows // items if items else 0
-        if given and any(n > 1 and s == 0 for n, s in zip(u.shape, u.stride())):
-            raise ValueError("a result must not be expanded: its elements would be written more than once")
-        self.to_shape = torch.Size((items * beams_out,) + tuple(t.shape[1:]))
-        size = t.element_size()
-        extent = lambda x: size * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) if x.numel() else 0  # noqa: E731
-        self.extent, self.to_extent = extent(t), extent(u)
-        self.pairs: List[Tuple[int, int]] = []
-        self.first = (t, u)
+    beams_in: int
+    to_shape: Tuple[int, ...]
+    extent: int     # bytes from a state's first element to its last
+    to_extent: int
+    expanded: bool  # whether elements of a result lie on each other
+    # (from_row, from_segment, to_row, to_segment, segments, bytes) and the segments' places in a state and in its result, in bytes
+    launches: Tuple[Tuple[Tuple[int, ...], Tuple[Tuple[int, int], ...]], ...]
 
-    def launches(self) -> List[Tuple[Tuple[int, ...], List[Tuple[int, int]]]]:
-        """For each kind of segment its sizes and strides in bytes and the two addresses of its first row in each pair; pairs in place apart from the others."""
-        t, u = self.first
-        size, t0, u0 = t.element_size(), t.data_ptr(), u.data_ptr()
-        row = t.stride(0) * size if t.shape[0] > 1 else 0
-        to_row = u.stride(0) * size if u.shape[0] > 1 else 0
-        found: dict = {}
-        for x, y, n, nbytes, step, to_step in _segments(t, u):
-            dx, dy = x.data_ptr() - t0, y.data_ptr() - u0
-            found.setdefault((row, step, to_row, to_step, n, nbytes), []).extend([(p + dx, q + dy) for p, q in self.pairs])
-        kinds = []
-        for sizes, pairs in found.items():
-            inside = [pair for pair in pairs if pair[0] == pair[1]]
-            kinds += [(sizes, some) for some in (([pair for pair in pairs if pair[0] != pair[1]], inside) if inside else (pairs,)) if some]
-        return kinds
+
+@functools.lru_cache(maxsize=256)
+def _layout(shape: Tuple[int, ...], strides: Tuple[int, ...], to_strides: Tuple[int, ...], dtype: torch.dtype, items: int, beams_out: int) -> _Layout:
+    if len(shape) < 1:
+        raise ValueError("a state has the beams of all prompts along its first dimension, got a scalar")
+    rows = int(shape[0])
+    if items == 0 and rows or items and rows % items:
+        raise ValueError(f"{rows} rows of a state {tuple(shape)} do not divide among {items} prompts")
+    size = dtype.itemsize
+    to_shape = (items * beams_out,) + tuple(shape[1:])
+
+    def extent(sizes, steps):
+        return 0 if 0 in sizes else size * (1 + sum((n - 1) * s for n, s in zip(sizes, steps)))
+
+    row = strides[0] * size if rows > 1 else 0
+    to_row = to_strides[0] * size if to_shape[0] > 1 else 0
+    found: dict = {}
+    if 0 not in to_shape:
+        for at, to_at, n, nbytes, step, to_step in _segments(tuple(shape[1:]), strides[1:], to_strides[1:], size):
+            found.setdefault((row, step, to_row, to_step, n, nbytes), []).append((at, to_at))
+    return _Layout(rows // items if items else 0, to_shape, extent(shape, strides), extent(to_shape, to_strides),
+                   any(n > 1 and s == 0 for n, s in zip(to_shape, to_strides)), tuple((sizes, tuple(places)) for sizes, places in found.items()))
 
 
 def _overlap(states: Sequence[Tuple[int, int]], results: Sequence[Tuple[int, int]]) -> bool:
@@ -203,34 +201,35 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         for kind, t, u in zip(kinds, states, results):
             some = groups.setdefault(kind, ([], []))
             some[0].append(t), some[1].append(u)
-    layouts = [_Layout(ts[0], us[0], N, B_out, given) for ts, us in groups.values()]
-    beams_in = layouts[0].beams_in
-    if any(layout.beams_in != beams_in for layout in layouts):
-        raise ValueError(f"states of unlike numbers of beams a prompt: {sorted({layout.beams_in for layout in layouts})}")
-    for layout, (ts, us) in zip(layouts, groups.values()):
-        if given and ([u.shape for u in us].count(layout.to_shape) < len(us) or [u.dtype for u in us].count(layout.dtype) < len(us)):
-            raise ValueError(f"a result must be {tuple(layout.to_shape)} {layout.dtype}, got " + ", ".join(f"{tuple(u.shape)} {u.dtype}" for u in us))
-        layout.pairs = list(zip([t.data_ptr() for t in ts], [u.data_ptr() for u in us]))
-    used = [layout for layout in layouts if layout.to_extent > 0]
+    used = []  # layouts with the addresses of each state and its result
+    beams_in = -1
+    for kind, (ts, us) in groups.items():
+        layout = _layout(*kind, N, B_out)
+        if beams_in not in (-1, layout.beams_in):
+            raise ValueError(f"states of {beams_in} and of {layout.beams_in} beams a prompt")
+        beams_in = layout.beams_in
+        if given and ([u.shape for u in us].count(layout.to_shape) < len(us) or [u.dtype for u in us].count(kind[3]) < len(us)):
+            raise ValueError(f"a result must be {layout.to_shape} {kind[3]}, got " + ", ".join(f"{tuple(u.shape)} {u.dtype}" for u in us))
+        if given and layout.expanded:
+            raise ValueError("a result must not be expanded: its elements would be written more than once")
+        if layout.to_extent > 0:
+            used.append((layout, kind[1] == kind[2] and beams_in == B_out, [t.data_ptr() for t in ts], [u.data_ptr() for u in us]))
     if not used:
         return results
     device = parents.get_device()
     if device < 0 or [t.get_device() for t in states + results].count(device) < 2 * len(states):
         _require_device(parents, *states, *results)
     if given:
-        apart = []  # the ranges of addresses of results that are not their states
-        for layout in used:
-            if layout.strides == layout.to_strides and layout.beams_in == B_out:
-                some = [q for p, q in layout.pairs if p != q]
-                if len(some) < len(layout.pairs) and B_out > MAX_BEAMS:
-                    raise ValueError(f"at most {MAX_BEAMS} beams are reordered in place, got {B_out}")
-            else:
-                some = [q for _, q in layout.pairs]
+        apart, to = [], []  # the ranges of addresses of results that are not their states; where results begin
+        for layout, may_be_same, ps, qs in used:
+            some = [q for p, q in zip(ps, qs) if p != q] if may_be_same else qs
+            if len(some) < len(qs) and B_out > MAX_BEAMS:
+                raise ValueError(f"at most {MAX_BEAMS} beams are reordered in place, got {B_out}")
             apart += [(q, q + layout.to_extent) for q in some]
-        to = [q for layout in used for _, q in layout.pairs]
+            to += qs
         if len(set(to)) < len(to):
             raise ValueError("a result is given twice")
-        if apart and _overlap([(p, p + layout.extent) for layout in used for p, _ in layout.pairs], apart):
+        if apart and _overlap([(p, p + layout.extent) for layout, _, ps, _ in used for p in ps], apart):
             raise ValueError("a result overlaps a state and is not that state: it would be read after it was written")
     dev = _require_device(parents, states[0])
     if beams_in == 0:  # no row to take
@@ -238,11 +237,15 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
     lib, parents = _lib.load(), parents.contiguous()
     with device_guard(dev):
         stream = raw_stream(dev)
-        for layout in used:
-            for sizes, pairs in layout.launches():
-                for at in range(0, len(pairs), _MAX_STATES):
-                    from_, to = zip(*pairs[at:at + _MAX_STATES])
-                    array = ctypes.c_void_p * len(from_)
-                    st = lib.skyrl_logits_beam_reorder(array(*from_), array(*to), len(from_), *sizes, parents.data_ptr(), N, beams_in, B_out, stream)
-                    _lib.check(st, "skyrl_logits_beam_reorder")
+        for layout, _, ps, qs in used:
+            pairs = list(zip(ps, qs))
+            inside = [pair for pair in pairs if pair[0] == pair[1]]
+            for some in (pairs,) if not inside or len(inside) == len(pairs) else (inside, [pair for pair in pairs if pair[0] != pair[1]]):
+                for sizes, places in layout.launches:
+                    every = [(p + x, q + y) for x, y in places for p, q in some] if places != ((0, 0),) else some
+                    for at in range(0, len(every), _MAX_STATES):
+                        from_, to = zip(*every[at:at + _MAX_STATES])
+                        array = ctypes.c_void_p * len(from_)
+                        st = lib.skyrl_logits_beam_reorder(array(*from_), array(*to), len(from_), *sizes, parents.data_ptr(), N, beams_in, B_out, stream)
+                        _lib.check(st, "skyrl_logits_beam_reorder")
     return results

@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libskyrl_lmhead.so"
 SOURCES = ["lmhead_kernels.hip", "few_tokens.hip", "packed_kernels.hip", "loss_kernels.hip", "logits_kernels.hip",
            "top_logits_kernels.hip", "adapter_tiles.hip", "adapter_kernels.hip", "embedding_kernels.hip", "beam_kernels.hip",
-           "int8_tiles.hip"]
+           "int8_tiles.hip", "int8_few.hip"]
 # -packed-fp32-ops off: the compiler must not form v_pk_{add,mul,fma}_f32 from the scalar fp32 epilogue code.
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

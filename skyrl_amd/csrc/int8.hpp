@@ -34,6 +34,10 @@ struct Int8LogitsArgs {
   int64_t ldo;
   int out_f32;
 };
+// Of few tokens, the weight streaming through registers (int8_few.hip).  Whether a call is one for it: forward tiles -> this, V=151936 and thereabouts, in
+// turn: 30.5 -> 27.6 us at T=1, H=896, 118 -> 107 at T=16, H=3584.
+bool int8_streams(int64_t T, int64_t K);
+hipError_t launch_int8_logits_stream(hipStream_t s, const Int8LogitsArgs& a, int ncu);
 hipError_t launch_int8_logits(hipStream_t s, const Int8LogitsArgs& a, bool half, bool shapes, int split, int workgroups);
 
 }  // namespace lmhead

@@ -94,77 +94,86 @@ __global__ __launch_bounds__(kRowThreads) void int8_rows(const char* __restrict_
 
 __device__ __forceinline__ Operand bytes_of(const Int8Rows& r, int row0, int rows) { return Operand{(const uint16_t*)r.values, (int)(r.ld / 2), row0, rows}; }
 
-// The sums of a wave's token block j times the scales of its vocabulary rows.
-struct RowScales {
-  f32x4 c[TM];  // of rows vbase + i * 16 + (lane >> 4) * 4 .. + 3
-  __device__ __forceinline__ RowScales(const float* __restrict__ scale, int vbase, int V) {
+// The scales of a wave's vocabulary rows and tokens, loaded behind the mainloop.  (In front of it they save nothing, because the branch for the vocabulary's last
+// rows makes the compiler wait there: 326 -> 400 us at T=2047, H=1536, V=128261; without that branch 322 -> 322.)
+template <int NB>
+struct Scales {
+  f32x4 c[TM];  // of rows v0 + i * 16 + (lane >> 4) * 4 .. + 3
+  float s[NB];  // of tokens t0 + j * 16 + (lane & 15)
+  int v0, t0;
+  __device__ __forceinline__ Scales(const Int8Rows& W, int v0_, int V, const Int8Rows& Hd, int t0_, int T) : v0(v0_), t0(t0_) {
     struct __attribute__((packed, aligned(4))) Four {
       f32x4 v;
     };
-    const int v0 = vbase + ((threadIdx.x & 63) >> 4) * 4;
-    if (vbase + WM <= V) {
+    const int lane = threadIdx.x & 63, first = v0 + (lane >> 4) * 4;
+    if (v0 + WM <= V) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) c[i] = ((const Four*)(scale + v0 + i * MT))->v;
+      for (int i = 0; i < TM; ++i) c[i] = ((const Four*)(W.scale + first + i * MT))->v;
     } else {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) c[i][r] = scale[v0 + i * MT + r < V ? v0 + i * MT + r : V - 1];
+        for (int r = 0; r < 4; ++r) c[i][r] = W.scale[first + i * MT + r < V ? first + i * MT + r : V - 1];
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int t = t0 + j * MT + (lane & 15);
+      s[j] = Hd.scale[t < T ? t : T - 1];
     }
   }
-  template <int NB>
-  __device__ __forceinline__ void apply(const f32x4 (&acc)[TM][NB], int j, float s, f32x4 (&z)[TM]) const {
+  // The sums of token block j times the scales of the rows.
+  __device__ __forceinline__ void rows(const f32x4 (&acc)[TM][NB], int j, f32x4 (&z)[TM]) const {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) z[i][r] = (float)__float_as_int(acc[i][j][r]) * c[i][r] * s;
+      for (int r = 0; r < 4; ++r) z[i][r] = (float)__float_as_int(acc[i][j][r]) * c[i][r];
   }
 };
 
-// Statistics of a wave's logits, as fwd_epilogue() (logits_tile.hpp) makes them; the token's scale enters with the temperature.
+// Statistics of a wave's logits, as fwd_epilogue() (logits_tile.hpp) makes them; the token's scale enters with the temperature.  Whether all of the wave's rows
+// exist is decided in front of the loop over token blocks: inside it, 330 us instead of 326 there, 284 instead of 274 at T=2048, H=896, V=151936.
 template <bool ENTROPY, int NB>
-__device__ __forceinline__ void int8_stats(const f32x4 (&acc)[TM][NB], const Int8FwdArgs& a, int part, int nparts, int t0) {
+__device__ __forceinline__ void int8_stats(const f32x4 (&acc)[TM][NB], const Scales<NB>& scales, const Int8FwdArgs& a, int nparts) {
   const int lane = threadIdx.x & 63, lrow = lane & 15, kq = lane >> 4;
-  const int vbase = part * WM;
+  const int vbase = scales.v0, part = vbase / WM;
+  const float per = a.rcp_temp * kLog2e;
   const int rows_kind = __builtin_amdgcn_readfirstlane(vbase + WM <= a.V ? 0 : (vbase < a.V ? 1 : 2));
-  const RowScales scales(a.W.scale, vbase, a.V);
-  float s_t[NB];
+  auto token_blocks = [&](auto kind) {
+    constexpr int KIND = decltype(kind)::value;
+    for_each_int(std::make_integer_sequence<int, NB>{}, [&](auto index) {
+      constexpr int j = decltype(index)::value;
+      const int t = scales.t0 + j * MT + lrow;
+      float m = -INFINITY, s = 0.f, e = 0.f;
+      if (KIND < 2) {
+        f32x4 x[TM], z[TM][1];
+        scales.rows(acc, j, x);
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const int t = t0 + j * MT + lrow;
-    s_t[j] = a.Hd.scale[t < a.T ? t : a.T - 1] * a.rcp_temp * kLog2e;
-  }
-  for_each_int(std::make_integer_sequence<int, NB>{}, [&](auto index) {
-    constexpr int j = decltype(index)::value;
-    const int t = t0 + j * MT + lrow;
-    float m = -INFINITY, s = 0.f, e = 0.f;
-    f32x4 z[TM][1];
-    {
-      f32x4 x[TM];
-      scales.apply(acc, j, 1.f, x);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) z[i][0] = x[i];
-    }
-    if (rows_kind == 0) fwd_tile_stats<ENTROPY, false, false>(z, 0, vbase, a.V, s_t[j], kq, m, s, e);
-    else if (rows_kind == 1) fwd_tile_stats<ENTROPY, true, false>(z, 0, vbase, a.V, s_t[j], kq, m, s, e);
-    if (kq == 0 && t < a.T) {
-      const size_t idx = part_index(part, t, nparts);
-      a.part_max[idx] = m;
-      a.part_sum[idx] = s;
-      if (ENTROPY) a.part_pz[idx] = e;
-    }
-  });
+        for (int i = 0; i < TM; ++i) z[i][0] = x[i];
+        fwd_tile_stats<ENTROPY, KIND == 1, false>(z, 0, vbase, a.V, scales.s[j] * per, kq, m, s, e);
+      }
+      if (kq == 0 && t < a.T) {
+        const size_t idx = part_index(part, t, nparts);
+        a.part_max[idx] = m;
+        a.part_sum[idx] = s;
+        if (ENTROPY) a.part_pz[idx] = e;
+      }
+    });
+  };
+  if (rows_kind == 0) token_blocks(std::integral_constant<int, 0>{});
+  else if (rows_kind == 1) token_blocks(std::integral_constant<int, 1>{});
+  else token_blocks(std::integral_constant<int, 2>{});
 }
 
-// epilogue(acc, first vocabulary row of the wave, first token of the wave) of a tile of whatever shape; v0: its first vocabulary row.
+// epilogue(acc, scales) of a tile of whatever shape; v0: its first vocabulary row.
 template <int SHAPE, bool EVEN, class Args, class Epilogue>
 __device__ __forceinline__ void int8_tile(const Args& a, int v0, int tn, char* lds, Epilogue epilogue) {
-  const int wave = threadIdx.x >> 6;
+  constexpr int NB = wave_cols(SHAPE);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // A part behind the vocabulary (the upper half of the last tile) is made of any row and dropped behind this.
   const Operand oa = bytes_of(a.W, SHAPE == kShort && v0 >= a.V ? a.V - 1 : v0, a.V), ob = bytes_of(a.Hd, tn * BN, a.T);
-  f32x4 acc[TM][wave_cols(SHAPE)];
+  f32x4 acc[TM][NB];
   tile_product<SHAPE, EVEN, true>(oa, ob, a.K / kInt8K, lds, acc);
-  epilogue(acc, v0 + wave / waves_n(SHAPE) * WM, tn * BN + wave % waves_n(SHAPE) * (wave_cols(SHAPE) * MT));
+  epilogue(acc, Scales<NB>(a.W, v0 + wave / waves_n(SHAPE) * WM, a.V, a.Hd, tn * BN + wave % waves_n(SHAPE) * (NB * MT), a.T));
 }
 
 template <class Args, class Epilogue>
@@ -172,10 +181,10 @@ __device__ __forceinline__ void int8_half_tile(const Args& a, char* lds, Epilogu
   const int tiles_m = (a.V + BM - 1) / BM, tiles_n = (a.T + kHalfBN - 1) / kHalfBN;
   int tm, tn;
   tile_coords(blockIdx.x, tiles_m, tiles_n, kGroupM, tm, tn);
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half_acc_t acc;
   half_tile_product<true>(bytes_of(a.W, tm * BM, a.V), bytes_of(a.Hd, tn * kHalfBN, a.T), a.K / kHalfRowBytes, lds, acc);
-  epilogue(acc, tm * BM + wave / WAVES_N * WM, tn * kHalfBN + wave % WAVES_N * kHalfWN);
+  epilogue(acc, Scales<kHalfTN>(a.W, tm * BM + wave / WAVES_N * WM, a.V, a.Hd, tn * kHalfBN + wave % WAVES_N * kHalfWN, a.T));
 }
 
 template <bool ENTROPY, bool EVEN, bool SHAPES>
@@ -185,27 +194,23 @@ __global__ __launch_bounds__(NTHREADS) void int8_fwd_tiles(const Int8FwdArgs a, 
   const Tile t = tile_of<false, SHAPES>(blockIdx.x, tiles_m, tiles_n, kGroupM, split);
   tile_of_shape<SHAPES>(t, a.T, [&](auto shape, int v0) {
     constexpr int SHAPE = decltype(shape)::value;
-    int8_tile<SHAPE, EVEN>(a, v0, t.tn, lds, [&](auto& acc, int vbase, int t0) { int8_stats<ENTROPY>(acc, a, vbase / WM, tiles_m * WAVES_M, t0); });
+    int8_tile<SHAPE, EVEN>(a, v0, t.tn, lds, [&](auto& acc, const auto& scales) { int8_stats<ENTROPY>(acc, scales, a, tiles_m * WAVES_M); });
   });
 }
 
 template <bool ENTROPY>
 __global__ __launch_bounds__(NTHREADS, 2) void int8_fwd_half_tiles(const Int8FwdArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[kHalfLdsBytes];
-  int8_half_tile(a, lds, [&](auto& acc, int vbase, int t0) { int8_stats<ENTROPY>(acc, a, vbase / WM, (a.V + BM - 1) / BM * WAVES_M, t0); });
+  int8_half_tile(a, lds, [&](auto& acc, const auto& scales) { int8_stats<ENTROPY>(acc, scales, a, (a.V + BM - 1) / BM * WAVES_M); });
 }
 
 template <bool F32, int NB>
-__device__ __forceinline__ void int8_store(const f32x4 (&acc)[TM][NB], const Int8LogitsArgs& a, int v0, int t0, char* lds) {
-  const RowScales scales(a.W.scale, v0, a.V);
-  const int lrow = threadIdx.x & 15;
-  float s_t[NB];
+__device__ __forceinline__ void int8_store(const f32x4 (&acc)[TM][NB], const Scales<NB>& scales, const Int8LogitsArgs& a, char* lds) {
+  store_logits_tile<F32, NB>(a.out, a.ldo, nullptr, a.T, a.V, scales.v0, scales.t0, lds, [&](int j, f32x4 (&z)[TM]) {
+    scales.rows(acc, j, z);
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const int t = t0 + j * MT + lrow;
-    s_t[j] = a.Hd.scale[t < a.T ? t : a.T - 1];
-  }
-  store_logits_tile<F32, NB>(a.out, a.ldo, nullptr, a.T, a.V, v0, t0, lds, [&](int j, f32x4 (&z)[TM]) { scales.apply(acc, j, s_t[j], z); });
+    for (int i = 0; i < TM; ++i) z[i] *= scales.s[j];
+  });
 }
 
 template <bool F32, bool EVEN, bool SHAPES>
@@ -215,14 +220,14 @@ __global__ __launch_bounds__(NTHREADS) void int8_logits_tiles(const Int8LogitsAr
   const Tile t = tile_of<false, SHAPES>(blockIdx.x, tiles_m, tiles_n, kGroupM, split);
   tile_of_shape<SHAPES>(t, a.T, [&](auto shape, int v0) {
     constexpr int SHAPE = decltype(shape)::value;
-    int8_tile<SHAPE, EVEN>(a, v0, t.tn, lds, [&](auto& acc, int vbase, int t0) { int8_store<F32>(acc, a, vbase, t0, lds); });
+    int8_tile<SHAPE, EVEN>(a, v0, t.tn, lds, [&](auto& acc, const auto& scales) { int8_store<F32>(acc, scales, a, lds); });
   });
 }
 
 template <bool F32>
 __global__ __launch_bounds__(NTHREADS, 2) void int8_logits_half_tiles(const Int8LogitsArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[kHalfLdsBytes];
-  int8_half_tile(a, lds, [&](auto& acc, int vbase, int t0) { int8_store<F32>(acc, a, vbase, t0, lds); });
+  int8_half_tile(a, lds, [&](auto& acc, const auto& scales) { int8_store<F32>(acc, scales, a, lds); });
 }
 
 // pick(x, y, z) for the three flags as compile-time constants.

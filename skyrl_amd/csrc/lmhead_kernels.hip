@@ -2363,9 +2363,8 @@ int skyrl_lmhead_int8_logits(const void* hidden, int hidden_dtype, int64_t ld_hi
     const bool half = half_tile_logits(Tb);
     const TileShapes shapes = tile_shapes(Tb, K / 2, tiles_m, compute_units());
     const int tiles = half ? tiles_m : tiles_m * (int)((Tb + BN - 1) / BN) + shapes.split;
-    e = launch_int8_logits(s, Int8LogitsArgs{W, Hd, (int)Tb, (int)K, (int)V, (char*)logits + (size_t)t0 * (size_t)ld_logits * (out_f32 ? 4 : 2), ld_logits,
-                                             out_f32 ? 1 : 0},
-                           half, shapes.used, shapes.split, tiles);
+    const Int8LogitsArgs a{W, Hd, (int)Tb, (int)K, (int)V, (char*)logits + (size_t)t0 * (size_t)ld_logits * (out_f32 ? 4 : 2), ld_logits, out_f32 ? 1 : 0};
+    e = int8_streams(Tb, K) ? launch_int8_logits_stream(s, a, compute_units()) : launch_int8_logits(s, a, half, shapes.used, shapes.split, tiles);
     if (e != hipSuccess) return (int)e;
   }
   return SKYRL_LMHEAD_OK;

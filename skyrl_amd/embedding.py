@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._launch import call, device_guard, raw_stream, registered_op
+from ._launch import call, device_guard, has_tangent, raw_stream, registered_op
 from .ops import _require_device
 
 __all__ = ["embedding_lookup", "embedding_backward_accumulate", "lmhead_embedding_fwd", "lmhead_embedding_bwd"]
@@ -132,9 +132,11 @@ def _walkable(rows: torch.Tensor) -> torch.Tensor:
 
 
 def _flat_ids(ids: torch.Tensor) -> torch.Tensor:
-    if ids.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
-    return ids.reshape(-1).to(torch.int64).contiguous()
+    if ids.dtype != torch.int64:
+        if ids.dtype != torch.int32:
+            raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
+        ids = ids.to(torch.int64)
+    return ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
 
 
 def _scale_of(scale: float) -> float:
@@ -158,10 +160,12 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, *, scale: float = 
     rounded once).  ``ids`` are int64 or int32; one outside ``[0, V)`` gives zeros and takes no gradient.  ``padding_idx``: the row that takes none
     either, as in ``torch.nn.functional.embedding``.  The gradient is dense, ``[V, H]`` in the table's dtype; at most 2^24 tokens with a gradient."""
     _check_table(weight)
-    flat, scale, padding_idx = _flat_ids(ids), _scale_of(scale), _padding_of(padding_idx, int(weight.shape[0]))
-    if weight.shape[1] > 1 and weight.stride(1) != 1 or _pitch(weight) < weight.shape[1]:
-        raise ValueError("the table must have unit stride in the last dimension and rows that do not overlap")
-    return _Lookup.apply(weight, flat, scale, padding_idx).reshape(ids.shape + (weight.shape[1],))
+    flat, scale, padding_idx = _flat_ids(ids), _scale_of(scale), _padding_of(padding_idx, weight.shape[0])
+    if torch.is_grad_enabled() and weight.requires_grad or has_tangent(weight):
+        rows = _Lookup.apply(weight, flat, scale, padding_idx)
+    else:
+        rows = call(lmhead_embedding_fwd, weight, flat, scale)
+    return rows if flat is ids else rows.reshape(ids.shape + (weight.shape[1],))
 
 
 def embedding_backward_accumulate(d_out: torch.Tensor, ids: torch.Tensor, d_weight_accum: torch.Tensor, *, scale: float = 1.0,

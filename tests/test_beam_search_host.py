@@ -90,10 +90,10 @@ def test_nothing_to_do():
     (torch.empty(6, 3)[:, :1], (1, 4, 0)), (torch.empty(6, 9, 10).transpose(1, 2), None), (torch.empty(6, 8, 3)[:, ::2], (4, 12, 24)),
 ])
 def test_segments_of_a_row(state, want):
-    into = torch.empty_strided(state.shape, state.stride())
-    got = BS._segments(state, into)
+    got = BS._segments(tuple(state.shape[1:]), state.stride()[1:], state.stride()[1:], 4)
     if want is None:  # columns that do not join: one element at a time, along the last dimension
         assert sum(n * b for _, _, n, b, _, _ in got) == state[0].numel() * 4
+        assert sorted(at + i * step for at, _, n, b, step, _ in got for i in range(n)) == list(range(0, state[0].numel() * 4, 4))
     else:
         assert [(n, b, step) for _, _, n, b, step, _ in got] == [want] and got[0][4] == got[0][5]
 
