@@ -26,7 +26,7 @@ using namespace logits;
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kInFlight = 4;  // 16-byte loads a thread has in flight
+constexpr int kInFlight = 8;  // 16-byte loads a thread has in flight
 constexpr int kMaxTop = SKYRL_LOGITS_TOP_MAX;
 constexpr int kMaxBeams = SKYRL_LOGITS_BEAMS_MAX;
 constexpr int kMaxLists = 512;  // of an item: beams * parts
@@ -68,7 +68,7 @@ struct Shared {
 __device__ __forceinline__ float difference(float z, float top) { return z - (top > -INFINITY ? top : 0.f); }  // -inf for -inf, never NaN of them
 
 template <bool F32>
-__global__ __launch_bounds__(kThreads, 6) void beam_rows(const BeamArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
   constexpr int E = Piece<F32>::kElems, ES = F32 ? 4 : 2;
   __shared__ Shared sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -25,6 +25,10 @@ struct Int8FwdArgs {
   float rcp_temp;
   float *part_max, *part_sum, *part_pz;  // part_pz NULL: no entropy
 };
+// Few tokens: the weight streams through registers (int8_few.hip).
+bool int8_streams(int64_t T, int64_t K);
+int int8_stream_parts(int64_t V, int ncu);  // partials a token of the statistics
+hipError_t launch_int8_fwd_stream(hipStream_t s, const Int8FwdArgs& a, int parts);
 hipError_t launch_int8_fwd_tiles(hipStream_t s, const Int8FwdArgs& a, bool half, bool shapes, int split, int workgroups);
 
 struct Int8LogitsArgs {
@@ -34,9 +38,6 @@ struct Int8LogitsArgs {
   int64_t ldo;
   int out_f32;
 };
-// Of few tokens, the weight streaming through registers (int8_few.hip).  Whether a call is one for it: forward tiles -> this, V=151936 and thereabouts, in
-// turn: 30.5 -> 27.6 us at T=1, H=896, 118 -> 107 at T=16, H=3584.
-bool int8_streams(int64_t T, int64_t K);
 hipError_t launch_int8_logits_stream(hipStream_t s, const Int8LogitsArgs& a, int ncu);
 hipError_t launch_int8_logits(hipStream_t s, const Int8LogitsArgs& a, bool half, bool shapes, int split, int workgroups);
 

@@ -2327,11 +2327,13 @@ int skyrl_lmhead_int8_fwd(const void* hidden, int hidden_dtype, int64_t ld_hidde
     const bool half = half_tile_logits(Tb);
     const TileShapes shapes = tile_shapes(Tb, K / 2, tiles_m, compute_units());
     const int tiles = half ? tiles_m : tiles_m * (int)((Tb + BN - 1) / BN) + shapes.split;
-    e = launch_int8_fwd_tiles(s, Int8FwdArgs{W, Hd, (int)Tb, (int)K, (int)V, rcp_temperature, pmax, psum, entropy ? ppz : nullptr}, half, shapes.used,
-                              shapes.split, tiles);
+    const Int8FwdArgs a{W, Hd, (int)Tb, (int)K, (int)V, rcp_temperature, pmax, psum, entropy ? ppz : nullptr};
+    const bool stream = int8_streams(Tb, K);
+    const int parts = stream ? int8_stream_parts(V, compute_units()) : (int)nparts;
+    e = stream ? launch_int8_fwd_stream(s, a, parts) : launch_int8_fwd_tiles(s, a, half, shapes.used, shapes.split, tiles);
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((merge_by_ten(nparts) ? &int8_fwd_merge<true, 10> : &int8_fwd_merge<true, 8>), dim3((unsigned)((Tb + kMergeTokens - 1) / kMergeTokens)),
-                       dim3(kMergeThreads), 0, s, pmax, psum, entropy ? ppz : (float*)nullptr, (int)nparts, (int)Tb, Hd, W, labels + t0, (int)K, (int)V,
+    hipLaunchKernelGGL((merge_by_ten(parts) ? &int8_fwd_merge<true, 10> : &int8_fwd_merge<true, 8>), dim3((unsigned)((Tb + kMergeTokens - 1) / kMergeTokens)),
+                       dim3(kMergeThreads), 0, s, pmax, psum, entropy ? ppz : (float*)nullptr, parts, (int)Tb, Hd, W, labels + t0, (int)K, (int)V,
                        rcp_temperature, logprobs + t0, entropy ? entropy + t0 : (float*)nullptr);
     if ((e = hipGetLastError()) != hipSuccess) return (int)e;
   }
