@@ -142,6 +142,7 @@ __global__ __launch_bounds__(64 * kRankWaves) void embedding_rank(const int64_t*
   const int from = wave * each, to = from + each;
   int before = 0;
   auto count = [&](int a, int b, auto sorts_before) {
+#pragma unroll 8
     for (int i = a; i < b; i += 4) {
       const int4 k = *(const int4*)(key + i);
       before += sorts_before(k.x, i) + sorts_before(k.y, i + 1) + sorts_before(k.z, i + 2) + sorts_before(k.w, i + 3);
@@ -331,29 +332,10 @@ __global__ __launch_bounds__(kRowThreads) void embedding_rows(const RowArgs a) {
   }
 }
 
-// A workgroup per window and slice; it has something to add where an id's tokens begin in the window and go on behind it.
-template <bool F32, bool ADD>
-__global__ __launch_bounds__(64 * kJoinWaves) void embedding_join(const RowArgs a) {
-  typedef Row16<F32> R;
-  constexpr int E = R::E;
-  __shared__ float sums[kJoinWaves][64][E];
-  const int64_t window = blockIdx.x / a.slices;
-  const int64_t at = window * kWindow, end = at + kWindow;
-  if (end >= a.T) return;
-  const int id = a.keys[end];
-  if (a.keys[end - 1] != id || id == (int)a.V) return;
-  if (a.keys[at] == id && at > 0 && a.keys[at - 1] == id) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pieces = R::pieces(a.H), piece = (int)(blockIdx.x - window * a.slices) * 64 + lane;
-  const int64_t stop = end + keys_before(a.keys + end, (int)(a.T - end), id, true);  // behind the id's last token
-  const int64_t parts = (stop - 1) / kWindow - window + 1, each = (parts + kJoinWaves - 1) / kJoinWaves;
-  const size_t row = (size_t)(pieces * E);
-  const float* base = a.partial + (size_t)window * 2 * row + (size_t)(piece < pieces ? piece : 0) * E;
-  float sum[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) sum[i] = 0.f;
-  const int64_t p1 = (wave + 1) * each < parts ? (wave + 1) * each : parts;
-  for (int64_t p = wave * each; p < p1; p += 4) {
+// The partial sums p0 .. p1 - 1 of an id whose tokens begin in window `window`, of one slice.
+template <int E>
+__device__ __forceinline__ void add_parts(const float* base, size_t row, int64_t p0, int64_t p1, float (&sum)[E]) {
+  for (int64_t p = p0; p < p1; p += 4) {
     f32x4 x[4][E / 4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -370,15 +352,61 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_join(const RowArgs 
       }
     }
   }
+}
+
+// A workgroup per kJoinWaves windows and slice.  A window has something to add where an id's tokens begin in it and go on behind it: its wave adds a few
+// partial sums alone, all waves many.  (A workgroup a window, nearly all of which had nothing to do, took 15 us for 16384 tokens.)
+constexpr int kAlone = 16;
+template <bool F32, bool ADD>
+__global__ __launch_bounds__(64 * kJoinWaves) void embedding_join(const RowArgs a) {
+  typedef Row16<F32> R;
+  constexpr int E = R::E;
+  __shared__ float sums[kJoinWaves][64][E];
+  __shared__ int many[kJoinWaves];  // partial sums of the windows that all waves add
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t group = blockIdx.x / a.slices, first = group * kJoinWaves;
+  const int pieces = R::pieces(a.H), piece = (int)(blockIdx.x - group * a.slices) * 64 + lane;
+  const bool there = piece < pieces;
+  const size_t row = (size_t)(pieces * E);
+  const float* const partial = a.partial + (size_t)(there ? piece : 0) * E;
+  const int64_t window = first + wave, at = window * kWindow, end = at + kWindow;
+  int parts = 0;
+  if (end < a.T) {
+    const int id = a.keys[end], before = at > 0 ? a.keys[at - 1] : -1;
+    if (a.keys[end - 1] == id && id != (int)a.V && !(a.keys[at] == id && before == id)) {
+      const int64_t stop = end + keys_before(a.keys + end, (int)(a.T - end), id, true);  // behind the id's last token
+      parts = (int)((stop - 1) / kWindow - window + 1);
+      if (parts <= kAlone) {
+        float sum[E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) sums[wave][lane][i] = sum[i];
+        for (int i = 0; i < E; ++i) sum[i] = 0.f;
+        add_parts<E>(partial + (size_t)window * 2 * row, row, 0, parts, sum);
+        if (there) finish<F32, ADD>(a, id, piece, sum);
+      }
+    }
+  }
+  if (lane == 0) many[wave] = parts > kAlone ? parts : 0;
   __syncthreads();
-  if (wave != 0 || piece >= pieces) return;
+  for (int x = 0; x < kJoinWaves; ++x) {
+    const int all = many[x];
+    if (all == 0) continue;
+    const int each = (all + kJoinWaves - 1) / kJoinWaves, p0 = wave * each;
+    float sum[E];
 #pragma unroll
-  for (int w = 1; w < kJoinWaves; ++w)
+    for (int i = 0; i < E; ++i) sum[i] = 0.f;
+    add_parts<E>(partial + (size_t)(first + x) * 2 * row, row, p0, p0 + each < all ? p0 + each : all, sum);
 #pragma unroll
-    for (int i = 0; i < E; ++i) sum[i] += sums[w][lane][i];
-  finish<F32, ADD>(a, id, piece, sum);
+    for (int i = 0; i < E; ++i) sums[wave][lane][i] = sum[i];
+    __syncthreads();
+    if (wave == 0 && there) {
+#pragma unroll
+      for (int w = 1; w < kJoinWaves; ++w)
+#pragma unroll
+        for (int i = 0; i < E; ++i) sum[i] += sums[w][lane][i];
+      finish<F32, ADD>(a, a.keys[(first + x + 1) * kWindow], piece, sum);
+    }
+    __syncthreads();
+  }
 }
 
 constexpr int64_t kMostTokens = (int64_t)1 << 24, kMostHidden = (int64_t)1 << 22;
@@ -396,7 +424,7 @@ int zero_rows(int pieces) {  // a multiple of 8, whose rows are whole 16-byte pi
 }
 bool fits_grid(int64_t T, int64_t V, int pieces) {
   const int64_t units = (T + kWindow - 1) / kWindow * ((pieces + 63) / 64), zeros = (V + zero_rows(pieces) - 1) / zero_rows(pieces);
-  return units * 64 * kJoinWaves < ((int64_t)1 << 32) && (units + zeros + kRowWaves) * kRowThreads < ((int64_t)1 << 32);
+  return (units + zeros + kRowWaves) * kRowThreads < ((int64_t)1 << 32);
 }
 
 size_t round_256(size_t x) { return (x + 255) / 256 * 256; }
@@ -422,7 +450,8 @@ hipError_t launch_rows(hipStream_t s, RowArgs a) {
   a.zero_rows = zero_rows(pieces);
   const int64_t groups = (a.units + kRowWaves - 1) / kRowWaves + (ADD ? 0 : (a.V + a.zero_rows - 1) / a.zero_rows);
   hipLaunchKernelGGL((embedding_rows<F32, ADD>), dim3((unsigned)groups), dim3(kRowThreads), 0, s, a);
-  if (a.T > kWindow) hipLaunchKernelGGL((embedding_join<F32, ADD>), dim3((unsigned)a.units), dim3(64 * kJoinWaves), 0, s, a);
+  const int64_t windows = (a.T + kWindow - 1) / kWindow, joins = (windows + kJoinWaves - 1) / kJoinWaves * a.slices;
+  if (windows > 1) hipLaunchKernelGGL((embedding_join<F32, ADD>), dim3((unsigned)joins), dim3(64 * kJoinWaves), 0, s, a);
   return hipGetLastError();
 }
 
