@@ -19,6 +19,7 @@ import math
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._launch import call, device_guard, has_tangent, raw_stream, registered_op
@@ -193,6 +194,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         return results
     if torch.is_grad_enabled() and any([t.requires_grad for t in states + results]) or has_tangent(*states):
         raise ValueError("beam_reorder has no gradient: call it under torch.no_grad()")
+    if True in [t.is_neg() for t in (states + results if given else states)] or any([t.is_conj() for t in states + results if t.dtype.is_complex]):
+        raise ValueError("a state whose memory is not its value (a negative or conjugate view): resolve it first")
     # What depends on the layout alone is looked at once for each: a model has many states and few layouts.
     kinds = list(zip([t.shape for t in states], [t.stride() for t in states], [u.stride() for u in results], [t.dtype for t in states]))
     groups = {kinds[0]: (states, results)}
@@ -248,4 +251,6 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
                         array = ctypes.c_void_p * len(from_)
                         st = lib.skyrl_logits_beam_reorder(array(*from_), array(*to), len(from_), *sizes, parents.data_ptr(), N, beams_in, B_out, stream)
                         _lib.check(st, "skyrl_logits_beam_reorder")
+    if given:
+        increment_version(results)
     return results

@@ -2124,15 +2124,18 @@ const char* skyrl_lmhead_strerror(int status) {
     case SKYRL_LMHEAD_ERR_NULL: return "a required pointer is NULL (or only some of seg_row, seg_col, seg_len are given)";
     case SKYRL_LMHEAD_ERR_SHAPE:
       return "bad shape: need T >= 1, V >= 1, H a positive multiple of 64, leading dimensions >= H and at most 4194304 elements; "
-             "packed-sequence calls: counts >= 0, rows == num_seqs with an attention mask";
-    case SKYRL_LMHEAD_ERR_ALIGN: return "bad alignment: pointers must be 16-byte aligned, leading dimensions multiples of 8";
+             "packed-sequence calls: counts >= 0, rows == num_seqs with an attention mask; the 8-bit head, the embedding and beam search: the "
+             "extents and strides that the header gives for them";
+    case SKYRL_LMHEAD_ERR_ALIGN:
+      return "bad alignment: pointers must be 16-byte aligned, leading dimensions multiples of 8 (entry points that walk rows of any alignment: of their "
+             "element type)";
     case SKYRL_LMHEAD_ERR_WORKSPACE: return "workspace is NULL or too small";
     case SKYRL_LMHEAD_ERR_TOO_LARGE:
       return "too large for the entry point that uses the library's fixed scratch array: V exceeds "
              "SKYRL_LMHEAD_STATIC_SCRATCH_MAX_V; use skyrl_lmhead_fwd with a caller-provided workspace";
     case SKYRL_LMHEAD_ERR_ARG:
       return "bad argument: rcp_temperature must be finite and > 0, vocab_chunk a multiple of 256; packed-sequence calls take "
-             "sub-sequence arrays or an attention mask, not both";
+             "sub-sequence arrays or an attention mask, not both; a type that is not SKYRL_LOGITS_*, a scale that is not finite, or states partly in place";
     default: break;
   }
   if (status > 0) return hipGetErrorString((hipError_t)status);

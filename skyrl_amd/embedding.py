@@ -17,9 +17,10 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
-from ._launch import call, device_guard, has_tangent, raw_stream, registered_op
+from ._launch import call, device_guard, direct, has_tangent, raw_stream, registered_op
 from .ops import _require_device
 
 __all__ = ["embedding_lookup", "embedding_backward_accumulate", "lmhead_embedding_fwd", "lmhead_embedding_bwd"]
@@ -31,6 +32,9 @@ _NO_PADDING = -1
 def _check_table(weight: torch.Tensor) -> None:
     if weight.dim() != 2 or weight.dtype not in _DTYPES:
         raise TypeError(f"the table must be a bf16 or fp32 matrix [V, H], got {weight.dtype} {tuple(weight.shape)}")
+    (V, H), (row, column) = weight.shape, weight.stride()
+    if column != 1 and H > 1 or row < H and V > 1:
+        raise ValueError("the table must have unit stride in the last dimension and rows that do not overlap")
 
 
 def _check_ids(ids: torch.Tensor) -> None:
@@ -38,29 +42,12 @@ def _check_ids(ids: torch.Tensor) -> None:
         raise ValueError(f"ids must be a contiguous int64 tensor of one dimension, got {ids.dtype} {tuple(ids.shape)}")
 
 
-def _pitch(rows: torch.Tensor) -> int:
-    return int(rows.stride(0) if rows.shape[0] > 1 else rows.shape[1])
-
-
 @registered_op("skyrl_amd::lmhead_embedding_fwd", mutates_args=())
 def lmhead_embedding_fwd(weight: torch.Tensor, ids: torch.Tensor, scale: float) -> torch.Tensor:
     """``[T, H]`` in the table's dtype."""
     _check_table(weight)
     _check_ids(ids)
-    V, H = (int(x) for x in weight.shape)
-    if weight.stride(1) != 1 and H > 1 or _pitch(weight) < H:
-        raise ValueError("the table must have unit stride in the last dimension and rows that do not overlap")
-    dev = _require_device(weight, ids)
-    out = torch.empty((ids.shape[0], H), dtype=weight.dtype, device=dev)
-    if out.numel() == 0:
-        return out
-    if V == 0:  # every id lies outside
-        return out.zero_()
-    with device_guard(dev):
-        st = _lib.load().skyrl_lmhead_embedding_fwd(weight.data_ptr(), _DTYPES[weight.dtype], _pitch(weight), ids.data_ptr(), ids.shape[0], H, V, float(scale),
-                                                    out.data_ptr(), raw_stream(dev))
-    _lib.check(st, "skyrl_lmhead_embedding_fwd")
-    return out
+    return _rows_of(weight, ids, scale)
 
 
 @lmhead_embedding_fwd.register_fake
@@ -68,17 +55,32 @@ def _(weight, ids, scale):
     return weight.new_empty((ids.shape[0], weight.shape[1]))
 
 
-def _backward_into(d_out: torch.Tensor, ids: torch.Tensor, scale: float, padding_idx: int, d_weight: torch.Tensor, accumulate: bool) -> None:
-    T, H = (int(x) for x in d_out.shape)
-    V, dev = int(d_weight.shape[0]), d_out.device
+def _rows_of(weight: torch.Tensor, ids: torch.Tensor, scale: float) -> torch.Tensor:
+    """The rows, of operands that have been checked but for their device."""
+    dev = _require_device(weight, ids)
+    (V, H), T = weight.shape, ids.shape[0]
+    out = torch.empty((T, H), dtype=weight.dtype, device=dev)
+    if T == 0 or H == 0:
+        return out
+    if V == 0:  # every id lies outside
+        return out.zero_()
+    with device_guard(dev):
+        st = _lib.load().skyrl_lmhead_embedding_fwd(weight.data_ptr(), _DTYPES[weight.dtype], weight.stride(0) if V > 1 else H, ids.data_ptr(), T, H, V, scale,
+                                                    out.data_ptr(), raw_stream(dev))
+    _lib.check(st, "skyrl_lmhead_embedding_fwd")
+    return out
+
+
+def _backward_into(d_out: torch.Tensor, ids: torch.Tensor, scale: float, padding_idx: int, d_weight: torch.Tensor, accumulate: int) -> None:
+    (T, H), V, dev = d_out.shape, d_weight.shape[0], d_out.device
     lib = _lib.load()
-    nbytes = int(lib.skyrl_lmhead_embedding_bwd_workspace_bytes(T, H, V))
+    nbytes = lib.skyrl_lmhead_embedding_bwd_workspace_bytes(T, H, V)
     if nbytes == 0:
         raise ValueError(f"no workspace for T={T}, H={H}, V={V}: an extent is out of range")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with device_guard(dev):
-        st = lib.skyrl_lmhead_embedding_bwd(d_out.data_ptr(), _DTYPES[d_out.dtype], int(d_out.stride(0)) if T > 1 else H, ids.data_ptr(), int(padding_idx), T, H,
-                                            V, float(scale), int(accumulate), d_weight.data_ptr(), ws.data_ptr(), nbytes, raw_stream(dev))
+        st = lib.skyrl_lmhead_embedding_bwd(d_out.data_ptr(), _DTYPES[d_out.dtype], d_out.stride(0) if T > 1 else H, ids.data_ptr(), padding_idx, T, H, V, scale,
+                                            accumulate, d_weight.data_ptr(), ws.data_ptr(), nbytes, raw_stream(dev))
     _lib.check(st, "skyrl_lmhead_embedding_bwd")
 
 
@@ -96,14 +98,19 @@ def _check_gradient(d_out: torch.Tensor, ids: torch.Tensor) -> None:
 def lmhead_embedding_bwd(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float, padding_idx: int) -> torch.Tensor:
     """``d_weight [vocab, H]`` in the dtype of ``d_out [T, H]``; ``padding_idx``: -1 where there is none."""
     _check_gradient(d_out, ids)
-    dev = _require_device(d_out, ids)
-    T, H = (int(x) for x in d_out.shape)
     if vocab < 0:
         raise ValueError(f"a table of {vocab} rows")
+    return _gradient_of(d_out, ids, vocab, scale, padding_idx)
+
+
+def _gradient_of(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float, padding_idx: int) -> torch.Tensor:
+    """The gradient, of operands that have been checked but for their device."""
+    dev = _require_device(d_out, ids)
+    T, H = d_out.shape
     if T == 0 or H == 0 or vocab == 0:
         return torch.zeros((vocab, H), dtype=d_out.dtype, device=dev)
     d_weight = torch.empty((vocab, H), dtype=d_out.dtype, device=dev)
-    _backward_into(d_out, ids, scale, padding_idx, d_weight, False)
+    _backward_into(d_out, ids, scale, padding_idx, d_weight, 0)
     return d_weight
 
 
@@ -116,19 +123,22 @@ class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale, padding_idx):
         ctx.save_for_backward(ids)
-        ctx.vocab, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
-        return call(lmhead_embedding_fwd, weight, ids, scale)
+        ctx.rest = (weight.shape[0], scale, padding_idx)
+        # Checked by embedding_lookup; the op, which checks for itself, where anything follows the call.
+        return _rows_of(weight, ids, scale) if direct(weight, ids) else lmhead_embedding_fwd(weight, ids, scale)
 
     @staticmethod
     def backward(ctx, d_out):
         (ids,) = ctx.saved_tensors
-        return call(lmhead_embedding_bwd, _walkable(d_out), ids, ctx.vocab, ctx.scale, ctx.padding_idx), None, None, None
+        d_out = _walkable(d_out)
+        d_weight = _gradient_of(d_out, ids, *ctx.rest) if direct(d_out, ids) else lmhead_embedding_bwd(d_out, ids, *ctx.rest)
+        return d_weight, None, None, None
 
 
 def _walkable(rows: torch.Tensor) -> torch.Tensor:
     T, H = rows.shape
-    fine = (H <= 1 or rows.stride(1) == 1) and (T <= 1 or rows.stride(0) == 0 or rows.stride(0) >= H)
-    return rows if fine else rows.contiguous()
+    row, column = rows.stride()
+    return rows if (column == 1 or H <= 1) and (row >= H or row == 0 or T <= 1) else rows.contiguous()
 
 
 def _flat_ids(ids: torch.Tensor) -> torch.Tensor:
@@ -158,7 +168,7 @@ def _padding_of(padding_idx: Optional[int], vocab: int) -> int:
 def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * weight[ids]``, shape ``ids.shape + (H,)``, in the dtype of ``weight [V, H]`` (bf16 or fp32; the product is formed in fp32 and
     rounded once).  ``ids`` are int64 or int32; one outside ``[0, V)`` gives zeros and takes no gradient.  ``padding_idx``: the row that takes none
-    either, as in ``torch.nn.functional.embedding``.  The gradient is dense, ``[V, H]`` in the table's dtype; at most 2^24 tokens with a gradient."""
+    either, as in ``torch.nn.functional.embedding``.  The gradient is dense, ``[V, H]`` in the table's dtype.  At most 2^24 tokens."""
     _check_table(weight)
     flat, scale, padding_idx = _flat_ids(ids), _scale_of(scale), _padding_of(padding_idx, weight.shape[0])
     if torch.is_grad_enabled() and weight.requires_grad or has_tangent(weight):
@@ -179,9 +189,10 @@ def embedding_backward_accumulate(d_out: torch.Tensor, ids: torch.Tensor, d_weig
     flat, scale, padding_idx = _flat_ids(ids), _scale_of(scale), _padding_of(padding_idx, int(d_weight_accum.shape[0]))
     if torch.is_grad_enabled() and d_weight_accum.requires_grad:
         raise ValueError("d_weight_accum is written in place and takes no gradient itself")
-    rows = _walkable(d_out.detach().reshape(flat.shape[0], d_weight_accum.shape[1]))
+    rows = _walkable(d_out.detach().resolve_neg().reshape(flat.shape[0], d_weight_accum.shape[1]))
     _check_gradient(rows, flat)
     _require_device(rows, flat, d_weight_accum)
     if rows.numel() and d_weight_accum.numel():
-        _backward_into(rows, flat, scale, padding_idx, d_weight_accum, True)
+        _backward_into(rows, flat, scale, padding_idx, d_weight_accum, 1)
+        increment_version(d_weight_accum)
     return d_weight_accum

@@ -258,3 +258,29 @@ def test_states_beyond_32_bit_offsets(cuda_device):
 def test_the_op_under_the_dispatcher(cuda_device):
     logits, scores = some_logits(2, 3, 40, F32, 3, cuda_device)
     torch.library.opcheck(BS.logits_beam_select, (logits, scores, 4, 1.0), test_utils=("test_schema", "test_faketensor"))
+
+
+def test_autograd_sees_what_is_written(cuda_device):
+    """A state that an eager graph has saved and that is then reordered in place: its backward refuses."""
+    t = torch.randn(4, 3, device=cuda_device)
+    w = torch.randn(4, 3, device=cuda_device, requires_grad=True)
+    loss = (w * t).sum()
+    before = t._version
+    BS.beam_reorder([t], torch.tensor([[1, 0, 2, 3]], device=cuda_device), out=[t])
+    assert t._version > before
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+def test_results_that_share_memory_with_states_are_refused(cuda_device):
+    base = torch.arange(40.0, device=cuda_device).reshape(10, 4)
+    parents = torch.zeros(1, 4, dtype=torch.int64, device=cuda_device)
+    for states, out in (([base[:4]], [base[2:6]]), ([base[:4], base[4:8]], [base[4:8], base[:4]]), ([base[:4], base[:4].clone()], [torch.empty_like(base[:4])] * 2),
+                        ([base[:4], base[:4]], [base[:4], base[:4]]), ([base[:4], base[4:8]], [base[:4], base[1:5]])):
+        with pytest.raises(ValueError):
+            BS.beam_reorder(states, parents, out=out)
+    wide = torch.zeros(130, 2, device=cuda_device)
+    with pytest.raises(ValueError):  # in place at most 128 beams
+        BS.beam_reorder([wide], torch.zeros(1, 130, dtype=torch.int64, device=cuda_device), out=[wide])
+    got = BS.beam_reorder([base[:4]], parents, out=[base[6:]])  # beside each other in one tensor
+    assert torch.equal(got[0], base[:1].expand(4, 4))

@@ -104,3 +104,13 @@ def test_shapes_under_fake_tensors():
     with FakeTensorMode():
         r = BS.beam_select(torch.empty(2, 3, 50, dtype=torch.bfloat16), torch.empty(2, 3), 7)
         assert r.scores.shape == r.parents.shape == r.tokens.shape == (2, 7) and r.tokens.dtype == torch.int64 and r.scores.dtype == torch.float32
+
+
+def test_views_whose_memory_is_not_their_value_are_refused():
+    c = torch.zeros(6, 4, dtype=torch.complex64)
+    p = torch.zeros(2, 3, dtype=torch.int64)
+    for state in (c.conj(), c.conj().imag):
+        with pytest.raises(ValueError):
+            BS.beam_reorder([state], p)
+        with pytest.raises(ValueError):
+            BS.beam_reorder([torch.zeros_like(state)], p, out=[state])
