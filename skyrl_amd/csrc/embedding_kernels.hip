@@ -6,14 +6,15 @@
 // Gradient.  Tokens are sorted by id, ties by position, so that the tokens of a row lie side by side.
 //   embedding_rank   sorts blocks of kSortBlock tokens by counting: a token's place is the number of keys that sort before its own, two
 //                    instructions a pair.  No passes, no atomics, one launch.
-//   embedding_merge  (more than one block) a token's place among all is its place in its block plus, by bisection, the keys of each other block
-//                    that sort before its own.
+//   embedding_merge  (more than one block) makes one block of kWay: a token's place in it is its place in its own block plus, by bisection, the keys
+//                    of each other that sort before its own.
 //   embedding_rows   the sorted tokens in windows of kWindow: a wave loads its window's rows of dout, 1 KiB of each, all at once and adds
 //                    up those of one id.  A sum that no other window adds to is a result; the others are kept as fp32 partial sums.  So every row
 //                    of dout is read once, by as many waves whatever the ids are: one id for all tokens or another one for each.  For a dense
 //                    result other workgroups of the same launch write the rows that no token names as zeros.
 //   embedding_join   adds the partial sums of an id whose tokens lie in several windows.
-// Bound by HBM: the table's gradient is written (almost all of it zeros), dout read.
+// Bound by HBM: the table's gradient is written (almost all of it zeros), dout read.  16384 tokens, H=3584, V=152064, bf16: lookup 46 us (5.1 TB/s),
+// rank 12, merge 7, rows 210 (5.8 TB/s), join 11.  Few tokens are bound by the zeros: 512 of H=896, V=151936 46 us (5.9 TB/s).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -27,12 +28,17 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSortBlock = 4096;
+constexpr int kSortBlock = 4096;  // 2048 and 4096 the same (250 us for the whole gradient there), 8192 260
 constexpr int kRankTokens = 64, kRankWaves = 8;  // a lane per token, a wave per eighth of the block's keys
-constexpr int kWindow = 16;                      // rows of dout that a wave has in flight
+// Rows of dout that a wave has in flight.  Ids as in text, one id, all ids alike: 255, 347, 247 us with 8, 250, 297, 267 with 16, 268, 280, 279 with 32.
+constexpr int kWindow = 16;
+// Sorted blocks that become one.  2^20 tokens of H=896: 1071 us with 8, 1141 with 16, 2375 with all blocks in one launch.
+constexpr int kWay = 8;
 constexpr int kRowThreads = 256, kRowWaves = kRowThreads / 64;
 constexpr int kJoinWaves = 8;
-constexpr int kZeroBytes = 65536;                // of the result that a workgroup looks after where it writes zeros
+// Of the result that a workgroup looks after where it writes zeros.  512 tokens of H=896 and 2047 of 1023 fp32 columns: 59 and 34 us with 16 KiB, 46 and
+// 34 with 64, 52 and 48 with 256.
+constexpr int kZeroBytes = 65536;
 
 // Sixteen bytes of a row from element e0 on.  Rows of odd sizes begin anywhere: loads and stores of unaligned 16 bytes.  The last piece of a row
 // ends with it and so may repeat elements of the one before; a row shorter than a piece goes element by element.
@@ -175,26 +181,26 @@ __device__ __forceinline__ int keys_before(const int* __restrict__ keys, int n, 
   return lo;
 }
 
-__global__ __launch_bounds__(256) void embedding_merge(const int* __restrict__ block_keys, const int* __restrict__ block_tokens, int64_t T,
+// Blocks of `block` tokens, the last one shorter.  All blocks in one launch would be as many bisections a token as there are blocks.
+__global__ __launch_bounds__(256) void embedding_merge(const int* __restrict__ block_keys, const int* __restrict__ block_tokens, int T, int block,
                                                        int* __restrict__ keys, int* __restrict__ tokens) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int i = (int)blockIdx.x * 256 + (int)threadIdx.x;
   if (i >= T) return;
-  const int blocks = (int)((T + kSortBlock - 1) / kSortBlock), own = (int)(i / kSortBlock);
+  const int own = i / block, first = own / kWay * kWay, all = (T + block - 1) / block, blocks = all < first + kWay ? all : first + kWay;
   const int k = block_keys[i];
-  int64_t place = i - (int64_t)own * kSortBlock;
+  int place = first * block + (i - own * block);
   // Four blocks at a time, whose bisections do not wait for each other.
-  for (int b0 = 0; b0 < blocks; b0 += 4) {
+  for (int b0 = first; b0 < blocks; b0 += 4) {
     const int* base[4];
     int lo[4], hi[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int b = b0 + u < blocks ? b0 + u : own;
-      const int64_t left = T - (int64_t)b * kSortBlock;
-      base[u] = block_keys + (int64_t)b * kSortBlock;
+      const int b = b0 + u < blocks ? b0 + u : own, left = T - b * block;
+      base[u] = block_keys + b * block;
       lo[u] = 0;
-      hi[u] = b == own ? 0 : (int)(left < kSortBlock ? left : kSortBlock);
+      hi[u] = b == own ? 0 : (left < block ? left : block);
     }
-    for (int step = 0; (kSortBlock >> step) > 0; ++step) {  // kSortBlock halves to nothing in as many steps
+    for (int step = 0; (block >> step) > 0; ++step) {  // a block halves to nothing in as many steps
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const bool open = lo[u] < hi[u];
@@ -258,8 +264,8 @@ __global__ __launch_bounds__(kRowThreads) void embedding_rows(const RowArgs a) {
       named[threadIdx.x] = at < (int)a.T && a.keys[at] == v ? 1 : 0;
     }
     __syncthreads();
-    // The rows as one run of memory in whole 16-byte pieces from the first row on (groups of rows begin on one, if the table does): rows of an odd
-    // size begin anywhere, and stores of unaligned pieces take three times as long (1023 fp32 columns x 32001 rows: 75 us against 25).
+    // The rows as one run of memory in whole 16-byte pieces from the first row on (groups of rows begin on one, if the table does), so that rows of any
+    // size keep all lanes at work.
     char* base = a.dtable + (size_t)v0 * (size_t)a.H * R::ES;
     const uint32_t H = (uint32_t)a.H, all = (uint32_t)rows * H;
     for (uint32_t e0 = threadIdx.x * E; e0 < all; e0 += kRowThreads * E) {
@@ -354,8 +360,9 @@ __device__ __forceinline__ void add_parts(const float* base, size_t row, int64_t
   }
 }
 
-// A workgroup per kJoinWaves windows and slice.  A window has something to add where an id's tokens begin in it and go on behind it: its wave adds a few
-// partial sums alone, all waves many.  (A workgroup a window, nearly all of which had nothing to do, took 15 us for 16384 tokens.)
+// A workgroup per kJoinWaves windows and slice.  A window has something to add where an id's tokens begin in it and go on behind it: its wave adds a
+// few partial sums alone, all waves many (a limit of 4, 16 or 64: within 1 %).  A workgroup a window, nearly all of which had nothing to do, took 15 us
+// for 16384 tokens.
 constexpr int kAlone = 16;
 template <bool F32, bool ADD>
 __global__ __launch_bounds__(64 * kJoinWaves) void embedding_join(const RowArgs a) {
@@ -430,14 +437,15 @@ bool fits_grid(int64_t T, int64_t V, int pieces) {
 size_t round_256(size_t x) { return (x + 255) / 256 * 256; }
 
 struct Scratch {
-  size_t keys, tokens, block_keys, block_tokens, partial, bytes;
+  size_t lists[2];  // of keys, each followed by its tokens; the second one where blocks are merged
+  size_t list, partial, bytes;
 };
 Scratch scratch(int64_t T, int64_t H) {
-  const size_t list = round_256((size_t)T * 4), windows = (size_t)((T + kWindow - 1) / kWindow);
+  const size_t windows = (size_t)((T + kWindow - 1) / kWindow);
   Scratch s;
-  s.keys = 0, s.tokens = list;
-  s.block_keys = T > kSortBlock ? 2 * list : 0, s.block_tokens = T > kSortBlock ? 3 * list : list;
-  s.partial = (T > kSortBlock ? 4 : 2) * list;
+  s.list = round_256((size_t)T * 4);
+  s.lists[0] = 0, s.lists[1] = 2 * s.list;
+  s.partial = (T > kSortBlock ? 4 : 2) * s.list;
   s.bytes = s.partial + (windows > 1 ? windows * 2 * (size_t)((H + 7) / 8 * 8) * 4 : 0);
   return s;
 }
@@ -496,13 +504,16 @@ int skyrl_lmhead_embedding_bwd(const void* dout, int dtype, int64_t ld_dout, con
   if ((uintptr_t)workspace & 255u) return SKYRL_LMHEAD_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   char* const base = (char*)workspace;
-  int *keys = (int*)(base + w.keys), *tokens = (int*)(base + w.tokens), *block_keys = (int*)(base + w.block_keys), *block_tokens = (int*)(base + w.block_tokens);
+  auto keys = [&](int x) { return (int*)(base + w.lists[x & 1]); };
+  auto tokens = [&](int x) { return (int*)(base + w.lists[x & 1] + w.list); };
   const int64_t blocks = (T + kSortBlock - 1) / kSortBlock;
   const int64_t groups = blocks > 1 ? blocks * (kSortBlock / kRankTokens) : (T + kRankTokens - 1) / kRankTokens;
-  hipLaunchKernelGGL(embedding_rank, dim3((unsigned)groups), dim3(64 * kRankWaves), 0, s, ids, T, V, padding, block_keys, block_tokens);
-  if (blocks > 1)
-    hipLaunchKernelGGL(embedding_merge, dim3((unsigned)((T + 255) / 256)), dim3(256), 0, s, (const int*)block_keys, (const int*)block_tokens, T, keys, tokens);
-  RowArgs a{(const char*)dout, ld_dout, T, V, (int)H, scale, keys, tokens, (float*)(base + w.partial), (char*)dtable, 0, 0, 0};
+  hipLaunchKernelGGL(embedding_rank, dim3((unsigned)groups), dim3(64 * kRankWaves), 0, s, ids, T, V, padding, keys(0), tokens(0));
+  int in = 0;  // where the sorted tokens are
+  for (int64_t block = kSortBlock; block < T; block *= kWay, ++in)
+    hipLaunchKernelGGL(embedding_merge, dim3((unsigned)((T + 255) / 256)), dim3(256), 0, s, (const int*)keys(in), (const int*)tokens(in), (int)T, (int)block,
+                       keys(in + 1), tokens(in + 1));
+  RowArgs a{(const char*)dout, ld_dout, T, V, (int)H, scale, keys(in), tokens(in), (float*)(base + w.partial), (char*)dtable, 0, 0, 0};
   hipError_t e;
   if (f32) e = add ? launch_rows<true, true>(s, a) : launch_rows<true, false>(s, a);
   else e = add ? launch_rows<false, true>(s, a) : launch_rows<false, false>(s, a);

@@ -274,3 +274,13 @@ def test_compiled_programs_see_the_ops(cuda_device):
     weight, ids = torch.randn(30, 16, device=cuda_device), torch.tensor([4, 29, 30], device=cuda_device)
     for op, args in ((E.lmhead_embedding_fwd, (weight, ids, 0.5)), (E.lmhead_embedding_bwd, (weight[:3].contiguous(), ids, 30, 0.5, 4))):
         torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("T,kind", [(65536, "text"), (65537, "text"), (70001, "some outside"), (1100003, "text"), (1100003, "apart"), (1100003, "one")])
+def test_more_blocks_than_one_launch_merges(cuda_device, T, kind):
+    """Whole numbers, whose sums are exact in fp32 (at most 1.1 million of them, 7 the largest): a token that the sort loses or counts twice shows."""
+    gen = torch.Generator().manual_seed(T)
+    ids = some_ids(kind, T, 40009, gen).to(cuda_device)
+    d = torch.randint(-7, 8, (T, 4), generator=gen).float()
+    want, _, _ = plain_gradient(d, ids, 40009, 1.0)
+    assert torch.equal(E.lmhead_embedding_bwd(d.to(cuda_device), ids, 40009, 1.0, -1).double().cpu(), want)
