@@ -101,6 +101,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, temperatu
         return BeamSelection(*call(logits_beam_select, rows, scores, k, 1.0 / temperature))
 
 
+_NOT_ITS_VALUE = "a state whose memory is not its value (a negative or conjugate view): resolve it first"
+
+
 def _segments(shape: Tuple[int, ...], strides: Tuple[int, ...], to_strides: Tuple[int, ...], size: int) -> List[Tuple[int, int, int, int, int, int]]:
     """``(place, place in the result, segments, bytes, from_segment, to_segment)``, in bytes, of a row of that shape: what it is in both, one run of
     equally spaced contiguous pieces.  Rows with more dimensions that do not join are taken apart along the first of them."""
@@ -121,6 +124,15 @@ def _segments(shape: Tuple[int, ...], strides: Tuple[int, ...], to_strides: Tupl
     return [(0, 0, n, inner * size, x * size, y * size)]
 
 
+def _folded(shape: Tuple[int, ...], strides: Tuple[int, ...]) -> bool:
+    end = 0  # of the dimensions so far, the closest elements first
+    for step, n in sorted((s, n) for n, s in zip(shape, strides) if n > 1):
+        if step <= end:
+            return True
+        end += (n - 1) * step
+    return False
+
+
 class _Layout(NamedTuple):
     """What states of one type, shape and strides and their results have in common."""
 
@@ -128,7 +140,7 @@ class _Layout(NamedTuple):
     to_shape: Tuple[int, ...]
     extent: int     # bytes from a state's first element to its last
     to_extent: int
-    expanded: bool  # whether elements of a result lie on each other
+    folded: bool    # whether elements of a result lie on each other, or might: their order in memory is not that of any order of the dimensions
     # (from_row, from_segment, to_row, to_segment, segments, bytes) and the segments' places in a state and in its result, in bytes
     launches: Tuple[Tuple[Tuple[int, ...], Tuple[Tuple[int, int], ...]], ...]
 
@@ -153,7 +165,7 @@ def _layout(shape: Tuple[int, ...], strides: Tuple[int, ...], to_strides: Tuple[
         for at, to_at, n, nbytes, step, to_step in _segments(tuple(shape[1:]), strides[1:], to_strides[1:], size):
             found.setdefault((row, step, to_row, to_step, n, nbytes), []).append((at, to_at))
     return _Layout(rows // items if items else 0, to_shape, extent(shape, strides), extent(to_shape, to_strides),
-                   any(n > 1 and s == 0 for n, s in zip(to_shape, to_strides)), tuple((sizes, tuple(places)) for sizes, places in found.items()))
+                   _folded(to_shape, to_strides), tuple((sizes, tuple(places)) for sizes, places in found.items()))
 
 
 def _overlap(states: Sequence[Tuple[int, int]], results: Sequence[Tuple[int, int]]) -> bool:
@@ -194,8 +206,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         return results
     if torch.is_grad_enabled() and any([t.requires_grad for t in states + results]) or has_tangent(*states):
         raise ValueError("beam_reorder has no gradient: call it under torch.no_grad()")
-    if True in [t.is_neg() for t in (states + results if given else states)] or any([t.is_conj() for t in states + results if t.dtype.is_complex]):
-        raise ValueError("a state whose memory is not its value (a negative or conjugate view): resolve it first")
+    if True in [t.is_neg() for t in (states + results if given else states)]:
+        raise ValueError(_NOT_ITS_VALUE)
     # What depends on the layout alone is looked at once for each: a model has many states and few layouts.
     kinds = list(zip([t.shape for t in states], [t.stride() for t in states], [u.stride() for u in results], [t.dtype for t in states]))
     groups = {kinds[0]: (states, results)}
@@ -213,8 +225,10 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         beams_in = layout.beams_in
         if given and ([u.shape for u in us].count(layout.to_shape) < len(us) or [u.dtype for u in us].count(kind[3]) < len(us)):
             raise ValueError(f"a result must be {layout.to_shape} {kind[3]}, got " + ", ".join(f"{tuple(u.shape)} {u.dtype}" for u in us))
-        if given and layout.expanded:
-            raise ValueError("a result must not be expanded: its elements would be written more than once")
+        if kind[3].is_complex and any([t.is_conj() for t in ts + us]):
+            raise ValueError(_NOT_ITS_VALUE)
+        if given and layout.folded:
+            raise ValueError("a result must not be expanded or overlap itself: its elements would be written more than once")
         if layout.to_extent > 0:
             used.append((layout, kind[1] == kind[2] and beams_in == B_out, [t.data_ptr() for t in ts], [u.data_ptr() for u in us]))
     if not used:

@@ -11,9 +11,11 @@
 // logit of +inf, or a score that is NaN or +inf offers the same columns with NaN, which sorts behind -inf.
 //
 // beam_rows   a workgroup per beam and part of its row: one pass for the largest logit, the sum and the k best (as logits_top_rows,
-//             top_logits_kernels.hip).  Bound by HBM and, for few beams, by the way through a workgroup.
+//             top_logits_kernels.hip).  Bound by HBM and, for few beams, by the way through a workgroup: 4 x 151936 in bf16 9 us, 16 x 8 x 128261 in
+//             fp32 19 (3.5 TB/s: four steps a workgroup, votes and candidates between them), 64 x 8 x 151936 in bf16 46 with the join (3.4 TB/s).
 // beam_join   a workgroup per item: joins the parts' sums; finds the k best of all parts' sorted lists.  Entry j of a list whose head r heads
 //             precede can only be among the k best if j + r < k, and must reach the k-th head: few entries are left, and each counts those before it.
+//             5 to 8 us, nearly all of it the latency of what it does one after the other.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -26,7 +28,9 @@ using namespace logits;
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kInFlight = 8;  // 16-byte loads a thread has in flight
+// 16-byte loads a thread has in flight; with eight the registers of four waves a SIMD have to do.  Four: 54 us for 64 x 8 x 151936 in bf16, 25.4 for
+// 16 x 8 x 128261 in fp32; eight: 46 and 24.5.
+constexpr int kInFlight = 8;
 constexpr int kMaxTop = SKYRL_LOGITS_TOP_MAX;
 constexpr int kMaxBeams = SKYRL_LOGITS_BEAMS_MAX;
 constexpr int kMaxLists = 512;  // of an item: beams * parts
@@ -304,9 +308,14 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
 // ------------------------------------------------------------------------------------------------------------
 // The states of the beams, rows [items * beams] of `segments` pieces of `bytes` contiguous bytes each: row j of an item becomes its row
 // parents[j].  One launch for all tensors of a layout.  Bound by HBM; rows that several beams take are read from the caches.
+// 16 x 8 rows of 4 MiB: 153 us (read and written 1.07 GB: 7.0 TB/s), in place, where rows that stay are left, 164.
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kStates = SKYRL_LOGITS_STATES_MAX;
-constexpr int kCopyThreads = 256, kCopyPieces = 4;  // pieces that a thread has in flight
+// Pieces that a thread has in flight.  A copy of 64 rows of 4 MiB: 78 us with one or two, 80 with four, 130 with eight.
+constexpr int kCopyThreads = 256, kCopyPieces = 2;
+// In place.  Eight, four and two: 203, 220 and 240 us for 128 beams of 2 MiB, 427, 409 and 333 for 16 x 16 of 4 MiB, whose pieces of one column, a power of
+// two apart, meet in the same channels of the memory; 157, 154 and 153 where they are 4000256 bytes apart, 16 x 8.
+constexpr int kHeldPieces = 2;
 
 struct ReorderArgs {
   const char* from[kStates];
@@ -353,6 +362,8 @@ __global__ __launch_bounds__(kCopyThreads) void beam_permute(const ReorderArgs a
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
   __shared__ int parent[kMaxBeams];
   __shared__ int wanted[kMaxBeams];
+  __shared__ int source[kMaxBeams];  // the beams that are wanted, one behind the other
+  __shared__ int sources;
   const uint32_t in_row = a.segments * a.blocks, item = blockIdx.x / in_row, rest = blockIdx.x - item * in_row;
   const uint32_t segment = rest / a.blocks, block = rest - segment * a.blocks;
   const int beams = a.beams_in;
@@ -364,13 +375,32 @@ __global__ __launch_bounds__(kCopyThreads) void beam_permute(const ReorderArgs a
     if (p >= 0 && p < beams && p != b) wanted[p] = 1;  // the same value from whichever beam
   }
   __syncthreads();
+  if (threadIdx.x < 64) {
+    int n = 0;
+    for (int b0 = 0; b0 < beams; b0 += 64) {
+      const int b = b0 + (int)threadIdx.x;
+      const bool take = b < beams && wanted[b];
+      const unsigned long long mask = __ballot(take);
+      if (take) source[n + __popcll(mask & ((1ull << threadIdx.x) - 1))] = b;
+      n += (int)__popcll(mask);
+    }
+    if (threadIdx.x == 0) sources = n;
+  }
+  __syncthreads();
   const uint32_t p = block * blockDim.x + threadIdx.x;
   if (p >= a.pieces) return;
   char* const base = a.to[blockIdx.y] + (int64_t)item * beams * a.to_row + (int64_t)segment * a.to_segment + (int64_t)p * (int64_t)sizeof(Unit);
   Unit* const mine = (Unit*)dynamic + threadIdx.x;
-#pragma unroll 4
-  for (int b = 0; b < beams; ++b)
-    if (wanted[b]) mine[b * blockDim.x] = *(const Unit*)(base + (int64_t)b * a.to_row);
+  const int n = __builtin_amdgcn_readfirstlane(sources);
+  for (int i = 0; i < n; i += kHeldPieces) {
+    Unit w[kHeldPieces];
+#pragma unroll
+    for (int u = 0; u < kHeldPieces; ++u)
+      if (i + u < n) w[u] = *(const Unit*)(base + (int64_t)source[i + u] * a.to_row);
+#pragma unroll
+    for (int u = 0; u < kHeldPieces; ++u)
+      if (i + u < n) mine[source[i + u] * blockDim.x] = w[u];
+  }
 #pragma unroll 4
   for (int b = 0; b < beams; ++b) {
     const int from = parent[b];
@@ -386,7 +416,8 @@ size_t most_left(int lists, int each, int k) {
   return n;
 }
 
-// Parts of a row: so many that 512 workgroups share the logits, of at least 8192 logits each.
+// Parts of a row: so many that 512 workgroups share the logits (two a CU, all at once), of at least 8192 logits each.  16 x 8 x 128261 in bf16 and fp32: 23
+// and 25 us with 512 workgroups, 26 and 25 with 768, 27 and 29 with 1024.
 int beam_parts(int64_t rows, int64_t beams, int64_t V) {
   int64_t n = 512 / rows;
   if (n > V / 8192) n = V / 8192;
@@ -404,8 +435,8 @@ template <class Unit>
 int launch_reorder(hipStream_t s, ReorderArgs& a, int64_t items, int64_t bytes, int count, bool in_place) {
   const int64_t pieces = bytes / (int64_t)sizeof(Unit);
   int threads = kCopyThreads;
-  if (in_place)
-    while (threads > 64 && (size_t)a.beams_in * threads * sizeof(Unit) > 65536) threads /= 2;  // two workgroups a CU, but for 128 beams
+  if (in_place)  // two workgroups a CU, but for 128 beams.  (One: within 4 % for 32 and 64 beams.)
+    while (threads > 64 && (size_t)a.beams_in * threads * sizeof(Unit) > 65536) threads /= 2;
   const int64_t each = in_place ? threads : kCopyThreads * kCopyPieces, blocks = (pieces + each - 1) / each;
   const int64_t rows = in_place ? items : items * a.beams_out;
   // In floats, which the products of what a caller passes cannot overflow.

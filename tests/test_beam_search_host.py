@@ -114,3 +114,13 @@ def test_views_whose_memory_is_not_their_value_are_refused():
             BS.beam_reorder([state], p)
         with pytest.raises(ValueError):
             BS.beam_reorder([torch.zeros_like(state)], p, out=[state])
+
+
+@pytest.mark.parametrize("size,stride,refused", [((6, 4), (4, 1), False), ((6, 4), (1, 6), False), ((6, 2, 5), (40, 20, 2), False), ((6, 4), (3, 1), True),
+                                                 ((6, 4), (1, 1), True), ((6, 4), (4, 0), True), ((6, 1), (1, 0), False)])
+def test_results_that_overlap_themselves_are_refused(size, stride, refused):
+    t = torch.zeros(300).as_strided(size, stride)
+    p = torch.zeros(2, 3, dtype=torch.int64)
+    with pytest.raises(ValueError if refused else RuntimeError) as e:  # RuntimeError: not on a GPU
+        BS.beam_reorder([torch.zeros(size)], p, out=[t])
+    assert ("overlap" in str(e.value)) == refused
