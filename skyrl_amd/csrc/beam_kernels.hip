@@ -15,7 +15,7 @@
 //             fp32 19 (3.5 TB/s: four steps a workgroup, votes and candidates between them), 64 x 8 x 151936 in bf16 46 with the join (3.4 TB/s).
 // beam_join   a workgroup per item: joins the parts' sums; finds the k best of all parts' sorted lists.  Entry j of a list whose head r heads
 //             precede can only be among the k best if j + r < k, and must reach the k-th head: few entries are left, and each counts those before it.
-//             5 to 8 us, nearly all of it the latency of what it does one after the other.
+//             5 to 7 us, nearly all of it the latency of what it does one after the other.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -245,6 +245,9 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t item = blockIdx.x, row0 = item * a.beams;
   const int lists = a.beams * parts, each = a.each, k = a.k;
+  // The first keys that a thread will look at, loaded beside the sums: what a list does not have is not looked at later.
+  const topkey_t* const keys = a.keys + row0 * parts * (int64_t)each;
+  const topkey_t head0 = keys[(int64_t)(tid < lists ? tid : 0) * each], key0 = keys[tid < lists * each ? tid : 0];
   for (int b = wave; b < a.beams; b += kJoinThreads / 64) {
     PartSum p{0.0, -INFINITY, 0};
     if (lane < parts) p = a.part[(row0 + b) * parts + lane];
@@ -265,15 +268,14 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
   }
   if (tid == 0) kept = 0, bound = Candidate{0, ~0ull};
   __syncthreads();
-  auto candidate = [&](int list, int j) {
+  auto candidate = [&](int list, int j, topkey_t key) {
     const int b = list / parts;
     const double off = offset[b];
     if (!(off - off == 0.0)) return Candidate{ordered_total(off), ((unsigned long long)b << 32) | (unsigned)j};
-    const topkey_t key = a.keys[(row0 * parts + list) * (int64_t)each + j];
     const double total = off + (double)value_of_bits(key_bits(key)) * a.rcp_temp;
     return Candidate{ordered_total(total), ((unsigned long long)b << 32) | (unsigned)key_column(key)};
   };
-  for (int l = tid; l < lists; l += kJoinThreads) heads[l] = have[l] > 0 ? candidate(l, 0) : Candidate{0, ~0ull};
+  for (int l = tid; l < lists; l += kJoinThreads) heads[l] = have[l] > 0 ? candidate(l, 0, l == tid ? head0 : keys[(int64_t)l * each]) : Candidate{0, ~0ull};
   __syncthreads();
   for (int l = tid; l < lists; l += kJoinThreads) {
     const Candidate mine = heads[l];
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
   for (int e = tid; e < lists * each; e += kJoinThreads) {
     const int l = e / each, j = e - l * each;
     if (j + rank[l] >= k || j >= have[l]) continue;
-    const Candidate c = candidate(l, j);
+    const Candidate c = candidate(l, j, e == tid ? key0 : keys[e]);
     if (!precedes(least, c)) left[atomicAdd(&kept, 1)] = c;  // in any order: places depend on the candidates alone
   }
   __syncthreads();
