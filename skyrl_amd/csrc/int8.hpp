@@ -15,8 +15,8 @@ struct Int8Rows {
   const float* scale;    // [rows]
 };
 
-// values[r, :H] = round(127 x / max |x|) of row r of src (bf16 or fp32), zeros up to the next multiple of kInt8K; scale[r] = max |x| / 127.  A row with NaN or an infinity
-// has values of zero and a scale of NaN.
+// values[r, :H] = round(127 x / max |x|) of row r of src (bf16 or fp32), zeros up to the next multiple of kInt8K; scale[r] = max |x| / 127.  A row with
+// NaN or an infinity has values of zero and a scale of NaN.
 hipError_t launch_int8_rows(hipStream_t s, const void* src, bool f32, int64_t ld_src, int64_t rows, int64_t H, int8_t* values, int64_t ld, float* scale);
 
 struct Int8FwdArgs {

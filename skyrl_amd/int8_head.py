@@ -6,8 +6,9 @@
 * ``int8_logits`` -- the logits of a decoding step, for a sampler, ``torch_utils.top_logprobs_from_logits`` or ``beam_search.beam_select``;
 * ``int8_logprobs_from_hidden`` -- log-probability and entropy of given tokens without a ``[T, V]`` tensor: scoring with a reference model.
 
-The hidden states are brought to integers inside the call, a scale a token (ties to even; the quotients are rounded as if they were exact).  Sums of products are exact;
-with weights and hidden states rounded to a step of max / 127, logits are those of the rounded operands to fp32 precision.  Neither has a gradient.
+The hidden states are brought to integers inside the call, a scale a token (ties to even; the quotients are rounded as if they were exact).  Sums of
+products are exact; with weights and hidden states rounded to a step of max / 127, logits are those of the rounded operands to fp32 precision.  Neither
+has a gradient.
 """
 
 from __future__ import annotations
