@@ -534,7 +534,7 @@ int skyrl_logits_top_bwd(const void* logits, int logits_dtype, int64_t ld_logits
 /* ---- the head in 8-bit integers ----------------------------------------------------------------------------------------
  * A frozen output weight as int8 values with one fp32 scale a row, and the hidden states brought to the same form in the call:
  *   q = round(127 x / max |x|), ties to even, s = max |x| / 127 of each hidden row x;    z[t, v] = s_t * scale_v * sum_i q[t, i] values[v, i]
- * The sums are exact.  A row of zeros has q = 0 and s = 0; a hidden row with NaN or an infinity has logits of NaN.  The quotients are rounded as if they
+ * The sums are exact for whatever values, -128 among them.  A row of zeros has q = 0 and s = 0; a hidden row with NaN or an infinity has logits of NaN.  The quotients are rounded as if they
  * were exact.
  *   skyrl_lmhead_int8_rows    brings the rows of a matrix (bf16 or fp32, SKYRL_LOGITS_*) to that form, zeros from H to the next multiple of 128: the
  *                             weight, once.  rows at most 2^23.
@@ -542,7 +542,7 @@ int skyrl_logits_top_bwd(const void* logits, int logits_dtype, int64_t ld_logits
  *                             log-probability 0
  *   skyrl_lmhead_int8_logits  the logits [T, ld_logits], bf16 or fp32
  * values: row v at values + v * ld_values, ld_values a multiple of 16, at least H rounded up to a multiple of 128 and at most 8388608; what lies between H and
- * that multiple is read but does not enter.  hidden rows of any pitch and alignment; 1 <= H <= 133120.  Workspaces: 256-byte aligned; a block of
+ * that multiple is read but does not enter.  hidden rows of any pitch and alignment; 1 <= H <= 132096.  Workspaces: 256-byte aligned; a block of
  * min(T, 32768) hidden rows as integers, and the partial sums of skyrl_lmhead_fwd. */
 int skyrl_lmhead_int8_rows(const void* src, int src_dtype, int64_t ld_src, int64_t rows, int64_t H, int8_t* values, int64_t ld_values, float* scale,
                            void* stream);

@@ -6,8 +6,8 @@
 namespace lmhead {
 
 constexpr int kInt8K = 128;  // k of a k-tile: rows of values are whole k-tiles long, zeros behind the hidden size
-// |sum of products| <= 127 * 127 * H stays below 2^31
-constexpr int64_t kInt8MostHidden = (((int64_t)1 << 31) - 1) / (127 * 127) / kInt8K * kInt8K;
+// |sum of products| <= 127 * 128 * H stays below 2^31: hidden values are 127 at most, weights from elsewhere may be -128
+constexpr int64_t kInt8MostHidden = (((int64_t)1 << 31) - 1) / (127 * 128) / kInt8K * kInt8K;
 
 struct Int8Rows {
   const int8_t* values;  // [rows, ld], ld a multiple of kInt8K bytes

@@ -24,7 +24,7 @@ from .ops import _require_device
 
 __all__ = ["Int8Head", "quantize_head", "int8_logits", "int8_logprobs_from_hidden", "lmhead_int8_rows", "lmhead_int8_fwd", "lmhead_int8_logits"]
 
-MAX_HIDDEN = 133120  # the largest sum of products, 127 * 127 * H, stays below 2^31
+MAX_HIDDEN = 132096  # the largest sum of products, 127 * 128 * H, stays below 2^31
 _K = 128             # rows of values are whole multiples of this long
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 

@@ -155,6 +155,22 @@ def test_the_largest_sums_are_exact(cuda_device):
         assert torch.equal(z, z[:1].expand_as(z))
 
 
+@pytest.mark.parametrize("T", [1, 40, 130])
+def test_the_largest_sums_of_a_weight_of_minus_128(cuda_device, T):
+    """-128, which quantize_head does not make, at the largest hidden size: a sum of 127 * 128 * H, on either side of zero."""
+    H = I.MAX_HIDDEN
+    assert 127 * 128 * H < 2 ** 31 <= 127 * 128 * (H + 128)
+    head = I.Int8Head(torch.full((70, H), -128, dtype=torch.int8, device=cuda_device), torch.ones(70, device=cuda_device))
+    hidden = torch.ones(T, H, device=cuda_device)
+    hidden[T // 2:] = -1
+    z = I.int8_logits(hidden, head, dtype=F32).double().cpu()
+    want = -128.0 * H * hidden[:, :1].double().cpu()
+    assert bool(((z - want).abs() <= 128.0 * H * 2 ** -22).all())
+    lp, _ = I.int8_logprobs_from_hidden(hidden, head, torch.zeros(T, dtype=torch.int64, device=cuda_device))
+    # 70 equal logits; the label's is summed on its own, and both are rounded to fp32 (1.7e7: steps of 1 or 2)
+    assert bool(((lp.double().cpu() + math.log(70)).abs() <= 128.0 * H * 2 ** -21).all())
+
+
 @pytest.mark.parametrize("T", [3, 40, 200])
 def test_what_lies_behind_the_hidden_size_does_not_enter(cuda_device, T):
     gen = torch.Generator().manual_seed(1)

@@ -22,13 +22,13 @@ def test_workspaces():
     assert head + 300 * 900 <= lib.skyrl_lmhead_int8_fwd_workspace_bytes(300, 896, 5000) <= head + 300 * 900 + 2048
     # of a block of tokens, however many there are
     assert lib.skyrl_lmhead_int8_fwd_workspace_bytes(1 << 30, 896, 5000) == lib.skyrl_lmhead_int8_fwd_workspace_bytes(32768, 896, 5000)
-    for T, H, V in ((0, 64, 8), (8, 0, 8), (8, 64, 0), (8, 133121, 8), ((1 << 30) + 1, 64, 8), (8, 64, 1 << 31), (BIG, BIG, BIG)):
+    for T, H, V in ((0, 64, 8), (8, 0, 8), (8, 64, 0), (8, 132097, 8), ((1 << 30) + 1, 64, 8), (8, 64, 1 << 31), (BIG, BIG, BIG)):
         assert lib.skyrl_lmhead_int8_fwd_workspace_bytes(T, H, V) == 0
-    assert lib.skyrl_lmhead_int8_logits_workspace_bytes(8, 133120) > 0 == lib.skyrl_lmhead_int8_logits_workspace_bytes(8, 133121)
+    assert lib.skyrl_lmhead_int8_logits_workspace_bytes(8, 132096) > 0 == lib.skyrl_lmhead_int8_logits_workspace_bytes(8, 132097)
 
 
 BAD = [(dict(hidden=None), NULL), (dict(values=None), NULL), (dict(scale=None), NULL), (dict(dtype=2), ARG), (dict(dtype=-1), ARG), (dict(T=0), SHAPE),
-       (dict(H=0), SHAPE), (dict(ld=99), SHAPE), (dict(ld=BIG), SHAPE), (dict(ldv=112), SHAPE), (dict(H=133121, ld=BIG - 1, ldv=1 << 20), SHAPE),
+       (dict(H=0), SHAPE), (dict(ld=99), SHAPE), (dict(ld=BIG), SHAPE), (dict(ldv=112), SHAPE), (dict(H=132097, ld=BIG - 1, ldv=1 << 20), SHAPE),
        (dict(ldv=(1 << 23) + 16), SHAPE), (dict(T=BIG), SHAPE), (dict(hidden=P + 1), ALIGN), (dict(dtype=1, hidden=P + 2), ALIGN), (dict(values=P + 8), ALIGN),
        (dict(ldv=136), ALIGN), (dict(scale=P + 2), ALIGN)]
 
@@ -99,7 +99,7 @@ def test_refusals():
     with pytest.raises(TypeError):
         I.quantize_head(torch.zeros(5, 64, dtype=torch.float16))
     with pytest.raises(ValueError):
-        I.quantize_head(torch.zeros(5, 133121))
+        I.quantize_head(torch.zeros(5, 132097))
 
 
 def test_shapes_under_fake_tensors():
