@@ -133,13 +133,26 @@ def _folded(shape: Tuple[int, ...], strides: Tuple[int, ...]) -> bool:
     return False
 
 
+class _Reach(NamedTuple):
+    """Where the elements of a tensor lie, from its address on, in bytes."""
+
+    extent: int                          # from the first element's begin to the last one's end
+    size: int                            # of an element
+    steps: Tuple[Tuple[int, int], ...]   # (stride, extent) of the dimensions with more than one element
+
+
+def _reach(shape: Tuple[int, ...], strides: Tuple[int, ...], size: int) -> _Reach:
+    steps = tuple((s * size, n) for n, s in zip(shape, strides) if n > 1)
+    return _Reach(0 if 0 in shape else size + sum(s * (n - 1) for s, n in steps), size, steps)
+
+
 class _Layout(NamedTuple):
     """What states of one type, shape and strides and their results have in common."""
 
     beams_in: int
     to_shape: Tuple[int, ...]
-    extent: int     # bytes from a state's first element to its last
-    to_extent: int
+    reach: _Reach
+    to_reach: _Reach
     folded: bool    # whether elements of a result lie on each other, or might: their order in memory is not that of any order of the dimensions
     # (from_row, from_segment, to_row, to_segment, segments, bytes) and the segments' places in a state and in its result, in bytes
     launches: Tuple[Tuple[Tuple[int, ...], Tuple[Tuple[int, int], ...]], ...]
@@ -154,33 +167,61 @@ def _layout(shape: Tuple[int, ...], strides: Tuple[int, ...], to_strides: Tuple[
         raise ValueError(f"{rows} rows of a state {tuple(shape)} do not divide among {items} prompts")
     size = dtype.itemsize
     to_shape = (items * beams_out,) + tuple(shape[1:])
-
-    def extent(sizes, steps):
-        return 0 if 0 in sizes else size * (1 + sum((n - 1) * s for n, s in zip(sizes, steps)))
-
     row = strides[0] * size if rows > 1 else 0
     to_row = to_strides[0] * size if to_shape[0] > 1 else 0
     found: dict = {}
     if 0 not in to_shape:
         for at, to_at, n, nbytes, step, to_step in _segments(tuple(shape[1:]), strides[1:], to_strides[1:], size):
             found.setdefault((row, step, to_row, to_step, n, nbytes), []).append((at, to_at))
-    return _Layout(rows // items if items else 0, to_shape, extent(shape, strides), extent(to_shape, to_strides),
+    return _Layout(rows // items if items else 0, to_shape, _reach(shape, strides, size), _reach(to_shape, to_strides, size),
                    _folded(to_shape, to_strides), tuple((sizes, tuple(places)) for sizes, places in found.items()))
 
 
-def _overlap(states: Sequence[Tuple[int, int]], results: Sequence[Tuple[int, int]]) -> bool:
-    """Whether one of the results' ranges of addresses meets one of the states'."""
-    if max(b for _, b in states) <= min(a for a, _ in results) or max(b for _, b in results) <= min(a for a, _ in states):
-        return False
-    end_of_state = end_of_result = 0
-    for start, end, is_result in sorted([(a, b, False) for a, b in states] + [(a, b, True) for a, b in results]):
-        if start < (end_of_state if is_result else end_of_result):
-            return True
-        if is_result:
-            end_of_result = max(end_of_result, end)
+def _clusters(some: list, turn: int) -> List[list]:
+    """The regions ``(begin, end, ...)`` that meet, directly or over others, in groups; on a circle of ``turn`` bytes, or a line where that is 0."""
+    groups, end = [], 0
+    for region in sorted(some):
+        if groups and region[0] < end:
+            groups[-1].append(region)
         else:
-            end_of_state = max(end_of_state, end)
-    return False
+            groups.append([region])
+        end = max(end, region[1])
+    while turn and len(groups) > 1 and groups[0][0][0] < end - turn:  # the last one goes over the end and begins anew
+        groups[-1] += groups.pop(0)
+    return groups
+
+
+def _clash(regions: list) -> bool:
+    """Whether a result may share memory with another region; regions are ``(begin, end, reach, whether it is a result)`` in addresses.
+
+    Ranges that do not meet share nothing.  Views of one buffer whose ranges interleave (keys and values side by side) are told apart by their addresses modulo
+    a stride: where all longer strides of the regions are multiples of it, each occupies one interval there, as long as its shorter strides make it, and
+    intervals that do not meet share nothing.  What no stride tells apart is taken to clash."""
+    end = 0
+    for region in sorted(regions):
+        if region[0] < end:
+            break
+        end = region[1]
+    else:
+        return False
+
+    def clash(some, moduli):
+        if len(some) < 2 or not any(r[3] for r in some):
+            return False
+        for i, turn in enumerate(moduli):
+            spans = {}
+            for reach in {r[2] for r in some}:
+                span = reach.size + sum(s * (n - 1) for s, n in reach.steps if s < turn)
+                if span > turn or any(s >= turn and s % turn for s, _ in reach.steps):
+                    break
+                spans[reach] = span
+            else:
+                groups = _clusters([(r[0] % turn, r[0] % turn + spans[r[2]], r) for r in some], turn)
+                if len(groups) > 1:
+                    return any(clash([r for _, _, r in group], moduli[i + 1:]) for group in groups)
+        return True
+
+    return any(clash(group, sorted({s for r in group for s, _ in r[2].steps if s > 0}, reverse=True)) for group in _clusters(regions, 0))
 
 
 def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
@@ -188,7 +229,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
     (the used part of a cache, say) and ``parents [N, B_out]`` int64; zeros where a parent lies outside ``[0, B_in)``.
 
     ``out``: tensors to write, new ones without it.  ``out=states`` reorders in place (``B_out == B_in``, at most 128 beams): rows that keep their place
-    are not moved.  A result is otherwise in memory of its own: one whose range of addresses meets a state's is refused.  Not differentiable."""
+    are not moved.  A result is otherwise in memory of its own: one that may share an element with another result, with a state but the one that it is, or with
+    ``parents`` is refused.  Views of one buffer that interleave without sharing an element are told apart.  Not differentiable."""
     states = list(states)
     if parents.dim() != 2:
         raise ValueError(f"expected parents [N, B], got {tuple(parents.shape)}")
@@ -229,25 +271,27 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
             raise ValueError(_NOT_ITS_VALUE)
         if given and layout.folded:
             raise ValueError("a result must not be expanded or overlap itself: its elements would be written more than once")
-        if layout.to_extent > 0:
+        if layout.to_reach.extent > 0:
             used.append((layout, kind[1] == kind[2] and beams_in == B_out, [t.data_ptr() for t in ts], [u.data_ptr() for u in us]))
     if not used:
         return results
+    if given:
+        regions = []
+        for layout, may_be_same, ps, qs in used:
+            reach, to_reach = layout.reach, layout.to_reach
+            regions += [(q, q + to_reach.extent, to_reach, True) for q in qs]
+            apart = [p for p, q in zip(ps, qs) if p != q] if may_be_same else ps
+            if len(apart) < len(ps) and B_out > MAX_BEAMS:
+                raise ValueError(f"at most {MAX_BEAMS} beams are reordered in place, got {B_out}")
+            if reach.extent > 0:
+                regions += [(p, p + reach.extent, reach, False) for p in apart]
+        read = _reach(parents.shape, parents.stride(), 8)
+        regions.append((parents.data_ptr(), parents.data_ptr() + read.extent, read, False))
+        if _clash(regions):
+            raise ValueError("a result shares memory with another result, with a state that it is not or with the parents, or may do so")
     device = parents.get_device()
     if device < 0 or [t.get_device() for t in states + results].count(device) < 2 * len(states):
         _require_device(parents, *states, *results)
-    if given:
-        apart, to = [], []  # the ranges of addresses of results that are not their states; where results begin
-        for layout, may_be_same, ps, qs in used:
-            some = [q for p, q in zip(ps, qs) if p != q] if may_be_same else qs
-            if len(some) < len(qs) and B_out > MAX_BEAMS:
-                raise ValueError(f"at most {MAX_BEAMS} beams are reordered in place, got {B_out}")
-            apart += [(q, q + layout.to_extent) for q in some]
-            to += qs
-        if len(set(to)) < len(to):
-            raise ValueError("a result is given twice")
-        if apart and _overlap([(p, p + layout.extent) for layout, _, ps, _ in used for p in ps], apart):
-            raise ValueError("a result overlaps a state and is not that state: it would be read after it was written")
     dev = _require_device(parents, states[0])
     if beams_in == 0:  # no row to take
         return [u.zero_() for u in results]
