@@ -6,8 +6,8 @@
 * ``beam_reorder`` -- key / value caches and whatever else a beam carries follow their parents, into other buffers or in place, all tensors of a
   layout in one launch.
 
-Among equal totals the lower beam and then the lower token comes first.  Totals are formed in 64 bits, so that candidates of different
-beams come in the order of their exact totals but where those differ by less than some 1e-7.  Neither waits for the GPU, and both may be
+Among equal totals the lower beam and then the lower token comes first.  Totals are formed in 64 bits from exponentials that are right to a unit of their
+last place in 32, so that candidates of different beams come in the order of their exact totals but where those differ by less than 2.4e-7.  Neither waits for the GPU, and both may be
 captured in a HIP graph.
 """
 

@@ -5,14 +5,16 @@
 //
 // Order: the larger total first, the lower beam and then the lower column first among equal ones.  A beam offers its k largest logits (the lower
 // column first among equal ones), so that is the order of a beam's candidates too.  Which of two candidates of different beams comes first hangs on
-// the last bits of their totals: those, the row's sum of exponentials and its logarithm are formed in 64 bits, from exponentials in 32 bits that
-// are relative to the row's largest logit and have no common error (the factor 1 / (temperature ln 2) enters as two floats).
+// the last bits of their totals: those, the row's sum of exponentials and its logarithm are formed in 64 bits, from exponentials in 32 bits that are relative
+// to the row's largest logit and off by no more than a unit of their last place: a logarithm is off by 2^-23 (1.2e-7) where all terms are alike, by less
+// elsewhere, so that candidates come in the order of their exact totals but where those differ by less than 2.4e-7.
 // A beam whose score is -inf, or that has no logit above -inf, offers columns 0 .. k - 1 with a total of -inf; one with NaN among its logits, a
 // logit of +inf, or a score that is NaN or +inf offers the same columns with NaN, which sorts behind -inf.
 //
 // beam_rows   a workgroup per beam and part of its row: one pass for the largest logit, the sum and the k best (as logits_top_rows,
-//             top_logits_kernels.hip).  Bound by HBM and, for few beams, by the way through a workgroup: 4 x 151936 in bf16 9 us, 16 x 8 x 128261 in
-//             fp32 19 (3.5 TB/s: four steps a workgroup, votes and candidates between them), 64 x 8 x 151936 in bf16 46 with the join (3.4 TB/s).
+//             top_logits_kernels.hip).  Bound by instructions where there are many beams (the sums, below), for few beams by the way through a workgroup:
+//             votes and candidates between the loads of its two steps.  Times of a call: 4 x 151936 in bf16 20 us, the host's; 16 x 8 x 128261 in fp32 29;
+//             64 x 8 x 151936 in bf16 56.
 // beam_join   a workgroup per item: joins the parts' sums; finds the k best of all parts' sorted lists.  Entry j of a list whose head r heads
 //             precede can only be among the k best if j + r < k, and must reach the k-th head: few entries are left, and each counts those before it.
 //             5 to 7 us, nearly all of it the latency of what it does one after the other.
@@ -89,21 +91,35 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
 
   float wave_top = -INFINITY;  // the largest logit of the wave so far
   double sum = 0.0;            // of this lane, relative to it
+  float rest = 0.f;            // sum 2^t r of the parts r of the exponents that t leaves
   float lane_max = -INFINITY;
   int count = 0;               // candidates in the wave's list
   topkey_t least = 0;          // candidates have larger keys
   float bound = -INFINITY;
   topkey_t* const list = sm.list[wave];
 
-  auto term = [&](float z) {
-    const float d = difference(z, wave_top);
-    return __builtin_amdgcn_exp2f(fmaf(d, a.scale_hi, fmaxf(d, kMostNegativeFactor) * a.scale_lo));
+  // 2^((z - top) scale) into the sums.  An exponent of 10 rounded to 32 bits is off by up to 5e-7, alike for equal logits: what the roundings of the
+  // difference and of its product leave, r, comes in with the derivative, ln 2 sum 2^t r.  Of the exponential's own error, a unit of its last place, equal
+  // logits have the same share.  Terms are added in 64 bits: beside one of 1 the small ones of a piece would all be rounded the same way.  With neither of the
+  // two 39 us instead of 56 for 64 x 8 x 151936 in bf16, bound by instructions, and 26 instead of 29 for 16 x 8 x 128261 in fp32, but sums off by up to 5e-7
+  // (with 32-bit sums that keep what each addition loses 59 and 29.5).
+  auto add = [&](float z) {
+#pragma clang fp contract(off)
+    const float top = wave_top > -INFINITY ? wave_top : 0.f;  // -inf - top is -inf and never NaN
+    const float d = z - top, back = d - z, lost = (z - (d - back)) + (-top - back);
+    const float t = d * a.scale_hi, p = __builtin_amdgcn_exp2f(t);
+    const float r = fmaf(lost, a.scale_hi, fmaf(d, a.scale_lo, fmaf(d, a.scale_hi, -t)));
+    sum += (double)p;
+    rest = fmaf(p, __builtin_amdgcn_fmed3f(r, -1e-3f, 1e-3f), rest);  // NaN or large only where p is 0, or NaN itself
   };
   auto raise = [&](float z) {  // the wave's largest logit, to the largest z of its lanes
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) z = fmaxf(z, __shfl_xor(z, o, 64));
     if (z > wave_top) {
-      if (wave_top > -INFINITY) sum *= exp2((double)(wave_top - z) * ((double)a.scale_hi + (double)a.scale_lo));
+      if (wave_top > -INFINITY) {
+        const double f = exp2((double)(wave_top - z) * ((double)a.scale_hi + (double)a.scale_lo));
+        sum *= f, rest *= (float)f;
+      }
       wave_top = z;
     }
   };
@@ -165,10 +181,8 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       if (p0 + u * kThreads < pieces) {
-        float s = 0.f;  // of one piece; pieces are added up in 64 bits
 #pragma unroll
-        for (int i = 0; i < E; ++i) s += term(pc[u].v[i]);
-        sum += (double)s;
+        for (int i = 0; i < E; ++i) add(pc[u].v[i]);
       }
     }
     if (__any(top >= bound)) {
@@ -186,13 +200,14 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
     const int c = all_pieces * E + (there ? tid : 0);
     const float z = load_one(base, (size_t)c, F32);
     raise(there ? z : -INFINITY);
-    if (there) sum += (double)term(z);
+    if (there) add(z);
     append(z, c, there);
   }
   if (count > k && __builtin_amdgcn_readfirstlane(count) > kThreads / kWaves) {  // so that all fit behind each other
     (void)keep_best(list, count, k);
     count = k;
   }
+  sum += 0.6931471805599453094 * (double)rest;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if (lane == 0) sm.count[wave] = count, sm.sum[wave] = sum, sm.top[wave] = wave_top;

@@ -1,0 +1,46 @@
+"""What error the sum of exponentials of a beam's row has (``skyrl_amd.beam_search.beam_select``), on rows whose terms are all alike, so that errors of the same
+sign show.
+
+Scores are chosen so that the totals are next to 0: what comes back is then the error, and not its rounding to fp32.  A term is one exponential in 32 bits of an
+exponent without error that counts: one unit of the last place, 2^-23 relative, which alike terms have in common.  Sums, the shifts between maxima and the
+logarithm are in 64 bits, so the total is off by 2^-23 (1.2e-7), and its rounding to fp32 by 2^-24 of a total below 2^-6.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from skyrl_amd import beam_search as BS
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+BOUND = 2.0 ** -23 + 2.0 ** -30  # and 2^-24 of the total
+
+
+def errors(logits, temperature):
+    """Each beam of ``logits [N, B, V]`` with the score that brings its best total next to 0: what comes back against the total in 64 bits."""
+    y = logits.double().cpu() / temperature
+    best = torch.log_softmax(y, 2).amax(2)
+    scores = (-best).float()
+    want = scores.double() + best
+    N, B, _ = logits.shape
+    got = BS.beam_select(logits, scores.to(logits.device), B, temperature=temperature)
+    off = got.scores.double().cpu() - want.gather(1, got.parents.cpu())
+    assert bool((got.parents.cpu().sort(1).values == torch.arange(B)).all())
+    return off.abs().max().item(), want.abs().max().item()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 1.3])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_terms_that_are_all_alike(cuda_device, dtype, temperature):
+    """64 rows of one background each, and of one logit a wave that is 8 or 7.75: the maxima's differences are exact, the background's error is the sum's."""
+    E, V = (8, 16376) if dtype == BF16 else (4, 16376)
+    background = 8.0 - torch.linspace(1.5, 12.0, 64) * temperature
+    logits = background[:, None].expand(64, V).clone()
+    logits[:, torch.arange(1, 8) * 64 * E] = 7.75
+    logits[:, 3] = 8.0
+    off, size = errors(logits.to(dtype).to(cuda_device)[None], temperature)
+    assert off <= BOUND + size * 2.0 ** -24, off
