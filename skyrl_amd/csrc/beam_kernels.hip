@@ -71,8 +71,6 @@ struct Shared {
   topkey_t all[kWaves * kMaxTop];
 };
 
-__device__ __forceinline__ float difference(float z, float top) { return z - (top > -INFINITY ? top : 0.f); }  // -inf for -inf, never NaN of them
-
 template <bool F32>
 __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
   constexpr int E = Piece<F32>::kElems, ES = F32 ? 4 : 2;
@@ -117,7 +115,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
     for (int o = 32; o >= 1; o >>= 1) z = fmaxf(z, __shfl_xor(z, o, 64));
     if (z > wave_top) {
       if (wave_top > -INFINITY) {
-        const double f = exp2((double)(wave_top - z) * ((double)a.scale_hi + (double)a.scale_lo));
+        const double f = exp2(((double)wave_top - (double)z) * ((double)a.scale_hi + (double)a.scale_lo));
         sum *= f, rest *= (float)f;
       }
       wave_top = z;
@@ -222,7 +220,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sm.top[w]);
     double s = 0.0;
     for (int w = 0; w < kWaves; ++w) {
-      const double d = (double)difference(sm.top[w], top) * ((double)a.scale_hi + (double)a.scale_lo);
+      const double d = ((double)sm.top[w] - (double)top) * ((double)a.scale_hi + (double)a.scale_lo);
       s += sm.top[w] == top ? sm.sum[w] : sm.top[w] > -INFINITY ? sm.sum[w] * exp2(d) : sm.sum[w];  // without a logit: 0, or NaN
     }
     a.part[row * parts + part] = PartSum{s, top, total < k ? total : k};
@@ -270,7 +268,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     double s = p.sum;
-    if (p.top > -INFINITY && p.top != top) s *= exp2((double)(p.top - top) * ((double)a.scale_hi + (double)a.scale_lo));
+    if (p.top > -INFINITY && p.top != top) s *= exp2(((double)p.top - (double)top) * ((double)a.scale_hi + (double)a.scale_lo));
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
     const float score = a.scores[row0 + b];

@@ -44,3 +44,16 @@ def test_terms_that_are_all_alike(cuda_device, dtype, temperature):
     logits[:, 3] = 8.0
     off, size = errors(logits.to(dtype).to(cuda_device)[None], temperature)
     assert off <= BOUND + size * 2.0 ** -24, off
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("peak_at", [0, 70000, 151935])
+def test_a_flat_row_with_one_peak(cuda_device, peak_at, dtype):
+    """The maximum comes to one wave of one part: all others' sums are relative to another one."""
+    gen = torch.Generator().manual_seed(peak_at)
+    flat = torch.tensor([0.1, -0.37, 1.7, 0.0123, -5.03, 2.9])
+    for peak in (8.4, 11.3, 14.77):
+        logits = flat[:, None].expand(6, 151936).clone()
+        logits[:, peak_at] = peak + torch.rand(6, generator=gen) * 0.1
+        off, size = errors(logits.to(dtype).to(cuda_device)[None], 1.0)
+        assert off <= BOUND + size * 2.0 ** -24, (peak, off)
