@@ -573,7 +573,7 @@ int skyrl_lmhead_embedding_bwd(const void* dout, int dtype, int64_t ld_dout, con
  * first: out_scores fp32, parents (the beam) and tokens (the column) int64, each [items, k].  Among equal totals the lower beam and then the
  * lower column comes first; a beam offers its k largest logits, the lower column first among equal ones.  Totals are formed in 64 bits from a sum in
  * 64 bits of exponentials that are off by a unit of their last place in 32, so that the order of candidates of different beams is that of the exact totals but
- * where they differ by less than 2.4e-7.  A beam whose score is -inf, or that has no logit above -inf, offers columns 0 .. with total -inf; one with a NaN or +inf among its logits, or whose
+ * where they differ by less than 2.4e-7, or 2^-45 of a total; those of one beam come in the order of its logits, however large its score is.  A beam whose score is -inf, or that has no logit above -inf, offers columns 0 .. with total -inf; one with a NaN or +inf among its logits, or whose
  * score is NaN or +inf, the same columns with NaN, behind those.  Parents and tokens are valid in every case.
  * logits: bf16 or fp32, item i's beam b at logits + i * ld_item + b * ld_beam elements (either may be 0: rows that beams share); scores fp32 [items, beams].
  * 1 <= k <= min(beams * V, SKYRL_LOGITS_TOP_MAX), beams <= SKYRL_LOGITS_BEAMS_MAX, items * beams <= 2^22.  workspace: 8-byte aligned.

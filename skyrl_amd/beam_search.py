@@ -7,7 +7,8 @@
   layout in one launch.
 
 Among equal totals the lower beam and then the lower token comes first.  Totals are formed in 64 bits from exponentials that are right to a unit of their
-last place in 32, so that candidates of different beams come in the order of their exact totals but where those differ by less than 2.4e-7.  Neither waits for the GPU, and both may be
+last place in 32, so that candidates of different beams come in the order of their exact totals but where those differ by less than 2.4e-7 (or, under scores of
+1e6 and more, than 2^-45 of them); candidates of one beam come in the order of their logits whatever its score is.  Neither waits for the GPU, and both may be
 captured in a HIP graph.
 """
 

@@ -4,7 +4,7 @@
 //   y[b, v] = z[b, v] / temperature;   total[b, v] = score_b + y[b, v] - log sum_v exp y[b, v]
 //
 // Order: the larger total first, the lower beam and then the lower column first among equal ones.  A beam offers its k largest logits (the lower
-// column first among equal ones), so that is the order of a beam's candidates too.  Which of two candidates of different beams comes first hangs on
+// column first among equal ones), and they come in that order.  Which of two candidates of different beams comes first hangs on
 // the last bits of their totals: those, the row's sum of exponentials and its logarithm are formed in 64 bits, from exponentials in 32 bits that are relative
 // to the row's largest logit and off by no more than a unit of their last place: a logarithm is off by 2^-23 (1.2e-7) where all terms are alike, by less
 // elsewhere, so that candidates come in the order of their exact totals but where those differ by less than 2.4e-7.
@@ -40,6 +40,7 @@ constexpr int kMaxParts = 64;
 constexpr int kGroupsPerWave = kGroups / kWaves;
 constexpr int kJoinThreads = 512;
 static_assert(kMaxTop <= kGroups && kMaxTop + 64 <= kWaveList && kMaxBeams <= kMaxLists && kMaxParts <= 64, "as in top_logits_kernels.hip; a part a lane");
+static_assert((kMaxBeams & (kMaxBeams - 1)) == 0, "a beam in the last bits of a total");
 
 // Of one part of a row: its largest logit, sum 2^((z - top) * scale2), how many keys it has found.
 struct PartSum {
@@ -234,18 +235,21 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
   }
 }
 
-// A candidate: a larger `total` first, a lower place among equal ones.  total: bits that compare as the 64-bit floats do; 1 for NaN, 0 for none.
+// A candidate: larger ones sort earlier, by `first` and then by the key.  first: the total's bits, so that they compare as the 64-bit floats do and all but the
+// last seven, and in their place the beam, lower ones larger.  So candidates of one beam come in the order of their keys even where its score is so large
+// that their totals are the same, which the lists of the parts rely on.  NaN is next to 0, none 0.
 struct Candidate {
-  unsigned long long total, place;
+  unsigned long long first, key;
 };
-__device__ __forceinline__ bool precedes(const Candidate& a, const Candidate& b) { return a.total > b.total || (a.total == b.total && a.place < b.place); }
+__device__ __forceinline__ bool precedes(const Candidate& a, const Candidate& b) { return a.first > b.first || (a.first == b.first && a.key > b.key); }
 __device__ __forceinline__ unsigned long long ordered_total(double x) {
   const unsigned long long b = (unsigned long long)__double_as_longlong(x + 0.0);
-  return x != x ? 1ull : b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
+  return x != x ? (unsigned long long)kMaxBeams : b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
 }
-__device__ __forceinline__ double value_of_total(unsigned long long t) {
-  return t == 1ull ? (double)NAN : __longlong_as_double((long long)(t ^ ((t >> 63) ? 0x8000000000000000ull : ~0ull)));
+__device__ __forceinline__ Candidate candidate_of(double total, int beam, topkey_t key) {
+  return Candidate{(ordered_total(total) & ~(unsigned long long)(kMaxBeams - 1)) | (unsigned)(kMaxBeams - 1 - beam), key};
 }
+__device__ __forceinline__ int beam_of(const Candidate& c) { return kMaxBeams - 1 - (int)(c.first & (kMaxBeams - 1)); }
 
 __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int parts) {
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
@@ -279,23 +283,25 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
     if (lane < parts) have[b * parts + lane] = off - off == 0.0 ? p.keys : lane == 0 ? each : 0;
     if (lane == 0) offset[b] = off;
   }
-  if (tid == 0) kept = 0, bound = Candidate{0, ~0ull};
+  if (tid == 0) kept = 0, bound = Candidate{0, 0};
   __syncthreads();
+  auto total_of = [&](int beam, topkey_t key) {
+    const double off = offset[beam];
+    return off - off == 0.0 ? off + (double)value_of_bits(key_bits(key)) * a.rcp_temp : off;
+  };
   auto candidate = [&](int list, int j, topkey_t key) {
     const int b = list / parts;
-    const double off = offset[b];
-    if (!(off - off == 0.0)) return Candidate{ordered_total(off), ((unsigned long long)b << 32) | (unsigned)j};
-    const double total = off + (double)value_of_bits(key_bits(key)) * a.rcp_temp;
-    return Candidate{ordered_total(total), ((unsigned long long)b << 32) | (unsigned)key_column(key)};
+    const topkey_t mine = offset[b] - offset[b] == 0.0 ? key : make_key(0.f, j);  // of a beam that has no order of its own: columns 0, 1, ...
+    return candidate_of(total_of(b, mine), b, mine);
   };
-  for (int l = tid; l < lists; l += kJoinThreads) heads[l] = have[l] > 0 ? candidate(l, 0, l == tid ? head0 : keys[(int64_t)l * each]) : Candidate{0, ~0ull};
+  for (int l = tid; l < lists; l += kJoinThreads) heads[l] = have[l] > 0 ? candidate(l, 0, l == tid ? head0 : keys[(int64_t)l * each]) : Candidate{0, 0};
   __syncthreads();
   for (int l = tid; l < lists; l += kJoinThreads) {
     const Candidate mine = heads[l];
     int r = 0;
     for (int i = 0; i < lists; ++i) r += precedes(heads[i], mine) ? 1 : 0;
     rank[l] = have[l] > 0 ? r : kMaxTop;
-    if (r == k - 1 && have[l] > 0) bound = mine;  // at most one: places differ
+    if (r == k - 1 && have[l] > 0) bound = mine;  // at most one: no two are equal
   }
   __syncthreads();
   const Candidate least = bound;
@@ -313,9 +319,10 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
     for (int i = 0; i < n; ++i) place += precedes(left[i], mine) ? 1 : 0;
     if (place < k) {
       const int64_t at = item * k + place;
-      a.out_scores[at] = (float)value_of_total(mine.total);
-      a.parents[at] = (int64_t)(mine.place >> 32);
-      a.tokens[at] = (int64_t)(mine.place & 0xffffffffull);
+      const int b = beam_of(mine);
+      a.out_scores[at] = (float)total_of(b, mine.key);
+      a.parents[at] = b;
+      a.tokens[at] = key_column(mine.key);
     }
   }
 }

@@ -57,3 +57,23 @@ def test_a_flat_row_with_one_peak(cuda_device, peak_at, dtype):
         logits[:, peak_at] = peak + torch.rand(6, generator=gen) * 0.1
         off, size = errors(logits.to(dtype).to(cuda_device)[None], 1.0)
         assert off <= BOUND + size * 2.0 ** -24, (peak, off)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("score", [-1e9, -1e20, -1e30, torch.finfo(F32).min, 1e25, 0.0])
+@pytest.mark.parametrize("V,k", [(300, 7), (70001, 16), (151936, 128)])
+def test_a_beam_of_a_far_score_keeps_the_order_of_its_logits(cuda_device, V, k, score, dtype):
+    """The totals of such a beam are all the same in 64 bits; its candidates are its largest logits all the same, in their order."""
+    gen = torch.Generator(device=cuda_device).manual_seed(V)
+    logits = (torch.randn(2, 1, V, generator=gen, device=cuda_device) * 3).to(dtype)
+    got = BS.beam_select(logits, torch.full((2, 1), score, device=cuda_device), k)
+    order = torch.sort(logits[:, 0].double(), dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(got.tokens, order) and not got.parents.any()
+    # Beside a beam of an ordinary score, and one of the same far one: that comes behind both, and the lower of the two first.
+    three = torch.cat([logits, logits.flip(2), logits], 1)
+    scores = torch.tensor([[score, -3.0, score]] * 2, device=cuda_device)
+    if score <= -1e20 and 2 * V >= k:
+        got = BS.beam_select(three, scores, min(V + 5, 128))
+        n = min(V, min(V + 5, 128))
+        assert bool((got.parents[:, :n] == 1).all()) and not got.parents[:, n:].any()
+        assert torch.equal(got.tokens[:, n:], order[:, :got.tokens.shape[1] - n])
