@@ -453,22 +453,41 @@ bool beam_extents(int64_t items, int64_t beams, int64_t V, int64_t k) {
          k <= beams * V;
 }
 
+// A launch for as many rows as one grid holds (2^32 threads), or as many segments of one row.
 template <class Unit>
-int launch_reorder(hipStream_t s, ReorderArgs& a, int64_t items, int64_t bytes, int count, bool in_place) {
+int launch_reorder(hipStream_t s, const ReorderArgs& all, int64_t items, int64_t bytes, int count, bool in_place) {
   const int64_t pieces = bytes / (int64_t)sizeof(Unit);
   int threads = kCopyThreads;
   if (in_place)  // two workgroups a CU, but for 128 beams.  (One: within 4 % for 32 and 64 beams.)
-    while (threads > 64 && (size_t)a.beams_in * threads * sizeof(Unit) > 65536) threads /= 2;
+    while (threads > 64 && (size_t)all.beams_in * threads * sizeof(Unit) > 65536) threads /= 2;
   const int64_t each = in_place ? threads : kCopyThreads * kCopyPieces, blocks = (pieces + each - 1) / each;
-  const int64_t rows = in_place ? items : items * a.beams_out;
-  // In floats, which the products of what a caller passes cannot overflow.
-  if (pieces >= ((int64_t)1 << 31) || (double)blocks * (double)a.segments * (double)rows * threads >= 4294967296.0) return SKYRL_LMHEAD_ERR_SHAPE;
-  a.pieces = (uint32_t)pieces, a.blocks = (uint32_t)blocks;
-  const dim3 grid((unsigned)(blocks * a.segments * rows), (unsigned)count);
-  if (in_place) hipLaunchKernelGGL(beam_permute<Unit>, grid, dim3((unsigned)threads), (size_t)a.beams_in * threads * sizeof(Unit), s, a);
-  else hipLaunchKernelGGL(beam_copy<Unit>, grid, dim3(kCopyThreads), 0, s, a);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? SKYRL_LMHEAD_OK : (int)e;
+  const int64_t most = (((int64_t)1 << 32) - 1) / threads;  // workgroups
+  if (pieces >= ((int64_t)1 << 31)) return SKYRL_LMHEAD_ERR_SHAPE;
+  const int64_t per_launch = most / blocks;  // segments
+  const int64_t segments = all.segments < per_launch ? all.segments : per_launch;
+  const int64_t rows = per_launch / segments;                                        // in place: items
+  const int64_t step_items = in_place ? rows : (rows >= all.beams_out ? rows / all.beams_out : 1);
+  const int64_t step_beams = in_place || rows >= all.beams_out ? all.beams_out : rows;  // of an item, where a launch has part of one
+  for (int64_t item = 0; item < items; item += step_items)
+    for (int64_t beam = 0; beam < all.beams_out; beam += step_beams)
+      for (int64_t segment = 0; segment < all.segments; segment += segments) {
+        ReorderArgs a = all;
+        const int64_t n_items = items - item < step_items ? items - item : step_items, n_beams = all.beams_out - beam < step_beams ? all.beams_out - beam : step_beams;
+        for (int t = 0; t < count; ++t) {
+          a.from[t] += item * all.beams_in * all.from_row + segment * all.from_segment;
+          a.to[t] += (item * all.beams_out + beam) * all.to_row + segment * all.to_segment;
+        }
+        a.parents += item * all.beams_out + beam;
+        a.beams_out = (int)n_beams;
+        a.segments = (uint32_t)(all.segments - segment < segments ? all.segments - segment : segments);
+        a.pieces = (uint32_t)pieces, a.blocks = (uint32_t)blocks;
+        const dim3 grid((unsigned)(blocks * a.segments * (in_place ? n_items : n_items * n_beams)), (unsigned)count);
+        if (in_place) hipLaunchKernelGGL(beam_permute<Unit>, grid, dim3((unsigned)threads), (size_t)a.beams_in * threads * sizeof(Unit), s, a);
+        else hipLaunchKernelGGL(beam_copy<Unit>, grid, dim3(kCopyThreads), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+      }
+  return SKYRL_LMHEAD_OK;
 }
 
 }  // namespace
@@ -517,6 +536,10 @@ int skyrl_logits_beam_reorder(const void* const* from, void* const* to, int64_t 
       items >= ((int64_t)1 << 31) || beams_in >= ((int64_t)1 << 31) || beams_out >= ((int64_t)1 << 31) || items * beams_out >= ((int64_t)1 << 31) ||
       items * beams_in >= ((int64_t)1 << 31) || from_row < 0 || from_segment < 0 || to_row < 0 || to_segment < 0 || from_row >= most || from_segment >= most ||
       to_row >= most || to_segment >= most)
+    return SKYRL_LMHEAD_ERR_SHAPE;
+  const double far = (double)((int64_t)1 << 62);  // no memory has such places, whose products might not be held in 64 bits
+  if ((double)items * (double)beams_in * (double)from_row + (double)segments * (double)from_segment >= far ||
+      (double)items * (double)beams_out * (double)to_row + (double)segments * (double)to_segment >= far)
     return SKYRL_LMHEAD_ERR_SHAPE;
   if ((uintptr_t)parents & 7u) return SKYRL_LMHEAD_ERR_ALIGN;
   const bool in_place = from[0] == to[0];
