@@ -13,11 +13,14 @@
 //
 // beam_rows   a workgroup per beam and part of its row: one pass for the largest logit, the sum and the k best (as logits_top_rows,
 //             top_logits_kernels.hip).  Bound by instructions where there are many beams (the sums, below), for few beams by the way through a workgroup:
-//             votes and candidates between the loads of its two steps.  Times of a call: 4 x 151936 in bf16 20 us, the host's; 16 x 8 x 128261 in fp32 29;
-//             64 x 8 x 151936 in bf16 56.
+//             votes and candidates between the loads of its two steps.  Times of a call: 4 x 151936 in bf16 20 us, the host's; 16 x 8 x 128261 in fp32 30;
+//             64 x 8 x 151936 in bf16 58.
 // beam_join   a workgroup per item: joins the parts' sums; finds the k best of all parts' sorted lists.  Entry j of a list whose head r heads
-//             precede can only be among the k best if j + r < k, and must reach the k-th head: few entries are left, and each counts those before it.
-//             5 to 7 us, nearly all of it the latency of what it does one after the other.
+//             precede can only be among the k best if j + r < k, and must reach the best of eight bounds, each from the m-th entries of the ceil(k / m) lists
+//             with the best heads.  Some 2 k to 8 k entries are left; where that is many, the rank of 64 of them cuts them again.  Each then counts those before
+//             it.  5 to 8 us where k is 8 or 16, nearly all of it the latency of what it does one after the other.  Calls of 4 x 151936 in bf16 with k = 8, 64,
+//             128: 20, 29, 72 us (elementary torch operations 300), of 16 x 8 x 128261 with k = 16, 64, 128: 30, 39, 107; of that with k = 128 the keys of the
+//             rows are the most, whose bound is the least of 128 groups' maxima.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -41,6 +44,7 @@ constexpr int kGroupsPerWave = kGroups / kWaves;
 constexpr int kJoinThreads = 512;
 static_assert(kMaxTop <= kGroups && kMaxTop + 64 <= kWaveList && kMaxBeams <= kMaxLists && kMaxParts <= 64, "as in top_logits_kernels.hip; a part a lane");
 static_assert((kMaxBeams & (kMaxBeams - 1)) == 0, "a beam in the last bits of a total");
+static_assert(1 << (kJoinThreads / 64 - 1) >= kMaxTop, "a wave for each power of two up to k");
 
 // Of one part of a row: its largest logit, sum 2^((z - top) * scale2), how many keys it has found.
 struct PartSum {
@@ -256,8 +260,9 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
   __shared__ Candidate heads[kMaxLists];
   __shared__ double offset[kMaxBeams];  // score - log-sum-exp; not finite: the beam's total whatever the column
   __shared__ int have[kMaxLists], rank[kMaxLists];
-  __shared__ Candidate bound;
-  __shared__ int kept;
+  __shared__ Candidate bounds[kJoinThreads / 64];
+  __shared__ int precede[64];
+  __shared__ int kept, fewer;
   Candidate* const left = (Candidate*)dynamic;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t item = blockIdx.x, row0 = item * a.beams;
@@ -283,7 +288,8 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
     if (lane < parts) have[b * parts + lane] = off - off == 0.0 ? p.keys : lane == 0 ? each : 0;
     if (lane == 0) offset[b] = off;
   }
-  if (tid == 0) kept = 0, bound = Candidate{0, 0};
+  if (tid < 64) precede[tid] = 0;
+  if (tid == 0) kept = 0, fewer = 0;
   __syncthreads();
   auto total_of = [&](int beam, topkey_t key) {
     const double off = offset[beam];
@@ -299,12 +305,36 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
   for (int l = tid; l < lists; l += kJoinThreads) {
     const Candidate mine = heads[l];
     int r = 0;
+#pragma unroll 8
     for (int i = 0; i < lists; ++i) r += precedes(heads[i], mine) ? 1 : 0;
-    rank[l] = have[l] > 0 ? r : kMaxTop;
-    if (r == k - 1 && have[l] > 0) bound = mine;  // at most one: no two are equal
+    rank[l] = have[l] > 0 ? r : kMaxLists;
   }
   __syncthreads();
-  const Candidate least = bound;
+  // Wave w: the m-th entries of the s lists of the best heads, s m >= k.  k candidates reach the last of them.  (The heads of k lists alone, m = 1: 31 us
+  // instead of 30 for 16 x 8 x 128261 and k = 16, and no bound where there are fewer lists.)
+  {
+    const int s = 1 << wave < k ? 1 << wave : k, m = (k + s - 1) / s;
+    Candidate last{~0ull, ~0ull};
+    int deep = 0;  // lists that have an m-th entry
+    for (int l = lane; l < lists; l += 64) {
+      if (rank[l] >= s || have[l] < m) continue;
+      const Candidate c = candidate(l, m - 1, keys[(int64_t)l * each + m - 1]);
+      if (precedes(last, c)) last = c;
+      ++deep;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const Candidate c{__shfl_xor(last.first, o, 64), __shfl_xor(last.key, o, 64)};
+      if (precedes(last, c)) last = c;
+      deep += __shfl_xor(deep, o, 64);
+    }
+    if (lane == 0) bounds[wave] = deep == s ? last : Candidate{0, 0};
+  }
+  __syncthreads();
+  Candidate least = bounds[0];
+#pragma unroll
+  for (int w = 1; w < kJoinThreads / 64; ++w)
+    if (precedes(bounds[w], least)) least = bounds[w];
   for (int e = tid; e < lists * each; e += kJoinThreads) {
     const int l = e / each, j = e - l * each;
     if (j + rank[l] >= k || j >= have[l]) continue;
@@ -312,11 +342,37 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
     if (!precedes(least, c)) left[atomicAdd(&kept, 1)] = c;  // in any order: places depend on the candidates alone
   }
   __syncthreads();
-  const int n = kept;
+  int n = kept;
+  const Candidate* some = left;
+  // Many: of 64 of them the first that k - 1 precede is another bound, behind which about k + n / 64 are left.  They go where the heads were.
+  if (n > 2 * kMaxTop) {
+    const Candidate sample = left[(int)((int64_t)n * lane / 64)];
+    int before = 0;
+#pragma unroll 8
+    for (int i = wave; i < n; i += kJoinThreads / 64) before += precedes(left[i], sample) ? 1 : 0;
+    atomicAdd(&precede[lane], before);
+    __syncthreads();
+    int b = precede[lane] >= k - 1 ? precede[lane] : 0x7fffffff, at = lane;  // of the sample with the fewest before it, k - 1 or more
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const int b1 = __shfl_xor(b, o, 64), at1 = __shfl_xor(at, o, 64);
+      if (b1 < b || (b1 == b && at1 < at)) b = b1, at = at1;
+    }
+    if (b < kMaxLists) {  // b + 1 are left
+      const Candidate last = left[(int)((int64_t)n * at / 64)];
+      for (int e = tid; e < n; e += kJoinThreads) {
+        const Candidate c = left[e];
+        if (!precedes(last, c)) heads[atomicAdd(&fewer, 1)] = c;
+      }
+      __syncthreads();
+      some = heads, n = b + 1;
+    }
+  }
   for (int e = tid; e < n; e += kJoinThreads) {
-    const Candidate mine = left[e];
+    const Candidate mine = some[e];
     int place = 0;
-    for (int i = 0; i < n; ++i) place += precedes(left[i], mine) ? 1 : 0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) place += precedes(some[i], mine) ? 1 : 0;
     if (place < k) {
       const int64_t at = item * k + place;
       const int b = beam_of(mine);
