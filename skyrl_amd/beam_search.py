@@ -231,7 +231,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
 
     ``out``: tensors to write, new ones without it.  ``out=states`` reorders in place (``B_out == B_in``, at most 128 beams): rows that keep their place
     are not moved.  A result is otherwise in memory of its own: one that may share an element with another result, with a state but the one that it is, or with
-    ``parents`` is refused.  Views of one buffer that interleave without sharing an element are told apart.  Not differentiable."""
+    ``parents`` is refused.  Views of one buffer that interleave without sharing an element are told apart.  Not differentiable, and no op that tracing sees: it
+    works on addresses, so a compiled program is left for the call and goes on behind it."""
     states = list(states)
     if parents.dim() != 2:
         raise ValueError(f"expected parents [N, B], got {tuple(parents.shape)}")

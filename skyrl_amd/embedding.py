@@ -181,7 +181,8 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, *, scale: float = 
 def embedding_backward_accumulate(d_out: torch.Tensor, ids: torch.Tensor, d_weight_accum: torch.Tensor, *, scale: float = 1.0,
                                   padding_idx: Optional[int] = None) -> torch.Tensor:
     """Adds the gradient of ``embedding_lookup`` for the upstream gradient ``d_out`` (``ids.shape + (H,)``, bf16 or fp32) into ``d_weight_accum``, a
-    contiguous fp32 ``[V, H]`` buffer, and returns it.  Rows that no token names are neither read nor written."""
+    contiguous fp32 ``[V, H]`` buffer, and returns it.  Rows that no token names are neither read nor written.  It works on addresses: a compiled program is
+    left for the call and goes on behind it."""
     if d_weight_accum.dim() != 2 or d_weight_accum.dtype != torch.float32 or not d_weight_accum.is_contiguous():
         raise ValueError(f"d_weight_accum must be a contiguous fp32 matrix [V, H], got {d_weight_accum.dtype} {tuple(d_weight_accum.shape)}")
     if tuple(d_out.shape) != tuple(ids.shape) + (d_weight_accum.shape[1],):
