@@ -178,10 +178,19 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, *, scale: float = 
     return rows if flat is ids else rows.reshape(ids.shape + (weight.shape[1],))
 
 
+def _meets(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the ranges of addresses of two tensors meet."""
+    def reach(t):
+        begin = t.data_ptr()
+        return begin, begin + (t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) if t.numel() else 0)
+    (a0, a1), (b0, b1) = reach(a), reach(b)
+    return a0 < b1 and b0 < a1
+
+
 def embedding_backward_accumulate(d_out: torch.Tensor, ids: torch.Tensor, d_weight_accum: torch.Tensor, *, scale: float = 1.0,
                                   padding_idx: Optional[int] = None) -> torch.Tensor:
     """Adds the gradient of ``embedding_lookup`` for the upstream gradient ``d_out`` (``ids.shape + (H,)``, bf16 or fp32) into ``d_weight_accum``, a
-    contiguous fp32 ``[V, H]`` buffer, and returns it.  Rows that no token names are neither read nor written.  It works on addresses: a compiled program is
+    contiguous fp32 ``[V, H]`` buffer in memory of its own, and returns it.  Rows that no token names are neither read nor written.  It works on addresses: a compiled program is
     left for the call and goes on behind it."""
     if d_weight_accum.dim() != 2 or d_weight_accum.dtype != torch.float32 or not d_weight_accum.is_contiguous():
         raise ValueError(f"d_weight_accum must be a contiguous fp32 matrix [V, H], got {d_weight_accum.dtype} {tuple(d_weight_accum.shape)}")
@@ -192,6 +201,8 @@ def embedding_backward_accumulate(d_out: torch.Tensor, ids: torch.Tensor, d_weig
         raise ValueError("d_weight_accum is written in place and takes no gradient itself")
     rows = _walkable(d_out.detach().resolve_neg().reshape(flat.shape[0], d_weight_accum.shape[1]))
     _check_gradient(rows, flat)
+    if _meets(rows, d_weight_accum) or _meets(flat, d_weight_accum):
+        raise ValueError("d_weight_accum shares memory with d_out or the ids: it would be written while they are read")
     _require_device(rows, flat, d_weight_accum)
     if rows.numel() and d_weight_accum.numel():
         _backward_into(rows, flat, scale, padding_idx, d_weight_accum, 1)
