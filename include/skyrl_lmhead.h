@@ -579,10 +579,10 @@ int skyrl_lmhead_embedding_bwd(const void* dout, int dtype, int64_t ld_dout, con
  * 1 <= k <= min(beams * V, SKYRL_LOGITS_TOP_MAX), beams <= SKYRL_LOGITS_BEAMS_MAX, items * beams <= 2^22.  workspace: 8-byte aligned.
  *
  * skyrl_logits_beam_reorder: row j of item i (of beams_out) of each of `count` tensors becomes row parents[i, j] of that item (of beams_in); zeros where
- * the parent lies outside [0, beams_in).  A row is `segments` pieces of `bytes` contiguous bytes: tensor t's at from[t] + (i * beams_in + parent) *
+ * the parent lies outside [0, beams_in).  A row is `segments` segments of `bytes` contiguous bytes: tensor t's at from[t] + (i * beams_in + parent) *
  * from_row + s * from_segment, written to to[t] + (i * beams_out + j) * to_row + s * to_segment; strides in bytes.  from and to are host arrays of
- * at most SKYRL_LOGITS_STATES_MAX device pointers, read before the call returns.  `bytes` below 2^31 (of strides and addresses that are multiples of 4 or 16:
- * 2^31 such units); what one grid does not hold takes several launches.  In place, to[t] == from[t] for every t with the same strides
+ * at most SKYRL_LOGITS_STATES_MAX device pointers, read before the call returns.  Any
+ * alignment; `bytes` below 2^35; what one grid does not hold takes several launches.  In place, to[t] == from[t] for every t with the same strides
  * and beams_in == beams_out <= SKYRL_LOGITS_BEAMS_MAX, rows that keep their place are neither read nor written for that; otherwise the two must not overlap. */
 #define SKYRL_LOGITS_BEAMS_MAX 128
 #define SKYRL_LOGITS_STATES_MAX 200

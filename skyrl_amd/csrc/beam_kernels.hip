@@ -384,9 +384,11 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(const BeamArgs a, int 
 }
 
 // ------------------------------------------------------------------------------------------------------------
-// The states of the beams, rows [items * beams] of `segments` pieces of `bytes` contiguous bytes each: row j of an item becomes its row
+// The states of the beams, rows [items * beams] of `segments` segments of `bytes` contiguous bytes each: row j of an item becomes its row
 // parents[j].  One launch for all tensors of a layout.  Bound by HBM; rows that several beams take are read from the caches.
-// 16 x 8 rows of 4 MiB: 153 us (read and written 1.07 GB: 7.0 TB/s), in place, where rows that stay are left, 164.
+// 16 x 8 rows of 4 MiB: 153 us (read and written 1.07 GB: 7.0 TB/s), in place, where rows that stay are left, 164.  16 tensors of 16 x 8 rows, 1.05 GB, as
+// segments of 128000 bytes 271 us, of 256 (a transposed cache) 315 (3020 with a workgroup a segment), of 81162 in bf16 at any place 203 us for half as much
+// (1040 a byte a lane).
 // ------------------------------------------------------------------------------------------------------------
 constexpr int kStates = SKYRL_LOGITS_STATES_MAX;
 // Pieces that a thread has in flight.  A copy of 64 rows of 4 MiB: 78 us with one or two, 80 with four, 130 with eight.
@@ -401,49 +403,95 @@ struct ReorderArgs {
   int64_t from_row, from_segment, to_row, to_segment;  // bytes
   const int64_t* parents;  // [items, beams_out]
   int beams_in, beams_out;
-  uint32_t segments, pieces;  // of a row, of a segment
-  uint32_t blocks;            // workgroups of a segment
+  uint32_t all, pieces;    // pieces of a row, below 2^31, and of a segment
+  uint32_t last;           // bytes of a segment's last piece
+  uint32_t magic, shift;   // p / pieces is p * magic >> shift
+  uint32_t blocks;         // workgroups of a row
 };
 
-template <class Unit>
-__device__ __forceinline__ Unit nothing() {
-  if constexpr (sizeof(Unit) == 16) return Unit{0, 0, 0, 0};
-  else return Unit{0};
-}
+// Sixteen bytes of a segment, whose begin, end and neighbours are multiples of G bytes; or the fewer that it ends with.
+template <int G>
+struct Piece16 {
+  struct __attribute__((packed, aligned(G))) Whole {
+    u32x4 v;
+  };
+  static __device__ __forceinline__ u32x4 load(const char* from, uint32_t bytes) {
+    if (G == 16 || bytes == 16) return ((const Whole*)from)->v;
+    u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16 / G; ++i) {
+      if (i * G >= (int)bytes) break;
+      if constexpr (G == 4) w[i] = ((const uint32_t*)from)[i];
+      if constexpr (G == 2) w[i / 2] |= (uint32_t)((const uint16_t*)from)[i] << (16 * (i % 2));
+      if constexpr (G == 1) w[i / 4] |= (uint32_t)((const uint8_t*)from)[i] << (8 * (i % 4));
+    }
+    return w;
+  }
+  static __device__ __forceinline__ void store(char* to, uint32_t bytes, const u32x4& w) {
+    if (G == 16 || bytes == 16) {
+      ((Whole*)to)->v = w;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / G; ++i) {
+      if (i * G >= (int)bytes) break;
+      if constexpr (G == 4) ((uint32_t*)to)[i] = w[i];
+      if constexpr (G == 2) ((uint16_t*)to)[i] = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+      if constexpr (G == 1) ((uint8_t*)to)[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+  }
+};
 
-template <class Unit>
+// Where piece p of a row lies: its segment, its place in that in bytes and how many it has.  Pieces are numbered through the segments, so that a workgroup has
+// as much to do where they are short.
+struct Place {
+  int64_t segment, at;
+  uint32_t bytes;
+  __device__ __forceinline__ Place(const ReorderArgs& a, uint32_t p) {
+    const uint32_t q = (uint32_t)(((uint64_t)p * a.magic) >> a.shift), r = p - q * a.pieces;
+    segment = q, at = (int64_t)r * 16, bytes = r + 1 == a.pieces ? a.last : 16u;
+  }
+};
+
+template <int G>
 __global__ __launch_bounds__(kCopyThreads) void beam_copy(const ReorderArgs a) {
-  const uint32_t in_row = a.segments * a.blocks, row = blockIdx.x / in_row, rest = blockIdx.x - row * in_row;
-  const uint32_t segment = rest / a.blocks, block = rest - segment * a.blocks;
+  const uint32_t row = blockIdx.x / a.blocks, block = blockIdx.x - row * a.blocks;
   const uint32_t item = row / (uint32_t)a.beams_out;
   const int64_t parent = a.parents[row];
   const bool has = parent >= 0 && parent < a.beams_in;
-  const Unit* from = (const Unit*)(a.from[blockIdx.y] + ((int64_t)item * a.beams_in + (has ? parent : 0)) * a.from_row + (int64_t)segment * a.from_segment);
-  Unit* to = (Unit*)(a.to[blockIdx.y] + (int64_t)row * a.to_row + (int64_t)segment * a.to_segment);
+  const char* const from = a.from[blockIdx.y] + ((int64_t)item * a.beams_in + (has ? parent : 0)) * a.from_row;
+  char* const to = a.to[blockIdx.y] + (int64_t)row * a.to_row;
   const uint32_t p0 = block * (kCopyThreads * kCopyPieces) + threadIdx.x;
-  Unit w[kCopyPieces];
+  u32x4 w[kCopyPieces];
 #pragma unroll
   for (int u = 0; u < kCopyPieces; ++u) {
     const uint32_t p = p0 + u * kCopyThreads;
-    w[u] = nothing<Unit>();
-    if (has && p < a.pieces) w[u] = from[p];
+    w[u] = u32x4{0, 0, 0, 0};
+    if (has && p < a.all) {
+      const Place x(a, p);
+      w[u] = Piece16<G>::load(from + x.segment * a.from_segment + x.at, x.bytes);
+    }
   }
 #pragma unroll
-  for (int u = 0; u < kCopyPieces; ++u)
-    if (p0 + u * kCopyThreads < a.pieces) to[p0 + u * kCopyThreads] = w[u];
+  for (int u = 0; u < kCopyPieces; ++u) {
+    const uint32_t p = p0 + u * kCopyThreads;
+    if (p < a.all) {
+      const Place x(a, p);
+      Piece16<G>::store(to + x.segment * a.to_segment + x.at, x.bytes, w[u]);
+    }
+  }
 }
 
 // In place: a thread reads one piece of all beams of an item into LDS before it writes any.  Rows that stay are not written, and those that no
 // other beam takes not read.
-template <class Unit>
+template <int G>
 __global__ __launch_bounds__(kCopyThreads) void beam_permute(const ReorderArgs a) {
   extern __shared__ __attribute__((aligned(16))) char dynamic[];
   __shared__ int parent[kMaxBeams];
   __shared__ int wanted[kMaxBeams];
   __shared__ int source[kMaxBeams];  // the beams that are wanted, one behind the other
   __shared__ int sources;
-  const uint32_t in_row = a.segments * a.blocks, item = blockIdx.x / in_row, rest = blockIdx.x - item * in_row;
-  const uint32_t segment = rest / a.blocks, block = rest - segment * a.blocks;
+  const uint32_t item = blockIdx.x / a.blocks, block = blockIdx.x - item * a.blocks;
   const int beams = a.beams_in;
   for (int b = threadIdx.x; b < beams; b += blockDim.x) wanted[b] = 0;
   __syncthreads();
@@ -466,15 +514,16 @@ __global__ __launch_bounds__(kCopyThreads) void beam_permute(const ReorderArgs a
   }
   __syncthreads();
   const uint32_t p = block * blockDim.x + threadIdx.x;
-  if (p >= a.pieces) return;
-  char* const base = a.to[blockIdx.y] + (int64_t)item * beams * a.to_row + (int64_t)segment * a.to_segment + (int64_t)p * (int64_t)sizeof(Unit);
-  Unit* const mine = (Unit*)dynamic + threadIdx.x;
+  if (p >= a.all) return;
+  const Place x(a, p);
+  char* const base = a.to[blockIdx.y] + (int64_t)item * beams * a.to_row + x.segment * a.to_segment + x.at;
+  u32x4* const mine = (u32x4*)dynamic + threadIdx.x;
   const int n = __builtin_amdgcn_readfirstlane(sources);
   for (int i = 0; i < n; i += kHeldPieces) {
-    Unit w[kHeldPieces];
+    u32x4 w[kHeldPieces];
 #pragma unroll
     for (int u = 0; u < kHeldPieces; ++u)
-      if (i + u < n) w[u] = *(const Unit*)(base + (int64_t)source[i + u] * a.to_row);
+      if (i + u < n) w[u] = Piece16<G>::load(base + (int64_t)source[i + u] * a.to_row, x.bytes);
 #pragma unroll
     for (int u = 0; u < kHeldPieces; ++u)
       if (i + u < n) mine[source[i + u] * blockDim.x] = w[u];
@@ -483,7 +532,7 @@ __global__ __launch_bounds__(kCopyThreads) void beam_permute(const ReorderArgs a
   for (int b = 0; b < beams; ++b) {
     const int from = parent[b];
     if (from == b) continue;
-    *(Unit*)(base + (int64_t)b * a.to_row) = from < 0 ? nothing<Unit>() : mine[from * blockDim.x];
+    Piece16<G>::store(base + (int64_t)b * a.to_row, x.bytes, from < 0 ? u32x4{0, 0, 0, 0} : mine[from * blockDim.x]);
   }
 }
 
@@ -510,36 +559,41 @@ bool beam_extents(int64_t items, int64_t beams, int64_t V, int64_t k) {
 }
 
 // A launch for as many rows as one grid holds (2^32 threads), or as many segments of one row.
-template <class Unit>
-int launch_reorder(hipStream_t s, const ReorderArgs& all, int64_t items, int64_t bytes, int count, bool in_place) {
-  const int64_t pieces = bytes / (int64_t)sizeof(Unit);
+template <int G>
+int launch_reorder(hipStream_t s, const ReorderArgs& whole, int64_t items, int64_t segments, int64_t bytes, int count, bool in_place) {
+  const int64_t pieces = (bytes + 15) / 16;
+  if (pieces >= ((int64_t)1 << 31)) return SKYRL_LMHEAD_ERR_SHAPE;
   int threads = kCopyThreads;
   if (in_place)  // two workgroups a CU, but for 128 beams.  (One: within 4 % for 32 and 64 beams.)
-    while (threads > 64 && (size_t)all.beams_in * threads * sizeof(Unit) > 65536) threads /= 2;
-  const int64_t each = in_place ? threads : kCopyThreads * kCopyPieces, blocks = (pieces + each - 1) / each;
+    while (threads > 64 && (size_t)whole.beams_in * threads * 16 > 65536) threads /= 2;
+  const int64_t each = in_place ? threads : kCopyThreads * kCopyPieces;
   const int64_t most = (((int64_t)1 << 32) - 1) / threads;  // workgroups
-  if (pieces >= ((int64_t)1 << 31)) return SKYRL_LMHEAD_ERR_SHAPE;
-  const int64_t per_launch = most / blocks;  // segments
-  const int64_t segments = all.segments < per_launch ? all.segments : per_launch;
-  const int64_t rows = per_launch / segments;                                        // in place: items
-  const int64_t step_items = in_place ? rows : (rows >= all.beams_out ? rows / all.beams_out : 1);
-  const int64_t step_beams = in_place || rows >= all.beams_out ? all.beams_out : rows;  // of an item, where a launch has part of one
+  int log = 0;
+  while (((int64_t)1 << log) < pieces) ++log;
+  const int64_t most_segments = (((int64_t)1 << 31) - 1) / pieces, step_segments = segments < most_segments ? segments : most_segments;
+  const int64_t blocks = (step_segments * pieces + each - 1) / each, rows = most / blocks;  // of a launch; 2^31 pieces are 2^23 or 2^25 workgroups
+  const int64_t step_items = in_place ? rows : (rows >= whole.beams_out ? rows / whole.beams_out : 1);
+  const int64_t step_beams = in_place || rows >= whole.beams_out ? whole.beams_out : rows;  // of an item, where a launch has part of one
   for (int64_t item = 0; item < items; item += step_items)
-    for (int64_t beam = 0; beam < all.beams_out; beam += step_beams)
-      for (int64_t segment = 0; segment < all.segments; segment += segments) {
-        ReorderArgs a = all;
-        const int64_t n_items = items - item < step_items ? items - item : step_items, n_beams = all.beams_out - beam < step_beams ? all.beams_out - beam : step_beams;
+    for (int64_t beam = 0; beam < whole.beams_out; beam += step_beams)
+      for (int64_t segment = 0; segment < segments; segment += step_segments) {
+        ReorderArgs a = whole;
+        const int64_t n_items = items - item < step_items ? items - item : step_items;
+        const int64_t n_beams = whole.beams_out - beam < step_beams ? whole.beams_out - beam : step_beams;
+        const int64_t n_segments = segments - segment < step_segments ? segments - segment : step_segments;
         for (int t = 0; t < count; ++t) {
-          a.from[t] += item * all.beams_in * all.from_row + segment * all.from_segment;
-          a.to[t] += (item * all.beams_out + beam) * all.to_row + segment * all.to_segment;
+          a.from[t] += item * whole.beams_in * whole.from_row + segment * whole.from_segment;
+          a.to[t] += (item * whole.beams_out + beam) * whole.to_row + segment * whole.to_segment;
         }
-        a.parents += item * all.beams_out + beam;
+        a.parents += item * whole.beams_out + beam;
         a.beams_out = (int)n_beams;
-        a.segments = (uint32_t)(all.segments - segment < segments ? all.segments - segment : segments);
-        a.pieces = (uint32_t)pieces, a.blocks = (uint32_t)blocks;
-        const dim3 grid((unsigned)(blocks * a.segments * (in_place ? n_items : n_items * n_beams)), (unsigned)count);
-        if (in_place) hipLaunchKernelGGL(beam_permute<Unit>, grid, dim3((unsigned)threads), (size_t)a.beams_in * threads * sizeof(Unit), s, a);
-        else hipLaunchKernelGGL(beam_copy<Unit>, grid, dim3(kCopyThreads), 0, s, a);
+        a.all = (uint32_t)(n_segments * pieces), a.pieces = (uint32_t)pieces, a.last = (uint32_t)(bytes - (pieces - 1) * 16);
+        // magic = 2^(31 + log) / pieces, rounded up, is too large by less than one part in 2^31, which no p < 2^31 sees.
+        a.magic = (uint32_t)((((uint64_t)1 << (31 + log)) + (uint64_t)pieces - 1) / (uint64_t)pieces), a.shift = (uint32_t)(31 + log);
+        a.blocks = (uint32_t)((n_segments * pieces + each - 1) / each);
+        const dim3 grid((unsigned)(a.blocks * (in_place ? n_items : n_items * n_beams)), (unsigned)count);
+        if (in_place) hipLaunchKernelGGL(beam_permute<G>, grid, dim3((unsigned)threads), (size_t)a.beams_in * threads * 16, s, a);
+        else hipLaunchKernelGGL(beam_copy<G>, grid, dim3(kCopyThreads), 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
       }
@@ -609,11 +663,12 @@ int skyrl_logits_beam_reorder(const void* const* from, void* const* to, int64_t 
     all |= (uintptr_t)from[i] | (uintptr_t)to[i];
   }
   a.from_row = from_row, a.from_segment = from_segment, a.to_row = to_row, a.to_segment = to_segment;
-  a.parents = parents, a.beams_in = (int)beams_in, a.beams_out = (int)beams_out, a.segments = (uint32_t)segments;
+  a.parents = parents, a.beams_in = (int)beams_in, a.beams_out = (int)beams_out;
   hipStream_t s = (hipStream_t)stream;
-  if (all % 16 == 0) return launch_reorder<u32x4>(s, a, items, bytes, (int)count, in_place);
-  if (all % 4 == 0) return launch_reorder<uint32_t>(s, a, items, bytes, (int)count, in_place);
-  return launch_reorder<uint8_t>(s, a, items, bytes, (int)count, in_place);
+  if (all % 16 == 0) return launch_reorder<16>(s, a, items, segments, bytes, (int)count, in_place);
+  if (all % 4 == 0) return launch_reorder<4>(s, a, items, segments, bytes, (int)count, in_place);
+  if (all % 2 == 0) return launch_reorder<2>(s, a, items, segments, bytes, (int)count, in_place);
+  return launch_reorder<1>(s, a, items, segments, bytes, (int)count, in_place);
 }
 
 }  // extern "C"
