@@ -134,6 +134,40 @@ def _folded(shape: Tuple[int, ...], strides: Tuple[int, ...]) -> bool:
     return False
 
 
+def _in_memory_order(shape: Tuple[int, ...], strides: Tuple[int, ...], to_strides: Tuple[int, ...]) -> Tuple[Tuple[int, ...], ...]:
+    """The dimensions of a row as the result has them in memory, outer first, which is where neighbours join; of several that do not, the longest is next to the
+    contiguous run, so that taking the others apart makes the fewest parts."""
+    dims: List[Tuple[int, int, int]] = []
+    for y, x, n in sorted(((y, x, n) for n, x, y in zip(shape, strides, to_strides) if n != 1), reverse=True):
+        if dims and dims[-1][1] == n * x and dims[-1][2] == n * y:
+            dims[-1] = (dims[-1][0] * n, x, y)
+        else:
+            dims.append((n, x, y))
+    run = [dims.pop()] if dims and dims[-1][1] == dims[-1][2] == 1 else []
+    dims.sort(key=lambda d: d[0])
+    return tuple(zip(*dims, *run)) or ((), (), ())
+
+
+@functools.lru_cache(maxsize=256)
+def _dense_order(shape: Tuple[int, ...], strides: Tuple[int, ...]) -> Optional[Tuple[int, ...]]:
+    """The order of a state's dimensions in which its rows are closest to one run of memory: None if that is their own."""
+    order = (0, *sorted(range(1, len(shape)), key=lambda i: -strides[i] if shape[i] != 1 else 0))
+    moving = [i for i in order if i == 0 or shape[i] != 1]
+    return None if moving == sorted(moving) else order
+
+
+def _new_result(state: torch.Tensor, rows: int) -> torch.Tensor:
+    """Dense, with the dimensions of a row in the order that they have in the state's memory."""
+    shape = state.shape
+    order = _dense_order(shape, state.stride()) if len(shape) > 2 else None
+    if order is None:
+        return state.new_empty((rows,) + tuple(shape[1:]))
+    back = [0] * len(order)
+    for at, i in enumerate(order):
+        back[i] = at
+    return state.new_empty([rows] + [shape[i] for i in order[1:]]).permute(back)
+
+
 class _Reach(NamedTuple):
     """Where the elements of a tensor lie, from its address on, in bytes."""
 
@@ -172,7 +206,7 @@ def _layout(shape: Tuple[int, ...], strides: Tuple[int, ...], to_strides: Tuple[
     to_row = to_strides[0] * size if to_shape[0] > 1 else 0
     found: dict = {}
     if 0 not in to_shape:
-        for at, to_at, n, nbytes, step, to_step in _segments(tuple(shape[1:]), strides[1:], to_strides[1:], size):
+        for at, to_at, n, nbytes, step, to_step in _segments(*_in_memory_order(shape[1:], strides[1:], to_strides[1:]), size):
             found.setdefault((row, step, to_row, to_step, n, nbytes), []).append((at, to_at))
     return _Layout(rows // items if items else 0, to_shape, _reach(shape, strides, size), _reach(to_shape, to_strides, size),
                    _folded(to_shape, to_strides), tuple((sizes, tuple(places)) for sizes, places in found.items()))
@@ -229,7 +263,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
     """Row ``n * B_out + j`` of each result is row ``n * B_in + parents[n, j]`` of its state, for states ``[N * B_in, ...]`` of any types and strides
     (the used part of a cache, say) and ``parents [N, B_out]`` int64; zeros where a parent lies outside ``[0, B_in)``.
 
-    ``out``: tensors to write, new ones without it.  ``out=states`` reorders in place (``B_out == B_in``, at most 128 beams): rows that keep their place
+    ``out``: tensors to write; without it new ones, dense, their rows' dimensions in memory as the states have them.  ``out=states`` reorders in place (``B_out == B_in``, at most 128 beams): rows that keep their place
     are not moved.  A result is otherwise in memory of its own: one that may share an element with another result, with a state but the one that it is, or with
     ``parents`` is refused.  Views of one buffer that interleave without sharing an element are told apart.  Not differentiable, and no op that tracing sees: it
     works on addresses, so a compiled program is left for the call and goes on behind it."""
@@ -245,7 +279,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         if len(results) != len(states):
             raise ValueError(f"{len(results)} results for {len(states)} states")
     else:
-        results = [t.new_empty((N * B_out,) + tuple(t.shape[1:])) for t in states]
+        results = [_new_result(t, N * B_out) for t in states]
     if not states:
         return results
     if torch.is_grad_enabled() and any([t.requires_grad for t in states + results]) or has_tangent(*states):
