@@ -49,13 +49,14 @@ def plain_eager() -> bool:
     return not (dispatch_modes() > 0 or function_modes() > 0 or transform() is not None or tracing() or profiling())
 
 
-def direct(*args) -> bool:
+def direct(*args, recorded: bool = False) -> bool:
     """Whether a registered function may be given these arguments itself: a plain eager call on real tensors, without a gradient to
-    record.  Not so for tensor subclasses, tensors on the meta device and those whose memory is not their value (negative views, such
-    as the imaginary part of a conjugate, and autograd's zero tensors, which have none)."""
+    record (``recorded``: whatever records it is the caller's own).  Not so for tensor subclasses, tensors on the meta device and those
+    whose memory is not their value (negative views, such as the imaginary part of a conjugate, and autograd's zero tensors, which have
+    none)."""
     if not plain_eager():
         return False
-    grad = torch.is_grad_enabled()
+    grad = not recorded and torch.is_grad_enabled()
     for a in args:
         if isinstance(a, torch.Tensor) and (type(a) not in _PLAIN or a.is_meta or (grad and a.requires_grad) or a.is_neg()
                                             or a._is_zerotensor()):

@@ -7,6 +7,8 @@ been built, or the symbol table does not match the header, loading raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
@@ -193,6 +195,31 @@ def load() -> ctypes.CDLL:
             raise LmHeadLibraryError(f"{_LIB_PATH} has ABI version {got}, this package expects {ABI_VERSION}; rebuild it")
         _lib = lib
         return lib
+
+
+_NODE_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "lookup_node.so")
+_node = None
+
+
+def load_node():
+    """Load (once) and return the autograd node of the embedding lookup, bound to the library.  Raises LmHeadLibraryError when it is not built."""
+    global _node
+    if _node is not None:
+        return _node
+    lib = load()
+    with _lock:
+        if _node is not None:
+            return _node
+        if not os.path.exists(_NODE_PATH):
+            raise LmHeadLibraryError(f"{_NODE_PATH} is not built. Run `python -m skyrl_amd.csrc.build` (needs hipcc and g++).")
+        loader = importlib.machinery.ExtensionFileLoader("lookup_node", _NODE_PATH)
+        spec = importlib.util.spec_from_file_location("lookup_node", _NODE_PATH, loader=loader)
+        node = importlib.util.module_from_spec(spec)
+        loader.exec_module(node)
+        node.bind(*[ctypes.cast(fn, ctypes.c_void_p).value for fn in (lib.skyrl_lmhead_embedding_fwd, lib.skyrl_lmhead_embedding_bwd,
+                                                                       lib.skyrl_lmhead_embedding_bwd_workspace_bytes, lib.skyrl_lmhead_strerror)])
+        _node = node
+        return node
 
 
 def strerror(status: int) -> str:

@@ -47,16 +47,6 @@ def lmhead_embedding_fwd(weight: torch.Tensor, ids: torch.Tensor, scale: float) 
     """``[T, H]`` in the table's dtype."""
     _check_table(weight)
     _check_ids(ids)
-    return _rows_of(weight, ids, scale)
-
-
-@lmhead_embedding_fwd.register_fake
-def _(weight, ids, scale):
-    return weight.new_empty((ids.shape[0], weight.shape[1]))
-
-
-def _rows_of(weight: torch.Tensor, ids: torch.Tensor, scale: float) -> torch.Tensor:
-    """The rows, of operands that have been checked but for their device."""
     dev = _require_device(weight, ids)
     (V, H), T = weight.shape, ids.shape[0]
     out = torch.empty((T, H), dtype=weight.dtype, device=dev)
@@ -69,6 +59,11 @@ def _rows_of(weight: torch.Tensor, ids: torch.Tensor, scale: float) -> torch.Ten
                                                     out.data_ptr(), raw_stream(dev))
     _lib.check(st, "skyrl_lmhead_embedding_fwd")
     return out
+
+
+@lmhead_embedding_fwd.register_fake
+def _(weight, ids, scale):
+    return weight.new_empty((ids.shape[0], weight.shape[1]))
 
 
 def _backward_into(d_out: torch.Tensor, ids: torch.Tensor, scale: float, padding_idx: int, d_weight: torch.Tensor, accumulate: int) -> None:
@@ -100,11 +95,6 @@ def lmhead_embedding_bwd(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, sca
     _check_gradient(d_out, ids)
     if vocab < 0:
         raise ValueError(f"a table of {vocab} rows")
-    return _gradient_of(d_out, ids, vocab, scale, padding_idx)
-
-
-def _gradient_of(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float, padding_idx: int) -> torch.Tensor:
-    """The gradient, of operands that have been checked but for their device."""
     dev = _require_device(d_out, ids)
     T, H = d_out.shape
     if T == 0 or H == 0 or vocab == 0:
@@ -120,19 +110,18 @@ def _(d_out, ids, vocab, scale, padding_idx):
 
 
 class _Lookup(torch.autograd.Function):
+    """What csrc/lookup_node.cpp is to a plain eager call: the same over the ops, where anything follows the call."""
+
     @staticmethod
     def forward(ctx, weight, ids, scale, padding_idx):
         ctx.save_for_backward(ids)
         ctx.rest = (weight.shape[0], scale, padding_idx)
-        # Checked by embedding_lookup; the op, which checks for itself, where anything follows the call.
-        return _rows_of(weight, ids, scale) if direct(weight, ids) else lmhead_embedding_fwd(weight, ids, scale)
+        return lmhead_embedding_fwd(weight, ids, scale)
 
     @staticmethod
     def backward(ctx, d_out):
         (ids,) = ctx.saved_tensors
-        d_out = _walkable(d_out)
-        d_weight = _gradient_of(d_out, ids, *ctx.rest) if direct(d_out, ids) else lmhead_embedding_bwd(d_out, ids, *ctx.rest)
-        return d_weight, None, None, None
+        return lmhead_embedding_bwd(_walkable(d_out), ids, *ctx.rest), None, None, None
 
 
 def _walkable(rows: torch.Tensor) -> torch.Tensor:
@@ -171,8 +160,13 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, *, scale: float = 
     either, as in ``torch.nn.functional.embedding``.  The gradient is dense, ``[V, H]`` in the table's dtype.  At most 2^24 tokens."""
     _check_table(weight)
     flat, scale, padding_idx = _flat_ids(ids), _scale_of(scale), _padding_of(padding_idx, weight.shape[0])
-    if torch.is_grad_enabled() and weight.requires_grad or has_tangent(weight):
-        rows = _Lookup.apply(weight, flat, scale, padding_idx)
+    tangent = has_tangent(weight)
+    if torch.is_grad_enabled() and weight.requires_grad or tangent:
+        if direct(weight, flat, recorded=True) and not tangent:
+            _require_device(weight, flat)
+            rows = _lib.load_node().lookup(weight, flat, scale, padding_idx)
+        else:
+            rows = _Lookup.apply(weight, flat, scale, padding_idx)
     else:
         rows = call(lmhead_embedding_fwd, weight, flat, scale)
     return rows if flat is ids else rows.reshape(ids.shape + (weight.shape[1],))
