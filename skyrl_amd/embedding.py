@@ -91,7 +91,9 @@ def _check_gradient(d_out: torch.Tensor, ids: torch.Tensor) -> None:
 
 @registered_op("skyrl_amd::lmhead_embedding_bwd", mutates_args=())
 def lmhead_embedding_bwd(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float, padding_idx: int) -> torch.Tensor:
-    """``d_weight [vocab, H]`` in the dtype of ``d_out [T, H]``; ``padding_idx``: -1 where there is none."""
+    """``d_weight [vocab, H]`` in the dtype of ``d_out [T, H]``, of whatever strides; ``padding_idx``: -1 where there is none."""
+    if d_out.dim() == 2:
+        d_out = _walkable(d_out)
     _check_gradient(d_out, ids)
     if vocab < 0:
         raise ValueError(f"a table of {vocab} rows")
@@ -121,7 +123,7 @@ class _Lookup(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_out):
         (ids,) = ctx.saved_tensors
-        return lmhead_embedding_bwd(_walkable(d_out), ids, *ctx.rest), None, None, None
+        return lmhead_embedding_bwd(d_out, ids, *ctx.rest), None, None, None
 
 
 def _walkable(rows: torch.Tensor) -> torch.Tensor:
