@@ -148,26 +148,6 @@ def _in_memory_order(shape: Tuple[int, ...], strides: Tuple[int, ...], to_stride
     return tuple(zip(*dims, *run)) or ((), (), ())
 
 
-@functools.lru_cache(maxsize=256)
-def _dense_order(shape: Tuple[int, ...], strides: Tuple[int, ...]) -> Optional[Tuple[int, ...]]:
-    """The order of a state's dimensions in which its rows are closest to one run of memory: None if that is their own."""
-    order = (0, *sorted(range(1, len(shape)), key=lambda i: -strides[i] if shape[i] != 1 else 0))
-    moving = [i for i in order if i == 0 or shape[i] != 1]
-    return None if moving == sorted(moving) else order
-
-
-def _new_result(state: torch.Tensor, rows: int) -> torch.Tensor:
-    """Dense, with the dimensions of a row in the order that they have in the state's memory."""
-    shape = state.shape
-    order = _dense_order(shape, state.stride()) if len(shape) > 2 else None
-    if order is None:
-        return state.new_empty((rows,) + tuple(shape[1:]))
-    back = [0] * len(order)
-    for at, i in enumerate(order):
-        back[i] = at
-    return state.new_empty([rows] + [shape[i] for i in order[1:]]).permute(back)
-
-
 class _Reach(NamedTuple):
     """Where the elements of a tensor lie, from its address on, in bytes."""
 
@@ -245,25 +225,25 @@ def _clash(regions: list) -> bool:
             return False
         for i, turn in enumerate(moduli):
             spans = {}
-            for reach in {r[2] for r in some}:
+            for reach in {id(r[2]): r[2] for r in some}.values():  # few, of many regions
                 span = reach.size + sum(s * (n - 1) for s, n in reach.steps if s < turn)
                 if span > turn or any(s >= turn and s % turn for s, _ in reach.steps):
                     break
-                spans[reach] = span
+                spans[id(reach)] = span
             else:
-                groups = _clusters([(r[0] % turn, r[0] % turn + spans[r[2]], r) for r in some], turn)
+                groups = _clusters([(r[0] % turn, r[0] % turn + spans[id(r[2])], r) for r in some], turn)
                 if len(groups) > 1:
                     return any(clash([r for _, _, r in group], moduli[i + 1:]) for group in groups)
         return True
 
-    return any(clash(group, sorted({s for r in group for s, _ in r[2].steps if s > 0}, reverse=True)) for group in _clusters(regions, 0))
+    return any(clash(group, sorted({s for reach in {id(r[2]): r[2] for r in group}.values() for s, _ in reach.steps if s > 0}, reverse=True)) for group in _clusters(regions, 0))
 
 
 def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
     """Row ``n * B_out + j`` of each result is row ``n * B_in + parents[n, j]`` of its state, for states ``[N * B_in, ...]`` of any types and strides
     (the used part of a cache, say) and ``parents [N, B_out]`` int64; zeros where a parent lies outside ``[0, B_in)``.
 
-    ``out``: tensors to write; without it new ones, dense, their rows' dimensions in memory as the states have them.  ``out=states`` reorders in place (``B_out == B_in``, at most 128 beams): rows that keep their place
+    ``out``: tensors to write, of any strides (a state's own are the fastest); without it new contiguous ones.  ``out=states`` reorders in place (``B_out == B_in``, at most 128 beams): rows that keep their place
     are not moved.  A result is otherwise in memory of its own: one that may share an element with another result, with a state but the one that it is, or with
     ``parents`` is refused.  Views of one buffer that interleave without sharing an element are told apart.  Not differentiable, and no op that tracing sees: it
     works on addresses, so a compiled program is left for the call and goes on behind it."""
@@ -279,7 +259,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, *, out: 
         if len(results) != len(states):
             raise ValueError(f"{len(results)} results for {len(states)} states")
     else:
-        results = [_new_result(t, N * B_out) for t in states]
+        results = [t.new_empty((N * B_out,) + tuple(t.shape[1:])) for t in states]
     if not states:
         return results
     if torch.is_grad_enabled() and any([t.requires_grad for t in states + results]) or has_tangent(*states):

@@ -26,7 +26,7 @@ def test_states_in_any_order_of_dimensions(cuda_device, layout):
     t = view(values((8, *shape), BF16, cuda_device, 1))
     want = moved(t, parents, 4)
     (new,) = BS.beam_reorder([t], parents)
-    assert torch.equal(new, want)
+    assert torch.equal(new, want) and new.is_contiguous()
     for like in (t, want.contiguous()):  # into the same strides, and into those of the shape's order
         out = torch.empty_strided(like.shape, like.stride(), dtype=BF16, device=cuda_device)
         BS.beam_reorder([t], parents, out=[out])
@@ -42,6 +42,7 @@ def test_they_take_no_longer_than_plain_indexing(cuda_device, layout):
     gen = torch.Generator(device=cuda_device).manual_seed(1)
     parents = torch.randint(0, 8, (16, 8), generator=gen, device=cuda_device)
     rows = (parents + torch.arange(0, 128, 8, device=cuda_device)[:, None]).reshape(-1)
-    own, inside = least_ms(lambda: BS.beam_reorder(states, parents)), least_ms(lambda: BS.beam_reorder(states, parents, out=states))
+    into = [torch.empty_strided(t.shape, t.stride(), dtype=BF16, device=cuda_device) for t in states]
+    own, inside = least_ms(lambda: BS.beam_reorder(states, parents, out=into)), least_ms(lambda: BS.beam_reorder(states, parents, out=states))
     plain = least_ms(lambda: [t[rows] for t in states])
     assert own <= plain and inside <= plain, (own, inside, plain)

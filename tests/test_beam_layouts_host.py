@@ -1,4 +1,4 @@
-"""How many runs of memory the rows of a state are taken as, and how new results lie in memory.  No GPU."""
+"""How many runs of memory the rows of a state are taken as.  No GPU."""
 
 from __future__ import annotations
 
@@ -36,18 +36,6 @@ def test_the_longest_dimension_is_the_one_that_is_stepped_through():
     """From [rows, length, heads, dim] into [rows, heads, length, dim]: 4 places of 500 segments, not 500 of 4."""
     ((sizes, places),) = launches(bf16(4, 500, 4, 128).transpose(1, 2), bf16(4, 4, 500, 128))
     assert sizes[4:] == (500, 256) and len(places) == 4
-
-
-def test_new_results_lie_as_their_states_do():
-    parents = torch.zeros(2, 3, dtype=torch.int64)
-    for state in (bf16(4, 500, 4, 128).transpose(1, 2), bf16(4, 512, 4, 128)[:, :500].transpose(1, 2), bf16(4, 3, 70, 40).transpose(2, 3), bf16(4, 2, 50, 8)[:, :, :7],
-                  bf16(4, 5), bf16(4), bf16(4, 6, 1, 3).transpose(1, 3), bf16(4, 2, 1, 5).expand(4, 2, 3, 5), bf16(9, 4, 8).transpose(0, 1)):
-        out = BS._new_result(state, parents.numel())
-        assert out.shape == (6, *state.shape[1:]) and out.dtype == state.dtype
-        assert sorted(n * s for n, s in zip(out.shape, out.stride()) if n > 1)[-1] == out.numel()  # dense, no gaps
-        if 0 not in state.stride():
-            layout = BS._layout(state.shape, state.stride(), out.stride(), state.dtype, 2, 3)
-            assert len(layout.launches) == 1 and len(layout.launches[0][1]) == 1
 
 
 def test_every_element_is_taken_to_its_place():
