@@ -18,7 +18,7 @@
 // beam_join   a workgroup per item: joins the parts' sums; finds the k best of all parts' sorted lists.  Entry j of a list whose head r heads
 //             precede can only be among the k best if j + r < k, and must reach the best of eight bounds, each from the m-th entries of the ceil(k / m) lists
 //             with the best heads.  Some 2 k to 8 k entries are left; where that is many, the rank of 64 of them cuts them again.  Each then counts those before
-//             it.  5 to 8 us where k is 8 or 16, nearly all of it the latency of what it does one after the other.  Calls of 4 x 151936 in bf16 with k = 8, 64,
+//             it.  8 to 9 us where k is 8 or 16, nearly all of it the latency of what it does one after the other.  Calls of 4 x 151936 in bf16 with k = 8, 64,
 //             128: 20, 29, 72 us (elementary torch operations 300), of 16 x 8 x 128261 with k = 16, 64, 128: 30, 39, 107; of that with k = 128 the keys of the
 //             rows are the most, whose bound is the least of 128 groups' maxima.
 #include <hip/hip_runtime.h>
