@@ -151,15 +151,13 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
       const int p = p0 + u * kThreads;
       pc[u].widen(((const Unaligned*)(base + (size_t)(p < pieces ? p : pieces - 1) * 16))->v);
     }
-    float mx[kInFlight], top = -INFINITY;
+    float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      mx[u] = -INFINITY;
       if (p0 + u * kThreads < pieces) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) mx[u] = fmaxf(mx[u], pc[u].v[i]);
+        for (int i = 0; i < E; ++i) top = fmaxf(top, pc[u].v[i]);
       }
-      top = fmaxf(top, mx[u]);
     }
     lane_max = fmaxf(lane_max, top);
     if (__any(top > wave_top)) raise(top);
@@ -192,7 +190,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows(const BeamArgs a) {
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) {
         const int p = p0 + u * kThreads;
-        if (!__any(mx[u] >= bound)) continue;
+        float mx = pc[u].v[0];  // again: held since then, the pieces' maxima would not fit the registers
+#pragma unroll
+        for (int i = 1; i < E; ++i) mx = fmaxf(mx, pc[u].v[i]);
+        if (!__any(p < pieces && mx >= bound)) continue;
 #pragma unroll
         for (int i = 0; i < E; ++i) append(pc[u].v[i], p * E + i, p < pieces);
       }
