@@ -6,6 +6,7 @@ import threading
 
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from skyrl_amd import embedding as E
@@ -140,6 +141,26 @@ def test_a_pass_both_ways_replays_from_a_graph(cuda_device):
         leaf = weight.detach().clone().requires_grad_()
         eager = E.embedding_lookup(leaf, ids, scale=2.0)
         assert torch.equal(out, eager) and torch.equal(grad, torch.autograd.grad(eager, leaf, d)[0])
+
+
+def test_saved_ids_that_travel_and_forwards_that_run_again(cuda_device):
+    weight, ids, d = inputs(cuda_device)
+    (want,) = torch.autograd.grad(E.embedding_lookup(weight, ids), weight, d)
+    with torch.autograd.graph.save_on_cpu():
+        out = E.embedding_lookup(weight, ids)
+    assert torch.equal(torch.autograd.grad(out, weight, d)[0], want)
+    for reentrant in (False, True):
+        leaf = weight.detach().clone().requires_grad_()
+        torch.utils.checkpoint.checkpoint(lambda w: E.embedding_lookup(w * 1.0, ids), leaf, use_reentrant=reentrant).backward(d)
+        assert torch.equal(leaf.grad, want)
+
+
+def test_a_compiled_backward(cuda_device):
+    weight, ids, d = inputs(cuda_device)
+    (want,) = torch.autograd.grad(E.embedding_lookup(weight, ids), weight, d)
+    with torch._dynamo.compiled_autograd._enable(torch.compile(backend="eager", dynamic=False)):
+        E.embedding_lookup(weight, ids).backward(d)
+    assert torch.equal(weight.grad, want)
 
 
 def test_too_many_tokens_are_a_value_error(cuda_device):
